@@ -76,7 +76,8 @@ enum hs_device_flag {
   HS_DEV_LRU_CORRUPT = 4,        /* an LRU entry outside [0, hot_rows) was skipped */
   HS_DEV_MISSES_EXCEED_HOT = 8,  /* more misses than hot rows: tags/lru left unchanged */
   HS_DEV_WAIT_TIMEOUT = 16,      /* a bounded wait for an async copy ran out (results invalid) */
-  HS_DEV_MISALIGNED = 32         /* a batched metadata pointer was not 16-byte aligned: skipped */
+  HS_DEV_MISALIGNED = 32,        /* a batched metadata pointer was not 16-byte aligned: skipped */
+  HS_DEV_TOKEN_OUT_OF_RANGE = 64 /* a given token beyond the vocabulary: its result is NaN */
 };
 
 typedef void *hs_stream; /* cudaStream_t */

@@ -1,0 +1,136 @@
+// (6) Per-head RMS norms of queries and keys with the position rotation.
+//
+// y = x / sqrt(mean(x^2) + eps) * w, then the pair (y_i, y_{i+R}) turns by the
+// angle positions[n] * inv_freq[i], R = head_dim / 2. Every element is read and
+// written once; the sums, the norm and the rotation are fp32 and the result is
+// rounded to the element type once.
+//
+// The angle: a position of one million times an inverse frequency of 1 is
+// 159,155 turns; fp32 would keep the angle to 0.03 rad only. The product is
+// formed in fp64 in units of a turn, its whole turns are dropped there, and
+// sincospif() takes the remaining fraction in fp32 (an error of at most
+// 2^-25 turn, 1.9e-7 rad).
+#include <math.h>
+
+#include "common.cuh"
+#include "hisparse_verify.h"
+
+namespace hs {
+namespace {
+
+constexpr int kRopeThreads = 256;
+constexpr int kRopeWarps = kRopeThreads / 32;
+constexpr int kRopeMaxDim = 256;
+
+struct RopeParams {
+  int64_t tokens;
+  const void *in[2];  // query, key
+  int64_t token_stride[2], head_stride[2];
+  int heads[2];
+  const void *weight[2];
+  void *out[2];
+  int head_dim;
+  const void *positions;
+  int positions64;
+  const double *inv_freq;
+  float eps;
+};
+
+__device__ __forceinline__ double position_of(const RopeParams &p, int64_t n) {
+  return p.positions64 ? (double)static_cast<const int64_t *>(p.positions)[n]
+                       : (double)static_cast<const int32_t *>(p.positions)[n];
+}
+
+// cos and sin of position * inv_freq
+__device__ __forceinline__ void turn(double position, double inv_freq, float &cosine,
+                                     float &sine) {
+  constexpr double kInvTwoPi = 0.15915494309189533577;
+  const double turns = position * inv_freq * kInvTwoPi;
+  sincospif(2.f * (float)(turns - rint(turns)), &sine, &cosine);
+}
+
+// One warp for each (token, head); lane l holds the pairs l, l + 32, ... Serves
+// every even head_dim, stride and alignment.
+template <typename T>
+__global__ void __launch_bounds__(kRopeThreads) norm_rope_any_kernel(RopeParams p) {
+  constexpr int kPairs = kRopeMaxDim / 2 / 32;
+  const int lane = threadIdx.x & 31;
+  const int all = p.heads[0] + p.heads[1];
+  const int64_t item = (int64_t)blockIdx.x * kRopeWarps + (threadIdx.x >> 5);
+  if (item >= p.tokens * all) return;
+  const int64_t n = item / all;
+  int h = (int)(item % all);
+  const int which = h >= p.heads[0];
+  if (which) h -= p.heads[0];
+  const int half = p.head_dim / 2;
+  const T *x = static_cast<const T *>(p.in[which]) + n * p.token_stride[which] +
+               h * p.head_stride[which];
+  float a[kPairs], b[kPairs], sum = 0.f;
+#pragma unroll
+  for (int j = 0; j < kPairs; ++j) {
+    const int i = lane + 32 * j;
+    a[j] = i < half ? to_f32(x[i]) : 0.f;
+    b[j] = i < half ? to_f32(x[i + half]) : 0.f;
+    sum = fmaf(a[j], a[j], fmaf(b[j], b[j], sum));
+  }
+  const T *w = static_cast<const T *>(p.weight[which]);
+  float scale = 1.f;
+  if (w != nullptr) scale = rsqrtf(warp_xor_tree_sum(sum) / (float)p.head_dim + p.eps);
+  const double position = position_of(p, n);
+  T *out = static_cast<T *>(p.out[which]) + (n * p.heads[which] + h) * p.head_dim;
+#pragma unroll
+  for (int j = 0; j < kPairs; ++j) {
+    const int i = lane + 32 * j;
+    if (i >= half) break;
+    float cosine, sine;
+    turn(position, p.inv_freq[i], cosine, sine);
+    const float ya = a[j] * scale * (w ? to_f32(w[i]) : 1.f);
+    const float yb = b[j] * scale * (w ? to_f32(w[i + half]) : 1.f);
+    out[i] = from_f32<T>(ya * cosine - yb * sine);
+    out[i + half] = from_f32<T>(yb * cosine + ya * sine);
+  }
+}
+
+template <typename T> int launch(const RopeParams &p, cudaStream_t s) {
+  const int64_t blocks = ceil_div(p.tokens * (p.heads[0] + p.heads[1]), kRopeWarps);
+  if (blocks > 0x7fffffff)
+    return set_error(HS_ERR_UNSUPPORTED, "norm_rope: too many tokens");
+  norm_rope_any_kernel<T><<<(unsigned)blocks, kRopeThreads, 0, s>>>(p);
+  return check_launch("norm_rope_any_kernel");
+}
+
+}  // namespace
+}  // namespace hs
+
+extern "C" int hs_qk_norm_rope(int64_t tokens, const void *query, int64_t query_token_stride,
+                               int64_t query_head_stride, int q_heads, const void *key,
+                               int64_t key_token_stride, int64_t key_head_stride, int kv_heads,
+                               int head_dim, int dtype, const void *positions,
+                               int positions_dtype, const double *inv_freq,
+                               const void *query_weight, const void *key_weight, float eps,
+                               void *query_out, void *key_out, hs_stream stream) {
+  using namespace hs;
+  if (tokens < 0 || q_heads < 1 || kv_heads < 1 || head_dim < 2 || head_dim % 2)
+    return set_error(HS_ERR_INVALID_ARGUMENT, "norm_rope: invalid sizes");
+  if (head_dim > kRopeMaxDim)
+    return set_error(HS_ERR_UNSUPPORTED, "norm_rope: head_dim %d > %d is not supported", head_dim,
+                     kRopeMaxDim);
+  if (positions_dtype != HS_INT32 && positions_dtype != HS_INT64)
+    return set_error(HS_ERR_INVALID_ARGUMENT, "norm_rope: positions must be int32 or int64");
+  if (!(eps >= 0.f))
+    return set_error(HS_ERR_INVALID_ARGUMENT, "norm_rope: eps must not be negative");
+  if (tokens == 0) return HS_OK;
+  if (!query || !key || !positions || !inv_freq || !query_out || !key_out)
+    return set_error(HS_ERR_INVALID_ARGUMENT, "norm_rope: null pointer");
+  const RopeParams p{tokens, {query, key}, {query_token_stride, key_token_stride},
+                     {query_head_stride, key_head_stride}, {q_heads, kv_heads},
+                     {query_weight, key_weight}, {query_out, key_out}, head_dim, positions,
+                     positions_dtype == HS_INT64, inv_freq, eps};
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  switch (dtype) {
+    case HS_FLOAT32: return launch<float>(p, s);
+    case HS_FLOAT16: return launch<__half>(p, s);
+    case HS_BFLOAT16: return launch<__nv_bfloat16>(p, s);
+  }
+  return set_error(HS_ERR_INVALID_ARGUMENT, "norm_rope: invalid dtype %d", dtype);
+}

@@ -1,4 +1,5 @@
-"""ctypes binding of libhisparse.so, whose C ABI is declared in include/hisparse.h.
+"""ctypes binding of libhisparse.so, whose C ABI is declared in include/hisparse.h
+and include/hisparse_verify.h.
 
 The shared library is built in-tree (nano-hisparse_b200/libhisparse.so) by
 ``make -C nano-hisparse_b200/csrc`` or ``__graft_entry__.build()``. There is no
@@ -7,6 +8,7 @@ fallback: importing an operator without the library raises immediately.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import threading
 from pathlib import Path
@@ -26,6 +28,7 @@ DEVICE_FLAGS = {
     8: "more misses than hot rows; tables left unchanged",
     16: "a bounded wait for an asynchronous copy ran out; results are invalid",
     32: "a batched metadata pointer was not 16-byte aligned; the request was skipped",
+    64: "a given token beyond the vocabulary was met; its log probability is NaN",
 }
 
 _DTYPES = {torch.float32: HS_FLOAT32, torch.float16: HS_FLOAT16, torch.bfloat16: HS_BFLOAT16}
@@ -64,6 +67,17 @@ _SIGNATURES = {
                                _I64, _INT, _INT, _INT, _INT, _P, _P], _INT),
 }
 
+# include/hisparse_verify.h
+_VERIFY_SIGNATURES = {
+    "hs_qk_norm_rope": ([_I64, _P, _I64, _I64, _INT, _P, _I64, _I64, _INT, _INT, _INT, _P, _INT,
+                         _P, _P, _P, ctypes.c_float, _P, _P, _P], _INT),
+    "hs_attend_tree_workspace_bytes": ([_INT, _INT, _INT, _INT, _INT, _I64, _INT], _SZ),
+    "hs_attend_tree": ([_INT, _INT, _P, _I64, _I64, _P, _P, _I64, _I64, _INT, _P, _P, _P, _I64,
+                        _P, _I64, _I64, _P, _P, _INT, _INT, _INT, _INT, _P, _SZ, _P, _P], _INT),
+    "hs_token_logprobs": ([_I64, _P, _I64, _INT, _I64, _P, _INT, _INT, _P, _P, _INT, _P, _P, _P,
+                           _P], _INT),
+}
+
 _lib = None
 _lock = threading.Lock()
 
@@ -81,7 +95,7 @@ def load():
                 f"{LIB_PATH} is missing: build it with `make -C nano-hisparse_b200/csrc` "
                 "(the sm_100a kernels have no fallback)")
         lib = ctypes.CDLL(str(LIB_PATH))
-        for name, (argtypes, restype) in _SIGNATURES.items():
+        for name, (argtypes, restype) in {**_SIGNATURES, **_VERIFY_SIGNATURES}.items():
             fn = getattr(lib, name)
             fn.argtypes, fn.restype = argtypes, restype
         if lib.hs_version() != ABI_VERSION:
@@ -116,6 +130,16 @@ def require_cuda(*tensors):
     for t in tensors:
         if t is not None and (not isinstance(t, torch.Tensor) or t.device.type != "cuda"):
             raise ValueError("hisparse_b200 operators take CUDA tensors; there is no CPU path")
+
+
+_CURRENT = contextlib.nullcontext()
+
+
+def on_device(device):
+    """Context in which `device` is the current one (a launch runs there)."""
+    if device.index == torch.cuda.current_device():
+        return _CURRENT
+    return torch.cuda.device(device)
 
 
 def ptr(t):

@@ -1,0 +1,63 @@
+"""Log probabilities of given tokens, the distribution's entropy and its
+largest alternatives, in one pass over the logits (``hs_token_logprobs``).
+
+The reference engine takes the argmax of fp32 logits only
+(nano_hisparse/model.py:179, engine.py:90-120); scoring drafted or given
+tokens needs the normaliser as well.
+"""
+
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+
+from . import _lib
+
+
+class TokenLogprobs(NamedTuple):
+    logprobs: torch.Tensor      # fp32, the shape of the given tokens ([N, 0] without)
+    entropy: torch.Tensor       # fp32 [N], nats
+    top_logprobs: torch.Tensor  # fp32 [N, top], largest first
+    top_tokens: torch.Tensor    # int64 [N, top]; equal logits by the lower token
+
+
+def token_logprobs(logits, tokens=None, top=0) -> TokenLogprobs:
+    """logits: CUDA [N, V] (fp32, fp16, bf16; any row stride). tokens: int32 or
+    int64 [N] or [N, C]; a negative token is padding (log probability 0), one
+    past the vocabulary gives NaN and raises the device flag. top: how many of
+    the largest entries to return (at most 32). All results are fp32 sums over
+    the given values; -inf logits have probability 0, and a row with nothing
+    above -inf has log probabilities -inf and entropy 0. Runs on the current
+    stream."""
+    _lib.require_cuda(logits, tokens)
+    if logits.ndim != 2 or logits.shape[1] < 1:
+        raise ValueError("logits must be [rows, vocab]")
+    rows, vocab = logits.shape
+    if not 0 <= top <= vocab:
+        raise ValueError("top must be between 0 and the vocabulary size")
+    device, given, code = logits.device, 0, _lib.HS_INT64
+    if tokens is not None:
+        if tokens.dtype not in (torch.int32, torch.int64) or tokens.ndim not in (1, 2) \
+                or tokens.shape[0] != rows:
+            raise ValueError("tokens must be int32 or int64 [rows] or [rows, given]")
+        if tokens.device != device:
+            raise ValueError("all tensors must be on one device")
+        given = 1 if tokens.ndim == 1 else tokens.shape[1]
+        code = _lib.HS_INT64 if tokens.dtype == torch.int64 else _lib.HS_INT32
+        tokens = tokens.contiguous()
+    if logits.stride(1) != 1:
+        logits = logits.contiguous()
+    out = TokenLogprobs(
+        torch.empty((rows, 0) if tokens is None else tokens.shape, dtype=torch.float32,
+                    device=device),
+        torch.empty(rows, dtype=torch.float32, device=device),
+        torch.empty((rows, top), dtype=torch.float32, device=device),
+        torch.empty((rows, top), dtype=torch.int64, device=device))
+    with _lib.on_device(device):
+        _lib.check(_lib.load().hs_token_logprobs(
+            rows, logits.data_ptr(), logits.stride(0), _lib.dtype_code(logits.dtype), vocab,
+            _lib.ptr(tokens), code, given, out.logprobs.data_ptr(), out.entropy.data_ptr(), top,
+            out.top_logprobs.data_ptr(), out.top_tokens.data_ptr(),
+            _lib.status_word(device).data_ptr(), _lib.stream_of(device)))
+    return out
