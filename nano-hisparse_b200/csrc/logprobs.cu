@@ -3,7 +3,20 @@
 // With m the row's maximum, s = sum exp(x - m) and t = sum (x - m) exp(x - m):
 // lse = m + log s, the entropy is log s - t / s. Both sums are carried over the
 // row with a running maximum: raising it by d scales s by exp(-d) and t to
-// exp(-d) (t - d s).
+// exp(-d) (t - d s). So one pass over the logits gives all of it, and the work is
+// bound by reading them once.
+//
+// The alternatives come out of the same pass: every thread keeps the order key
+// of its best entry. The r-th best key of each warp, r = ceil(top / warps), the
+// smallest of them over the warps, is passed by at least `top` entries of the
+// block's part, so every one of its `top` largest entries has a key of at least
+// that. Threads whose own best passes it (a few more than `top`) read their
+// entries again, from L2, and collect those that pass; the collected keys are
+// ranked by counting.
+//
+// A row is split over a cluster of 1 to 8 blocks, which join their sums and their
+// best keys in the first block's shared memory: few rows reach many SMs without
+// a workspace or a second launch.
 #include <math.h>
 
 #include "common.cuh"
@@ -14,7 +27,13 @@ namespace {
 
 constexpr int kLogprobThreads = 256;
 constexpr int kLogprobWarps = kLogprobThreads / 32;
+constexpr int kLogprobBlocks = 4;   // blocks resident on an SM
 constexpr int kMaxTop = 32;
+constexpr int kMaxCluster = 8;
+constexpr int kAhead = 4;           // 16-byte vectors in flight per thread
+constexpr int kCandidates = 1024;   // keys collected before the exact threshold is taken
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kFar = -16384.f;    // exp(kFar) is 0 in fp32
 
 struct LogprobParams {
   const void *logits;
@@ -27,6 +46,7 @@ struct LogprobParams {
   float *top_logprobs;
   int64_t *top_tokens;
   int32_t *status;
+  int cluster;
 };
 
 // Order of an entry as one unsigned word: larger values first, equal values by
@@ -39,61 +59,333 @@ __device__ __forceinline__ uint32_t value_order(float x) {
 __device__ __forceinline__ uint64_t entry_order(float x, uint32_t index) {
   return (uint64_t)value_order(x) << 32 | (uint32_t)~index;
 }
+__device__ __forceinline__ float order_value(uint64_t order) {
+  const uint32_t u = (uint32_t)(order >> 32);
+  return u == 0xfffffffeu ? NAN : __uint_as_float((u & 0x80000000u) ? u & 0x7fffffffu : ~u);
+}
 
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// 16 bytes of logits
+template <typename T> struct Vector {
+  static constexpr int n = 16 / sizeof(T);
+  static __device__ __forceinline__ void widen(const uint4 &raw, float (&x)[n]) {
+    const T *e = reinterpret_cast<const T *>(&raw);
+#pragma unroll
+    for (int i = 0; i < n; ++i) x[i] = to_f32(e[i]);
+  }
+  static __device__ __forceinline__ float largest(const uint4 &raw) {
+    float x[n];
+    widen(raw, x);
+    float m = x[0];
+#pragma unroll
+    for (int i = 1; i < n; ++i) m = max_nan(m, x[i]);
+    return m;
+  }
+};
+// the 16-bit types in pairs
+template <typename T2> __device__ __forceinline__ float pair_largest(const uint4 &raw) {
+  const T2 *e = reinterpret_cast<const T2 *>(&raw);
+  const T2 m = __hmax2_nan(__hmax2_nan(e[0], e[1]), __hmax2_nan(e[2], e[3]));
+  return max_nan(to_f32(m.x), to_f32(m.y));
+}
+template <> __device__ __forceinline__ float Vector<__half>::largest(const uint4 &raw) {
+  return pair_largest<__half2>(raw);
+}
+template <> __device__ __forceinline__ float Vector<__nv_bfloat16>::largest(const uint4 &raw) {
+  return pair_largest<__nv_bfloat162>(raw);
+}
+
+// Differences are held above kFar where they multiply: a masked entry of -inf or
+// of the type's lowest value then adds 0 to t, not 0 * -inf. What that takes from
+// NaN and +inf comes back through s, whose own terms stay NaN.
 struct Softmax {
-  float m, s, t;
-  __device__ __forceinline__ void add(float x) {
-    if (x > m || x != x) {  // a new maximum, or NaN, which then stays
-      const float d = m - x, f = m == -INFINITY ? 0.f : expf(d);
-      t = m == -INFINITY ? 0.f : f * (t + d * s);
+  float m, s, t;  // maximum, sum exp(x - m), sum (x - m) exp(x - m)
+  __device__ __forceinline__ void raise(float to) {
+    if (m != -INFINITY) {
+      const float d = fmaxf(m - to, kFar), f = exp2f(d * kLog2e);
+      t = f * fmaf(d, s, t);
       s *= f;
-      m = x;
     }
-    const float d = x - m, e = m == -INFINITY ? 0.f : expf(d);
+    m = to;
+  }
+  __device__ __forceinline__ void add(float x) {  // x <= m
+    const float d = x - m, e = exp2f(d * kLog2e);
     s += e;
-    t += e * fmaxf(d, -200.f);  // exp(-200) is 0 in fp32
+    t = fmaf(e, fmaxf(d, kFar), t);
   }
   __device__ __forceinline__ void join(float m2, float s2, float t2) {
-    const float top = m2 > m || m2 != m2 ? m2 : m;
-    const float d1 = m - top, d2 = m2 - top;
-    const float f1 = m == -INFINITY ? 0.f : expf(d1), f2 = m2 == -INFINITY ? 0.f : expf(d2);
-    const float t1 = m == -INFINITY ? 0.f : f1 * (t + d1 * s);
-    t = t1 + (m2 == -INFINITY ? 0.f : f2 * (t2 + d2 * s2));
+    const float top = max_nan(m, m2);
+    const float d1 = fmaxf(m - top, kFar), d2 = fmaxf(m2 - top, kFar);
+    const float f1 = m == -INFINITY ? 0.f : exp2f(d1 * kLog2e);
+    const float f2 = m2 == -INFINITY ? 0.f : exp2f(d2 * kLog2e);
+    t = (m == -INFINITY ? 0.f : f1 * fmaf(d1, s, t)) +
+        (m2 == -INFINITY ? 0.f : f2 * fmaf(d2, s2, t2));
     s = f1 * s + f2 * s2;
     m = top;
   }
 };
 
-// One block for each row; the alternatives by one pass over the row for each.
+__device__ __forceinline__ uint64_t warp_largest(uint64_t v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const uint64_t other = __shfl_xor_sync(kFullMask, v, o);
+    if (other > v) v = other;
+  }
+  return v;
+}
+
+struct LogprobShared {
+  float m[kLogprobWarps], s[kLogprobWarps], t[kLogprobWarps];
+  uint64_t warp_best[kLogprobWarps];
+  uint64_t candidates[kCandidates];
+  uint64_t best[kMaxTop];
+  int found;
+  // written by every block of the cluster into the first one's
+  float joined[kMaxCluster][3];
+  uint64_t joined_best[kMaxCluster * kMaxTop];
+};
+
+// The part of a row that a block reads: whole 16-byte vectors, and for the first
+// block of a cluster the up to 2 (n - 1) entries before and after them.
+template <typename T> struct RowPart {
+  static constexpr int n = Vector<T>::n;
+  const T *x;
+  int head;          // entries before the first vector
+  int first, count;  // vectors
+  int edge;          // this thread's entry outside the vectors, or -1
+
+  __device__ __forceinline__ RowPart(const LogprobParams &p, const T *row, int rank) : x(row) {
+    const int misaligned = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+    head = min(p.vocab, (n - misaligned) % n);
+    const int vectors = (p.vocab - head) / n, tail = head + vectors * n;
+    const int share = (int)ceil_div(vectors, p.cluster);
+    first = min(vectors, rank * share);
+    count = min(vectors, first + share) - first;
+    const int i = threadIdx.x;
+    edge = rank != 0 ? -1 : i < head ? i : tail + i - head < p.vocab ? tail + i - head : -1;
+  }
+  __device__ __forceinline__ uint4 vector(int v) const {
+    return __ldg(reinterpret_cast<const uint4 *>(x + head) + first + v);
+  }
+  __device__ __forceinline__ uint32_t index(int v, int i) const {
+    return (uint32_t)(head + (first + v) * n + i);
+  }
+  // f(vector, its number) for this thread's vectors, kAhead loads at a time
+  template <typename F> __device__ __forceinline__ void each(F f) const {
+    for (int v0 = threadIdx.x; v0 < count; v0 += kAhead * kLogprobThreads) {
+      uint4 raw[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (v0 + u * kLogprobThreads < count) raw[u] = vector(v0 + u * kLogprobThreads);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (v0 + u * kLogprobThreads < count) f(raw[u], v0 + u * kLogprobThreads);
+    }
+  }
+};
+
+// Collects the block's entries with a key of at least `threshold`; returns their
+// number, of which the first kCandidates are kept. `mine`: a key that no entry of
+// this thread passes.
 template <typename T>
-__global__ void __launch_bounds__(kLogprobThreads) logprobs_kernel(LogprobParams p) {
-  __shared__ float sm[kLogprobWarps], ss[kLogprobWarps], st[kLogprobWarps];
-  __shared__ uint64_t best[kLogprobWarps];
-  const int64_t row = blockIdx.x;
+__device__ __forceinline__ int collect(LogprobShared &sh, const RowPart<T> &part, uint64_t mine,
+                                       uint64_t threshold) {
+  if (threadIdx.x == 0) sh.found = 0;
+  __syncthreads();
+  if (mine >= threshold) {
+    auto take = [&](uint64_t key) {
+      if (key < threshold) return;
+      const int at = atomicAdd(&sh.found, 1);
+      if (at < kCandidates) sh.candidates[at] = key;
+    };
+    const uint32_t least = (uint32_t)(threshold >> 32);
+    part.each([&](const uint4 &raw, int v) {
+      if (value_order(Vector<T>::largest(raw)) < least) return;
+      float x[Vector<T>::n];
+      Vector<T>::widen(raw, x);
+#pragma unroll
+      for (int i = 0; i < Vector<T>::n; ++i) take(entry_order(x[i], part.index(v, i)));
+    });
+    if (part.edge >= 0) take(entry_order(to_f32(part.x[part.edge]), (uint32_t)part.edge));
+  }
+  __syncthreads();
+  return sh.found;
+}
+
+// The block's `top` largest keys into sh.best (0 where it has fewer entries).
+// `mine` is this thread's best key, `bound` one that no entry of it passes.
+template <typename T>
+__device__ __forceinline__ void block_best(LogprobShared &sh, const RowPart<T> &part, int top,
+                                           uint64_t mine, uint64_t bound) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int deep = (top + kLogprobWarps - 1) / kLogprobWarps;
+  uint64_t left = mine, nth = 0;
+  for (int i = 0; i < deep; ++i) {  // keys are distinct unless 0
+    nth = warp_largest(left);
+    if (left == nth) left = 0;
+  }
+  if (lane == 0) sh.warp_best[warp] = nth;
+  if (threadIdx.x < kMaxTop) sh.best[threadIdx.x] = 0;
+  __syncthreads();
+  uint64_t threshold = sh.warp_best[0];
+  for (int w = 1; w < kLogprobWarps; ++w)
+    if (sh.warp_best[w] < threshold) threshold = sh.warp_best[w];
+  if (threshold == 0) threshold = 1;  // fewer entries than warps: all of them
+  int found = collect(sh, part, bound, threshold);
+  if (found > kCandidates) {
+    // Many entries pass (equal values, or the largest ones in few threads): take
+    // the top-th best of the threads' keys, the largest key that `top` threads
+    // reach, bit by bit.
+    uint64_t exact = 0;
+    for (int bit = 63; bit >= 0; --bit) {
+      const uint64_t trial = exact | 1ull << bit;
+      if (__syncthreads_count(mine >= trial) >= top) exact = trial;
+    }
+    if (exact > threshold) {
+      threshold = exact;
+      found = collect(sh, part, bound, threshold);
+    }
+  }
+  if (found <= kCandidates) {
+    for (int i = threadIdx.x; i < found; i += kLogprobThreads) {
+      const uint64_t key = sh.candidates[i];
+      int rank = 0;
+      for (int j = 0; j < found; ++j) rank += sh.candidates[j] > key;
+      if (rank < top) sh.best[rank] = key;
+    }
+  } else {  // one pass over the part for each
+    uint64_t below = ~0ull;
+    for (int k = 0; k < top; ++k) {
+      uint64_t next = 0;
+      auto take = [&](uint64_t key) {
+        if (key < below && key > next) next = key;
+      };
+      part.each([&](const uint4 &raw, int v) {
+        float x[Vector<T>::n];
+        Vector<T>::widen(raw, x);
+#pragma unroll
+        for (int i = 0; i < Vector<T>::n; ++i) take(entry_order(x[i], part.index(v, i)));
+      });
+      if (part.edge >= 0) take(entry_order(to_f32(part.x[part.edge]), (uint32_t)part.edge));
+      next = warp_largest(next);
+      __syncthreads();
+      if (lane == 0) sh.warp_best[warp] = next;
+      __syncthreads();
+      below = sh.warp_best[0];
+      for (int w = 1; w < kLogprobWarps; ++w)
+        if (sh.warp_best[w] > below) below = sh.warp_best[w];
+      if (threadIdx.x == 0) sh.best[k] = below;
+    }
+  }
+  __syncthreads();
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kLogprobThreads, kLogprobBlocks)
+    logprobs_kernel(LogprobParams p) {
+  __shared__ LogprobShared sh;
+  const int rank = (int)cluster_rank(), cluster = p.cluster;
+  const int64_t row = blockIdx.x / cluster;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // all blocks of the cluster run before any writes to the first one's memory
+  if (cluster > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;\n" ::: "memory");
   const T *x = static_cast<const T *>(p.logits) + row * p.row_stride;
+  const RowPart<T> part(p, x, rank);
+
   Softmax acc{-INFINITY, 0.f, 0.f};
-  for (int i = threadIdx.x; i < p.vocab; i += kLogprobThreads) acc.add(to_f32(x[i]));
+  int at = -1;  // the vector that first held this thread's maximum
+  for (int v0 = threadIdx.x; v0 < part.count; v0 += kAhead * kLogprobThreads) {
+    uint4 raw[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (v0 + u * kLogprobThreads < part.count) raw[u] = part.vector(v0 + u * kLogprobThreads);
+    float largest = -INFINITY;
+    int where = v0;
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (v0 + u * kLogprobThreads < part.count) {
+        const float m = Vector<T>::largest(raw[u]);
+        if (m > largest || (m != m && largest == largest)) {
+          largest = m;
+          where = v0 + u * kLogprobThreads;
+        }
+      }
+    if (at < 0 || largest > acc.m || (largest != largest && acc.m == acc.m)) {
+      at = where;
+      acc.raise(largest);
+    }
+    if (acc.m == -INFINITY) continue;
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (v0 + u * kLogprobThreads < part.count) {
+        float e[Vector<T>::n];
+        Vector<T>::widen(raw[u], e);
+#pragma unroll
+        for (int i = 0; i < Vector<T>::n; ++i) acc.add(e[i]);
+      }
+  }
+  // This thread's best entry is at most `bound` and at least `mine` in the order:
+  // the vector is known, the place in it is not.
+  uint64_t mine = 0, bound = 0;
+  if (at >= 0) {
+    mine = entry_order(acc.m, part.index(at, Vector<T>::n - 1));
+    bound = entry_order(acc.m, part.index(at, 0));
+  }
+  if (part.edge >= 0) {
+    const float e = to_f32(x[part.edge]);
+    const uint64_t key = entry_order(e, (uint32_t)part.edge);
+    if (key > mine) mine = key;
+    if (key > bound) bound = key;
+    if (e != -INFINITY) {
+      if (e > acc.m || e != e) acc.raise(e);
+      acc.add(e);
+    }
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1)
     acc.join(__shfl_xor_sync(kFullMask, acc.m, o), __shfl_xor_sync(kFullMask, acc.s, o),
              __shfl_xor_sync(kFullMask, acc.t, o));
   if (lane == 0) {
-    sm[warp] = acc.m;
-    ss[warp] = acc.s;
-    st[warp] = acc.t;
+    sh.m[warp] = acc.m;
+    sh.s[warp] = acc.s;
+    sh.t[warp] = acc.t;
   }
-  __syncthreads();
-  acc = Softmax{sm[0], ss[0], st[0]};
-  for (int w = 1; w < kLogprobWarps; ++w) acc.join(sm[w], ss[w], st[w]);
+  if (p.top > 0) block_best(sh, part, p.top, mine, bound);
+  else __syncthreads();
+
+  if (cluster > 1) asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+  LogprobShared &out = *(cluster > 1 ? map_rank(&sh, 0) : &sh);
+  if (threadIdx.x == 0) {
+    acc = Softmax{sh.m[0], sh.s[0], sh.t[0]};
+    for (int w = 1; w < kLogprobWarps; ++w) acc.join(sh.m[w], sh.s[w], sh.t[w]);
+    out.joined[rank][0] = acc.m;
+    out.joined[rank][1] = acc.s;
+    out.joined[rank][2] = acc.t;
+  }
+  if (threadIdx.x < p.top) out.joined_best[rank * p.top + threadIdx.x] = sh.best[threadIdx.x];
+  if (cluster > 1) {
+    cluster_barrier();
+    if (rank != 0) return;
+  } else {
+    __syncthreads();
+  }
+
+  acc = Softmax{sh.joined[0][0], sh.joined[0][1], sh.joined[0][2]};
+  for (int r = 1; r < cluster; ++r)
+    acc.join(sh.joined[r][0], sh.joined[r][1], sh.joined[r][2]);
   const bool empty = acc.m == -INFINITY;
   const float log_s = logf(acc.s);
   // (x - m) - log s: one rounding less than x - lse for entries near the maximum
   auto logprob = [&](float v) { return empty ? -INFINITY : (v - acc.m) - log_s; };
   for (int c = threadIdx.x; c < p.given; c += kLogprobThreads) {
-    const int64_t at = row * p.given + c;
-    const int64_t token = p.tokens64 ? static_cast<const int64_t *>(p.tokens)[at]
-                                     : static_cast<const int32_t *>(p.tokens)[at];
+    const int64_t where = row * p.given + c;
+    const int64_t token = p.tokens64 ? static_cast<const int64_t *>(p.tokens)[where]
+                                     : static_cast<const int32_t *>(p.tokens)[where];
     float v = 0.f;
     if (token >= p.vocab) {
       flag(p.status, HS_DEV_TOKEN_OUT_OF_RANGE);
@@ -101,38 +393,48 @@ __global__ void __launch_bounds__(kLogprobThreads) logprobs_kernel(LogprobParams
     } else if (token >= 0) {
       v = logprob(to_f32(x[token]));
     }
-    p.logprobs[at] = v;
+    p.logprobs[where] = v;
   }
   if (threadIdx.x == 0 && p.entropy != nullptr)
     p.entropy[row] = empty ? 0.f : log_s - acc.t / acc.s;
-  uint64_t below = ~0ull;
-  for (int k = 0; k < p.top; ++k) {
-    uint64_t mine = 0;
-    for (int i = threadIdx.x; i < p.vocab; i += kLogprobThreads) {
-      const uint64_t e = entry_order(to_f32(x[i]), (uint32_t)i);
-      if (e < below && e > mine) mine = e;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const uint64_t other = __shfl_xor_sync(kFullMask, mine, o);
-      if (other > mine) mine = other;
-    }
-    __syncthreads();
-    if (lane == 0) best[warp] = mine;
-    __syncthreads();
-    below = best[0];
-    for (int w = 1; w < kLogprobWarps; ++w)
-      if (best[w] > below) below = best[w];
-    if (threadIdx.x == 0) {
-      const uint32_t index = ~(uint32_t)below;
-      p.top_tokens[row * p.top + k] = index;
-      p.top_logprobs[row * p.top + k] = logprob(to_f32(x[index]));
+  const int keys = cluster * p.top;  // distinct but for the 0 of a block with fewer entries
+  if ((int)threadIdx.x < keys) {
+    const uint64_t key = sh.joined_best[threadIdx.x];
+    int rank_of = 0;
+    for (int j = 0; j < keys; ++j) rank_of += sh.joined_best[j] > key;
+    if (key != 0 && rank_of < p.top) {
+      p.top_tokens[row * p.top + rank_of] = (int64_t)~(uint32_t)key;
+      p.top_logprobs[row * p.top + rank_of] = logprob(order_value(key));
     }
   }
 }
 
-template <typename T> int launch(const LogprobParams &p, int64_t rows, cudaStream_t s) {
-  logprobs_kernel<T><<<(unsigned)rows, kLogprobThreads, 0, s>>>(p);
+// Blocks of a row: as many as give every SM's kLogprobBlocks places work, while a
+// block still has two rounds of loads to do.
+int logprob_cluster(int64_t rows, int64_t row_bytes) {
+  const int64_t places = (int64_t)kLogprobBlocks * sm_count();
+  const int64_t least = 2 * kAhead * kLogprobThreads * 16;
+  int c = 1;
+  while (c < kMaxCluster && rows * c * 2 <= places && row_bytes >= least * c * 2) c *= 2;
+  return c;
+}
+
+template <typename T> int launch(LogprobParams &p, int64_t rows, cudaStream_t s) {
+  static_assert(kMaxCluster * kMaxTop <= kLogprobThreads, "one thread for each joined key");
+  p.cluster = logprob_cluster(rows, (int64_t)p.vocab * sizeof(T));
+  if (rows * p.cluster > 0x7fffffff)
+    return set_error(HS_ERR_UNSUPPORTED, "logprobs: too many rows");
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3((unsigned)(rows * p.cluster));
+  config.blockDim = dim3(kLogprobThreads);
+  config.stream = s;
+  cudaLaunchAttribute attribute{};
+  attribute.id = cudaLaunchAttributeClusterDimension;
+  attribute.val.clusterDim.x = (unsigned)p.cluster;
+  attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+  config.attrs = &attribute;
+  config.numAttrs = p.cluster > 1 ? 1 : 0;
+  cudaLaunchKernelEx(&config, logprobs_kernel<T>, p);
   return check_launch("logprobs_kernel");
 }
 
@@ -156,9 +458,9 @@ extern "C" int hs_token_logprobs(int64_t rows, const void *logits, int64_t row_s
   if (!logits || (given > 0 && (!tokens || !out_logprobs)) ||
       (top > 0 && (!out_top_logprobs || !out_top_tokens)))
     return set_error(HS_ERR_INVALID_ARGUMENT, "logprobs: null pointer");
-  const LogprobParams p{logits, row_stride, (int)vocab, tokens, tokens_dtype == HS_INT64, given,
-                        out_logprobs, out_entropy, top, out_top_logprobs, out_top_tokens,
-                        device_status};
+  LogprobParams p{logits, row_stride, (int)vocab, tokens, tokens_dtype == HS_INT64, given,
+                  out_logprobs, out_entropy, top, out_top_logprobs, out_top_tokens,
+                  device_status, 1};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (dtype) {
     case HS_FLOAT32: return launch<float>(p, rows, s);

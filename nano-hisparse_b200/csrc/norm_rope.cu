@@ -91,7 +91,147 @@ __global__ void __launch_bounds__(kRopeThreads) norm_rope_any_kernel(RopeParams 
   }
 }
 
+// The same with 16-byte loads: lane j of a group of kGroup lanes holds the pairs
+// j * kVec .. of one head, a warp 32 / kGroup heads at once. A warp walks `span`
+// head sets of one token with the lane's cosines and sines in registers; the
+// loads of kRopeAhead head sets are issued together, the first of them before
+// the angles are computed.
+constexpr int kRopeAhead = 2;
+
+template <typename T, int kVec>
+__device__ __forceinline__ void unpack(const uint4 &raw, float (&x)[kVec]) {
+  const T *e = reinterpret_cast<const T *>(&raw);
+#pragma unroll
+  for (int i = 0; i < kVec; ++i) x[i] = to_f32(e[i]);
+}
+
+__device__ __forceinline__ uint4 choose(bool first, const uint4 &a, const uint4 &b) {
+  return make_uint4(first ? a.x : b.x, first ? a.y : b.y, first ? a.z : b.z, first ? a.w : b.w);
+}
+
+template <typename T, int kGroup>
+__global__ void __launch_bounds__(kRopeThreads) norm_rope_kernel(RopeParams p, int spans,
+                                                                 int span) {
+  constexpr int kVec = 16 / sizeof(T), kHeads = 32 / kGroup;
+  const int lane = threadIdx.x & 31, j = lane % kGroup;
+  const int all = p.heads[0] + p.heads[1], half = p.head_dim / 2;
+  const int64_t item = (int64_t)blockIdx.x * kRopeWarps + (threadIdx.x >> 5);
+  const int64_t n = item / spans;
+  if (n >= p.tokens) return;
+  const int first = (int)(item % spans) * span * kHeads + lane / kGroup;
+  const int last = min(all, ((int)(item % spans) + 1) * span * kHeads);
+  const bool in_head = j * kVec < half;
+  const T *in[2] = {static_cast<const T *>(p.in[0]) + n * p.token_stride[0] + j * kVec,
+                    static_cast<const T *>(p.in[1]) + n * p.token_stride[1] + j * kVec};
+
+  uint4 lo[kRopeAhead], hi[kRopeAhead];
+  auto fetch = [&](int h0) {
+#pragma unroll
+    for (int u = 0; u < kRopeAhead; ++u) {
+      const int h = h0 + u * kHeads;
+      lo[u] = hi[u] = make_uint4(0, 0, 0, 0);
+      if (h < last && in_head) {
+        const T *x = h < p.heads[0] ? in[0] + h * p.head_stride[0]
+                                    : in[1] + (h - p.heads[0]) * p.head_stride[1];
+        lo[u] = __ldcs(reinterpret_cast<const uint4 *>(x));
+        hi[u] = __ldcs(reinterpret_cast<const uint4 *>(x + half));
+      }
+    }
+  };
+  fetch(first);
+  uint4 w_lo[2], w_hi[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const T *w = static_cast<const T *>(p.weight[k]) + j * kVec;
+    if (p.weight[k] != nullptr && in_head) {
+      w_lo[k] = __ldg(reinterpret_cast<const uint4 *>(w));
+      w_hi[k] = __ldg(reinterpret_cast<const uint4 *>(w + half));
+    }
+  }
+  float cosine[kVec], sine[kVec];
+  const double position = position_of(p, n);
+#pragma unroll
+  for (int i = 0; i < kVec; ++i) {
+    cosine[i] = sine[i] = 0.f;
+    if (in_head) turn(position, __ldg(p.inv_freq + j * kVec + i), cosine[i], sine[i]);
+  }
+  // every lane of the warp takes every step: the norms are sums over its group
+  for (int h0 = first; h0 - lane / kGroup < last; h0 += kRopeAhead * kHeads) {
+    float a[kRopeAhead][kVec], b[kRopeAhead][kVec];
+#pragma unroll
+    for (int u = 0; u < kRopeAhead; ++u) {
+      unpack<T, kVec>(lo[u], a[u]);
+      unpack<T, kVec>(hi[u], b[u]);
+    }
+    if (h0 - lane / kGroup + kRopeAhead * kHeads < last) fetch(h0 + kRopeAhead * kHeads);
+#pragma unroll
+    for (int u = 0; u < kRopeAhead; ++u) {
+      const int h = h0 + u * kHeads;
+      const int which = h >= p.heads[0];
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) sum = fmaf(a[u][i], a[u][i], fmaf(b[u][i], b[u][i], sum));
+#pragma unroll
+      for (int o = kGroup / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(kFullMask, sum, o);
+      if (h >= last || !in_head) continue;
+      if (p.weight[which] != nullptr) {
+        const float scale = rsqrtf(sum / (float)p.head_dim + p.eps);
+        float wa[kVec], wb[kVec];
+        unpack<T, kVec>(choose(which, w_lo[1], w_lo[0]), wa);
+        unpack<T, kVec>(choose(which, w_hi[1], w_hi[0]), wb);
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) {
+          a[u][i] *= scale * wa[i];
+          b[u][i] *= scale * wb[i];
+        }
+      }
+      uint4 out_lo, out_hi;
+      T *ol = reinterpret_cast<T *>(&out_lo), *oh = reinterpret_cast<T *>(&out_hi);
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) {
+        ol[i] = from_f32<T>(a[u][i] * cosine[i] - b[u][i] * sine[i]);
+        oh[i] = from_f32<T>(b[u][i] * cosine[i] + a[u][i] * sine[i]);
+      }
+      T *out = static_cast<T *>(p.out[which]) +
+               (n * p.heads[which] + (which ? h - p.heads[0] : h)) * p.head_dim + j * kVec;
+      *reinterpret_cast<uint4 *>(out) = out_lo;
+      *reinterpret_cast<uint4 *>(out + half) = out_hi;
+    }
+  }
+}
+
+template <typename T, int kGroup> int launch_vector(const RopeParams &p, cudaStream_t s) {
+  // One token's heads are split over warps until every SM has 16 of them: few
+  // tokens spread out, many tokens compute their angles once.
+  const int sets = (int)ceil_div(p.heads[0] + p.heads[1], 32 / kGroup);
+  const int64_t want = ceil_div((int64_t)16 * sm_count(), p.tokens);
+  const int spans0 = (int)(want < 1 ? 1 : (want > sets ? sets : want));
+  const int span = (int)ceil_div(sets, spans0), spans = (int)ceil_div(sets, span);
+  const int64_t blocks = ceil_div(p.tokens * spans, kRopeWarps);
+  if (blocks > 0x7fffffff)
+    return set_error(HS_ERR_UNSUPPORTED, "norm_rope: too many tokens");
+  norm_rope_kernel<T, kGroup><<<(unsigned)blocks, kRopeThreads, 0, s>>>(p, spans, span);
+  return check_launch("norm_rope_kernel");
+}
+
 template <typename T> int launch(const RopeParams &p, cudaStream_t s) {
+  // 16-byte vectors: half a head is a whole number of them, and every address
+  // is a multiple of 16 bytes
+  constexpr int kVec = 16 / sizeof(T);
+  const int half = p.head_dim / 2;
+  bool vector = half % kVec == 0;
+  for (int k = 0; k < 2; ++k)
+    vector = vector && p.token_stride[k] % kVec == 0 && p.head_stride[k] % kVec == 0 &&
+             ((reinterpret_cast<uintptr_t>(p.in[k]) | reinterpret_cast<uintptr_t>(p.out[k]) |
+               reinterpret_cast<uintptr_t>(p.weight[k])) & 15) == 0;
+  if (vector) {
+    const int lanes = half / kVec;
+    if (lanes <= 4) return launch_vector<T, 4>(p, s);
+    if (lanes <= 8) return launch_vector<T, 8>(p, s);
+    if constexpr (kVec == 4)  // the largest half holds 32 vectors of fp32
+      if (lanes > 16) return launch_vector<T, 32>(p, s);
+    return launch_vector<T, 16>(p, s);
+  }
   const int64_t blocks = ceil_div(p.tokens * (p.heads[0] + p.heads[1]), kRopeWarps);
   if (blocks > 0x7fffffff)
     return set_error(HS_ERR_UNSUPPORTED, "norm_rope: too many tokens");
