@@ -132,14 +132,33 @@ def require_cuda(*tensors):
             raise ValueError("hisparse_b200 operators take CUDA tensors; there is no CPU path")
 
 
+def one_device(first, *others) -> int:
+    """Index of the CUDA device that holds every given tensor (None is skipped)."""
+    try:
+        index = first.get_device()
+        same = index >= 0
+        for t in others:
+            if t is not None and t.get_device() != index:
+                same = False
+    except AttributeError:
+        same = False
+    if not same:
+        require_cuda(first, *others)
+        raise ValueError("all tensors must be on one device")
+    return index
+
+
 _CURRENT = contextlib.nullcontext()
 
 
-def on_device(device):
-    """Context in which `device` is the current one (a launch runs there)."""
-    if device.index == torch.cuda.current_device():
-        return _CURRENT
-    return torch.cuda.device(device)
+def on_device(index: int):
+    """Context in which device `index` is the current one (a launch runs there)."""
+    return _CURRENT if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
+
+
+def raw_stream(index: int) -> int:
+    """stream_of for a device index, without making a Stream object."""
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def ptr(t):
@@ -160,6 +179,21 @@ def status_word(device) -> torch.Tensor:
             word = torch.zeros(1, dtype=torch.int32, device=f"cuda:{index}")
         _status_words[index] = word
     return word
+
+
+_status_pointers: dict = {}
+
+
+def status_pointer(index: int) -> int:
+    """Address of status_word of device `index`; 0 (no flags are recorded) when the
+    first call on the device is being captured, since the word would belong to
+    that graph."""
+    pointer = _status_pointers.get(index)
+    if pointer is None:
+        if torch.cuda.is_current_stream_capturing() and index not in _status_words:
+            return 0
+        pointer = _status_pointers[index] = status_word(f"cuda:{index}").data_ptr()
+    return pointer
 
 
 def device_flags(device, reset=True) -> list[str]:

@@ -14,6 +14,8 @@ import torch
 
 from . import _lib
 
+_TOKENS = {torch.int32: _lib.HS_INT32, torch.int64: _lib.HS_INT64}
+
 
 class TokenLogprobs(NamedTuple):
     logprobs: torch.Tensor      # fp32, the shape of the given tokens ([N, 0] without)
@@ -30,34 +32,31 @@ def token_logprobs(logits, tokens=None, top=0) -> TokenLogprobs:
     the given values; -inf logits have probability 0, and a row with nothing
     above -inf has log probabilities -inf and entropy 0. Runs on the current
     stream."""
-    _lib.require_cuda(logits, tokens)
+    index = _lib.one_device(logits, tokens)
     if logits.ndim != 2 or logits.shape[1] < 1:
         raise ValueError("logits must be [rows, vocab]")
     rows, vocab = logits.shape
     if not 0 <= top <= vocab:
         raise ValueError("top must be between 0 and the vocabulary size")
-    device, given, code = logits.device, 0, _lib.HS_INT64
+    shape, given, code = (rows, 0), 0, _lib.HS_INT64
     if tokens is not None:
-        if tokens.dtype not in (torch.int32, torch.int64) or tokens.ndim not in (1, 2) \
-                or tokens.shape[0] != rows:
+        shape = tokens.shape
+        if tokens.dtype not in _TOKENS or len(shape) not in (1, 2) or shape[0] != rows:
             raise ValueError("tokens must be int32 or int64 [rows] or [rows, given]")
-        if tokens.device != device:
-            raise ValueError("all tensors must be on one device")
-        given = 1 if tokens.ndim == 1 else tokens.shape[1]
-        code = _lib.HS_INT64 if tokens.dtype == torch.int64 else _lib.HS_INT32
+        given = 1 if len(shape) == 1 else shape[1]
+        code = _TOKENS[tokens.dtype]
         tokens = tokens.contiguous()
     if logits.stride(1) != 1:
         logits = logits.contiguous()
-    out = TokenLogprobs(
-        torch.empty((rows, 0) if tokens is None else tokens.shape, dtype=torch.float32,
-                    device=device),
-        torch.empty(rows, dtype=torch.float32, device=device),
-        torch.empty((rows, top), dtype=torch.float32, device=device),
-        torch.empty((rows, top), dtype=torch.int64, device=device))
-    with _lib.on_device(device):
+    device = logits.device
+    logprobs = torch.empty(shape, dtype=torch.float32, device=device)
+    entropy = torch.empty(rows, dtype=torch.float32, device=device)
+    top_logprobs = torch.empty((rows, top), dtype=torch.float32, device=device)
+    top_tokens = torch.empty((rows, top), dtype=torch.int64, device=device)
+    with _lib.on_device(index):
         _lib.check(_lib.load().hs_token_logprobs(
             rows, logits.data_ptr(), logits.stride(0), _lib.dtype_code(logits.dtype), vocab,
-            _lib.ptr(tokens), code, given, out.logprobs.data_ptr(), out.entropy.data_ptr(), top,
-            out.top_logprobs.data_ptr(), out.top_tokens.data_ptr(),
-            _lib.status_word(device).data_ptr(), _lib.stream_of(device)))
-    return out
+            _lib.ptr(tokens), code, given, logprobs.data_ptr(), entropy.data_ptr(), top,
+            top_logprobs.data_ptr(), top_tokens.data_ptr(), _lib.status_pointer(index),
+            _lib.raw_stream(index)))
+    return TokenLogprobs(logprobs, entropy, top_logprobs, top_tokens)

@@ -13,6 +13,8 @@ import torch
 
 from . import _lib
 
+_POSITIONS = {torch.int32: _lib.HS_INT32, torch.int64: _lib.HS_INT64}
+
 
 def rope_frequencies(head_dim: int, theta: float, device="cuda") -> torch.Tensor:
     """theta^(-2i/head_dim) for i < head_dim / 2, in fp64 (the angles of far
@@ -44,38 +46,35 @@ def qk_norm_rope(query, key, positions, inv_freq, query_weight=None, key_weight=
     same dtype. Returns new contiguous (query, key); fp32 arithmetic with one
     rounding. Runs on the current stream.
     """
-    _lib.require_cuda(query, key, positions, inv_freq, query_weight, key_weight)
+    index = _lib.one_device(query, key, positions, inv_freq, query_weight, key_weight)
     if query.ndim != 3:
         raise ValueError("query must be [tokens, heads, head_dim]")
     tokens, q_heads, dim = query.shape
-    query = _check_heads("query", query, tokens, dim, query.dtype)
-    key = _check_heads("key", key, tokens, dim, query.dtype)
+    dtype = query.dtype
+    query = _check_heads("query", query, tokens, dim, dtype)
+    key = _check_heads("key", key, tokens, dim, dtype)
     if dim < 2 or dim % 2:
         raise ValueError("head_dim must be even")
-    if positions.shape != (tokens,) or positions.dtype not in (torch.int32, torch.int64):
+    if positions.shape != (tokens,) or positions.dtype not in _POSITIONS:
         raise ValueError("positions must be int32 or int64 [tokens]")
     if inv_freq.shape != (dim // 2,) or inv_freq.dtype != torch.float64:
         raise ValueError("inv_freq must be float64 [head_dim / 2]")
-    for w in (query_weight, key_weight):
-        if w is not None and (w.shape != (dim,) or w.dtype != query.dtype):
-            raise ValueError("norm weights must be [head_dim] of the query's dtype")
-    device = query.device
-    for t in (key, positions, inv_freq, query_weight, key_weight):
-        if t is not None and t.device != device:
-            raise ValueError("all tensors must be on one device")
+    weights = [None, None]
+    for i, w in enumerate((query_weight, key_weight)):
+        if w is not None:
+            if w.shape != (dim,) or w.dtype != dtype:
+                raise ValueError("norm weights must be [head_dim] of the query's dtype")
+            weights[i] = w = w.contiguous()
     positions, inv_freq = positions.contiguous(), inv_freq.contiguous()
-    if query_weight is not None:
-        query_weight = query_weight.contiguous()
-    if key_weight is not None:
-        key_weight = key_weight.contiguous()
-    query_out = torch.empty((tokens, q_heads, dim), dtype=query.dtype, device=device)
-    key_out = torch.empty((tokens, key.shape[1], dim), dtype=query.dtype, device=device)
-    with _lib.on_device(device):
+    query_out = torch.empty_like(query, memory_format=torch.contiguous_format)
+    key_out = torch.empty_like(key, memory_format=torch.contiguous_format)
+    q_token, q_head, _ = query.stride()
+    k_token, k_head, _ = key.stride()
+    with _lib.on_device(index):
         _lib.check(_lib.load().hs_qk_norm_rope(
-            tokens, query.data_ptr(), query.stride(0), query.stride(1), q_heads, key.data_ptr(),
-            key.stride(0), key.stride(1), key.shape[1], dim, _lib.dtype_code(query.dtype),
-            positions.data_ptr(),
-            _lib.HS_INT64 if positions.dtype == torch.int64 else _lib.HS_INT32,
-            inv_freq.data_ptr(), _lib.ptr(query_weight), _lib.ptr(key_weight), eps,
-            query_out.data_ptr(), key_out.data_ptr(), _lib.stream_of(device)))
+            tokens, query.data_ptr(), q_token, q_head, q_heads, key.data_ptr(), k_token, k_head,
+            key.shape[1], dim, _lib.dtype_code(dtype), positions.data_ptr(),
+            _POSITIONS[positions.dtype], inv_freq.data_ptr(), _lib.ptr(weights[0]),
+            _lib.ptr(weights[1]), eps, query_out.data_ptr(), key_out.data_ptr(),
+            _lib.raw_stream(index)))
     return query_out, key_out

@@ -56,7 +56,7 @@ def attend_tree(query, key, value, mask, pool, rows, config, counts=None, nodes=
     throughout; any batch and node stride of query, key and value with adjacent
     heads. Returns a new [B, T, Hq, D]. Runs on the current stream.
     """
-    _lib.require_cuda(query, key, value, mask, pool, rows, counts, nodes)
+    index = _lib.one_device(query, key, value, mask, pool, rows, counts, nodes)
     if query.ndim != 4 or query.shape[3] != config.head_dim:
         raise ValueError("query must be [batch, nodes, heads, head_dim]")
     batch, width, q_heads, dim = query.shape
@@ -76,31 +76,28 @@ def attend_tree(query, key, value, mask, pool, rows, config, counts=None, nodes=
         raise ValueError("mask must be int64 [batch, nodes]")
     if rows.ndim != 2 or rows.shape[0] != batch or rows.dtype != torch.int64:
         raise ValueError("rows must be int64 [batch, rows]")
-    device = query.device
-    for t in (key, value, mask, pool, rows):
-        if t.device != device:
-            raise ValueError("all tensors must be on one device")
     for name, t in (("counts", counts), ("nodes", nodes)):
         if t is not None and (t.shape != (batch,) or t.dtype != torch.int32
-                              or t.device != device or not t.is_contiguous()):
-            raise ValueError(f"{name} must be contiguous int32 [batch] on the query's device")
+                              or not t.is_contiguous()):
+            raise ValueError(f"{name} must be contiguous int32 [batch]")
     query, key, value, mask = (_heads_adjacent(query), _heads_adjacent(key),
                                _heads_adjacent(value), mask.contiguous())
     if key.stride() != value.stride():
         key, value = key.contiguous(), value.contiguous()
     if rows.stride(1) != 1 and rows.shape[1] > 1:
         rows = rows.contiguous()
-    out = torch.empty((batch, width, q_heads, dim), dtype=query.dtype, device=device)
+    out = torch.empty_like(query, memory_format=torch.contiguous_format)
     lib, code, count = _lib.load(), _lib.dtype_code(query.dtype), rows.shape[1]
-    with _lib.on_device(device):
+    q_batch, q_node, _, _ = query.stride()
+    kv_batch, kv_node, _, _ = key.stride()
+    with _lib.on_device(index):
         nbytes = lib.hs_attend_tree_workspace_bytes(batch, width, q_heads, config.kv_heads, dim,
                                                     count, code)
-        ws = _lib.workspace(nbytes, device)
+        ws = _lib.workspace(nbytes, query.device)
         _lib.check(lib.hs_attend_tree(
-            batch, width, query.data_ptr(), query.stride(0), query.stride(1), key.data_ptr(),
-            value.data_ptr(), key.stride(0), key.stride(1), code, mask.data_ptr(),
-            _lib.ptr(nodes), pool.data_ptr(), pool.shape[0], rows.data_ptr(), rows.stride(0),
-            count, _lib.ptr(counts), out.data_ptr(), q_heads, config.kv_heads, dim,
-            config.page_size, _lib.ptr(ws), nbytes, _lib.status_word(device).data_ptr(),
-            _lib.stream_of(device)))
+            batch, width, query.data_ptr(), q_batch, q_node, key.data_ptr(), value.data_ptr(),
+            kv_batch, kv_node, code, mask.data_ptr(), _lib.ptr(nodes), pool.data_ptr(),
+            pool.shape[0], rows.data_ptr(), rows.stride(0), count, _lib.ptr(counts),
+            out.data_ptr(), q_heads, config.kv_heads, dim, config.page_size, _lib.ptr(ws), nbytes,
+            _lib.status_pointer(index), _lib.raw_stream(index)))
     return out
