@@ -4,7 +4,7 @@
 // the M = 128 tile of tcgen05.mma, its rows the TMEM lanes). With more than 128
 // rows stream w owns rows 128 w .. and both work on every block of 64 keys; with
 // fewer, both own the same rows and take the key blocks in turn, so that one
-// stream's softmax runs beside the other's products, and join at the end. 13 warps:
+// stream's softmax runs beside the other's products, and join at the end. 14 warps:
 //   warps 0-3, 4-7  softmax of stream 0, 1: a thread has one query row. Scores
 //                   from TMEM, P = exp2(s - m) rounded to the 16-bit type back to
 //                   TMEM. The maximum is raised only when a score passes it by
@@ -14,12 +14,11 @@
 //                   of stages in the 128-byte-swizzled layout of the descriptors:
 //                   rows are scattered over the pool, so there is no tile for the
 //                   TMA engine, and a row's slice of one KV head is 256 bytes.
-//   warp 12         one thread issues the products:
-//                     S = Q K^T  both operands in shared memory, K-major
-//                     O += P V   P in TMEM, V in shared memory, MN-major (as
-//                                stored: a key's elements are adjacent)
-// Scores of the next block are issued before the output of this one, so the
-// tensor pipe and the softmax overlap. What bounds it: up to about 50 nodes the
+//   warp 12         issues S = Q K^T, both operands in shared memory, K-major
+//   warp 13         issues O += P V, P in TMEM, V in shared memory, MN-major (as
+//                   stored: a key's elements are adjacent)
+// The next block's scores do not wait for this one's output, so the tensor pipe and
+// the softmax overlap. What bounds it: up to about 50 nodes the
 // reads of K and V, beyond that the exponentials (16 a clock on an SM).
 //
 // TMEM columns of a stream: O 0..127, S 128..191, P (two buffers) 192..255.
@@ -33,27 +32,23 @@ namespace hs {
 namespace {
 
 constexpr int kSoftmaxWarps = 8, kLoadWarps = 4;
-constexpr int kLoadThreads = 32 * kLoadWarps;
-constexpr int kTensorThreads = 32 * (kSoftmaxWarps + kLoadWarps + 1);
+constexpr int kScoreWarp = kSoftmaxWarps + kLoadWarps, kOutputWarp = kScoreWarp + 1;
+constexpr int kTensorThreads = 32 * (kOutputWarp + 1);
 constexpr int kTile = 128;     // query rows of a stream
 constexpr int kKeys = 64;      // keys of a block
+constexpr int kLook = 6;       // blocks that row numbers are read ahead
 constexpr int kColumnsS = 128, kColumnsP = 192, kStreamColumns = 256;
 
 // Shared memory of a block. kDim: head_dim rounded up to 64 or 128, the rest zero.
 // Operands are panels of 64 elements (128 bytes) a row, 8 rows to the swizzle atom.
 template <int kDim> struct TensorShape {
-  static constexpr int panels = kDim / 64;
   static constexpr int q_bytes = kTile * kDim * 2;       // of one stream
   static constexpr int plane_bytes = kKeys * kDim * 2;   // K or V of a stage
   static constexpr int stages = kDim == 64 ? 8 : 5;
-  static constexpr int ahead = kDim == 64 ? 4 : 2;       // stages left in flight
   static constexpr int ring = 2 * q_bytes;
   static constexpr int bytes = ring + stages * 2 * plane_bytes;
   static constexpr size_t dynamic = bytes + 1024;        // alignment to a swizzle atom
   static constexpr int join_pitch = kDim + 1;            // floats; the streams' join
-  // The first product of a stream's next block is issued two blocks ahead of the
-  // one whose stage is waited for; stages copied but not yet announced come on top.
-  static_assert(ahead <= stages - 3, "the loader would wait for blocks it has not announced");
   static_assert(kTile * join_pitch * 4 <= stages * 2 * plane_bytes, "join fits the ring");
 };
 
@@ -70,17 +65,24 @@ __device__ __forceinline__ void tmem_load32(uint32_t (&r)[32], uint32_t addr) {
                  "=r"(r[30]), "=r"(r[31])
                : "r"(addr));
 }
-__device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t (&r)[32]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, "
-               "%8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, "
-               "%23, %24, %25, %26, %27, %28, %29, %30, %31, %32};\n"
+__device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, "
+               "%8, %9, %10, %11, %12, %13, %14, %15, %16};\n"
                ::"r"(addr),
                  "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]),
                  "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
-                 "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-                 "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
-                 "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]),
-                 "r"(r[31])
+                 "r"(r[13]), "r"(r[14]), "r"(r[15])
+               : "memory");
+}
+// 16 columns, waited for
+__device__ __forceinline__ void tmem_load16_wait(uint32_t (&r)[16], uint32_t addr) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, "
+               "%9, %10, %11, %12, %13, %14, %15}, [%16];\n"
+               "tcgen05.wait::ld.sync.aligned;\n"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]),
+                 "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+                 "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(addr)
                : "memory");
 }
 // The loads are done; the registers pass through so that no use moves ahead of it.
@@ -107,35 +109,72 @@ __device__ __forceinline__ void fence_after() {
 __device__ __forceinline__ void fence_async_proxy() {
   asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
 }
+// fp32 pairs: one instruction for two products or sums
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n .reg .b64 a, b, c, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n"
+      " mov.b64 c, {%6, %7};\n fma.rn.f32x2 d, a, b, c;\n mov.b64 {%0, %1}, d;\n}\n"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n .reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n"
+      " add.rn.f32x2 d, a, b;\n mov.b64 {%0, %1}, d;\n}\n"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// Arrives on `bar` once this thread's copies so far have landed.
+__device__ __forceinline__ void copies_arrive(uint64_t *bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];\n" ::"r"(smem_addr(bar))
+               : "memory");
+}
 // Arrives on `bar` once the products issued so far are done.
 __device__ __forceinline__ void commit(uint64_t *bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(
                    smem_addr(bar))
                : "memory");
 }
+// Shared-memory descriptor, 128-byte swizzle: the low word has the address and, for
+// MN-major operands that span several panels, the panels' distance; the high word
+// the distance of 8-row atoms, the same for all operands here. Adding bytes / 16 to
+// the low word moves the address.
+constexpr uint32_t kDescriptorHigh = (1024 >> 4) | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint32_t descriptor(uint32_t addr, uint32_t panel) {
+  return (addr >> 4) | (panel >> 4) << 16;
+}
 // D = A B (+ D), both operands in shared memory
-__device__ __forceinline__ void mma_shared(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+__device__ __forceinline__ void mma_shared(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc,
                                            bool accumulate) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+      "{\n .reg .pred p;\n .reg .b64 a, b;\n setp.ne.b32 p, %4, 0;\n"
+      " mov.b64 a, {%1, %5};\n mov.b64 b, {%2, %5};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)accumulate), "r"(kDescriptorHigh)
       : "memory");
 }
 // A in TMEM
-__device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
+__device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc,
                                          bool accumulate) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+      "{\n .reg .pred p;\n .reg .b64 b;\n setp.ne.b32 p, %4, 0;\n mov.b64 b, {%2, %5};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)accumulate), "r"(kDescriptorHigh)
       : "memory");
 }
-// Shared-memory descriptor, 128-byte swizzle: `group` is the distance of panels
-// (used by MN-major operands that span several), `atom` that of 8-row atoms.
-__device__ __forceinline__ uint64_t descriptor(uint32_t addr, uint32_t group, uint32_t atom) {
-  return (uint64_t)((addr >> 4) & 0x3fff) | (uint64_t)(group >> 4) << 16 |
-         (uint64_t)(atom >> 4) << 32 | 1ull << 46 | 2ull << 61;
+__device__ __forceinline__ bool elect_one() {
+  uint32_t chosen;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n"
+               : "=r"(chosen));
+  return chosen != 0;
 }
 // Instruction descriptor: fp32 accumulator, M = 128, n columns; b_mn: B is MN-major
 template <typename T> __device__ __forceinline__ uint32_t instruction(int n, bool b_mn) {
@@ -196,18 +235,18 @@ __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreePara
   // live rows of each stream's tile; a warp without any only takes part in barriers
   const int live0 = min(kTile, live - r0);
   const int live1 = apart ? max(0, min(kTile, live - r0 - kTile)) : live0;
-  if (warp == kSoftmaxWarps + kLoadWarps) {
+  if (warp == kScoreWarp) {
     if (lane == 0) {
       for (int i = 0; i < Shape::stages; ++i) {
-        mbar_init(&bar.kv_full[i], kLoadThreads);
+        mbar_init(&bar.kv_full[i], kLoadWarps * (32 + 1));
         mbar_init(&bar.kv_free[i], apart ? 2 : 1);
       }
       for (int w = 0; w < 2; ++w) {
-        const int threads = 32 * max(1, (int)ceil_div(w ? live1 : live0, 32));
+        const int warps = max(1, (int)ceil_div(w ? live1 : live0, 32));
         mbar_init(&bar.s_full[w], 1);
-        mbar_init(&bar.s_free[w], threads);
+        mbar_init(&bar.s_free[w], warps);
         for (int i = 0; i < 2; ++i) {
-          mbar_init(&bar.p_full[w][i], threads);
+          mbar_init(&bar.p_full[w][i], warps);
           mbar_init(&bar.pv_done[w][i], 1);
         }
       }
@@ -274,18 +313,19 @@ __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreePara
       tmem_load_wait(s[0]);
       tmem_load_wait(s[1]);
       fence_before();
-      mbar_arrive(&bar.s_free[w]);
-      float top = -INFINITY;
-      if (__all_sync(kFullMask, seen == ~0ull)) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar.s_free[w]);
+      if (!__all_sync(kFullMask, seen == ~0ull)) {
 #pragma unroll
-        for (int i = 0; i < 64; ++i) top = fmaxf(top, __uint_as_float(s[i / 32][i % 32]));
-      } else {
-#pragma unroll
-        for (int i = 0; i < 64; ++i) {
+        for (int i = 0; i < 64; ++i)
           if (!(seen >> i & 1)) s[i / 32][i % 32] = 0xff800000u;  // -inf
-          top = fmaxf(top, __uint_as_float(s[i / 32][i % 32]));
-        }
       }
+      float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int i = 0; i < 64; i += 2)
+        tops[i / 2 % 4] = max3(tops[i / 2 % 4], __uint_as_float(s[i / 32][i % 32]),
+                               __uint_as_float(s[i / 32][i % 32 + 1]));
+      float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]);
       top *= p.scale_log2;
       if (__any_sync(kFullMask, top > m + kLazy)) {
         const float to = fmaxf(m, top);
@@ -294,14 +334,13 @@ __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreePara
           ok = mbar_wait(&bar.pv_done[w][buffer ^ 1], (k - 1) >> 1 & 1, p.status);
           if (!__all_sync(kFullMask, ok)) break;
           fence_after();
+#pragma unroll 1
+          for (int c = 0; c < kDim; c += 16) {
+            uint32_t o[16];
+            tmem_load16_wait(o, lanes + c);
 #pragma unroll
-          for (int c = 0; c < kDim; c += 32) {
-            uint32_t o[32];
-            tmem_load32(o, lanes + c);
-            tmem_load_wait(o);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-            tmem_store32(lanes + c, o);
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+            tmem_store16(lanes + c, o);
           }
           tmem_store_wait();
         }
@@ -310,24 +349,34 @@ __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreePara
       }
       // a row that has seen nothing keeps m = -inf: its weights are exp2(-inf) = 0
       const float base = m == -INFINITY ? 0.f : kLift<T> - m;
-      uint32_t packed[32];
-#pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        const float a = tree_exp2(fmaf(__uint_as_float(s[i / 16][2 * i % 32]), p.scale_log2, base));
-        const float c =
-            tree_exp2(fmaf(__uint_as_float(s[i / 16][2 * i % 32 + 1]), p.scale_log2, base));
-        l += a + c;
-        packed[i] = pack2<T>(a, c);
-      }
-      if (k >= 2) {  // the products that read this buffer last
+      if (k >= 2) {  // the products that read this P buffer last
         ok = mbar_wait(&bar.pv_done[w][buffer], (k - 2) >> 1 & 1, p.status);
         if (!__all_sync(kFullMask, ok)) break;
         fence_after();
       }
-      tmem_store32(lanes + kColumnsP + buffer * 32, packed);
+      const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
+      const float2 base2 = make_float2(base, base);
+      float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t packed[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float2 e = fma2(
+              make_float2(__uint_as_float(s[h][2 * i]), __uint_as_float(s[h][2 * i + 1])),
+              scale2, base2);
+          const float2 w2 = make_float2(tree_exp2(e.x), tree_exp2(e.y));
+          sums[i % 2] = add2(sums[i % 2], w2);
+          packed[i] = pack2<T>(w2.x, w2.y);
+        }
+        tmem_store16(lanes + kColumnsP + buffer * 32 + h * 16, packed);
+      }
+      sums[0] = add2(sums[0], sums[1]);
+      l += sums[0].x + sums[0].y;
       tmem_store_wait();
       fence_before();
-      mbar_arrive(&bar.p_full[w][buffer]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar.p_full[w][buffer]);
     }
     // ---- the result ---------------------------------------------------------------------
     if (ok && mine > 0)
@@ -435,13 +484,18 @@ __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreePara
     const T *value = static_cast<const T *>(p.value) + node_base;
     const int64_t *rows = p.rows + b * p.rows_batch_stride;
     constexpr int mine = kKeys / kLoadWarps;  // keys of a block that this warp copies
-    // lane i < mine reads the row number of the warp's i-th key, a block ahead
+    // lane i < mine reads the row number of the warp's i-th key, kLook blocks ahead:
+    // a block's time is shorter than the read's
     auto look = [&](int block) -> int64_t {
       const int64_t at = begin + (int64_t)block * kKeys + lw * mine + lane;
       return lane < mine && at < end && at < valid ? __ldg(rows + at) : -1;
     };
-    int64_t next = look(0);
-    int announced = 0;
+    int64_t next[kLook];
+#pragma unroll
+    for (int i = 0; i < kLook; ++i) next[i] = look(i);
+    // Where this lane's first chunk goes; i keys further it is i rows down, and the
+    // row's part of the swizzle differs by i (the lane's own part is below `together`).
+    const uint32_t to0 = place(lw * mine + lane / chunks, c, kKeys);
     bool ok = true;
     for (int block = 0; block < blocks; ++block) {
       const int slot = block % Shape::stages;
@@ -449,92 +503,117 @@ __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreePara
         ok = mbar_wait(&bar.kv_free[slot], (block / Shape::stages - 1) & 1, p.status);
         if (!__all_sync(kFullMask, ok)) break;
       }
-      const int64_t offset = row_offset(p, next, row_elems);
-      next = look(block + 1);
+      const int64_t offset = row_offset(p, next[0], row_elems);
+#pragma unroll
+      for (int i = 0; i + 1 < kLook; ++i) next[i] = next[i + 1];
+      next[kLook - 1] = look(block + kLook);
       const unsigned cached = __ballot_sync(kFullMask, offset >= 0);
       if (lane == 0) s_cached[slot][lw] = (uint16_t)cached;
       unsigned char *stage = ring + slot * 2 * Shape::plane_bytes;
+      const uint32_t stage_addr = smem_addr(stage);
       const int64_t at0 = begin + (int64_t)block * kKeys + lw * mine;
+      int64_t off[mine / together];
 #pragma unroll
-      for (int i = 0; i < mine; i += together) {
-        const int mk = i + lane / chunks, k = lw * mine + mk;
-        const int64_t off = __shfl_sync(kFullMask, offset, mk);
-        const uint32_t to = place(k, c, kKeys);
-        if (at0 + mk >= valid && at0 + mk < end) {  // a node
-          const int64_t j = at0 + mk - valid;
-          uint4 kx = make_uint4(0, 0, 0, 0), vx = kx;
-          if (in_dim) {
-            kx = *reinterpret_cast<const uint4 *>(key + j * p.kv_node_stride);
-            vx = *reinterpret_cast<const uint4 *>(value + j * p.kv_node_stride);
+      for (int i = 0; i < mine; i += together)
+        off[i / together] = __shfl_sync(kFullMask, offset, i + lane / chunks);
+      if (at0 + mine <= valid) {
+#pragma unroll
+        for (int i = 0; i < mine; i += together) {
+          const uint32_t to = stage_addr + (to0 ^ ((i & 7) << 4)) + i * 128;
+          const bool in = off[i / together] >= 0;
+          const T *src = in ? pool + off[i / together] : pool;
+          tree_cp_async16(to, src, in && in_dim);
+          tree_cp_async16(to + Shape::plane_bytes, in ? src + plane : src, in && in_dim);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < mine / together; ++i) {
+          const int mk = i * together + lane / chunks;
+          const uint32_t to = place(lw * mine + mk, c, kKeys);
+          if (at0 + mk >= valid && at0 + mk < end) {  // a node
+            const int64_t j = at0 + mk - valid;
+            uint4 kx = make_uint4(0, 0, 0, 0), vx = kx;
+            if (in_dim) {
+              kx = *reinterpret_cast<const uint4 *>(key + j * p.kv_node_stride);
+              vx = *reinterpret_cast<const uint4 *>(value + j * p.kv_node_stride);
+            }
+            if (clear_nonfinite<T>(vx)) atomicOr(&s_bad, 1ull << j);
+            *reinterpret_cast<uint4 *>(stage + to) = kx;
+            *reinterpret_cast<uint4 *>(stage + Shape::plane_bytes + to) = vx;
+          } else {
+            const int64_t from = off[i];
+            const bool in = from >= 0;
+            const T *src = in ? pool + from : pool;
+            tree_cp_async16(stage_addr + to, src, in && in_dim);
+            tree_cp_async16(stage_addr + to + Shape::plane_bytes, in ? src + plane : src,
+                            in && in_dim);
           }
-          if (clear_nonfinite<T>(vx)) atomicOr(&s_bad, 1ull << j);
-          *reinterpret_cast<uint4 *>(stage + to) = kx;
-          *reinterpret_cast<uint4 *>(stage + Shape::plane_bytes + to) = vx;
-        } else {
-          const bool in = off >= 0;
-          const T *src = in ? pool + off : pool;
-          tree_cp_async16(smem_addr(stage + to), src, in && in_dim);
-          tree_cp_async16(smem_addr(stage + Shape::plane_bytes + to), in ? src + plane : src,
-                          in && in_dim);
         }
       }
-      asm volatile("cp.async.commit_group;\n" ::: "memory");
-      if (block >= Shape::ahead) {
-        asm volatile("cp.async.wait_group %0;\n" ::"n"(Shape::ahead) : "memory");
-        fence_async_proxy();
-        mbar_arrive(&bar.kv_full[announced % Shape::stages]);
-        ++announced;
-      }
+      // Every lane's copies announce themselves when they land; lane 0's arrival
+      // carries what was written with plain stores.
+      if (at0 + mine > valid) fence_async_proxy();
+      __syncwarp();
+      copies_arrive(&bar.kv_full[slot]);
+      if (lane == 0) mbar_arrive(&bar.kv_full[slot]);
     }
-    asm volatile("cp.async.wait_group 0;\n" ::: "memory");
-    fence_async_proxy();
-    if (ok)
-      for (; announced < blocks; ++announced) mbar_arrive(&bar.kv_full[announced % Shape::stages]);
-  } else if (lane == 0) {
-    // ---- the products ---------------------------------------------------------------
-    const uint32_t i_scores = instruction<T>(kKeys, false), i_output = instruction<T>(kDim, true);
-    const uint32_t q_base = smem_addr(smem), kv_base = smem_addr(ring);
-    auto scores = [&](int n) -> bool {
-      const int w = n & 1, k = n >> 1, block = apart ? k : n, slot = block % Shape::stages;
-      if (!mbar_wait(&bar.kv_full[slot], block / Shape::stages & 1, p.status)) return false;
-      if (k > 0 && !mbar_wait(&bar.s_free[w], (k - 1) & 1, p.status)) return false;
+    asm volatile("cp.async.wait_all;\n" ::: "memory");
+  } else {
+    // ---- the products: one warp issues the scores, one the outputs ------------------
+    // The whole warp walks the items, so that addresses stay in uniform registers;
+    // one lane issues.
+    const bool outputs = warp == kOutputWarp;
+    const uint32_t idesc = instruction<T>(outputs ? kDim : kKeys, outputs);
+    const uint32_t q0 = descriptor(smem_addr(smem), 16);
+    const uint32_t k0 = descriptor(smem_addr(ring), 16);
+    const uint32_t v0 = descriptor(smem_addr(ring) + Shape::plane_bytes, kKeys * 128);
+    int slot = 0, turn = 0;  // block % stages, block / stages & 1
+    for (int n = 0; n < items; ++n) {
+      const int w = n & 1, k = n >> 1;
+      bool ready = mbar_wait(&bar.kv_full[slot], turn, p.status);
+      if (!outputs) {
+        if (k > 0) ready = ready && mbar_wait(&bar.s_free[w], (k - 1) & 1, p.status);
+      } else {
+        ready = ready && mbar_wait(&bar.p_full[w][k & 1], k >> 1 & 1, p.status);
+      }
+      if (!__all_sync(kFullMask, ready)) break;
       fence_after();
-      const uint32_t q = q_base + (apart ? w * Shape::q_bytes : 0);
-      const uint32_t kp = kv_base + slot * 2 * Shape::plane_bytes;
+      fence_async_proxy();  // the copies are visible to this thread; now to its products
+      const uint32_t d = tmem + w * kStreamColumns;
+      if (!outputs) {
+        const uint32_t q = q0 + (apart ? w * (Shape::q_bytes >> 4) : 0);
+        const uint32_t kd = k0 + slot * (2 * Shape::plane_bytes >> 4);
+        if (elect_one()) {
 #pragma unroll
-      for (int kk = 0; kk < kDim / 16; ++kk)
-        mma_shared(tmem + w * kStreamColumns + kColumnsS,
-                   descriptor(q + kk / 4 * kTile * 128 + kk % 4 * 32, 16, 1024),
-                   descriptor(kp + kk / 4 * kKeys * 128 + kk % 4 * 32, 16, 1024), i_scores,
-                   kk > 0);
-      commit(&bar.s_full[w]);
-      return true;
-    };
-    auto output = [&](int n) -> bool {
-      const int w = n & 1, k = n >> 1, block = apart ? k : n, slot = block % Shape::stages;
-      if (!mbar_wait(&bar.p_full[w][k & 1], k >> 1 & 1, p.status)) return false;
-      fence_after();
-      const uint32_t vp = kv_base + slot * 2 * Shape::plane_bytes + Shape::plane_bytes;
+          for (int kk = 0; kk < kDim / 16; ++kk)
+            mma_shared(d + kColumnsS, q + ((kk / 4 * kTile * 128 + kk % 4 * 32) >> 4),
+                       kd + ((kk / 4 * kKeys * 128 + kk % 4 * 32) >> 4), idesc, kk > 0);
+          commit(&bar.s_full[w]);
+        }
+      } else {
+        const uint32_t vd = v0 + slot * (2 * Shape::plane_bytes >> 4);
+        const uint32_t a = d + kColumnsP + (k & 1) * 32;
+        if (elect_one()) {
 #pragma unroll
-      for (int kk = 0; kk < kKeys / 16; ++kk)
-        mma_tmem(tmem + w * kStreamColumns,
-                 tmem + w * kStreamColumns + kColumnsP + (k & 1) * 32 + kk * 8,
-                 descriptor(vp + kk * 2048, kKeys * 128, 1024), i_output, k > 0 || kk > 0);
-      commit(&bar.pv_done[w][k & 1]);
-      commit(&bar.kv_free[slot]);
-      return true;
-    };
-    bool ok = true;
-    for (int n = 0; ok && n < 2 && n < items; ++n) ok = scores(n);
-    for (int n = 0; ok && n < items; ++n) {
-      if (n + 2 < items) ok = scores(n + 2);
-      if (ok) ok = output(n);
+          for (int kk = 0; kk < kKeys / 16; ++kk)
+            mma_tmem(d, a + kk * 8, vd + (kk * 2048 >> 4), idesc, k > 0 || kk > 0);
+          commit(&bar.pv_done[w][k & 1]);
+          commit(&bar.kv_free[slot]);
+        }
+      }
+      __syncwarp();
+      if (!apart || w == 1) {
+        if (++slot == Shape::stages) {
+          slot = 0;
+          turn ^= 1;
+        }
+      }
     }
   }
   __syncwarp();
   fence_before();
   __syncthreads();
-  if (warp == kSoftmaxWarps + kLoadWarps) {
+  if (warp == kScoreWarp) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem),
                  "r"(2 * kStreamColumns));
