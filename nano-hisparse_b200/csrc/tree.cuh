@@ -71,6 +71,12 @@ __device__ __forceinline__ int64_t partial_number(const TreeParams &p, int b, in
   return (((int64_t)b * p.kv_heads + kh) * (p.nodes * p.groups) + r) * p.splits + split;
 }
 
+// Where query row r of KV head kh starts in the output.
+__device__ __forceinline__ int64_t out_offset(const TreeParams &p, int b, int kh, int r) {
+  const int t = r / p.groups;
+  return (((int64_t)b * p.nodes + t) * p.q_heads + kh * p.groups + r - t * p.groups) * p.head_dim;
+}
+
 __device__ __forceinline__ float tree_exp2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));

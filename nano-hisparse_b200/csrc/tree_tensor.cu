@@ -4,24 +4,25 @@
 // the M = 128 tile of tcgen05.mma, its rows the TMEM lanes). With more than 128
 // rows stream w owns rows 128 w .. and both work on every block of 64 keys; with
 // fewer, both own the same rows and take the key blocks in turn, so that one
-// stream's softmax runs beside the other's products, and join at the end. 14 warps:
+// stream's softmax runs beside the other's products, and join at the end. 18 warps:
 //   warps 0-3, 4-7  softmax of stream 0, 1: a thread has one query row. Scores
 //                   from TMEM, P = exp2(s - m) rounded to the 16-bit type back to
 //                   TMEM. The maximum is raised only when a score passes it by
 //                   more than 8 (a factor of 256, inside fp16's range), so the
 //                   output, which stays in TMEM, is rescaled rarely.
-//   warps 8-11      copy key blocks, 16 bytes a thread with cp.async, into a ring
+//   warps 8-15      copy key blocks, 16 bytes a thread with cp.async, into a ring
 //                   of stages in the 128-byte-swizzled layout of the descriptors:
 //                   rows are scattered over the pool, so there is no tile for the
 //                   TMA engine, and a row's slice of one KV head is 256 bytes.
-//   warp 12         issues S = Q K^T, both operands in shared memory, K-major
-//   warp 13         issues O += P V, P in TMEM, V in shared memory, MN-major (as
+//   warp 16         issues S = Q K^T, both operands in shared memory, K-major
+//   warp 17         issues O += P V, P in TMEM, V in shared memory, MN-major (as
 //                   stored: a key's elements are adjacent)
 // The next block's scores do not wait for this one's output, so the tensor pipe and
 // the softmax overlap. What bounds it: up to about 50 nodes the
 // reads of K and V, beyond that the exponentials (16 a clock on an SM).
 //
-// TMEM columns of a stream: O 0..127, S 128..191, P (two buffers) 192..255.
+// TMEM columns of a stream: O 0..127, two buffers of S from 128 on; P takes the
+// second half of its S.
 // Every wait is bounded; one that runs out sets HS_DEV_WAIT_TIMEOUT, ends its
 // warp's loop, and so lets every other wait run out.
 #include <type_traits>
@@ -31,13 +32,13 @@
 namespace hs {
 namespace {
 
-constexpr int kSoftmaxWarps = 8, kLoadWarps = 4;
+constexpr int kSoftmaxWarps = 8, kLoadWarps = 8;
 constexpr int kScoreWarp = kSoftmaxWarps + kLoadWarps, kOutputWarp = kScoreWarp + 1;
 constexpr int kTensorThreads = 32 * (kOutputWarp + 1);
 constexpr int kTile = 128;     // query rows of a stream
 constexpr int kKeys = 64;      // keys of a block
 constexpr int kLook = 6;       // blocks that row numbers are read ahead
-constexpr int kColumnsS = 128, kColumnsP = 192, kStreamColumns = 256;
+constexpr int kColumnsS = 128, kStreamColumns = 256;
 
 // Shared memory of a block. kDim: head_dim rounded up to 64 or 128, the rest zero.
 // Operands are panels of 64 elements (128 bytes) a row, 8 rows to the swizzle atom.
@@ -48,8 +49,9 @@ template <int kDim> struct TensorShape {
   static constexpr int ring = 2 * q_bytes;
   static constexpr int bytes = ring + stages * 2 * plane_bytes;
   static constexpr size_t dynamic = bytes + 1024;        // alignment to a swizzle atom
-  static constexpr int join_pitch = kDim + 1;            // floats; the streams' join
-  static_assert(kTile * join_pitch * 4 <= stages * 2 * plane_bytes, "join fits the ring");
+  static constexpr int join_pitch = kDim + 4;            // floats of a result's row in the ring
+  static_assert(kKeys / kLoadWarps == 8, "a byte of s_cached for each loading warp");
+  static_assert(2 * kTile * join_pitch * 4 <= stages * 2 * plane_bytes, "results fit the ring");
 };
 
 // 32 columns of this thread's TMEM lane
@@ -131,6 +133,20 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
+// Scores of keys that are not seen become -inf.
+__device__ __forceinline__ void hide(uint32_t (&s)[32], uint32_t seen) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i)
+    if (!(seen >> i & 1)) s[i] = 0xff800000u;
+}
+__device__ __forceinline__ float largest(uint32_t (&s)[32], bool plain, uint32_t seen) {
+  if (!plain) hide(s, seen);
+  float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int i = 0; i < 32; i += 2)
+    tops[i / 2 % 4] = max3(tops[i / 2 % 4], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+  return fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]);
+}
 
 // Arrives on `bar` once this thread's copies so far have landed.
 __device__ __forceinline__ void copies_arrive(uint64_t *bar) {
@@ -189,8 +205,7 @@ __device__ __forceinline__ uint32_t place(int r, int c, int rows) {
 
 struct TensorBarriers {
   uint64_t kv_full[8], kv_free[8];
-  uint64_t s_full[2], s_free[2];        // by stream
-  uint64_t p_full[2][2], pv_done[2][2];  // by stream and P buffer
+  uint64_t s_full[2][2], p_full[2][2], pv_done[2][2];  // by stream and buffer
 };
 
 template <typename T, int kDim>
@@ -198,7 +213,7 @@ __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreePara
   using Shape = TensorShape<kDim>;
   extern __shared__ unsigned char tensor_smem[];
   __shared__ TensorBarriers bar;
-  __shared__ uint16_t s_cached[8][kLoadWarps];  // by stage: its keys that are cache rows
+  __shared__ __align__(8) uint8_t s_cached[8][kLoadWarps];  // by stage: its keys that are cache rows
   __shared__ uint32_t s_tmem;
   __shared__ unsigned long long s_bad;  // nodes whose V held a non-finite element
   __shared__ float2 s_stats[kTile];
@@ -206,28 +221,27 @@ __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreePara
       (reinterpret_cast<uintptr_t>(tensor_smem) + 1023) & ~(uintptr_t)1023);
   unsigned char *ring = smem + Shape::ring;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, split = blockIdx.x;
-  const int D = p.head_dim, G = p.groups, all = p.nodes * G;
-  const int tiles = (int)ceil_div(all, p.tile_rows);
-  const int kh = blockIdx.y / tiles, r0 = blockIdx.y % tiles * p.tile_rows, b = blockIdx.z;
-  const int n_nodes = nodes_of(p, b), live = n_nodes * G;
+  const int D = p.head_dim, G = p.groups, all = p.nodes * G, b = blockIdx.z;
+  const int n_nodes = nodes_of(p, b), valid = (int)rows_of(p, b), live = n_nodes * G;
+  const int tiles = (all + p.tile_rows - 1) / p.tile_rows;
+  const int kh = blockIdx.y / tiles, r0 = blockIdx.y % tiles * p.tile_rows;
   const bool apart = p.tile_rows > kTile;  // the streams own different rows
-  const int64_t valid = rows_of(p, b);
-  const int64_t total = r0 < live ? valid + n_nodes : 0;
-  const int64_t chunk = ceil_div(ceil_div(total, p.splits), kKeys) * kKeys;
-  const int64_t begin = min(total, split * chunk), end = min(total, begin + chunk);
-  const int blocks = (int)ceil_div(end - begin, kKeys);
-  const int items = apart ? 2 * blocks : blocks;
-  T *out = static_cast<T *>(p.out) + (int64_t)b * p.nodes * p.q_heads * D;
-  auto out_row = [&](int row) {
-    return out + (int64_t)(row / G) * p.q_heads * D + (int64_t)(kh * G + row % G) * D;
-  };
+  // the keys of this split: begin .. end - 1
+  const unsigned total = r0 < live ? (unsigned)(valid + n_nodes) : 0;
+  const unsigned share = ((total + p.splits - 1) / p.splits + kKeys - 1) / kKeys * kKeys;
+  const int begin = (int)min((unsigned long long)total, (unsigned long long)split * share);
+  const int end = (int)min(total, begin + share);
+  const int blocks = (end - begin + kKeys - 1) / kKeys, items = apart ? 2 * blocks : blocks;
 
   if (blocks == 0) {  // nothing is seen here: zeros, or a split without weight
     for (int i = warp; i < p.tile_rows && r0 + i < all; i += kTensorThreads / 32) {
-      if (p.splits == 1)
-        for (int d = lane; d < D; d += 32) out_row(r0 + i)[d] = from_f32<T>(0.f);
-      else if (lane == 0)
-        p.stats[partial_number(p, b, kh, r0 + i, split)] = make_float2(-INFINITY, 0.f);
+      if (p.splits > 1) {
+        if (lane == 0)
+          p.stats[partial_number(p, b, kh, r0 + i, split)] = make_float2(-INFINITY, 0.f);
+      } else {
+        T *out = static_cast<T *>(p.out) + out_offset(p, b, kh, r0 + i);
+        for (int d = lane; d < D; d += 32) out[d] = from_f32<T>(0.f);
+      }
     }
     return;
   }
@@ -235,243 +249,23 @@ __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreePara
   // live rows of each stream's tile; a warp without any only takes part in barriers
   const int live0 = min(kTile, live - r0);
   const int live1 = apart ? max(0, min(kTile, live - r0 - kTile)) : live0;
-  if (warp == kScoreWarp) {
-    if (lane == 0) {
-      for (int i = 0; i < Shape::stages; ++i) {
-        mbar_init(&bar.kv_full[i], kLoadWarps * (32 + 1));
-        mbar_init(&bar.kv_free[i], apart ? 2 : 1);
-      }
-      for (int w = 0; w < 2; ++w) {
-        const int warps = max(1, (int)ceil_div(w ? live1 : live0, 32));
-        mbar_init(&bar.s_full[w], 1);
-        mbar_init(&bar.s_free[w], warps);
-        for (int i = 0; i < 2; ++i) {
-          mbar_init(&bar.p_full[w][i], warps);
-          mbar_init(&bar.pv_done[w][i], 1);
-        }
-      }
-      s_bad = 0;
-      asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  if (tid == 32 * kScoreWarp) {
+    for (int i = 0; i < Shape::stages; ++i) {
+      mbar_init(&bar.kv_full[i], kLoadWarps * (32 + 1));
+      mbar_init(&bar.kv_free[i], apart ? 2 : 1);
     }
-    __syncwarp();
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(
-                     smem_addr(&s_tmem)),
-                 "r"(2 * kStreamColumns)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n");
-  } else if (warp < kSoftmaxWarps) {
-    // Q into both streams' tiles (one tile when they share it), dead rows zero
-    const T *query = static_cast<const T *>(p.query) + b * p.q_batch_stride;
-    constexpr int chunks = kDim / 8;
-    for (int i = tid; i < p.tile_rows * chunks; i += 32 * kSoftmaxWarps) {
-      const int r = i / chunks, c = i % chunks, row = r0 + r;
-      uint4 x = make_uint4(0, 0, 0, 0);
-      if (row < live && c * 8 < D)
-        x = *reinterpret_cast<const uint4 *>(query + row / G * p.q_node_stride +
-                                             (int64_t)(kh * G + row % G) * D + c * 8);
-      *reinterpret_cast<uint4 *>(smem + r / kTile * Shape::q_bytes + place(r % kTile, c, kTile)) =
-          x;
-    }
-    fence_async_proxy();
+    for (int w = 0; w < 2; ++w)
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&bar.s_full[w][i], 1);
+        mbar_init(&bar.p_full[w][i], max(1, ((w ? live1 : live0) + 31) / 32));
+        mbar_init(&bar.pv_done[w][i], 1);
+      }
+    s_bad = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
-  fence_before();
   __syncthreads();
-  fence_after();
-  const uint32_t tmem = s_tmem;
 
-  if (warp < kSoftmaxWarps) {
-    // ---- softmax of stream w --------------------------------------------------------
-    const int w = warp / 4, quarter = warp % 4;
-    const int mine = apart ? blocks : (blocks + 1 - w) / 2;
-    const int live_here = w ? live1 : live0;
-    const int r = quarter * 32 + lane;           // row of the tile
-    const int row = r0 + (apart ? w * kTile : 0) + r;
-    const uint32_t lanes = tmem + w * kStreamColumns + ((uint32_t)(quarter * 32) << 16);
-    const bool here = quarter < max(1, (int)ceil_div(live_here, 32));
-    const uint64_t see =
-        r < live_here ? (uint64_t)p.mask[(int64_t)b * p.nodes + row / G] : 0;
-    float m = -INFINITY, l = 0.f;
-    bool ok = true;
-    for (int k = 0; here && ok && k < mine; ++k) {
-      const int block = apart ? k : 2 * k + w, slot = block % Shape::stages, buffer = k & 1;
-      ok = mbar_wait(&bar.kv_full[slot], block / Shape::stages & 1, p.status) &&
-           mbar_wait(&bar.s_full[w], k & 1, p.status);
-      if (!__all_sync(kFullMask, ok)) break;
-      // keys this row sees: cache rows, then nodes from position n0 on
-      uint64_t seen = *reinterpret_cast<const uint64_t *>(s_cached[slot]);
-      const int64_t k0 = begin + (int64_t)block * kKeys;
-      if (k0 + kKeys > valid) {
-        const int n0 = (int)(valid > k0 ? valid - k0 : 0), j0 = (int)(k0 + n0 - valid);
-        const int n = (int)(min(end, k0 + kKeys) - (k0 + n0));  // nodes in the block
-        const uint64_t nodes = n >= 64 ? ~0ull : (1ull << n) - 1;
-        seen |= (see >> j0 & nodes) << n0;
-      }
-      uint32_t s[2][32];
-      fence_after();
-      tmem_load32(s[0], lanes + kColumnsS);
-      tmem_load32(s[1], lanes + kColumnsS + 32);
-      tmem_load_wait(s[0]);
-      tmem_load_wait(s[1]);
-      fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bar.s_free[w]);
-      if (!__all_sync(kFullMask, seen == ~0ull)) {
-#pragma unroll
-        for (int i = 0; i < 64; ++i)
-          if (!(seen >> i & 1)) s[i / 32][i % 32] = 0xff800000u;  // -inf
-      }
-      float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (int i = 0; i < 64; i += 2)
-        tops[i / 2 % 4] = max3(tops[i / 2 % 4], __uint_as_float(s[i / 32][i % 32]),
-                               __uint_as_float(s[i / 32][i % 32 + 1]));
-      float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]);
-      top *= p.scale_log2;
-      if (__any_sync(kFullMask, top > m + kLazy)) {
-        const float to = fmaxf(m, top);
-        const float f = m == -INFINITY ? 0.f : tree_exp2(m - to);
-        if (k > 0) {  // the output so far
-          ok = mbar_wait(&bar.pv_done[w][buffer ^ 1], (k - 1) >> 1 & 1, p.status);
-          if (!__all_sync(kFullMask, ok)) break;
-          fence_after();
-#pragma unroll 1
-          for (int c = 0; c < kDim; c += 16) {
-            uint32_t o[16];
-            tmem_load16_wait(o, lanes + c);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-            tmem_store16(lanes + c, o);
-          }
-          tmem_store_wait();
-        }
-        l *= f;
-        m = to;
-      }
-      // a row that has seen nothing keeps m = -inf: its weights are exp2(-inf) = 0
-      const float base = m == -INFINITY ? 0.f : kLift<T> - m;
-      if (k >= 2) {  // the products that read this P buffer last
-        ok = mbar_wait(&bar.pv_done[w][buffer], (k - 2) >> 1 & 1, p.status);
-        if (!__all_sync(kFullMask, ok)) break;
-        fence_after();
-      }
-      const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
-      const float2 base2 = make_float2(base, base);
-      float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t packed[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float2 e = fma2(
-              make_float2(__uint_as_float(s[h][2 * i]), __uint_as_float(s[h][2 * i + 1])),
-              scale2, base2);
-          const float2 w2 = make_float2(tree_exp2(e.x), tree_exp2(e.y));
-          sums[i % 2] = add2(sums[i % 2], w2);
-          packed[i] = pack2<T>(w2.x, w2.y);
-        }
-        tmem_store16(lanes + kColumnsP + buffer * 32 + h * 16, packed);
-      }
-      sums[0] = add2(sums[0], sums[1]);
-      l += sums[0].x + sums[0].y;
-      tmem_store_wait();
-      fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bar.p_full[w][buffer]);
-    }
-    // ---- the result ---------------------------------------------------------------------
-    if (ok && mine > 0)
-      ok = mbar_wait(&bar.pv_done[w][(mine - 1) & 1], (mine - 1) >> 1 & 1, p.status);
-    __syncwarp();
-    fence_after();
-    // Streams of the same rows join through the ring's memory: its last products
-    // are done when both streams' are, which the named barrier brings together.
-    float *join = reinterpret_cast<float *>(ring);
-    asm volatile("bar.sync 1, %0;\n" ::"n"(32 * kSoftmaxWarps) : "memory");
-    if (!apart) {
-      if (w == 1 && here) {
-        s_stats[r] = make_float2(m, l);
-#pragma unroll
-        for (int c = 0; c < kDim; c += 32) {
-          uint32_t o[32];
-          tmem_load32(o, lanes + c);
-          tmem_load_wait(o);
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            join[r * Shape::join_pitch + c + i] = mine > 0 ? __uint_as_float(o[i]) : 0.f;
-        }
-      }
-      __syncwarp();
-      asm volatile("bar.sync 1, %0;\n" ::"n"(32 * kSoftmaxWarps) : "memory");
-    }
-    if (here && (apart || w == 0)) {
-      float f = 1.f, g = 0.f;
-      if (!apart) {
-        const float2 other = s_stats[r];
-        const float to = fmaxf(m, other.x);
-        f = m == -INFINITY ? 0.f : tree_exp2(m - to);
-        g = other.x == -INFINITY ? 0.f : tree_exp2(other.x - to);
-        // a sum of NaN scores has no maximum: let it through
-        l = (m == -INFINITY ? l : l * f) + (other.x == -INFINITY ? other.y : other.y * g);
-        m = to;
-      }
-      const bool in = row < all;
-      const uint64_t bad = r < live_here ? s_bad & see : 0;
-      const float inv = r < live_here && (l > 0.f || l != l) ? 1.f / l : 0.f;
-      const int64_t at = in ? partial_number(p, b, kh, row, split) : 0;
-#pragma unroll
-      for (int c = 0; c < kDim; c += 32) {
-        uint32_t o[32];
-        __syncwarp();
-        tmem_load32(o, lanes + c);
-        tmem_load_wait(o);
-        if (!in || c >= D) continue;
-        float x[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          x[i] = __uint_as_float(o[i]) * f;
-          if (!apart) x[i] = fmaf(g, join[r * Shape::join_pitch + c + i], x[i]);
-        }
-        if (r >= live_here)
-#pragma unroll
-          for (int i = 0; i < 32; ++i) x[i] = 0.f;
-        if (p.splits == 1) {
-          T *to = out_row(row) + c;
-#pragma unroll
-          for (int i = 0; i < 32; i += 8)
-            if (c + i < D) {
-              uint4 v;
-              v.x = pack2<T>(x[i] * inv, x[i + 1] * inv);
-              v.y = pack2<T>(x[i + 2] * inv, x[i + 3] * inv);
-              v.z = pack2<T>(x[i + 4] * inv, x[i + 5] * inv);
-              v.w = pack2<T>(x[i + 6] * inv, x[i + 7] * inv);
-              *reinterpret_cast<uint4 *>(to + i) = v;
-            }
-        } else {
-          float *to = p.partials + at * D + c;
-#pragma unroll
-          for (int i = 0; i < 32; i += 4)
-            if (c + i < D)
-              *reinterpret_cast<float4 *>(to + i) =
-                  make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
-        }
-      }
-      if (bad != 0)
-        for (int d = 0; d < D; ++d) {
-          const float x = nonfinite_sum<T>(p, b, kh, d, bad);
-          if (p.splits == 1) out_row(row)[d] = from_f32<T>(to_f32(out_row(row)[d]) + x);
-          else p.partials[at * D + d] += x;
-        }
-      if (in && p.splits > 1) p.stats[at] = make_float2(m, r < live_here ? l : 0.f);
-    }
-    // rows of padded nodes that no live warp covers
-    if (!here && (apart || w == 0) && row < all) {
-      if (p.splits == 1)
-        for (int d = 0; d < D; d += 8)
-          *reinterpret_cast<uint4 *>(out_row(row) + d) = make_uint4(0, 0, 0, 0);
-      else
-        p.stats[partial_number(p, b, kh, row, split)] = make_float2(-INFINITY, 0.f);
-    }
-  } else if (warp < kSoftmaxWarps + kLoadWarps) {
+  if (warp >= kSoftmaxWarps && warp < kSoftmaxWarps + kLoadWarps) {
     // ---- key blocks into the ring ---------------------------------------------------
     const int lw = warp - kSoftmaxWarps;
     constexpr int chunks = kDim / 8, together = 32 / chunks;  // keys of a warp's copy
@@ -486,32 +280,32 @@ __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreePara
     constexpr int mine = kKeys / kLoadWarps;  // keys of a block that this warp copies
     // lane i < mine reads the row number of the warp's i-th key, kLook blocks ahead:
     // a block's time is shorter than the read's
+    const int last = min(end, valid);
     auto look = [&](int block) -> int64_t {
-      const int64_t at = begin + (int64_t)block * kKeys + lw * mine + lane;
-      return lane < mine && at < end && at < valid ? __ldg(rows + at) : -1;
+      const int at = begin + block * kKeys + lw * mine + lane;
+      return lane < mine && at < last ? __ldg(rows + at) : -1;
     };
     int64_t next[kLook];
 #pragma unroll
-    for (int i = 0; i < kLook; ++i) next[i] = look(i);
+    for (int i = 0; i < kLook; ++i) next[i] = i < blocks ? look(i) : -1;
     // Where this lane's first chunk goes; i keys further it is i rows down, and the
     // row's part of the swizzle differs by i (the lane's own part is below `together`).
     const uint32_t to0 = place(lw * mine + lane / chunks, c, kKeys);
-    bool ok = true;
+    int slot = 0, turn = 1;
     for (int block = 0; block < blocks; ++block) {
-      const int slot = block % Shape::stages;
       if (block >= Shape::stages) {
-        ok = mbar_wait(&bar.kv_free[slot], (block / Shape::stages - 1) & 1, p.status);
+        const bool ok = mbar_wait(&bar.kv_free[slot], turn, p.status);
         if (!__all_sync(kFullMask, ok)) break;
       }
       const int64_t offset = row_offset(p, next[0], row_elems);
 #pragma unroll
       for (int i = 0; i + 1 < kLook; ++i) next[i] = next[i + 1];
-      next[kLook - 1] = look(block + kLook);
+      next[kLook - 1] = block + kLook < blocks ? look(block + kLook) : -1;
       const unsigned cached = __ballot_sync(kFullMask, offset >= 0);
-      if (lane == 0) s_cached[slot][lw] = (uint16_t)cached;
+      if (lane == 0) s_cached[slot][lw] = (uint8_t)cached;
       unsigned char *stage = ring + slot * 2 * Shape::plane_bytes;
       const uint32_t stage_addr = smem_addr(stage);
-      const int64_t at0 = begin + (int64_t)block * kKeys + lw * mine;
+      const int at0 = begin + block * kKeys + lw * mine;
       int64_t off[mine / together];
 #pragma unroll
       for (int i = 0; i < mine; i += together)
@@ -526,7 +320,7 @@ __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreePara
           tree_cp_async16(to + Shape::plane_bytes, in ? src + plane : src, in && in_dim);
         }
       } else {
-#pragma unroll
+#pragma unroll 1
         for (int i = 0; i < mine / together; ++i) {
           const int mk = i * together + lane / chunks;
           const uint32_t to = place(lw * mine + mk, c, kKeys);
@@ -541,7 +335,9 @@ __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreePara
             *reinterpret_cast<uint4 *>(stage + to) = kx;
             *reinterpret_cast<uint4 *>(stage + Shape::plane_bytes + to) = vx;
           } else {
-            const int64_t from = off[i];
+            int64_t from = -1;
+#pragma unroll
+            for (int e = 0; e < mine / together; ++e) from = e == i ? off[e] : from;
             const bool in = from >= 0;
             const T *src = in ? pool + from : pool;
             tree_cp_async16(stage_addr + to, src, in && in_dim);
@@ -549,74 +345,291 @@ __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreePara
                             in && in_dim);
           }
         }
+        fence_async_proxy();
       }
       // Every lane's copies announce themselves when they land; lane 0's arrival
       // carries what was written with plain stores.
-      if (at0 + mine > valid) fence_async_proxy();
       __syncwarp();
       copies_arrive(&bar.kv_full[slot]);
       if (lane == 0) mbar_arrive(&bar.kv_full[slot]);
+      if (++slot == Shape::stages) {
+        slot = 0;
+        turn ^= 1;
+      }
     }
     asm volatile("cp.async.wait_all;\n" ::: "memory");
   } else {
-    // ---- the products: one warp issues the scores, one the outputs ------------------
-    // The whole warp walks the items, so that addresses stay in uniform registers;
-    // one lane issues.
-    const bool outputs = warp == kOutputWarp;
-    const uint32_t idesc = instruction<T>(outputs ? kDim : kKeys, outputs);
-    const uint32_t q0 = descriptor(smem_addr(smem), 16);
-    const uint32_t k0 = descriptor(smem_addr(ring), 16);
-    const uint32_t v0 = descriptor(smem_addr(ring) + Shape::plane_bytes, kKeys * 128);
-    int slot = 0, turn = 0;  // block % stages, block / stages & 1
-    for (int n = 0; n < items; ++n) {
-      const int w = n & 1, k = n >> 1;
-      bool ready = mbar_wait(&bar.kv_full[slot], turn, p.status);
-      if (!outputs) {
-        if (k > 0) ready = ready && mbar_wait(&bar.s_free[w], (k - 1) & 1, p.status);
-      } else {
-        ready = ready && mbar_wait(&bar.p_full[w][k & 1], k >> 1 & 1, p.status);
+    if (warp < kSoftmaxWarps) {
+      // Q into both streams' tiles (one tile when they share it), dead rows zero
+      const T *query = static_cast<const T *>(p.query) + b * p.q_batch_stride;
+      constexpr int chunks = kDim / 8, step = 32 * kSoftmaxWarps / chunks;
+      const int c = tid % chunks;
+#pragma unroll 4
+      for (int r = tid / chunks; r < p.tile_rows; r += step) {
+        const int row = r0 + r, t = row / G;
+        const bool in = row < live && c * 8 < D;
+        tree_cp_async16(
+            smem_addr(smem + r / kTile * Shape::q_bytes + place(r % kTile, c, kTile)),
+            in ? query + t * p.q_node_stride + (int64_t)(kh * G + row - t * G) * D + c * 8 : query,
+            in);
       }
-      if (!__all_sync(kFullMask, ready)) break;
-      fence_after();
-      fence_async_proxy();  // the copies are visible to this thread; now to its products
-      const uint32_t d = tmem + w * kStreamColumns;
-      if (!outputs) {
-        const uint32_t q = q0 + (apart ? w * (Shape::q_bytes >> 4) : 0);
-        const uint32_t kd = k0 + slot * (2 * Shape::plane_bytes >> 4);
-        if (elect_one()) {
-#pragma unroll
-          for (int kk = 0; kk < kDim / 16; ++kk)
-            mma_shared(d + kColumnsS, q + ((kk / 4 * kTile * 128 + kk % 4 * 32) >> 4),
-                       kd + ((kk / 4 * kKeys * 128 + kk % 4 * 32) >> 4), idesc, kk > 0);
-          commit(&bar.s_full[w]);
+      asm volatile("cp.async.wait_all;\n" ::: "memory");
+      fence_async_proxy();
+    } else if (warp == kOutputWarp) {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(
+                       smem_addr(&s_tmem)),
+                   "r"(2 * kStreamColumns)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n");
+    }
+    fence_before();
+    __syncwarp();
+    asm volatile("bar.sync 2, %0;\n" ::"n"(32 * (kSoftmaxWarps + 2)) : "memory");
+    fence_after();
+    const uint32_t tmem = s_tmem;
+
+    if (warp < kSoftmaxWarps) {
+      // ---- softmax of stream w ------------------------------------------------------
+      const int w = warp / 4, quarter = warp % 4;
+      const int mine = apart ? blocks : (blocks + 1 - w) / 2;
+      const int live_here = w ? live1 : live0;
+      const int r = quarter * 32 + lane;  // row of the tile
+      const int row = r0 + (apart ? w * kTile : 0) + r;
+      const uint32_t lanes = tmem + w * kStreamColumns + ((uint32_t)(quarter * 32) << 16);
+      const bool here = quarter < max(1, (live_here + 31) / 32);
+      const uint64_t see = r < live_here ? (uint64_t)p.mask[(int64_t)b * p.nodes + row / G] : 0;
+      const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
+      float m = -INFINITY, l = 0.f;
+      bool ok = true;
+      int slot = apart ? 0 : w, turn = 0;
+      for (int k = 0; here && k < mine; ++k) {
+        const int block = apart ? k : 2 * k + w, buffer = k & 1;
+        const uint32_t scores = lanes + kColumnsS + buffer * kKeys, weights = scores + kKeys / 2;
+        ok = mbar_wait(&bar.s_full[w][buffer], k >> 1 & 1, p.status) &&
+             mbar_wait(&bar.kv_full[slot], turn, p.status);  // for s_cached
+        if (!__all_sync(kFullMask, ok)) break;
+        fence_after();
+        uint32_t s[32];
+        tmem_load32(s, scores);
+        // keys this row sees: cache rows, then nodes from position n0 on
+        uint64_t seen = *reinterpret_cast<const uint64_t *>(s_cached[slot]);
+        const int k0 = begin + block * kKeys;
+        if (k0 + kKeys > valid) {
+          const int n0 = max(valid - k0, 0), j0 = k0 + n0 - valid;
+          const int n = min(end, k0 + kKeys) - (k0 + n0);  // nodes in the block
+          const uint64_t nodes = n >= 64 ? ~0ull : (1ull << n) - 1;
+          seen |= (see >> j0 & nodes) << n0;
         }
-      } else {
-        const uint32_t vd = v0 + slot * (2 * Shape::plane_bytes >> 4);
-        const uint32_t a = d + kColumnsP + (k & 1) * 32;
-        if (elect_one()) {
+        const bool plain = __all_sync(kFullMask, seen == ~0ull);
+        tmem_load_wait(s);
+        float top = largest(s, plain, (uint32_t)seen);
+        tmem_load32(s, scores + 32);
+        tmem_load_wait(s);
+        top = fmaxf(top, largest(s, plain, (uint32_t)(seen >> 32))) * p.scale_log2;
+        if (__any_sync(kFullMask, top > m + kLazy)) {
+          const float to = fmaxf(m, top);
+          const float f = m == -INFINITY ? 0.f : tree_exp2(m - to);
+          if (k > 0) {  // the output so far
+            ok = mbar_wait(&bar.pv_done[w][buffer ^ 1], (k - 1) >> 1 & 1, p.status);
+            if (!__all_sync(kFullMask, ok)) break;
+            fence_after();
+#pragma unroll 1
+            for (int c = 0; c < kDim; c += 16) {
+              uint32_t o[16];
+              tmem_load16_wait(o, lanes + c);
 #pragma unroll
-          for (int kk = 0; kk < kKeys / 16; ++kk)
-            mma_tmem(d, a + kk * 8, vd + (kk * 2048 >> 4), idesc, k > 0 || kk > 0);
-          commit(&bar.pv_done[w][k & 1]);
-          commit(&bar.kv_free[slot]);
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+              tmem_store16(lanes + c, o);
+            }
+          }
+          l *= f;
+          m = to;
         }
-      }
-      __syncwarp();
-      if (!apart || w == 1) {
-        if (++slot == Shape::stages) {
-          slot = 0;
+        // a row that has seen nothing keeps m = -inf: its weights are exp2(-inf) = 0
+        const float base = m == -INFINITY ? 0.f : kLift<T> - m;
+        // P takes the columns of the second half of S, which is in registers; the
+        // first half is read again (64 scores at once cost too many registers)
+#pragma unroll
+        for (int h = 1; h >= 0; --h) {
+          if (h == 0) {
+            tmem_load32(s, scores);
+            tmem_load_wait(s);
+            if (!plain) hide(s, (uint32_t)seen);
+          }
+          float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+          uint32_t packed[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float2 e =
+                fma2(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), scale2,
+                     make_float2(base, base));
+            const float2 w2 = make_float2(tree_exp2(e.x), tree_exp2(e.y));
+            sums[i % 2] = add2(sums[i % 2], w2);
+            packed[i] = pack2<T>(w2.x, w2.y);
+          }
+          tmem_store16(weights + h * 16, packed);
+          sums[0] = add2(sums[0], sums[1]);
+          l += sums[0].x + sums[0].y;
+        }
+        tmem_store_wait();
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar.p_full[w][buffer]);
+        slot += apart ? 1 : 2;
+        if (slot >= Shape::stages) {
+          slot -= Shape::stages;
           turn ^= 1;
         }
       }
+      // ---- the result -----------------------------------------------------------------
+      if (ok && mine > 0)
+        mbar_wait(&bar.pv_done[w][(mine - 1) & 1], (mine - 1) >> 1 & 1, p.status);
+      __syncwarp();
+      fence_after();
+      // With both streams' last products done the ring's memory is free: a row of
+      // fp32 for each query row, so that rows leave in whole lines.
+      asm volatile("bar.sync 1, %0;\n" ::"n"(32 * kSoftmaxWarps) : "memory");
+      constexpr int pitch = Shape::join_pitch;
+      float *stage = reinterpret_cast<float *>(ring) + (apart ? w * kTile * pitch : 0);
+      float *own = stage + r * pitch;
+      if (!apart) {
+        if (w == 1 && here) {
+          s_stats[r] = make_float2(m, l);
+#pragma unroll 1
+          for (int c = 0; c < kDim; c += 16) {
+            uint32_t o[16];
+            tmem_load16_wait(o, lanes + c);
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+              *reinterpret_cast<uint4 *>(own + c + i) =
+                  mine > 0 ? make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]) : make_uint4(0, 0, 0, 0);
+          }
+        }
+        asm volatile("bar.sync 1, %0;\n" ::"n"(32 * kSoftmaxWarps) : "memory");
+      }
+      if (apart || w == 0) {
+        float f = 1.f, g = 0.f;
+        if (!apart && here) {
+          const float2 other = s_stats[r];
+          const float to = fmaxf(m, other.x);
+          f = m == -INFINITY ? 0.f : tree_exp2(m - to);
+          g = other.x == -INFINITY ? 0.f : tree_exp2(other.x - to);
+          // a sum of NaN scores has no maximum: let it through
+          l = (m == -INFINITY ? l : l * f) + (other.x == -INFINITY ? other.y : other.y * g);
+          m = to;
+        }
+        const bool alive = here && r < live_here;
+        if (!alive) l = 0.f;
+        // with one split the result itself, with more the unnormalised output
+        const float scale = p.splits > 1 ? 1.f : l > 0.f || l != l ? 1.f / l : 0.f;
+        f *= scale;
+        g *= scale;
+        if (here) {
+          const uint64_t bad = alive ? s_bad & see : 0;
+#pragma unroll 1
+          for (int c = 0; c < kDim; c += 16) {
+            uint32_t o[16];
+            __syncwarp();
+            tmem_load16_wait(o, lanes + c);
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+              float4 x = make_float4(__uint_as_float(o[i]) * f, __uint_as_float(o[i + 1]) * f,
+                                     __uint_as_float(o[i + 2]) * f, __uint_as_float(o[i + 3]) * f);
+              if (!apart) {
+                const float4 y = *reinterpret_cast<const float4 *>(own + c + i);
+                x.x = fmaf(g, y.x, x.x);
+                x.y = fmaf(g, y.y, x.y);
+                x.z = fmaf(g, y.z, x.z);
+                x.w = fmaf(g, y.w, x.w);
+              }
+              *reinterpret_cast<float4 *>(own + c + i) = x;
+            }
+          }
+          if (bad != 0)
+            for (int d = 0; d < D; ++d) own[d] += nonfinite_sum<T>(p, b, kh, d, bad);
+        }
+        __syncwarp();
+        // the warp's 32 rows, four elements a lane
+        const int first = row - lane, rows_here = max(0, min(32, all - first));
+        const unsigned alive_rows = __ballot_sync(kFullMask, alive);
+        const int d = 4 * lane;
+        for (int i = 0; i < rows_here; ++i) {
+          float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+          if ((alive_rows >> i & 1) && d < D)
+            x = *reinterpret_cast<const float4 *>(stage + (quarter * 32 + i) * pitch + d);
+          if (d >= D) continue;
+          if (p.splits > 1) {
+            *reinterpret_cast<float4 *>(
+                p.partials + partial_number(p, b, kh, first + i, split) * D + d) = x;
+          } else {
+            uint2 v;
+            v.x = pack2<T>(x.x, x.y);
+            v.y = pack2<T>(x.z, x.w);
+            *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + out_offset(p, b, kh, first + i) +
+                                       d) = v;
+          }
+        }
+        if (p.splits > 1 && row < all)
+          p.stats[partial_number(p, b, kh, row, split)] = make_float2(alive ? m : -INFINITY, l);
+      }
+    } else {
+      // ---- the products: one warp issues the scores, one the outputs ----------------
+      // The whole warp walks the items, so that addresses stay in uniform registers;
+      // one lane issues.
+      const bool outputs = warp == kOutputWarp;
+      const uint32_t idesc = instruction<T>(outputs ? kDim : kKeys, outputs);
+      const uint32_t q0 = descriptor(smem_addr(smem), 16);
+      const uint32_t k0 = descriptor(smem_addr(ring), 16);
+      const uint32_t v0 = descriptor(smem_addr(ring) + Shape::plane_bytes, kKeys * 128);
+      int slot = 0, turn = 0;
+      for (int n = 0; n < items; ++n) {
+        const int w = n & 1, k = n >> 1, buffer = k & 1;
+        bool ready = mbar_wait(&bar.kv_full[slot], turn, p.status);
+        if (outputs)
+          ready = ready && mbar_wait(&bar.p_full[w][buffer], k >> 1 & 1, p.status);
+        else if (k >= 2)  // the products that read this buffer's P
+          ready = ready && mbar_wait(&bar.pv_done[w][buffer], (k - 2) >> 1 & 1, p.status);
+        if (!__all_sync(kFullMask, ready)) break;
+        fence_after();
+        fence_async_proxy();  // the copies are visible to this thread; now to its products
+        const uint32_t d = tmem + w * kStreamColumns, s = d + kColumnsS + buffer * kKeys;
+        if (!outputs) {
+          const uint32_t q = q0 + (apart ? w * (Shape::q_bytes >> 4) : 0);
+          const uint32_t kd = k0 + slot * (2 * Shape::plane_bytes >> 4);
+          if (elect_one()) {
+#pragma unroll
+            for (int kk = 0; kk < kDim / 16; ++kk)
+              mma_shared(s, q + ((kk / 4 * kTile * 128 + kk % 4 * 32) >> 4),
+                         kd + ((kk / 4 * kKeys * 128 + kk % 4 * 32) >> 4), idesc, kk > 0);
+            commit(&bar.s_full[w][buffer]);
+          }
+        } else {
+          const uint32_t vd = v0 + slot * (2 * Shape::plane_bytes >> 4);
+          if (elect_one()) {
+#pragma unroll
+            for (int kk = 0; kk < kKeys / 16; ++kk)
+              mma_tmem(d, s + kKeys / 2 + kk * 8, vd + (kk * 2048 >> 4), idesc, k > 0 || kk > 0);
+            commit(&bar.pv_done[w][buffer]);
+            commit(&bar.kv_free[slot]);
+          }
+        }
+        __syncwarp();
+        if (!apart || w == 1) {
+          if (++slot == Shape::stages) {
+            slot = 0;
+            turn ^= 1;
+          }
+        }
+      }
     }
-  }
-  __syncwarp();
-  fence_before();
-  __syncthreads();
-  if (warp == kScoreWarp) {
-    fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem),
-                 "r"(2 * kStreamColumns));
+    __syncwarp();
+    fence_before();
+    asm volatile("bar.sync 2, %0;\n" ::"n"(32 * (kSoftmaxWarps + 2)) : "memory");
+    if (warp == kOutputWarp) {
+      fence_after();
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem),
+                   "r"(2 * kStreamColumns));
+    }
   }
 }
 
