@@ -38,6 +38,7 @@ constexpr int kTensorThreads = 32 * (kOutputWarp + 1);
 constexpr int kTile = 128;     // query rows of a stream
 constexpr int kKeys = 64;      // keys of a block
 constexpr int kLook = 6;       // blocks that row numbers are read ahead
+constexpr unsigned long long kWaitNanoseconds = 4000000000ull;  // then a wait gives up
 constexpr int kColumnsS = 128, kStreamColumns = 256;
 
 // Shared memory of a block. kDim: head_dim rounded up to 64 or 128, the rest zero.
@@ -148,6 +149,29 @@ __device__ __forceinline__ float largest(uint32_t (&s)[32], bool plain, uint32_t
   return fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]);
 }
 
+// As mbar_wait, without the hint to sleep: waits here are a few hundred clocks, and
+// waking from a hinted sleep was measured to take more than a thousand.
+__device__ __forceinline__ bool wait_phase(uint64_t *bar, unsigned parity, int32_t *status) {
+  unsigned long long first = 0;
+  for (unsigned i = 0;; ++i) {
+    unsigned done;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+        " selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(done)
+        : "r"(smem_addr(bar)), "r"(parity)
+        : "memory");
+    if (done) return true;
+    if ((i & 1023) == 1023) {
+      unsigned long long now;
+      asm volatile("mov.u64 %0, %%globaltimer;\n" : "=l"(now));
+      if (first == 0) first = now;
+      if (now - first > kWaitNanoseconds) break;
+    }
+  }
+  flag(status, HS_DEV_WAIT_TIMEOUT);
+  return false;
+}
 // Arrives on `bar` once this thread's copies so far have landed.
 __device__ __forceinline__ void copies_arrive(uint64_t *bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];\n" ::"r"(smem_addr(bar))
@@ -294,7 +318,7 @@ __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreePara
     int slot = 0, turn = 1;
     for (int block = 0; block < blocks; ++block) {
       if (block >= Shape::stages) {
-        const bool ok = mbar_wait(&bar.kv_free[slot], turn, p.status);
+        const bool ok = wait_phase(&bar.kv_free[slot], turn, p.status);
         if (!__all_sync(kFullMask, ok)) break;
       }
       const int64_t offset = row_offset(p, next[0], row_elems);
@@ -320,26 +344,30 @@ __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreePara
           tree_cp_async16(to + Shape::plane_bytes, in ? src + plane : src, in && in_dim);
         }
       } else {
-#pragma unroll 1
-        for (int i = 0; i < mine / together; ++i) {
-          const int mk = i * together + lane / chunks;
-          const uint32_t to = place(lw * mine + mk, c, kKeys);
-          if (at0 + mk >= valid && at0 + mk < end) {  // a node
-            const int64_t j = at0 + mk - valid;
-            uint4 kx = make_uint4(0, 0, 0, 0), vx = kx;
-            if (in_dim) {
-              kx = *reinterpret_cast<const uint4 *>(key + j * p.kv_node_stride);
-              vx = *reinterpret_cast<const uint4 *>(value + j * p.kv_node_stride);
-            }
-            if (clear_nonfinite<T>(vx)) atomicOr(&s_bad, 1ull << j);
-            *reinterpret_cast<uint4 *>(stage + to) = kx;
-            *reinterpret_cast<uint4 *>(stage + Shape::plane_bytes + to) = vx;
-          } else {
-            int64_t from = -1;
+        constexpr int steps = mine / together;
+        uint4 kx[steps], vx[steps];  // all loads before the first use
+        const auto node = [&](int i) {
+          const int at = at0 + i * together + lane / chunks;
+          return at >= valid && at < end ? at - valid : -1;
+        };
 #pragma unroll
-            for (int e = 0; e < mine / together; ++e) from = e == i ? off[e] : from;
-            const bool in = from >= 0;
-            const T *src = in ? pool + from : pool;
+        for (int i = 0; i < steps; ++i) {
+          kx[i] = vx[i] = make_uint4(0, 0, 0, 0);
+          if (node(i) >= 0 && in_dim) {
+            kx[i] = *reinterpret_cast<const uint4 *>(key + node(i) * p.kv_node_stride);
+            vx[i] = *reinterpret_cast<const uint4 *>(value + node(i) * p.kv_node_stride);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < steps; ++i) {
+          const uint32_t to = place(lw * mine + i * together + lane / chunks, c, kKeys);
+          if (node(i) >= 0) {
+            if (clear_nonfinite<T>(vx[i])) atomicOr(&s_bad, 1ull << node(i));
+            *reinterpret_cast<uint4 *>(stage + to) = kx[i];
+            *reinterpret_cast<uint4 *>(stage + Shape::plane_bytes + to) = vx[i];
+          } else {
+            const bool in = off[i] >= 0;
+            const T *src = in ? pool + off[i] : pool;
             tree_cp_async16(stage_addr + to, src, in && in_dim);
             tree_cp_async16(stage_addr + to + Shape::plane_bytes, in ? src + plane : src,
                             in && in_dim);
@@ -405,8 +433,8 @@ __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreePara
       for (int k = 0; here && k < mine; ++k) {
         const int block = apart ? k : 2 * k + w, buffer = k & 1;
         const uint32_t scores = lanes + kColumnsS + buffer * kKeys, weights = scores + kKeys / 2;
-        ok = mbar_wait(&bar.s_full[w][buffer], k >> 1 & 1, p.status) &&
-             mbar_wait(&bar.kv_full[slot], turn, p.status);  // for s_cached
+        ok = wait_phase(&bar.s_full[w][buffer], k >> 1 & 1, p.status) &&
+             wait_phase(&bar.kv_full[slot], turn, p.status);  // for s_cached
         if (!__all_sync(kFullMask, ok)) break;
         fence_after();
         uint32_t s[32];
@@ -430,7 +458,7 @@ __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreePara
           const float to = fmaxf(m, top);
           const float f = m == -INFINITY ? 0.f : tree_exp2(m - to);
           if (k > 0) {  // the output so far
-            ok = mbar_wait(&bar.pv_done[w][buffer ^ 1], (k - 1) >> 1 & 1, p.status);
+            ok = wait_phase(&bar.pv_done[w][buffer ^ 1], (k - 1) >> 1 & 1, p.status);
             if (!__all_sync(kFullMask, ok)) break;
             fence_after();
 #pragma unroll 1
@@ -483,7 +511,7 @@ __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreePara
       }
       // ---- the result -----------------------------------------------------------------
       if (ok && mine > 0)
-        mbar_wait(&bar.pv_done[w][(mine - 1) & 1], (mine - 1) >> 1 & 1, p.status);
+        wait_phase(&bar.pv_done[w][(mine - 1) & 1], (mine - 1) >> 1 & 1, p.status);
       __syncwarp();
       fence_after();
       // With both streams' last products done the ring's memory is free: a row of
@@ -553,24 +581,24 @@ __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreePara
         const int first = row - lane, rows_here = max(0, min(32, all - first));
         const unsigned alive_rows = __ballot_sync(kFullMask, alive);
         const int d = 4 * lane;
-        for (int i = 0; i < rows_here; ++i) {
+        // lane i knows where row i goes: its partial number or its offset in `out`
+        const int64_t number = row < all ? partial_number(p, b, kh, row, split) : 0;
+        const int64_t place_of = p.splits > 1 ? number * D : row < all ? out_offset(p, b, kh, row) : 0;
+        const float *from = stage + quarter * 32 * pitch + d;
+#pragma unroll 8
+        for (int i = 0; i < 32; ++i) {
+          const int64_t to = __shfl_sync(kFullMask, place_of, i) + d;
+          if (i >= rows_here || d >= D) continue;
           float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-          if ((alive_rows >> i & 1) && d < D)
-            x = *reinterpret_cast<const float4 *>(stage + (quarter * 32 + i) * pitch + d);
-          if (d >= D) continue;
-          if (p.splits > 1) {
-            *reinterpret_cast<float4 *>(
-                p.partials + partial_number(p, b, kh, first + i, split) * D + d) = x;
-          } else {
-            uint2 v;
-            v.x = pack2<T>(x.x, x.y);
-            v.y = pack2<T>(x.z, x.w);
-            *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + out_offset(p, b, kh, first + i) +
-                                       d) = v;
-          }
+          if (alive_rows >> i & 1) x = *reinterpret_cast<const float4 *>(from + i * pitch);
+          if (p.splits > 1)
+            *reinterpret_cast<float4 *>(p.partials + to) = x;
+          else
+            *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + to) =
+                make_uint2(pack2<T>(x.x, x.y), pack2<T>(x.z, x.w));
         }
         if (p.splits > 1 && row < all)
-          p.stats[partial_number(p, b, kh, row, split)] = make_float2(alive ? m : -INFINITY, l);
+          p.stats[number] = make_float2(alive ? m : -INFINITY, l);
       }
     } else {
       // ---- the products: one warp issues the scores, one the outputs ----------------
@@ -584,11 +612,11 @@ __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreePara
       int slot = 0, turn = 0;
       for (int n = 0; n < items; ++n) {
         const int w = n & 1, k = n >> 1, buffer = k & 1;
-        bool ready = mbar_wait(&bar.kv_full[slot], turn, p.status);
+        bool ready = wait_phase(&bar.kv_full[slot], turn, p.status);
         if (outputs)
-          ready = ready && mbar_wait(&bar.p_full[w][buffer], k >> 1 & 1, p.status);
+          ready = ready && wait_phase(&bar.p_full[w][buffer], k >> 1 & 1, p.status);
         else if (k >= 2)  // the products that read this buffer's P
-          ready = ready && mbar_wait(&bar.pv_done[w][buffer], (k - 2) >> 1 & 1, p.status);
+          ready = ready && wait_phase(&bar.pv_done[w][buffer], (k - 2) >> 1 & 1, p.status);
         if (!__all_sync(kFullMask, ready)) break;
         fence_after();
         fence_async_proxy();  // the copies are visible to this thread; now to its products
