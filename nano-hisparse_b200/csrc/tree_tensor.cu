@@ -10,10 +10,11 @@
 //                   TMEM. The maximum is raised only when a score passes it by
 //                   more than 8 (a factor of 256, inside fp16's range), so the
 //                   output, which stays in TMEM, is rescaled rarely.
-//   warps 8-15      copy key blocks, 16 bytes a thread with cp.async, into a ring
-//                   of stages in the 128-byte-swizzled layout of the descriptors:
-//                   rows are scattered over the pool, so there is no tile for the
-//                   TMA engine, and a row's slice of one KV head is 256 bytes.
+//   warps 8-15      copy key blocks (four warps K, four V), 16 bytes a thread with
+//                   cp.async, into rings of stages in the 128-byte-swizzled layout of
+//                   the descriptors: rows are scattered over the pool, so there is no
+//                   tile for the TMA engine, and its gather of four rows of 128 bytes
+//                   was measured at 73 clocks each, a third of this path's rate.
 //   warp 16         issues S = Q K^T, both operands in shared memory, K-major
 //   warp 17         issues O += P V, P in TMEM, V in shared memory, MN-major (as
 //                   stored: a key's elements are adjacent)
@@ -32,7 +33,9 @@
 namespace hs {
 namespace {
 
-constexpr int kSoftmaxWarps = 8, kLoadWarps = 8;
+constexpr int kSoftmaxWarps = 8, kLoadWarps = 8;  // half of the latter for K, half for V
+constexpr int kMaxStages = 8;
+constexpr int kMarks = 16;     // blocks whose marks (which keys are cache rows) are kept
 constexpr int kScoreWarp = kSoftmaxWarps + kLoadWarps, kOutputWarp = kScoreWarp + 1;
 constexpr int kTensorThreads = 32 * (kOutputWarp + 1);
 constexpr int kTile = 128;     // query rows of a stream
@@ -43,16 +46,21 @@ constexpr int kColumnsS = 128, kStreamColumns = 256;
 
 // Shared memory of a block. kDim: head_dim rounded up to 64 or 128, the rest zero.
 // Operands are panels of 64 elements (128 bytes) a row, 8 rows to the swizzle atom.
+// K and V have rings of their own: a stage of K is free when its scores are done, a
+// stage of V only when its output is. Streams of the same rows need one tile of Q and
+// take the other's place for two more stages.
 template <int kDim> struct TensorShape {
   static constexpr int q_bytes = kTile * kDim * 2;       // of one stream
-  static constexpr int plane_bytes = kKeys * kDim * 2;   // K or V of a stage
-  static constexpr int stages = kDim == 64 ? 8 : 5;
-  static constexpr int ring = 2 * q_bytes;
-  static constexpr int bytes = ring + stages * 2 * plane_bytes;
+  static constexpr int plane_bytes = kKeys * kDim * 2;   // a stage: K or V of a block
+  static constexpr int k_stages = kDim == 64 ? 8 : 4, v_stages = kDim == 64 ? 8 : 6;
+  static constexpr int more = kDim == 64 ? 0 : 1;        // of each, with one tile of Q
+  static constexpr int bytes = 2 * q_bytes + (k_stages + v_stages) * plane_bytes;
   static constexpr size_t dynamic = bytes + 1024;        // alignment to a swizzle atom
-  static constexpr int join_pitch = kDim + 4;            // floats of a result's row in the ring
-  static_assert(kKeys / kLoadWarps == 8, "a byte of s_cached for each loading warp");
-  static_assert(2 * kTile * join_pitch * 4 <= stages * 2 * plane_bytes, "results fit the ring");
+  static constexpr int join_pitch = kDim + 4;            // floats of a result's row in the rings
+  static_assert(k_stages + more <= kMaxStages && v_stages + more <= kMaxStages, "barriers");
+  static_assert(2 * more * plane_bytes <= q_bytes, "the second tile of Q makes room for them");
+  static_assert(2 * kTile * join_pitch * 4 <= (k_stages + v_stages) * plane_bytes,
+                "results fit the rings");
 };
 
 // 32 columns of this thread's TMEM lane
@@ -228,7 +236,7 @@ __device__ __forceinline__ uint32_t place(int r, int c, int rows) {
 }
 
 struct TensorBarriers {
-  uint64_t kv_full[8], kv_free[8];
+  uint64_t k_full[kMaxStages], k_free[kMaxStages], v_full[kMaxStages], v_free[kMaxStages];
   uint64_t s_full[2][2], p_full[2][2], pv_done[2][2];  // by stream and buffer
 };
 
@@ -237,19 +245,23 @@ __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreePara
   using Shape = TensorShape<kDim>;
   extern __shared__ unsigned char tensor_smem[];
   __shared__ TensorBarriers bar;
-  __shared__ __align__(8) uint8_t s_cached[8][kLoadWarps];  // by stage: its keys that are cache rows
+  __shared__ __align__(8) uint16_t s_cached[kMarks][kLoadWarps / 2];  // keys that are cache rows
   __shared__ uint32_t s_tmem;
   __shared__ unsigned long long s_bad;  // nodes whose V held a non-finite element
   __shared__ float2 s_stats[kTile];
   unsigned char *smem = reinterpret_cast<unsigned char *>(
       (reinterpret_cast<uintptr_t>(tensor_smem) + 1023) & ~(uintptr_t)1023);
-  unsigned char *ring = smem + Shape::ring;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, split = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31, split = blockIdx.y;
+  const int warp = __shfl_sync(kFullMask, tid >> 5, 0);  // the same for every lane, to the compiler too
   const int D = p.head_dim, G = p.groups, all = p.nodes * G, b = blockIdx.z;
   const int n_nodes = nodes_of(p, b), valid = (int)rows_of(p, b), live = n_nodes * G;
   const int tiles = (all + p.tile_rows - 1) / p.tile_rows;
-  const int kh = blockIdx.y / tiles, r0 = blockIdx.y % tiles * p.tile_rows;
+  const int kh = blockIdx.x / tiles, r0 = blockIdx.x % tiles * p.tile_rows;
   const bool apart = p.tile_rows > kTile;  // the streams own different rows
+  const int k_stages = Shape::k_stages + (apart ? 0 : Shape::more);
+  const int v_stages = Shape::v_stages + (apart ? 0 : Shape::more);
+  unsigned char *k_ring = smem + (apart ? 2 : 1) * Shape::q_bytes;
+  unsigned char *v_ring = k_ring + k_stages * Shape::plane_bytes;
   // the keys of this split: begin .. end - 1
   const unsigned total = r0 < live ? (unsigned)(valid + n_nodes) : 0;
   const unsigned share = ((total + p.splits - 1) / p.splits + kKeys - 1) / kKeys * kKeys;
@@ -274,13 +286,15 @@ __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreePara
   const int live0 = min(kTile, live - r0);
   const int live1 = apart ? max(0, min(kTile, live - r0 - kTile)) : live0;
   if (tid == 32 * kScoreWarp) {
-    for (int i = 0; i < Shape::stages; ++i) {
-      mbar_init(&bar.kv_full[i], kLoadWarps * (32 + 1));
-      mbar_init(&bar.kv_free[i], apart ? 2 : 1);
+    for (int i = 0; i < kMaxStages; ++i) {
+      mbar_init(&bar.k_full[i], kLoadWarps / 2 * (32 + 1));
+      mbar_init(&bar.v_full[i], kLoadWarps / 2 * (32 + 1));
+      mbar_init(&bar.k_free[i], apart ? 2 : 1);
+      mbar_init(&bar.v_free[i], apart ? 2 : 1);
     }
     for (int w = 0; w < 2; ++w)
       for (int i = 0; i < 2; ++i) {
-        mbar_init(&bar.s_full[w][i], 1);
+        mbar_init(&bar.s_full[w][i], 2);  // the products, and the marks that came with their keys
         mbar_init(&bar.p_full[w][i], max(1, ((w ? live1 : live0) + 31) / 32));
         mbar_init(&bar.pv_done[w][i], 1);
       }
@@ -290,18 +304,22 @@ __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreePara
   __syncthreads();
 
   if (warp >= kSoftmaxWarps && warp < kSoftmaxWarps + kLoadWarps) {
-    // ---- key blocks into the ring ---------------------------------------------------
-    const int lw = warp - kSoftmaxWarps;
-    constexpr int chunks = kDim / 8, together = 32 / chunks;  // keys of a warp's copy
-    const int c = lane % chunks;
+    // ---- K or V of the key blocks into its ring -------------------------------------
+    constexpr int warps = kLoadWarps / 2, mine = kKeys / warps;  // keys of a block a warp copies
+    constexpr int chunks = kDim / 8, together = 32 / chunks, steps = mine / together;
+    const bool values = warp >= kSoftmaxWarps + warps;
+    const int lw = (warp - kSoftmaxWarps) % warps, c = lane % chunks;
     const bool in_dim = c * 8 < D;
-    const int64_t row_elems = (int64_t)p.kv_heads * D, plane = p.page_size * row_elems;
-    const T *pool = static_cast<const T *>(p.pool) + (int64_t)kh * D + c * 8;
-    const int64_t node_base = (int64_t)b * p.kv_batch_stride + (int64_t)kh * D + c * 8;
-    const T *key = static_cast<const T *>(p.key) + node_base;
-    const T *value = static_cast<const T *>(p.value) + node_base;
+    const int64_t row_elems = (int64_t)p.kv_heads * D;
+    const T *pool = static_cast<const T *>(p.pool) + (int64_t)kh * D + c * 8 +
+                    (values ? p.page_size * row_elems : 0);
+    const T *drafted = static_cast<const T *>(values ? p.value : p.key) +
+                       (int64_t)b * p.kv_batch_stride + (int64_t)kh * D + c * 8;
     const int64_t *rows = p.rows + b * p.rows_batch_stride;
-    constexpr int mine = kKeys / kLoadWarps;  // keys of a block that this warp copies
+    uint64_t *full = values ? bar.v_full : bar.k_full, *free = values ? bar.v_free : bar.k_free;
+    const int stages = values ? v_stages : k_stages;
+    const uint32_t ring_addr = smem_addr(values ? v_ring : k_ring);
+    unsigned char *ring = values ? v_ring : k_ring;
     // lane i < mine reads the row number of the warp's i-th key, kLook blocks ahead:
     // a block's time is shorter than the read's
     const int last = min(end, valid);
@@ -317,60 +335,52 @@ __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreePara
     const uint32_t to0 = place(lw * mine + lane / chunks, c, kKeys);
     int slot = 0, turn = 1;
     for (int block = 0; block < blocks; ++block) {
-      if (block >= Shape::stages) {
-        const bool ok = wait_phase(&bar.kv_free[slot], turn, p.status);
+      if (block >= stages) {
+        const bool ok = wait_phase(&free[slot], turn, p.status);
         if (!__all_sync(kFullMask, ok)) break;
       }
       const int64_t offset = row_offset(p, next[0], row_elems);
 #pragma unroll
       for (int i = 0; i + 1 < kLook; ++i) next[i] = next[i + 1];
       next[kLook - 1] = block + kLook < blocks ? look(block + kLook) : -1;
-      const unsigned cached = __ballot_sync(kFullMask, offset >= 0);
-      if (lane == 0) s_cached[slot][lw] = (uint8_t)cached;
-      unsigned char *stage = ring + slot * 2 * Shape::plane_bytes;
-      const uint32_t stage_addr = smem_addr(stage);
+      if (!values) {
+        const unsigned cached = __ballot_sync(kFullMask, offset >= 0);
+        if (lane == 0) s_cached[block % kMarks][lw] = (uint16_t)cached;
+      }
+      const uint32_t stage_addr = ring_addr + slot * Shape::plane_bytes;
       const int at0 = begin + block * kKeys + lw * mine;
-      int64_t off[mine / together];
+      int64_t off[steps];
 #pragma unroll
-      for (int i = 0; i < mine; i += together)
-        off[i / together] = __shfl_sync(kFullMask, offset, i + lane / chunks);
+      for (int i = 0; i < steps; ++i)
+        off[i] = __shfl_sync(kFullMask, offset, i * together + lane / chunks);
       if (at0 + mine <= valid) {
 #pragma unroll
-        for (int i = 0; i < mine; i += together) {
-          const uint32_t to = stage_addr + (to0 ^ ((i & 7) << 4)) + i * 128;
-          const bool in = off[i / together] >= 0;
-          const T *src = in ? pool + off[i / together] : pool;
-          tree_cp_async16(to, src, in && in_dim);
-          tree_cp_async16(to + Shape::plane_bytes, in ? src + plane : src, in && in_dim);
+        for (int i = 0; i < steps; ++i) {
+          const int key = i * together;
+          tree_cp_async16(stage_addr + (to0 ^ ((key & 7) << 4)) + key * 128,
+                          off[i] >= 0 ? pool + off[i] : pool, off[i] >= 0 && in_dim);
         }
       } else {
-        constexpr int steps = mine / together;
-        uint4 kx[steps], vx[steps];  // all loads before the first use
+        uint4 raw[steps];  // all loads before the first use
         const auto node = [&](int i) {
           const int at = at0 + i * together + lane / chunks;
           return at >= valid && at < end ? at - valid : -1;
         };
 #pragma unroll
         for (int i = 0; i < steps; ++i) {
-          kx[i] = vx[i] = make_uint4(0, 0, 0, 0);
-          if (node(i) >= 0 && in_dim) {
-            kx[i] = *reinterpret_cast<const uint4 *>(key + node(i) * p.kv_node_stride);
-            vx[i] = *reinterpret_cast<const uint4 *>(value + node(i) * p.kv_node_stride);
-          }
+          raw[i] = make_uint4(0, 0, 0, 0);
+          if (node(i) >= 0 && in_dim)
+            raw[i] = *reinterpret_cast<const uint4 *>(drafted + node(i) * p.kv_node_stride);
         }
 #pragma unroll
         for (int i = 0; i < steps; ++i) {
           const uint32_t to = place(lw * mine + i * together + lane / chunks, c, kKeys);
           if (node(i) >= 0) {
-            if (clear_nonfinite<T>(vx[i])) atomicOr(&s_bad, 1ull << node(i));
-            *reinterpret_cast<uint4 *>(stage + to) = kx[i];
-            *reinterpret_cast<uint4 *>(stage + Shape::plane_bytes + to) = vx[i];
+            if (values && clear_nonfinite<T>(raw[i])) atomicOr(&s_bad, 1ull << node(i));
+            *reinterpret_cast<uint4 *>(ring + slot * Shape::plane_bytes + to) = raw[i];
           } else {
-            const bool in = off[i] >= 0;
-            const T *src = in ? pool + off[i] : pool;
-            tree_cp_async16(stage_addr + to, src, in && in_dim);
-            tree_cp_async16(stage_addr + to + Shape::plane_bytes, in ? src + plane : src,
-                            in && in_dim);
+            tree_cp_async16(stage_addr + to, off[i] >= 0 ? pool + off[i] : pool,
+                            off[i] >= 0 && in_dim);
           }
         }
         fence_async_proxy();
@@ -378,9 +388,9 @@ __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreePara
       // Every lane's copies announce themselves when they land; lane 0's arrival
       // carries what was written with plain stores.
       __syncwarp();
-      copies_arrive(&bar.kv_full[slot]);
-      if (lane == 0) mbar_arrive(&bar.kv_full[slot]);
-      if (++slot == Shape::stages) {
+      copies_arrive(&full[slot]);
+      if (lane == 0) mbar_arrive(&full[slot]);
+      if (++slot == stages) {
         slot = 0;
         turn ^= 1;
       }
@@ -414,7 +424,7 @@ __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreePara
     __syncwarp();
     asm volatile("bar.sync 2, %0;\n" ::"n"(32 * (kSoftmaxWarps + 2)) : "memory");
     fence_after();
-    const uint32_t tmem = s_tmem;
+    const uint32_t tmem = __shfl_sync(kFullMask, s_tmem, 0);
 
     if (warp < kSoftmaxWarps) {
       // ---- softmax of stream w ------------------------------------------------------
@@ -429,18 +439,16 @@ __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreePara
       const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
       float m = -INFINITY, l = 0.f;
       bool ok = true;
-      int slot = apart ? 0 : w, turn = 0;
       for (int k = 0; here && k < mine; ++k) {
         const int block = apart ? k : 2 * k + w, buffer = k & 1;
         const uint32_t scores = lanes + kColumnsS + buffer * kKeys, weights = scores + kKeys / 2;
-        ok = wait_phase(&bar.s_full[w][buffer], k >> 1 & 1, p.status) &&
-             wait_phase(&bar.kv_full[slot], turn, p.status);  // for s_cached
+        ok = wait_phase(&bar.s_full[w][buffer], k >> 1 & 1, p.status);
         if (!__all_sync(kFullMask, ok)) break;
         fence_after();
         uint32_t s[32];
         tmem_load32(s, scores);
         // keys this row sees: cache rows, then nodes from position n0 on
-        uint64_t seen = *reinterpret_cast<const uint64_t *>(s_cached[slot]);
+        uint64_t seen = *reinterpret_cast<const uint64_t *>(s_cached[block % kMarks]);
         const int k0 = begin + block * kKeys;
         if (k0 + kKeys > valid) {
           const int n0 = max(valid - k0, 0), j0 = k0 + n0 - valid;
@@ -503,22 +511,17 @@ __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreePara
         fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar.p_full[w][buffer]);
-        slot += apart ? 1 : 2;
-        if (slot >= Shape::stages) {
-          slot -= Shape::stages;
-          turn ^= 1;
-        }
       }
       // ---- the result -----------------------------------------------------------------
       if (ok && mine > 0)
         wait_phase(&bar.pv_done[w][(mine - 1) & 1], (mine - 1) >> 1 & 1, p.status);
       __syncwarp();
       fence_after();
-      // With both streams' last products done the ring's memory is free: a row of
+      // With both streams' last products done the rings' memory is free: a row of
       // fp32 for each query row, so that rows leave in whole lines.
       asm volatile("bar.sync 1, %0;\n" ::"n"(32 * kSoftmaxWarps) : "memory");
       constexpr int pitch = Shape::join_pitch;
-      float *stage = reinterpret_cast<float *>(ring) + (apart ? w * kTile * pitch : 0);
+      float *stage = reinterpret_cast<float *>(k_ring) + (apart ? w * kTile * pitch : 0);
       float *own = stage + r * pitch;
       if (!apart) {
         if (w == 1 && here) {
@@ -600,53 +603,66 @@ __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreePara
         if (p.splits > 1 && row < all)
           p.stats[number] = make_float2(alive ? m : -INFINITY, l);
       }
-    } else {
-      // ---- the products: one warp issues the scores, one the outputs ----------------
+    } else if (warp == kScoreWarp) {
+      // ---- S = Q K^T ------------------------------------------------------------------
       // The whole warp walks the items, so that addresses stay in uniform registers;
       // one lane issues.
-      const bool outputs = warp == kOutputWarp;
-      const uint32_t idesc = instruction<T>(outputs ? kDim : kKeys, outputs);
+      const uint32_t idesc = instruction<T>(kKeys, false);
       const uint32_t q0 = descriptor(smem_addr(smem), 16);
-      const uint32_t k0 = descriptor(smem_addr(ring), 16);
-      const uint32_t v0 = descriptor(smem_addr(ring) + Shape::plane_bytes, kKeys * 128);
+      const uint32_t k0 = descriptor(smem_addr(k_ring), 16);
       int slot = 0, turn = 0;
       for (int n = 0; n < items; ++n) {
         const int w = n & 1, k = n >> 1, buffer = k & 1;
-        bool ready = wait_phase(&bar.kv_full[slot], turn, p.status);
-        if (outputs)
-          ready = ready && wait_phase(&bar.p_full[w][buffer], k >> 1 & 1, p.status);
-        else if (k >= 2)  // the products that read this buffer's P
-          ready = ready && wait_phase(&bar.pv_done[w][buffer], (k - 2) >> 1 & 1, p.status);
+        // the products that read this buffer's P, then the keys
+        bool ready = k < 2 || wait_phase(&bar.pv_done[w][buffer], (k - 2) >> 1 & 1, p.status);
+        ready = ready && wait_phase(&bar.k_full[slot], turn, p.status);
         if (!__all_sync(kFullMask, ready)) break;
         fence_after();
         fence_async_proxy();  // the copies are visible to this thread; now to its products
-        const uint32_t d = tmem + w * kStreamColumns, s = d + kColumnsS + buffer * kKeys;
-        if (!outputs) {
-          const uint32_t q = q0 + (apart ? w * (Shape::q_bytes >> 4) : 0);
-          const uint32_t kd = k0 + slot * (2 * Shape::plane_bytes >> 4);
-          if (elect_one()) {
+        const uint32_t q = q0 + (apart ? w * (Shape::q_bytes >> 4) : 0);
+        const uint32_t kd = k0 + slot * (Shape::plane_bytes >> 4);
+        const uint32_t d = tmem + w * kStreamColumns + kColumnsS + buffer * kKeys;
+        if (elect_one()) {
 #pragma unroll
-            for (int kk = 0; kk < kDim / 16; ++kk)
-              mma_shared(s, q + ((kk / 4 * kTile * 128 + kk % 4 * 32) >> 4),
-                         kd + ((kk / 4 * kKeys * 128 + kk % 4 * 32) >> 4), idesc, kk > 0);
-            commit(&bar.s_full[w][buffer]);
-          }
-        } else {
-          const uint32_t vd = v0 + slot * (2 * Shape::plane_bytes >> 4);
-          if (elect_one()) {
-#pragma unroll
-            for (int kk = 0; kk < kKeys / 16; ++kk)
-              mma_tmem(d, s + kKeys / 2 + kk * 8, vd + (kk * 2048 >> 4), idesc, k > 0 || kk > 0);
-            commit(&bar.pv_done[w][buffer]);
-            commit(&bar.kv_free[slot]);
-          }
+          for (int kk = 0; kk < kDim / 16; ++kk)
+            mma_shared(d, q + ((kk / 4 * kTile * 128 + kk % 4 * 32) >> 4),
+                       kd + ((kk / 4 * kKeys * 128 + kk % 4 * 32) >> 4), idesc, kk > 0);
+          commit(&bar.s_full[w][buffer]);
+          mbar_arrive(&bar.s_full[w][buffer]);
+          commit(&bar.k_free[slot]);
         }
         __syncwarp();
-        if (!apart || w == 1) {
-          if (++slot == Shape::stages) {
-            slot = 0;
-            turn ^= 1;
-          }
+        if ((!apart || w == 1) && ++slot == k_stages) {
+          slot = 0;
+          turn ^= 1;
+        }
+      }
+    } else {
+      // ---- O += P V -------------------------------------------------------------------
+      const uint32_t idesc = instruction<T>(kDim, true);
+      const uint32_t v0 = descriptor(smem_addr(v_ring), kKeys * 128);
+      int slot = 0, turn = 0;
+      for (int n = 0; n < items; ++n) {
+        const int w = n & 1, k = n >> 1, buffer = k & 1;
+        bool ready = wait_phase(&bar.v_full[slot], turn, p.status);
+        ready = ready && wait_phase(&bar.p_full[w][buffer], k >> 1 & 1, p.status);
+        if (!__all_sync(kFullMask, ready)) break;
+        fence_after();
+        fence_async_proxy();
+        const uint32_t vd = v0 + slot * (Shape::plane_bytes >> 4);
+        const uint32_t d = tmem + w * kStreamColumns;
+        const uint32_t weights = d + kColumnsS + buffer * kKeys + kKeys / 2;
+        if (elect_one()) {
+#pragma unroll
+          for (int kk = 0; kk < kKeys / 16; ++kk)
+            mma_tmem(d, weights + kk * 8, vd + (kk * 2048 >> 4), idesc, k > 0 || kk > 0);
+          commit(&bar.pv_done[w][buffer]);
+          commit(&bar.v_free[slot]);
+        }
+        __syncwarp();
+        if ((!apart || w == 1) && ++slot == v_stages) {
+          slot = 0;
+          turn ^= 1;
         }
       }
     }
@@ -666,7 +682,8 @@ template <typename T, int kDim> int launch(const TreeParams &p, cudaStream_t s) 
   const size_t bytes = TensorShape<kDim>::dynamic;
   if (int e = reserve_smem(reinterpret_cast<const void *>(kernel), bytes, "attend_tree")) return e;
   const int64_t tiles = ceil_div((int64_t)p.nodes * p.groups, p.tile_rows);
-  const dim3 grid((unsigned)p.splits, (unsigned)(p.kv_heads * tiles), (unsigned)p.batch);
+  // heads side by side: their slices of a cache row are neighbours in memory
+  const dim3 grid((unsigned)(p.kv_heads * tiles), (unsigned)p.splits, (unsigned)p.batch);
   kernel<<<grid, kTensorThreads, bytes, s>>>(p);
   return check_launch("tree_tensor_kernel");
 }
