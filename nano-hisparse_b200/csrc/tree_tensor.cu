@@ -26,6 +26,9 @@
 // second half of its S.
 // Every wait is bounded; one that runs out sets HS_DEV_WAIT_TIMEOUT, ends its
 // warp's loop, and so lets every other wait run out.
+#include <cuda.h>
+
+#include <atomic>
 #include <type_traits>
 
 #include "tree.cuh"
@@ -35,6 +38,8 @@ namespace {
 
 constexpr int kSoftmaxWarps = 8, kLoadWarps = 8;  // half of the latter for K, half for V
 constexpr int kMaxStages = 8;
+constexpr int kPanel = 1024;   // bytes of 8 rows x 64 elements
+constexpr int kRun = 16;       // rows of a tiled copy
 constexpr int kMarks = 16;     // blocks whose marks (which keys are cache rows) are kept
 constexpr int kScoreWarp = kSoftmaxWarps + kLoadWarps, kOutputWarp = kScoreWarp + 1;
 constexpr int kTensorThreads = 32 * (kOutputWarp + 1);
@@ -45,11 +50,14 @@ constexpr unsigned long long kWaitNanoseconds = 4000000000ull;  // then a wait g
 constexpr int kColumnsS = 128, kStreamColumns = 256;
 
 // Shared memory of a block. kDim: head_dim rounded up to 64 or 128, the rest zero.
-// Operands are panels of 64 elements (128 bytes) a row, 8 rows to the swizzle atom.
+// An operand is a list of 8-row groups, each of one or two panels of 64 elements
+// (128 bytes) a row: a panel of a group is a swizzle atom, and a run of rows in the
+// pool lands in it with one tiled copy.
 // K and V have rings of their own: a stage of K is free when its scores are done, a
 // stage of V only when its output is. Streams of the same rows need one tile of Q and
 // take the other's place for two more stages.
 template <int kDim> struct TensorShape {
+  static constexpr int atom = kDim / 64 * kPanel;        // bytes of an 8-row group
   static constexpr int q_bytes = kTile * kDim * 2;       // of one stream
   static constexpr int plane_bytes = kKeys * kDim * 2;   // a stage: K or V of a block
   static constexpr int k_stages = kDim == 64 ? 8 : 4, v_stages = kDim == 64 ? 8 : 6;
@@ -180,6 +188,20 @@ __device__ __forceinline__ bool wait_phase(uint64_t *bar, unsigned parity, int32
   flag(status, HS_DEV_WAIT_TIMEOUT);
   return false;
 }
+__device__ __forceinline__ void mbar_arrive_many(uint64_t *bar, unsigned count) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;\n" ::"r"(smem_addr(bar)), "r"(count)
+               : "memory");
+}
+// kRun rows of one KV head (panels `panel` on) from row 8 * group of the pool's rows,
+// completing on `bar`
+__device__ __forceinline__ void tile_copy(uint32_t dst, const CUtensorMap *map, int panel,
+                                          int group, uint64_t *bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, "
+      "{%2, %2, %3, %4}], [%5];\n" ::"r"(dst),
+      "l"(map), "r"(0), "r"(panel), "r"(group), "r"(smem_addr(bar))
+      : "memory");
+}
 // Arrives on `bar` once this thread's copies so far have landed.
 __device__ __forceinline__ void copies_arrive(uint64_t *bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];\n" ::"r"(smem_addr(bar))
@@ -193,29 +215,31 @@ __device__ __forceinline__ void commit(uint64_t *bar) {
 }
 // Shared-memory descriptor, 128-byte swizzle: the low word has the address and, for
 // MN-major operands that span several panels, the panels' distance; the high word
-// the distance of 8-row atoms, the same for all operands here. Adding bytes / 16 to
-// the low word moves the address.
-constexpr uint32_t kDescriptorHigh = (1024 >> 4) | 1u << 14 | 2u << 29;
-__device__ __forceinline__ uint32_t descriptor(uint32_t addr, uint32_t panel) {
-  return (addr >> 4) | (panel >> 4) << 16;
+// the distance of 8-row groups. Adding bytes / 16 to the low word moves the address.
+template <int kDim>
+constexpr uint32_t kDescriptorHigh = (TensorShape<kDim>::atom >> 4) | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint32_t descriptor(uint32_t addr) {
+  return (addr >> 4) | (kPanel >> 4) << 16;
 }
 // D = A B (+ D), both operands in shared memory
+template <int kDim>
 __device__ __forceinline__ void mma_shared(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc,
                                            bool accumulate) {
   asm volatile(
       "{\n .reg .pred p;\n .reg .b64 a, b;\n setp.ne.b32 p, %4, 0;\n"
       " mov.b64 a, {%1, %5};\n mov.b64 b, {%2, %5};\n"
       " tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n}\n" ::"r"(d),
-      "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)accumulate), "r"(kDescriptorHigh)
+      "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)accumulate), "r"(kDescriptorHigh<kDim>)
       : "memory");
 }
 // A in TMEM
+template <int kDim>
 __device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc,
                                          bool accumulate) {
   asm volatile(
       "{\n .reg .pred p;\n .reg .b64 b;\n setp.ne.b32 p, %4, 0;\n mov.b64 b, {%2, %5};\n"
       " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n}\n" ::"r"(d),
-      "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)accumulate), "r"(kDescriptorHigh)
+      "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)accumulate), "r"(kDescriptorHigh<kDim>)
       : "memory");
 }
 __device__ __forceinline__ bool elect_one() {
@@ -230,9 +254,10 @@ template <typename T> __device__ __forceinline__ uint32_t instruction(int n, boo
   return 1u << 4 | type << 7 | type << 10 | (uint32_t)b_mn << 16 | (uint32_t)(n >> 3) << 17 |
          (uint32_t)(kTile >> 4) << 24;
 }
-// Place of 16-byte chunk c of row r in a panelled, swizzled operand of `rows` rows
-__device__ __forceinline__ uint32_t place(int r, int c, int rows) {
-  return (uint32_t)((c >> 3) * rows * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+// Place of 16-byte chunk c of row r of an operand
+template <int kDim> __device__ __forceinline__ uint32_t place(int r, int c) {
+  return (uint32_t)((r >> 3) * TensorShape<kDim>::atom + (c >> 3) * kPanel + (r & 7) * 128 +
+                    (((c & 7) ^ (r & 7)) << 4));
 }
 
 struct TensorBarriers {
@@ -241,7 +266,7 @@ struct TensorBarriers {
 };
 
 template <typename T, int kDim>
-__global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreeParams p) {
+__global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreeParams p, const __grid_constant__ CUtensorMap map, bool tiled) {
   using Shape = TensorShape<kDim>;
   extern __shared__ unsigned char tensor_smem[];
   __shared__ TensorBarriers bar;
@@ -332,14 +357,18 @@ __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreePara
     for (int i = 0; i < kLook; ++i) next[i] = i < blocks ? look(i) : -1;
     // Where this lane's first chunk goes; i keys further it is i rows down, and the
     // row's part of the swizzle differs by i (the lane's own part is below `together`).
-    const uint32_t to0 = place(lw * mine + lane / chunks, c, kKeys);
+    const uint32_t to0 = place<kDim>(lw * mine + lane / chunks, c);
     int slot = 0, turn = 1;
     for (int block = 0; block < blocks; ++block) {
       if (block >= stages) {
         const bool ok = wait_phase(&free[slot], turn, p.status);
-        if (!__all_sync(kFullMask, ok)) break;
+        if (!__all_sync(kFullMask, ok)) {  // leave no copy behind
+          for (int i = max(0, block - stages); i < block; ++i)
+            wait_phase(&full[i % stages], i / stages & 1, p.status);
+          break;
+        }
       }
-      const int64_t offset = row_offset(p, next[0], row_elems);
+      const int64_t now = next[0], offset = row_offset(p, now, row_elems);
 #pragma unroll
       for (int i = 0; i + 1 < kLook; ++i) next[i] = next[i + 1];
       next[kLook - 1] = block + kLook < blocks ? look(block + kLook) : -1;
@@ -349,6 +378,26 @@ __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreePara
       }
       const uint32_t stage_addr = ring_addr + slot * Shape::plane_bytes;
       const int at0 = begin + block * kKeys + lw * mine;
+      // Rows that follow one another from a multiple of 8 on, as those of a page do: one
+      // tiled copy. The copy engine keeps more reads in flight than cp.async does.
+      const int64_t row = now, row0 = __shfl_sync(kFullMask, row, 0);
+      const bool run = tiled && (row0 & 7) == 0 &&
+                       (row0 & (p.page_size - 1)) + kRun <= p.page_size;
+      if (__all_sync(kFullMask, run && (lane >= mine || (offset >= 0 && row == row0 + lane)))) {
+        if (lane == 0) {
+          const int group = (int)(((row0 >> p.page_shift) * 2 * p.page_size +
+                                   (values ? p.page_size : 0) + (row0 & (p.page_size - 1))) >> 3);
+          mbar_arrive_many(&full[slot], 32);
+          mbar_expect_tx(&full[slot], mine * kDim * 2);
+          tile_copy(stage_addr + lw * mine * kDim * 2, &map, kh * (kDim / 64), group, &full[slot]);
+        }
+        __syncwarp();
+        if (++slot == stages) {
+          slot = 0;
+          turn ^= 1;
+        }
+        continue;
+      }
       int64_t off[steps];
 #pragma unroll
       for (int i = 0; i < steps; ++i)
@@ -357,7 +406,8 @@ __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreePara
 #pragma unroll
         for (int i = 0; i < steps; ++i) {
           const int key = i * together;
-          tree_cp_async16(stage_addr + (to0 ^ ((key & 7) << 4)) + key * 128,
+          tree_cp_async16(stage_addr + (to0 ^ ((key & 7) << 4)) + (key >> 3) * Shape::atom +
+                              (key & 7) * 128,
                           off[i] >= 0 ? pool + off[i] : pool, off[i] >= 0 && in_dim);
         }
       } else {
@@ -374,7 +424,7 @@ __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreePara
         }
 #pragma unroll
         for (int i = 0; i < steps; ++i) {
-          const uint32_t to = place(lw * mine + i * together + lane / chunks, c, kKeys);
+          const uint32_t to = place<kDim>(lw * mine + i * together + lane / chunks, c);
           if (node(i) >= 0) {
             if (values && clear_nonfinite<T>(raw[i])) atomicOr(&s_bad, 1ull << node(i));
             *reinterpret_cast<uint4 *>(ring + slot * Shape::plane_bytes + to) = raw[i];
@@ -407,7 +457,7 @@ __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreePara
         const int row = r0 + r, t = row / G;
         const bool in = row < live && c * 8 < D;
         tree_cp_async16(
-            smem_addr(smem + r / kTile * Shape::q_bytes + place(r % kTile, c, kTile)),
+            smem_addr(smem + r / kTile * Shape::q_bytes + place<kDim>(r % kTile, c)),
             in ? query + t * p.q_node_stride + (int64_t)(kh * G + row - t * G) * D + c * 8 : query,
             in);
       }
@@ -608,8 +658,8 @@ __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreePara
       // The whole warp walks the items, so that addresses stay in uniform registers;
       // one lane issues.
       const uint32_t idesc = instruction<T>(kKeys, false);
-      const uint32_t q0 = descriptor(smem_addr(smem), 16);
-      const uint32_t k0 = descriptor(smem_addr(k_ring), 16);
+      const uint32_t q0 = descriptor(smem_addr(smem));
+      const uint32_t k0 = descriptor(smem_addr(k_ring));
       int slot = 0, turn = 0;
       for (int n = 0; n < items; ++n) {
         const int w = n & 1, k = n >> 1, buffer = k & 1;
@@ -625,8 +675,8 @@ __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreePara
         if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < kDim / 16; ++kk)
-            mma_shared(d, q + ((kk / 4 * kTile * 128 + kk % 4 * 32) >> 4),
-                       kd + ((kk / 4 * kKeys * 128 + kk % 4 * 32) >> 4), idesc, kk > 0);
+            mma_shared<kDim>(d, q + ((kk / 4 * kPanel + kk % 4 * 32) >> 4),
+                             kd + ((kk / 4 * kPanel + kk % 4 * 32) >> 4), idesc, kk > 0);
           commit(&bar.s_full[w][buffer]);
           mbar_arrive(&bar.s_full[w][buffer]);
           commit(&bar.k_free[slot]);
@@ -640,7 +690,7 @@ __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreePara
     } else {
       // ---- O += P V -------------------------------------------------------------------
       const uint32_t idesc = instruction<T>(kDim, true);
-      const uint32_t v0 = descriptor(smem_addr(v_ring), kKeys * 128);
+      const uint32_t v0 = descriptor(smem_addr(v_ring));
       int slot = 0, turn = 0;
       for (int n = 0; n < items; ++n) {
         const int w = n & 1, k = n >> 1, buffer = k & 1;
@@ -655,7 +705,8 @@ __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreePara
         if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < kKeys / 16; ++kk)
-            mma_tmem(d, weights + kk * 8, vd + (kk * 2048 >> 4), idesc, k > 0 || kk > 0);
+            mma_tmem<kDim>(d, weights + kk * 8, vd + (kk * 2 * Shape::atom >> 4), idesc,
+                           k > 0 || kk > 0);
           commit(&bar.pv_done[w][buffer]);
           commit(&bar.v_free[slot]);
         }
@@ -677,14 +728,52 @@ __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreePara
   }
 }
 
-template <typename T, int kDim> int launch(const TreeParams &p, cudaStream_t s) {
+// The pool as 8-row groups of 64-element panels: (element, row of the group, panel,
+// group). Groups are whole where page_size is a multiple of 8. False when the driver
+// has no encoder or refuses the sizes: then all rows go through cp.async.
+bool encode_pool(CUtensorMap *map, const TreeParams &p, int dtype) {
+  using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *,
+                              const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                              const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static std::atomic<void *> found{nullptr};
+  void *fn = found.load(std::memory_order_relaxed);
+  if (fn == nullptr) {
+    cudaDriverEntryPointQueryResult result;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &result) !=
+            cudaSuccess ||
+        result != cudaDriverEntryPointSuccess || fn == nullptr) {
+      cudaGetLastError();
+      return false;
+    }
+    found.store(fn, std::memory_order_relaxed);
+  }
+  const cuuint64_t row_bytes = (cuuint64_t)p.kv_heads * p.head_dim * 2;
+  const cuuint64_t groups = (cuuint64_t)p.pool_blocks * 2 * p.page_size / 8;
+  if (groups < 2 || groups > 0x7fffffff) return false;
+  const cuuint64_t dims[4] = {64, 8, (cuuint64_t)p.kv_heads * p.head_dim / 64, groups};
+  const cuuint64_t strides[3] = {row_bytes, 128, 8 * row_bytes};
+  const cuuint32_t box[4] = {64, 8, (cuuint32_t)p.head_dim / 64, kRun / 8}, ones[4] = {1, 1, 1, 1};
+  return reinterpret_cast<Encode>(fn)(
+             map, dtype == HS_FLOAT16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                      : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+             4, const_cast<void *>(p.pool), dims, strides, box, ones,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int kDim> int launch(const TreeParams &p, int dtype, cudaStream_t s) {
   auto kernel = tree_tensor_kernel<T, kDim>;
   const size_t bytes = TensorShape<kDim>::dynamic;
   if (int e = reserve_smem(reinterpret_cast<const void *>(kernel), bytes, "attend_tree")) return e;
   const int64_t tiles = ceil_div((int64_t)p.nodes * p.groups, p.tile_rows);
   // heads side by side: their slices of a cache row are neighbours in memory
   const dim3 grid((unsigned)(p.kv_heads * tiles), (unsigned)p.splits, (unsigned)p.batch);
-  kernel<<<grid, kTensorThreads, bytes, s>>>(p);
+  CUtensorMap map{};
+  const bool tiled = p.head_dim == kDim && p.count >= kRun && p.page_size % kRun == 0 &&
+                     p.page_shift >= 0 && encode_pool(&map, p, dtype);
+  kernel<<<grid, kTensorThreads, bytes, s>>>(p, map, tiled);
   return check_launch("tree_tensor_kernel");
 }
 
@@ -692,8 +781,9 @@ template <typename T, int kDim> int launch(const TreeParams &p, cudaStream_t s) 
 
 int launch_tree_tensor(const TreeParams &p, int dtype, cudaStream_t s) {
   if (dtype == HS_FLOAT16)
-    return p.head_dim <= 64 ? launch<__half, 64>(p, s) : launch<__half, 128>(p, s);
-  return p.head_dim <= 64 ? launch<__nv_bfloat16, 64>(p, s) : launch<__nv_bfloat16, 128>(p, s);
+    return p.head_dim <= 64 ? launch<__half, 64>(p, dtype, s) : launch<__half, 128>(p, dtype, s);
+  return p.head_dim <= 64 ? launch<__nv_bfloat16, 64>(p, dtype, s)
+                          : launch<__nv_bfloat16, 128>(p, dtype, s);
 }
 
 }  // namespace hs
