@@ -220,6 +220,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) tree_merge_kernel(TreeParams
     return;
   }
   const int64_t first = partial_number(p, b, h / p.groups, t * p.groups + h % p.groups, 0);
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");  // the splits are written
   static_assert(kTreeMaxSplits <= 64, "two splits a lane");
   float2 part[2];
 #pragma unroll
@@ -266,10 +267,18 @@ template <typename T> int launch_merge(const TreeParams &p, cudaStream_t s) {
   if (p.splits == 1) return HS_OK;
   const dim3 grid((unsigned)ceil_div((int64_t)p.nodes * p.q_heads, kMergeWarps),
                   (unsigned)p.batch);
-  if (p.head_dim % 4 == 0)
-    tree_merge_kernel<T, true><<<grid, 32 * kMergeWarps, 0, s>>>(p);
-  else
-    tree_merge_kernel<T, false><<<grid, 32 * kMergeWarps, 0, s>>>(p);
+  // its launch overlaps the end of the kernel before it, which it waits for itself
+  cudaLaunchConfig_t config{};
+  config.gridDim = grid;
+  config.blockDim = dim3(32 * kMergeWarps);
+  config.stream = s;
+  cudaLaunchAttribute attribute{};
+  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  cudaLaunchKernelEx(&config, p.head_dim % 4 == 0 ? tree_merge_kernel<T, true>
+                                                  : tree_merge_kernel<T, false>, p);
   return check_launch("tree_merge_kernel");
 }
 

@@ -60,7 +60,7 @@ template <int kDim> struct TensorShape {
   static constexpr int atom = kDim / 64 * kPanel;        // bytes of an 8-row group
   static constexpr int q_bytes = kTile * kDim * 2;       // of one stream
   static constexpr int plane_bytes = kKeys * kDim * 2;   // a stage: K or V of a block
-  static constexpr int k_stages = kDim == 64 ? 8 : 4, v_stages = kDim == 64 ? 8 : 6;
+  static constexpr int k_stages = kDim == 64 ? 8 : 4, v_stages = kDim == 64 ? 8 : 5;
   static constexpr int more = kDim == 64 ? 0 : 1;        // of each, with one tile of Q
   static constexpr int bytes = 2 * q_bytes + (k_stages + v_stages) * plane_bytes;
   static constexpr size_t dynamic = bytes + 1024;        // alignment to a swizzle atom
@@ -84,6 +84,14 @@ __device__ __forceinline__ void tmem_load32(uint32_t (&r)[32], uint32_t addr) {
                  "=r"(r[30]), "=r"(r[31])
                : "r"(addr));
 }
+__device__ __forceinline__ void tmem_load16(uint32_t (&r)[16], uint32_t addr) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, "
+               "%9, %10, %11, %12, %13, %14, %15}, [%16];\n"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]),
+                 "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+                 "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(addr));
+}
 __device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t (&r)[16]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, "
                "%8, %9, %10, %11, %12, %13, %14, %15, %16};\n"
@@ -91,17 +99,6 @@ __device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t (&r)[
                  "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]),
                  "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
                  "r"(r[13]), "r"(r[14]), "r"(r[15])
-               : "memory");
-}
-// 16 columns, waited for
-__device__ __forceinline__ void tmem_load16_wait(uint32_t (&r)[16], uint32_t addr) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, "
-               "%9, %10, %11, %12, %13, %14, %15}, [%16];\n"
-               "tcgen05.wait::ld.sync.aligned;\n"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]),
-                 "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
-                 "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-               : "r"(addr)
                : "memory");
 }
 // The loads are done; the registers pass through so that no use moves ahead of it.
@@ -113,6 +110,25 @@ __device__ __forceinline__ void tmem_load_wait(uint32_t (&r)[32]) {
                  "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
                  "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
                  "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void tmem_load16_done(uint32_t (&a)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;\n"
+               : "+r"(a[0]), "+r"(a[1]), "+r"(a[2]), "+r"(a[3]), "+r"(a[4]), "+r"(a[5]),
+                 "+r"(a[6]), "+r"(a[7]), "+r"(a[8]), "+r"(a[9]), "+r"(a[10]), "+r"(a[11]),
+                 "+r"(a[12]), "+r"(a[13]), "+r"(a[14]), "+r"(a[15])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void tmem_load16_done(uint32_t (&a)[16], uint32_t (&b)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;\n"
+               : "+r"(a[0]), "+r"(a[1]), "+r"(a[2]), "+r"(a[3]), "+r"(a[4]), "+r"(a[5]),
+                 "+r"(a[6]), "+r"(a[7]), "+r"(a[8]), "+r"(a[9]), "+r"(a[10]), "+r"(a[11]),
+                 "+r"(a[12]), "+r"(a[13]), "+r"(a[14]), "+r"(a[15]),
+                 "+r"(b[0]), "+r"(b[1]), "+r"(b[2]), "+r"(b[3]), "+r"(b[4]), "+r"(b[5]),
+                 "+r"(b[6]), "+r"(b[7]), "+r"(b[8]), "+r"(b[9]), "+r"(b[10]), "+r"(b[11]),
+                 "+r"(b[12]), "+r"(b[13]), "+r"(b[14]), "+r"(b[15])
                :
                : "memory");
 }
@@ -265,6 +281,38 @@ struct TensorBarriers {
   uint64_t s_full[2][2], p_full[2][2], pv_done[2][2];  // by stream and buffer
 };
 
+// This thread's 16-byte chunks of the 128 rows from row r0 of Q into a tile,
+// kThreads threads taking part; rows past the last live one become zero. One division:
+// from row to row the pointer moves by a constant, but for a node's last head.
+template <typename T, int kDim, int kThreads>
+__device__ __forceinline__ void copy_q(const TreeParams &p, int b, int kh, int r0, int live,
+                                       unsigned char *tile, int thread) {
+  constexpr int chunks = kDim / 8, step = kThreads / chunks;
+  static_assert(step % 8 == 0, "a thread's rows have one place in the swizzle");
+  const int D = p.head_dim, G = p.groups, c = thread % chunks, r = thread / chunks;
+  int left = c * 8 < D ? live - (r0 + r) : 0;  // rows to the last live one
+  const int t = (r0 + r) / G, skip = step / G;
+  int g = r0 + r - t * G;
+  const T *from = static_cast<const T *>(p.query) + b * p.q_batch_stride +
+                  t * p.q_node_stride + (int64_t)(kh * G + g) * D + c * 8;
+  const int64_t stride = skip * p.q_node_stride + (int64_t)(step - skip * G) * D;
+  const int64_t wrap = p.q_node_stride - (int64_t)G * D;
+  const int rest = step - skip * G;
+  uint32_t to = smem_addr(tile + place<kDim>(r, c));
+#pragma unroll
+  for (int i = 0; i < kTile / step; ++i) {
+    tree_cp_async16(to, left > 0 ? from : static_cast<const T *>(p.query), left > 0);
+    left -= step;
+    to += step / 8 * TensorShape<kDim>::atom;
+    from += stride;
+    g += rest;
+    if (g >= G) {
+      g -= G;
+      from += wrap;
+    }
+  }
+}
+
 template <typename T, int kDim>
 __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreeParams p, const __grid_constant__ CUtensorMap map, bool tiled) {
   using Shape = TensorShape<kDim>;
@@ -273,7 +321,8 @@ __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreePara
   __shared__ __align__(8) uint16_t s_cached[kMarks][kLoadWarps / 2];  // keys that are cache rows
   __shared__ uint32_t s_tmem;
   __shared__ unsigned long long s_bad;  // nodes whose V held a non-finite element
-  __shared__ float2 s_stats[kTile];
+  __shared__ float2 s_stats[2][kTile];
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
   unsigned char *smem = reinterpret_cast<unsigned char *>(
       (reinterpret_cast<uintptr_t>(tensor_smem) + 1023) & ~(uintptr_t)1023);
   const int tid = threadIdx.x, lane = tid & 31, split = blockIdx.y;
@@ -310,6 +359,8 @@ __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreePara
   // live rows of each stream's tile; a warp without any only takes part in barriers
   const int live0 = min(kTile, live - r0);
   const int live1 = apart ? max(0, min(kTile, live - r0 - kTile)) : live0;
+  if (tid == 32 * kSoftmaxWarps)
+    asm volatile("prefetch.tensormap [%0];\n" ::"l"(&map) : "memory");
   if (tid == 32 * kScoreWarp) {
     for (int i = 0; i < kMaxStages; ++i) {
       mbar_init(&bar.k_full[i], kLoadWarps / 2 * (32 + 1));
@@ -448,19 +499,12 @@ __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreePara
     asm volatile("cp.async.wait_all;\n" ::: "memory");
   } else {
     if (warp < kSoftmaxWarps) {
-      // Q into both streams' tiles (one tile when they share it), dead rows zero
-      const T *query = static_cast<const T *>(p.query) + b * p.q_batch_stride;
-      constexpr int chunks = kDim / 8, step = 32 * kSoftmaxWarps / chunks;
-      const int c = tid % chunks;
-#pragma unroll 4
-      for (int r = tid / chunks; r < p.tile_rows; r += step) {
-        const int row = r0 + r, t = row / G;
-        const bool in = row < live && c * 8 < D;
-        tree_cp_async16(
-            smem_addr(smem + r / kTile * Shape::q_bytes + place<kDim>(r % kTile, c)),
-            in ? query + t * p.q_node_stride + (int64_t)(kh * G + row - t * G) * D + c * 8 : query,
-            in);
-      }
+      // Q into both streams' tiles (one tile when they share it)
+      if (apart)
+        copy_q<T, kDim, kTile>(p, b, kh, r0 + tid / kTile * kTile, live,
+                               smem + tid / kTile * Shape::q_bytes, tid % kTile);
+      else
+        copy_q<T, kDim, 2 * kTile>(p, b, kh, r0, live, smem, tid);
       asm volatile("cp.async.wait_all;\n" ::: "memory");
       fence_async_proxy();
     } else if (warp == kOutputWarp) {
@@ -522,7 +566,8 @@ __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreePara
 #pragma unroll 1
             for (int c = 0; c < kDim; c += 16) {
               uint32_t o[16];
-              tmem_load16_wait(o, lanes + c);
+              tmem_load16(o, lanes + c);
+              tmem_load16_done(o);
 #pragma unroll
               for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
               tmem_store16(lanes + c, o);
@@ -568,91 +613,80 @@ __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreePara
       __syncwarp();
       fence_after();
       // With both streams' last products done the rings' memory is free: a row of
-      // fp32 for each query row, so that rows leave in whole lines.
+      // fp32 for each query row, so that rows leave in whole lines. Streams of the same
+      // rows have the other's output in their own lanes, and write half the elements each.
+      s_stats[w][r] = here && mine > 0 ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
       asm volatile("bar.sync 1, %0;\n" ::"n"(32 * kSoftmaxWarps) : "memory");
       constexpr int pitch = Shape::join_pitch;
-      float *stage = reinterpret_cast<float *>(k_ring) + (apart ? w * kTile * pitch : 0);
-      float *own = stage + r * pitch;
+      float *stage = reinterpret_cast<float *>(k_ring) +
+                     ((apart ? w * kTile : 0) + quarter * 32) * pitch;
+      const int d0 = apart ? 0 : w * (kDim / 2), dn = apart ? kDim : kDim / 2;
+      const bool other_mine = !apart && (w == 0 ? blocks > 1 : true);  // it had a block
+      const bool alive = here && r < live_here;
+      float f = 1.f, g = 0.f;  // weights of this stream's output and the other's
       if (!apart) {
-        if (w == 1 && here) {
-          s_stats[r] = make_float2(m, l);
-#pragma unroll 1
-          for (int c = 0; c < kDim; c += 16) {
-            uint32_t o[16];
-            tmem_load16_wait(o, lanes + c);
-#pragma unroll
-            for (int i = 0; i < 16; i += 4)
-              *reinterpret_cast<uint4 *>(own + c + i) =
-                  mine > 0 ? make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]) : make_uint4(0, 0, 0, 0);
-          }
-        }
-        asm volatile("bar.sync 1, %0;\n" ::"n"(32 * kSoftmaxWarps) : "memory");
+        const float2 other = s_stats[w ^ 1][r];
+        const float to = fmaxf(m, other.x);
+        f = m == -INFINITY ? 0.f : tree_exp2(m - to);
+        g = other.x == -INFINITY ? 0.f : tree_exp2(other.x - to);
+        // a sum of NaN scores has no maximum: let it through
+        l = (m == -INFINITY ? l : l * f) + (other.x == -INFINITY ? other.y : other.y * g);
+        m = to;
       }
-      if (apart || w == 0) {
-        float f = 1.f, g = 0.f;
-        if (!apart && here) {
-          const float2 other = s_stats[r];
-          const float to = fmaxf(m, other.x);
-          f = m == -INFINITY ? 0.f : tree_exp2(m - to);
-          g = other.x == -INFINITY ? 0.f : tree_exp2(other.x - to);
-          // a sum of NaN scores has no maximum: let it through
-          l = (m == -INFINITY ? l : l * f) + (other.x == -INFINITY ? other.y : other.y * g);
-          m = to;
-        }
-        const bool alive = here && r < live_here;
-        if (!alive) l = 0.f;
-        // with one split the result itself, with more the unnormalised output
-        const float scale = p.splits > 1 ? 1.f : l > 0.f || l != l ? 1.f / l : 0.f;
+      if (!alive) l = 0.f;
+      if (p.splits == 1) {  // the result itself; otherwise the unnormalised output
+        const float scale = l > 0.f || l != l ? 1.f / l : 0.f;
         f *= scale;
         g *= scale;
-        if (here) {
-          const uint64_t bad = alive ? s_bad & see : 0;
-#pragma unroll 1
-          for (int c = 0; c < kDim; c += 16) {
-            uint32_t o[16];
-            __syncwarp();
-            tmem_load16_wait(o, lanes + c);
-#pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-              float4 x = make_float4(__uint_as_float(o[i]) * f, __uint_as_float(o[i + 1]) * f,
-                                     __uint_as_float(o[i + 2]) * f, __uint_as_float(o[i + 3]) * f);
-              if (!apart) {
-                const float4 y = *reinterpret_cast<const float4 *>(own + c + i);
-                x.x = fmaf(g, y.x, x.x);
-                x.y = fmaf(g, y.y, x.y);
-                x.z = fmaf(g, y.z, x.z);
-                x.w = fmaf(g, y.w, x.w);
-              }
-              *reinterpret_cast<float4 *>(own + c + i) = x;
-            }
-          }
-          if (bad != 0)
-            for (int d = 0; d < D; ++d) own[d] += nonfinite_sum<T>(p, b, kh, d, bad);
-        }
-        __syncwarp();
-        // the warp's 32 rows, four elements a lane
-        const int first = row - lane, rows_here = max(0, min(32, all - first));
-        const unsigned alive_rows = __ballot_sync(kFullMask, alive);
-        const int d = 4 * lane;
-        // lane i knows where row i goes: its partial number or its offset in `out`
-        const int64_t number = row < all ? partial_number(p, b, kh, row, split) : 0;
-        const int64_t place_of = p.splits > 1 ? number * D : row < all ? out_offset(p, b, kh, row) : 0;
-        const float *from = stage + quarter * 32 * pitch + d;
-#pragma unroll 8
-        for (int i = 0; i < 32; ++i) {
-          const int64_t to = __shfl_sync(kFullMask, place_of, i) + d;
-          if (i >= rows_here || d >= D) continue;
-          float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (alive_rows >> i & 1) x = *reinterpret_cast<const float4 *>(from + i * pitch);
-          if (p.splits > 1)
-            *reinterpret_cast<float4 *>(p.partials + to) = x;
-          else
-            *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + to) =
-                make_uint2(pack2<T>(x.x, x.y), pack2<T>(x.z, x.w));
-        }
-        if (p.splits > 1 && row < all)
-          p.stats[number] = make_float2(alive ? m : -INFINITY, l);
       }
+      if (here) {
+        const uint64_t bad = alive ? s_bad & see : 0;
+        float *own = stage + lane * pitch;
+#pragma unroll 2
+        for (int c = d0; c < d0 + dn; c += 16) {
+          uint32_t x[16], y[16];
+          __syncwarp();
+          tmem_load16(x, lanes + c);
+          tmem_load16(y, (apart ? lanes : lanes ^ kStreamColumns) + c);
+          tmem_load16_done(x, y);
+#pragma unroll
+          for (int i = 0; i < 16; i += 4) {
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              // a stream without a block left nothing in its columns
+              v[e] = mine > 0 ? __uint_as_float(x[i + e]) * f : 0.f;
+              if (other_mine) v[e] = fmaf(g, __uint_as_float(y[i + e]), v[e]);
+            }
+            *reinterpret_cast<float4 *>(own + c + i) = make_float4(v[0], v[1], v[2], v[3]);
+          }
+        }
+        if (bad != 0)
+          for (int d = d0; d < min(D, d0 + dn); ++d)
+            own[d] += nonfinite_sum<T>(p, b, kh, d, bad);
+      }
+      __syncwarp();
+      // The warp's 32 rows, four elements a lane, several rows at once. Lane i knows where
+      // row i goes: its partial number or its offset in `out`.
+      const int first = row - lane, rows_here = max(0, min(32, all - first));
+      const unsigned alive_rows = __ballot_sync(kFullMask, alive);
+      const int64_t number = row < all ? partial_number(p, b, kh, row, split) : 0;
+      const int64_t place_of = p.splits > 1 ? number * D : row < all ? out_offset(p, b, kh, row) : 0;
+      const int lanes_of = dn / 4, d = d0 + lane % lanes_of * 4;
+#pragma unroll 4
+      for (int i = lane / lanes_of; i < 32; i += 32 / lanes_of) {
+        const int64_t to = __shfl_sync(kFullMask, place_of, i) + d;
+        if (i >= rows_here || d >= D) continue;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (alive_rows >> i & 1) x = *reinterpret_cast<const float4 *>(stage + i * pitch + d);
+        if (p.splits > 1)
+          *reinterpret_cast<float4 *>(p.partials + to) = x;
+        else
+          *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + to) =
+              make_uint2(pack2<T>(x.x, x.y), pack2<T>(x.z, x.w));
+      }
+      if (p.splits > 1 && row < all && (apart || w == 0))
+        p.stats[number] = make_float2(alive ? m : -INFINITY, l);
     } else if (warp == kScoreWarp) {
       // ---- S = Q K^T ------------------------------------------------------------------
       // The whole warp walks the items, so that addresses stay in uniform registers;
