@@ -310,7 +310,7 @@ TreeShape tree_shape(int batch, int nodes, int q_heads, int kv_heads, int head_d
   }
   s.keys = 64;
   // The split count with the least (rounds of blocks) x (keys of a block and what a
-  // block costs besides, about 128 keys); more splits than two tiles each are not
+  // block costs besides, as much as about 384 keys); more splits than two tiles each are not
   // worth joining.
   const int64_t blocks = (int64_t)batch * kv_heads * ceil_div(queries, s.rows);
   const int64_t places = (int64_t)s.resident * sm_count(), total = count + nodes;
@@ -319,7 +319,7 @@ TreeShape tree_shape(int batch, int nodes, int q_heads, int kv_heads, int head_d
   for (int n = 1; n <= kTreeMaxSplits; ++n) {
     const int64_t part = ceil_div(ceil_div(total, n), s.keys) * s.keys;
     if (n > 1 && part < 2 * s.keys) break;
-    const int64_t cost = ceil_div(blocks * n, places) * (part + 128) + (n > 1 ? 64 : 0);
+    const int64_t cost = ceil_div(blocks * n, places) * (part + 384) + (n > 1 ? 64 : 0);
     if (n == 1 || cost < least) {
       least = cost;
       s.splits = n;

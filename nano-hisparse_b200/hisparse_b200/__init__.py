@@ -27,6 +27,7 @@ from .attention import row_attention
 from .batched import DecodeBatch
 from .cache import LayerTables, RowCache, RowLease
 from .config import ACTIVE_TAIL_PAGES, CacheConfig, CapacityError, HotConfig
+from .draft import PromptLookup
 from .logprobs import TokenLogprobs, token_logprobs
 from .norm_rope import qk_norm_rope, rope_frequencies
 from .row_index import LogicalTopK, RowPlan, resolve_rows
@@ -36,7 +37,7 @@ from .tree import attend_tree, tree_mask
 
 __all__ = [
     "ACTIVE_TAIL_PAGES", "CacheConfig", "CapacityError", "DecodeBatch", "HotConfig",
-    "LayerTables", "LogicalTopK", "MappedHost", "RowCache", "RowLease", "RowPlan", "Selection",
+    "LayerTables", "LogicalTopK", "MappedHost", "PromptLookup", "RowCache", "RowLease", "RowPlan", "Selection",
     "TokenLogprobs", "attend_rows", "attend_tree", "gather_rows", "qk_norm_rope",
     "quest_selection", "resolve_rows", "rope_frequencies", "row_attention", "token_logprobs",
     "tree_mask",

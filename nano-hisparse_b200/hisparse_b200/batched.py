@@ -227,6 +227,60 @@ class DecodeBatch:
         st.last_use.record(compute)
         return out
 
+    def layer_tree(self, layer: int, query, key, value, mask, nodes, positions, row_counts):
+        """Attention of a drafted tree of every request (``attend_tree``) over the
+        history rows that `positions` name: resolve, miss gather, then one pass
+        over the physical rows and the nodes' own key/value, on the batch's compute
+        stream. query [B, T, Hq, D], key/value [B, T, Hkv, D], mask int64 [B, T],
+        nodes int32 [B] (see attend_tree); positions int32 [B, width], -1 padded
+        behind row_counts int32 [B] leading ones. Returns [B, T, Hq, D]."""
+        from .tree import attend_tree
+
+        cfg, st, compute = self.config, self.layers[layer], self.compute
+        if torch.cuda.current_stream(self.device) != compute:
+            raise RuntimeError("DecodeBatch.layer_tree must run on the batch's compute stream")
+        if query.ndim != 4 or query.shape[0] != self.batch or query.shape[2] != self.q_heads:
+            raise ValueError("query must be [batch, nodes, q_heads, head_dim]")
+        if (positions.shape != (self.batch, self.width) or positions.dtype != torch.int32
+                or positions.device != self.device or not positions.is_contiguous()):
+            raise ValueError("positions must be a contiguous int32 [batch, width] tensor "
+                             "on the batch's device")
+        if st.ready is not None:
+            compute.wait_event(st.ready)
+        self._resolve_and_gather(layer, positions.data_ptr(), st.counts)
+        compute.wait_event(st.ready)
+        out = attend_tree(query, key, value, mask, self.cache.pool, self.physical, cfg,
+                          counts=row_counts, nodes=nodes)
+        st.last_use = torch.cuda.Event()
+        st.last_use.record(compute)
+        return out
+
+    def _resolve_and_gather(self, layer, positions, counts):
+        """The resolver on the compute stream, then the miss gather on the transfer
+        stream; st.ready is recorded behind the gather."""
+        cache, cfg, st, lib = self.cache, self.config, self.layers[layer], _lib.load()
+        compute, transfer, status = self.compute, self.transfer, self.status.data_ptr()
+        b = self.batch
+        _lib.check(lib.hs_resolve_rows_batched(
+            b, positions, self.width, st.src_ptrs.data_ptr(), st.res_ptrs.data_ptr(),
+            st.table_pages, st.hot_ptrs.data_ptr(), cache.hot_blocks, st.tag_ptrs.data_ptr(),
+            st.lru_ptrs.data_ptr(), self.hot_rows, st.lengths.data_ptr(), cfg.page_size,
+            self.physical.data_ptr(), self.miss_host.data_ptr(), self.miss_device.data_ptr(),
+            counts.data_ptr(), None, _lib.ptr(self.resolve_ws), self.resolve_ws_bytes, status,
+            compute.cuda_stream))
+        resolved = torch.cuda.Event()
+        resolved.record(compute)
+        transfer.wait_event(resolved)
+        if st.last_use is not None:
+            transfer.wait_event(st.last_use)
+        _lib.check(lib.hs_gather_rows(
+            cache.mapped.data_ptr(), cache.host.shape[0], cache.pool.data_ptr(),
+            cache.pool.shape[0], self.miss_host.data_ptr(), self.miss_device.data_ptr(),
+            b * self.width, self.width, cfg.page_size, self._row_bytes, status,
+            transfer.cuda_stream))
+        st.ready = torch.cuda.Event()
+        st.ready.record(transfer)
+
     def exchange(self):
         """All-gather of the partial scores over the group, on the current
         stream (nothing without a group)."""

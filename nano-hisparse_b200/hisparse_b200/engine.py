@@ -32,6 +32,15 @@ and older pages stay resident while the pool has unreserved blocks
 (borrowed, revoked when an admission needs them). Placement decides only
 where rows are read from; the selected rows and their values, and so the
 tokens, do not depend on it.
+
+Beyond the reference: models whose query and key heads are normalised before
+the rotation (``DecoderConfig.qk_norm``, through ``qk_norm_rope``); the log
+probability, entropy and alternatives of every emitted token (``logprobs``,
+through ``token_logprobs``); and drafted decoding (``drafter``): a request's
+turn checks a small tree of drafted tokens in one forward, whose nodes attend
+over the request's rows and over each other (``attend_tree``), emits the
+longest drafted path that greedy decoding would have taken and one token
+more, and appends the accepted rows.
 """
 
 from __future__ import annotations
@@ -47,6 +56,10 @@ from .append import append_chunks
 from .batched import DecodeBatch
 from .cache import LayerTables, RowCache
 from .config import ACTIVE_TAIL_PAGES, CacheConfig, CapacityError, HotConfig
+from .draft import tree_of
+from .logprobs import token_logprobs
+from .norm_rope import qk_norm_rope, rope_frequencies
+from .tree import MAX_NODES, tree_mask
 
 
 @dataclass
@@ -61,11 +74,26 @@ class Request:
     decode_count: int = 0
     finished: bool = False
     cancelled: bool = False
+    # with BatchedEngine(logprobs=k): one TokenScore for each generated token
+    scores: list = field(default_factory=list)
+
+
+@dataclass(frozen=True)
+class TokenScore:
+    """What the model gave an emitted token: its log probability, the entropy of
+    the distribution it came from (nats) and the largest alternatives as
+    (token, log probability), largest first."""
+
+    logprob: float
+    entropy: float
+    top: tuple
 
 
 @dataclass
 class DecoderConfig:
-    """Dimensions of the Qwen2-shaped decoder (model.py:18-40), same fields."""
+    """Dimensions of the Qwen2-shaped decoder (model.py:18-40), same fields.
+    qk_norm: every query and key head is RMS-normalised, with a weight, before
+    the rotation (no counterpart in the reference model)."""
 
     vocab_size: int = 256
     hidden_size: int = 128
@@ -75,6 +103,7 @@ class DecoderConfig:
     num_key_value_heads: int = 2
     rms_norm_eps: float = 1e-6
     rope_theta: float = 10000.0
+    qk_norm: bool = False
 
     @property
     def head_dim(self):
@@ -88,6 +117,11 @@ class DecoderConfig:
 
 _CONFIG_FIELDS = ("vocab_size", "hidden_size", "intermediate_size", "num_hidden_layers",
                   "num_attention_heads", "num_key_value_heads", "rms_norm_eps", "rope_theta")
+
+
+def _norm_keys(i):
+    base = f"model.layers.{i}.self_attn."
+    return {"q_norm": base + "q_norm.weight", "k_norm": base + "k_norm.weight"}
 
 
 def _layer_keys(i):
@@ -134,7 +168,11 @@ class DecoderWeights:
                 "gate_up_w": torch.cat((w["gate_w"], w["up_w"])).contiguous(),
                 "down_w": w["down_w"],
             })
+            if config.qk_norm:
+                self.layers[-1].update({name: get(k) for name, k in _norm_keys(i).items()})
         cfg = config
+        if cfg.qk_norm:
+            self.rope = rope_frequencies(cfg.head_dim, cfg.rope_theta, self.device)
         self.inv_freq = cfg.rope_theta ** (
             -torch.arange(0, cfg.head_dim, 2, device=self.device).float() / cfg.head_dim)
 
@@ -142,7 +180,8 @@ class DecoderWeights:
     def from_model(cls, model, device=None, dtype=None):
         """From a reference ``Model`` (or any module with its state_dict names
         and a config carrying the DecoderConfig fields)."""
-        cfg = DecoderConfig(**{name: getattr(model.config, name) for name in _CONFIG_FIELDS})
+        cfg = DecoderConfig(**{name: getattr(model.config, name) for name in _CONFIG_FIELDS},
+                            qk_norm=getattr(model.config, "qk_norm", False))
         return cls(cfg, model.state_dict(), device, dtype)
 
     @classmethod
@@ -175,6 +214,9 @@ class DecoderWeights:
             state[key["up_w"]] = uniform((cfg.intermediate_size, h), pow2_scale(h))
             state[key["down_w"]] = uniform((h, cfg.intermediate_size),
                                            pow2_scale(cfg.intermediate_size))
+            if cfg.qk_norm:
+                for k in _norm_keys(i).values():
+                    state[k] = 1.0 + uniform((cfg.head_dim,), 1 / 8)
         state["model.norm.weight"] = 1.0 + uniform((h,), 1 / 8)
         state["lm_head.weight"] = uniform((cfg.vocab_size, h), pow2_scale(h))
         return cls(cfg, state, device, dtype)
@@ -195,6 +237,8 @@ class DecoderWeights:
                         key["q_w"]: q_w, key["k_w"]: k_w, key["v_w"]: v_w, key["q_b"]: q_b,
                         key["k_b"]: k_b, key["v_b"]: v_b, key["o_w"]: w["o_w"],
                         key["gate_w"]: gate, key["up_w"]: up, key["down_w"]: w["down_w"]})
+            if cfg.qk_norm:
+                out.update({k: w[name] for name, k in _norm_keys(i).items()})
         return {k: v.detach().float().cpu().contiguous() for k, v in out.items()}
 
     # -- the dense math of model.py:45-179, batched over rows ------------------------
@@ -205,14 +249,19 @@ class DecoderWeights:
         return normalized.to(x.dtype) * weight
 
     def project(self, layer, x, positions):
-        """model.py:136-155 for rows x [N, hidden] at float positions [N]:
-        returns q [N, Hq, D], k and v [N, Hkv, D], RoPE applied to q and k."""
+        """model.py:136-155 for rows x [N, hidden] at float positions [N] (with
+        qk_norm: integer positions, on a CUDA device): returns q [N, Hq, D], k
+        and v [N, Hkv, D], RoPE (and the head norms) applied to q and k."""
         cfg, w = self.config, self.layers[layer]
         n, d = x.shape[0], cfg.head_dim
         h = self.rms_norm(x, w["input_norm"])
         qkv = F.linear(h, w["qkv_w"], w["qkv_b"])
         hq, hkv = cfg.num_attention_heads, cfg.num_key_value_heads
         q, k, v = qkv.split((hq * d, hkv * d, hkv * d), dim=-1)
+        if cfg.qk_norm:
+            q, k = qk_norm_rope(q.unflatten(-1, (hq, d)), k.unflatten(-1, (hkv, d)), positions,
+                                self.rope, w["q_norm"], w["k_norm"], eps=cfg.rms_norm_eps)
+            return q, k, v.reshape(n, hkv, d)
         q, k, v = q.view(n, hq, d), k.view(n, hkv, d), v.reshape(n, hkv, d)
         angles = positions[:, None] * self.inv_freq[None, :]
         angles = torch.cat((angles, angles), -1)[:, None, :]
@@ -231,9 +280,17 @@ class DecoderWeights:
         gate, up = F.linear(self.rms_norm(x, w["post_norm"]), w["gate_up_w"]).chunk(2, -1)
         return x + F.linear(F.silu(gate) * up, w["down_w"])
 
+    def positions(self, positions):
+        """Integer positions [N] in the form that ``project`` takes."""
+        return positions if self.config.qk_norm else positions.float()
+
+    def head(self, x):
+        """Logits of rows x [N, hidden] in the model's dtype."""
+        return F.linear(self.rms_norm(x, self.norm), self.lm_head)
+
     def logits(self, x):
         """model.py:179 / 221: fp32 logits of rows x [N, hidden]."""
-        return F.linear(self.rms_norm(x, self.norm), self.lm_head).float()
+        return self.head(x).float()
 
 
 def _staged(values: torch.Tensor, device) -> torch.Tensor:
@@ -499,6 +556,39 @@ class ServingCache:
         return (staged[5 * L * B:5 * L * B + B], ints[:B], ints[B:2 * B], ints[2 * B:3 * B],
                 staged[:5 * L * B].view(5, L, B))
 
+    def plan_append(self, request_ids, counts):
+        """Stages the append of counts[b] >= 1 rows at the end of each request's
+        history, within one page each (a step that crosses pages appends page by
+        page): returns (within int32 [B], count int32 [B], meta int64 [5, L, B])
+        as plan_decode does."""
+        import numpy as np
+
+        P, B = self.config.page_size, len(request_ids)
+        L = self.requests[request_ids[0]].layers
+        words = np.empty(5 * L * B + B, dtype=np.int64)
+        meta, halves = words[:5 * L * B].reshape(5, L, B), words[5 * L * B:].view(np.int32)
+        updates = []
+        for b, (request_id, rows) in enumerate(zip(request_ids, counts)):
+            res = self.requests[request_id]
+            if res.length + rows > res.max_tokens:
+                raise CapacityError("request exceeds its reserved host capacity")
+            page, within = divmod(res.length, P)
+            if not 1 <= rows <= P - within:
+                raise ValueError("append chunk leaves its page")
+            for layer in range(L):
+                if within == 0:
+                    self._enter_tail(res, layer, page, updates)
+                meta[0, layer, b] = res.tail[layer, page % ACTIVE_TAIL_PAGES]
+                meta[1, layer, b] = res.host[layer, page]
+                meta[2, layer, b], meta[3, layer, b], meta[4, layer, b] = self._pointers(
+                    res, layer, page)
+            halves[b], halves[B + b] = within, rows
+        with torch.cuda.stream(self.compute):
+            self._apply(updates)
+            staged = _staged(torch.from_numpy(words), self.device)
+        ints = staged[5 * L * B:].view(torch.int32)
+        return ints[:B], ints[B:], staged[:5 * L * B].view(5, L, B)
+
     def append(self, layer, k, v, within, count, meta, mapped=True):
         """One append launch for `layer`: chunk b of k/v [B, T, Hkv, D] goes
         where plan_prompt / plan_decode staged it."""
@@ -574,10 +664,22 @@ class BatchedEngine:
     reference's quest_selection top_pages, sink and tail pages included), or
     None for the full causal history. backend is accepted for signature
     parity; every path runs libhisparse. selector: "quest" only (the mean
-    indexer of selection.py:127 is not part of this path)."""
+    indexer of selection.py:127 is not part of this path).
+
+    logprobs: None, or how many alternatives (0 to 32) to keep with the log
+    probability and entropy of every emitted token, in ``Request.scores``.
+
+    drafter: None, or an object whose ``propose(tokens, limit)`` returns a tree
+    of likely continuations of a token list as (token, parent) pairs, parents
+    first, -1 for a child of the last token, at most `limit` of them
+    (``hisparse_b200.PromptLookup`` drafts from the request's own text). A
+    request's turn then emits one or more tokens, those that greedy decoding
+    would emit one by one. Needs the full causal history (top_k=None): with a
+    page budget every token selects its own pages."""
 
     def __init__(self, model, cache: ServingCache, top_k=None, backend="auto",
-                 eos_token_id: int | None = None, selector: str = "quest"):
+                 eos_token_id: int | None = None, selector: str = "quest",
+                 logprobs: int | None = None, drafter=None):
         weights = model if isinstance(model, DecoderWeights) else DecoderWeights.from_model(model)
         cfg, kv = weights.config, cache.config
         if (cfg.num_key_value_heads, cfg.head_dim) != (kv.kv_heads, kv.head_dim):
@@ -588,6 +690,12 @@ class BatchedEngine:
             raise ValueError("top_k must be positive or None")
         if selector != "quest":
             raise ValueError("selector must be quest")
+        if logprobs is not None and not 0 <= logprobs <= min(32, cfg.vocab_size):
+            raise ValueError("logprobs must be None or between 0 and 32")
+        if drafter is not None and top_k is not None:
+            raise ValueError("drafted decoding reads the full history: top_k must be None")
+        self.logprobs, self.drafter = logprobs, drafter
+        self.draft_stats = {"steps": 0, "drafted": 0, "accepted": 0}
         self.model, self.cache, self.top_k, self.backend = weights, cache, top_k, backend
         self.eos_token_id, self.selector = eos_token_id, selector
         self.requests: dict[str, Request] = {}
@@ -658,10 +766,15 @@ class BatchedEngine:
                     self.running.append(request)
         batch = list(self.running)
         if batch:
-            tokens = self._decode(batch)
-            for request, token in zip(batch, tokens):
+            trees = [self._draft(request) for request in batch] if self.drafter else None
+            if trees and any(trees):
+                turns = self._decode_drafted(batch, trees)
+            else:
+                turns = [[token] for token in self._decode(batch)]
+            for request, tokens in zip(batch, turns):
                 request.decode_count += 1
-                emitted.append((request.request_id, self._emit(request, token)))
+                for token in tokens:
+                    emitted.append((request.request_id, self._emit(request, token)))
             self.running = deque(r for r in batch if not r.finished)
         return emitted
 
@@ -694,7 +807,7 @@ class BatchedEngine:
         with torch.cuda.stream(cache.compute):
             within, count, meta = cache.plan_prompt(request.request_id, n)
             x = F.embedding(torch.tensor(request.prompt, device=w.device), w.embed)
-            positions = torch.arange(n, device=w.device).float()
+            positions = w.positions(torch.arange(n, device=w.device))
             pad = pages * P - n
             for layer in range(cfg.num_hidden_layers):
                 q, k, v = w.project(layer, x, positions)
@@ -706,9 +819,132 @@ class BatchedEngine:
                     v.repeat_interleave(groups, 1).transpose(0, 1), is_causal=True,
                 ).transpose(0, 1)
                 x = w.finish(layer, x, attention)
-            token = int(w.logits(x[-1:])[0].argmax().item())
+            token = int(self._choose([request], x[-1:])[0])
         cache.advance(request.request_id, n)
         return token
+
+    def _choose(self, requests, x):
+        """The greedy token of each row of x (one a request), and its score."""
+        w = self.model
+        if self.logprobs is None:
+            return w.logits(x).argmax(-1).cpu().tolist()
+        logits = w.head(x)
+        tokens = logits.float().argmax(-1)
+        scores = token_logprobs(logits, tokens, top=self.logprobs)
+        tokens, *scores = (t.cpu().tolist() for t in (tokens, *scores))
+        for request, *score in zip(requests, *scores):
+            self._score(request, *score)
+        return tokens
+
+    def _score(self, request, logprob, entropy, top_logprobs, top_tokens):
+        request.scores.append(TokenScore(logprob, entropy, tuple(zip(top_tokens, top_logprobs))))
+
+    # -- drafted decoding -----------------------------------------------------------
+    def _draft(self, request):
+        """The drafted tree of a request's next turn as (token, parent) pairs; node
+        0 of the step is its last token, so parents are counted from there."""
+        left = request.max_new_tokens - len(request.generated) - 1  # beyond the sure token
+        if left < 1:
+            return []
+        limit = MAX_NODES - 1
+        drafted = list(self.drafter.propose(request.prompt + request.generated, limit))
+        return tree_of(drafted, limit, left, self.model.config.vocab_size)
+
+    @torch.inference_mode()
+    def _decode_drafted(self, requests, trees):
+        """One turn of every running request over its drafted tree: returns the
+        emitted tokens of each. Row t of request b is node t; the history stays
+        as it was until the accepted rows are appended."""
+        w, cache, cfg = self.model, self.cache, self.model.config
+        ids = [r.request_id for r in requests]
+        batch = self._decode_batch(ids)
+        nodes = [1 + len(tree) for tree in trees]
+        b, width = len(ids), max(nodes)
+        parents = [[-1] + [parent + 1 for _, parent in tree] for tree in trees]
+        tokens = torch.zeros((b, width), dtype=torch.int64)
+        positions = torch.zeros((b, width), dtype=torch.int64)
+        for i, (request, tree) in enumerate(zip(requests, trees)):
+            length, depth = cache.length(ids[i]), [0]
+            depth += [0] * len(tree)
+            tokens[i, 0] = request.generated[-1]
+            for t, (token, _) in enumerate(tree, 1):
+                tokens[i, t], depth[t] = token, depth[parents[i][t]] + 1
+            positions[i, :nodes[i]] = length + torch.tensor(depth)
+        with torch.cuda.stream(cache.compute):
+            host = torch.cat((tokens.flatten(), positions.flatten(),
+                              tree_mask(parents, "cpu").flatten(),
+                              torch.tensor([cache.length(r) for r in ids] + nodes)))
+            staged = _staged(host, cache.device)
+            n = b * width
+            mask, ints = staged[2 * n:3 * n].view(b, width), staged[3 * n:].to(torch.int32)
+            lengths, counts = ints[:b], ints[b:]
+            self._lengths.copy_(lengths)
+            x = F.embedding(staged[:n], w.embed)
+            at = w.positions(staged[n:2 * n])
+            selected = self._history(batch, lengths)
+            kept = []
+            for layer in range(cfg.num_hidden_layers):
+                q, k, v = w.project(layer, x, at)
+                kept.append((k, v))
+                attention = batch.layer_tree(
+                    layer, *(t.unflatten(0, (b, width)) for t in (q, k, v)), mask, counts,
+                    selected, lengths)
+                x = w.finish(layer, x, attention.flatten(0, 1))
+            cache.rows.row_stats.add_(batch.last_counts().sum((0, 1)))
+            scores = token_logprobs(w.head(x), top=max(1, self.logprobs or 0))
+            best = scores.top_tokens[:, 0].view(b, width).cpu().tolist()
+            if self.logprobs is not None:
+                _, entropy, top_logprobs, top_tokens = (t.cpu().tolist() for t in scores)
+        turns, paths = [], []
+        for i, (request, tree) in enumerate(zip(requests, trees)):
+            node, turn, path = 0, [], []
+            while True:
+                token = best[i][node]
+                turn.append(token)
+                path.append(node)
+                if self.logprobs is not None:
+                    row = i * width + node
+                    self._score(request, top_logprobs[row][0], entropy[row],
+                                top_logprobs[row][:self.logprobs], top_tokens[row][:self.logprobs])
+                if token == self.eos_token_id or \
+                        len(request.generated) + len(turn) >= request.max_new_tokens:
+                    path = []  # the request ends here: its rows are not needed
+                    break
+                node = next((t for t in range(1, nodes[i])
+                             if parents[i][t] == node and tree[t - 1][0] == token), None)
+                if node is None:
+                    break
+            turns.append(turn)
+            paths.append(path)
+            self.draft_stats["drafted"] += len(tree)
+            self.draft_stats["accepted"] += len(turn) - 1
+        self.draft_stats["steps"] += 1
+        self._append_paths(ids, paths, kept, width)
+        return turns
+
+    def _append_paths(self, ids, paths, kept, width):
+        """Appends the K/V rows of each request's accepted nodes (`kept`: every
+        layer's (k, v) of all nodes), one page of each request at a time."""
+        cache, page = self.cache, self.cache.config.page_size
+        done = [0] * len(ids)
+        while True:
+            todo = [i for i, path in enumerate(paths) if done[i] < len(path)]
+            if not todo:
+                return
+            names = [ids[i] for i in todo]
+            counts = [min(len(paths[i]) - done[i], page - cache.length(ids[i]) % page)
+                      for i in todo]
+            rows = torch.zeros((len(todo), max(counts)), dtype=torch.int64)
+            for j, (i, count) in enumerate(zip(todo, counts)):
+                rows[j, :count] = i * width + torch.tensor(paths[i][done[i]:done[i] + count])
+                done[i] += count
+            with torch.cuda.stream(cache.compute):
+                within, count, meta = cache.plan_append(names, counts)
+                index = _staged(rows, cache.device)
+                for layer, (k, v) in enumerate(kept):
+                    cache.append(layer, k[index], v[index], within, count, meta)
+            for name, count in zip(names, counts):
+                cache.advance(name, count)
 
     def _decode_batch(self, ids):
         """The DecodeBatch of the running set, rebuilt when the set changes."""
@@ -738,20 +974,23 @@ class BatchedEngine:
                 ids, [r.generated[-1] for r in requests])
             self._lengths.copy_(lengths)
             x = F.embedding(tokens, w.embed)
-            positions = (lengths - 1).float()
+            positions = w.positions(lengths - 1)
             selected = None
             if self.top_k is None:  # the full causal history (selection.py:127-135)
-                width = batch.width
-                ar = torch.arange(width, dtype=torch.int32, device=cache.device)
-                selected = torch.where(ar[None, :] < lengths[:, None], ar[None, :],
-                                       torch.full_like(ar[None, :], -1)).contiguous()
+                selected = self._history(batch, lengths)
             for layer in range(cfg.num_hidden_layers):
                 q, k, v = w.project(layer, x, positions)
                 cache.append(layer, k.unsqueeze(1), v.unsqueeze(1), within, count, meta)
                 attention = batch.layer(layer, q.contiguous(), positions=selected)
                 x = w.finish(layer, x, attention)
             cache.rows.row_stats.add_(batch.last_counts().sum((0, 1)))
-            out = w.logits(x).argmax(-1).cpu()
+            out = self._choose(requests, x)
         for r in ids:
             cache.advance(r, 1)
-        return out.tolist()
+        return out
+
+    @staticmethod
+    def _history(batch, lengths):
+        """int32 [B, width]: every position below each request's length, then -1."""
+        ar = torch.arange(batch.width, dtype=torch.int32, device=lengths.device)[None, :]
+        return torch.where(ar < lengths[:, None], ar, torch.full_like(ar, -1)).contiguous()
