@@ -6,13 +6,13 @@
 // exp(-d) (t - d s). So one pass over the logits gives all of it, and the work is
 // bound by reading them once.
 //
-// The alternatives come out of the same pass: every thread keeps the order key
-// of its best entry. The r-th best key of each warp, r = ceil(top / warps), the
-// smallest of them over the warps, is passed by at least `top` entries of the
-// block's part, so every one of its `top` largest entries has a key of at least
-// that. Threads whose own best passes it (a few more than `top`) read their
-// entries again, from L2, and collect those that pass; the collected keys are
-// ranked by counting.
+// The alternatives come out of the same pass: every thread keeps its best entry. At
+// least `top` entries of the block's part reach the top-th best of the threads' best
+// values, so every one of its `top` largest entries does. Threads whose own best reaches
+// it (`top` of them, and equals) read their entries again and collect those that do; the
+// collected keys are ranked by counting. (A looser bound, the smallest of the warps'
+// best, is found in half the time, but made a fifth of the threads read again: half as
+// much traffic again on rows that L2 does not hold.)
 //
 // A row is split over a cluster of 1 to 8 blocks, which join their sums and their
 // best keys in the first block's shared memory: few rows reach many SMs without
@@ -118,15 +118,23 @@ struct Softmax {
     s += e;
     t = fmaf(e, fmaxf(d, kFar), t);
   }
-  __device__ __forceinline__ void join(float m2, float s2, float t2) {
-    const float top = max_nan(m, m2);
-    const float d1 = fmaxf(m - top, kFar), d2 = fmaxf(m2 - top, kFar);
-    const float f1 = m == -INFINITY ? 0.f : exp2f(d1 * kLog2e);
-    const float f2 = m2 == -INFINITY ? 0.f : exp2f(d2 * kLog2e);
-    t = (m == -INFINITY ? 0.f : f1 * fmaf(d1, s, t)) +
-        (m2 == -INFINITY ? 0.f : f2 * fmaf(d2, s2, t2));
-    s = f1 * s + f2 * s2;
+  // the sums over the warp's lanes, in every lane
+  __device__ __forceinline__ void join_warp() {
+    float top = m;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(kFullMask, top, o));
+    if (m != -INFINITY) {
+      const float d = fmaxf(m - top, kFar), f = exp2f(d * kLog2e);
+      t = f * fmaf(d, s, t);
+      s *= f;
+    }
     m = top;
+    s = warp_xor_tree_sum(s);
+    t = warp_xor_tree_sum(t);
+  }
+  // this lane's part as it was left in shared memory, or none
+  __device__ __forceinline__ static Softmax part(const float *from, bool there) {
+    return there ? Softmax{from[0], from[1], from[2]} : Softmax{-INFINITY, 0.f, 0.f};
   }
 };
 
@@ -140,7 +148,7 @@ __device__ __forceinline__ uint64_t warp_largest(uint64_t v) {
 }
 
 struct LogprobShared {
-  float m[kLogprobWarps], s[kLogprobWarps], t[kLogprobWarps];
+  float parts[kLogprobWarps][3];  // maximum and sums of each warp
   uint64_t warp_best[kLogprobWarps];
   uint64_t candidates[kCandidates];
   uint64_t best[kMaxTop];
@@ -175,13 +183,17 @@ template <typename T> struct RowPart {
   __device__ __forceinline__ uint32_t index(int v, int i) const {
     return (uint32_t)(head + (first + v) * n + i);
   }
+  // this thread's kAhead vectors from number v0 on
+  __device__ __forceinline__ void load(int v0, uint4 (&raw)[kAhead]) const {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (v0 + u * kLogprobThreads < count) raw[u] = vector(v0 + u * kLogprobThreads);
+  }
   // f(vector, its number) for this thread's vectors, kAhead loads at a time
   template <typename F> __device__ __forceinline__ void each(F f) const {
     for (int v0 = threadIdx.x; v0 < count; v0 += kAhead * kLogprobThreads) {
       uint4 raw[kAhead];
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u)
-        if (v0 + u * kLogprobThreads < count) raw[u] = vector(v0 + u * kLogprobThreads);
+      load(v0, raw);
 #pragma unroll
       for (int u = 0; u < kAhead; ++u)
         if (v0 + u * kLogprobThreads < count) f(raw[u], v0 + u * kLogprobThreads);
@@ -223,29 +235,22 @@ template <typename T>
 __device__ __forceinline__ void block_best(LogprobShared &sh, const RowPart<T> &part, int top,
                                            uint64_t mine, uint64_t bound) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int deep = (top + kLogprobWarps - 1) / kLogprobWarps;
-  uint64_t left = mine, nth = 0;
-  for (int i = 0; i < deep; ++i) {  // keys are distinct unless 0
-    nth = warp_largest(left);
-    if (left == nth) left = 0;
-  }
-  if (lane == 0) sh.warp_best[warp] = nth;
   if (threadIdx.x < kMaxTop) sh.best[threadIdx.x] = 0;
-  __syncthreads();
-  uint64_t threshold = sh.warp_best[0];
-  for (int w = 1; w < kLogprobWarps; ++w)
-    if (sh.warp_best[w] < threshold) threshold = sh.warp_best[w];
-  if (threshold == 0) threshold = 1;  // fewer entries than warps: all of them
+  // the largest value that the best entries of `top` threads reach, bit by bit
+  const auto search = [&](uint64_t known, int from, int to) {
+    for (int bit = from; bit >= to; --bit) {
+      const uint64_t trial = known | 1ull << bit;
+      if (__syncthreads_count(mine >= trial) >= top) known = trial;
+    }
+    return known;
+  };
+  uint64_t threshold = search(0, 63, 32);
+  if (threshold == 0) threshold = 1;  // fewer threads with entries than `top`: all of them
   int found = collect(sh, part, bound, threshold);
   if (found > kCandidates) {
-    // Many entries pass (equal values, or the largest ones in few threads): take
-    // the top-th best of the threads' keys, the largest key that `top` threads
-    // reach, bit by bit.
-    uint64_t exact = 0;
-    for (int bit = 63; bit >= 0; --bit) {
-      const uint64_t trial = exact | 1ull << bit;
-      if (__syncthreads_count(mine >= trial) >= top) exact = trial;
-    }
+    // Many entries have that value: those of lower index go first, which the rest of
+    // the key says.
+    const uint64_t exact = search(threshold >> 32 << 32, 31, 0);
     if (exact > threshold) {
       threshold = exact;
       found = collect(sh, part, bound, threshold);
@@ -299,11 +304,12 @@ __global__ void __launch_bounds__(kLogprobThreads, kLogprobBlocks)
 
   Softmax acc{-INFINITY, 0.f, 0.f};
   int at = -1;  // the vector that first held this thread's maximum
+  uint4 raw[kAhead], next[kAhead];
+  part.load(threadIdx.x, next);
   for (int v0 = threadIdx.x; v0 < part.count; v0 += kAhead * kLogprobThreads) {
-    uint4 raw[kAhead];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u)
-      if (v0 + u * kLogprobThreads < part.count) raw[u] = part.vector(v0 + u * kLogprobThreads);
+    for (int u = 0; u < kAhead; ++u) raw[u] = next[u];
+    part.load(v0 + kAhead * kLogprobThreads, next);  // while these are summed
     float largest = -INFINITY;
     int where = v0;
 #pragma unroll
@@ -346,26 +352,21 @@ __global__ void __launch_bounds__(kLogprobThreads, kLogprobBlocks)
       acc.add(e);
     }
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    acc.join(__shfl_xor_sync(kFullMask, acc.m, o), __shfl_xor_sync(kFullMask, acc.s, o),
-             __shfl_xor_sync(kFullMask, acc.t, o));
+  acc.join_warp();
   if (lane == 0) {
-    sh.m[warp] = acc.m;
-    sh.s[warp] = acc.s;
-    sh.t[warp] = acc.t;
+    sh.parts[warp][0] = acc.m;
+    sh.parts[warp][1] = acc.s;
+    sh.parts[warp][2] = acc.t;
   }
   if (p.top > 0) block_best(sh, part, p.top, mine, bound);
   else __syncthreads();
 
   if (cluster > 1) asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
   LogprobShared &out = *(cluster > 1 ? map_rank(&sh, 0) : &sh);
-  if (threadIdx.x == 0) {
-    acc = Softmax{sh.m[0], sh.s[0], sh.t[0]};
-    for (int w = 1; w < kLogprobWarps; ++w) acc.join(sh.m[w], sh.s[w], sh.t[w]);
-    out.joined[rank][0] = acc.m;
-    out.joined[rank][1] = acc.s;
-    out.joined[rank][2] = acc.t;
+  if (warp == 0) {
+    acc = Softmax::part(sh.parts[lane % kLogprobWarps], lane < kLogprobWarps);
+    acc.join_warp();
+    if (lane < 3) out.joined[rank][lane] = lane == 0 ? acc.m : lane == 1 ? acc.s : acc.t;
   }
   if (threadIdx.x < p.top) out.joined_best[rank * p.top + threadIdx.x] = sh.best[threadIdx.x];
   if (cluster > 1) {
@@ -375,9 +376,8 @@ __global__ void __launch_bounds__(kLogprobThreads, kLogprobBlocks)
     __syncthreads();
   }
 
-  acc = Softmax{sh.joined[0][0], sh.joined[0][1], sh.joined[0][2]};
-  for (int r = 1; r < cluster; ++r)
-    acc.join(sh.joined[r][0], sh.joined[r][1], sh.joined[r][2]);
+  acc = Softmax::part(sh.joined[lane % kMaxCluster], lane < cluster);
+  acc.join_warp();
   const bool empty = acc.m == -INFINITY;
   const float log_s = logf(acc.s);
   // (x - m) - log s: one rounding less than x - lse for entries near the maximum

@@ -34,8 +34,23 @@ template <int NJ> struct SimtShape {
       sizeof(float) * ((kSimtRows + 2 * kSimtKeys) * pitch + kSimtRows * kSimtPPitch);
 };
 
+// Elements d .. d + 3 of a row of head_dim D as fp32, zero past its end. `four`: one
+// vector load reads them (D a multiple of 4, addresses of the vector's size).
+template <typename T>
+__device__ __forceinline__ float4 load_four(const T *row, int d, int D, bool four) {
+  float x[4] = {0.f, 0.f, 0.f, 0.f};
+  if (four) {
+    if (d < D) load_f32<T, 4>(row + d, x, true);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (d + i < D) x[i] = to_f32(row[d + i]);
+  }
+  return make_float4(x[0], x[1], x[2], x[3]);
+}
+
 template <typename T, int NJ>
-__global__ void __launch_bounds__(kSimtThreads) tree_simt_kernel(TreeParams p) {
+__global__ void __launch_bounds__(kSimtThreads) tree_simt_kernel(TreeParams p, bool four) {
   using Shape = SimtShape<NJ>;
   constexpr int dim = Shape::dim, pitch = Shape::pitch;
   extern __shared__ __align__(16) float smem[];
@@ -54,12 +69,13 @@ __global__ void __launch_bounds__(kSimtThreads) tree_simt_kernel(TreeParams p) {
   const int tx = tid & 15, ty = tid >> 4;  // keys / elements; rows 4 ty .. 4 ty + 3
 
   const T *query = static_cast<const T *>(p.query) + b * p.q_batch_stride;
-  for (int i = tid; i < kSimtRows * dim; i += kSimtThreads) {
-    const int r = i / dim, d = i % dim, row = r0 + r;
-    sq[r * pitch + d] =
-        row < live && d < D
-            ? to_f32(query[row / G * p.q_node_stride + (kh * G + row % G) * (int64_t)D + d])
-            : 0.f;
+  constexpr int fours = dim / 4;  // a power of two or 48
+  for (int i = tid; i < kSimtRows * fours; i += kSimtThreads) {
+    const int r = i / fours, d = i % fours * 4, row = r0 + r, t = row / G;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (row < live)
+      x = load_four(query + t * p.q_node_stride + (kh * G + row - t * G) * (int64_t)D, d, D, four);
+    *reinterpret_cast<float4 *>(&sq[r * pitch + d]) = x;
   }
   if (tid < kSimtRows) {
     const int row = r0 + tid;
@@ -90,19 +106,19 @@ __global__ void __launch_bounds__(kSimtThreads) tree_simt_kernel(TreeParams p) {
                                : -2 - (i - valid);
     }
     __syncthreads();
-    for (int i = tid; i < kSimtKeys * dim; i += kSimtThreads) {
-      const int k = i / dim, d = i % dim;
+#pragma unroll 4
+    for (int i = tid; i < kSimtKeys * fours; i += kSimtThreads) {
+      const int k = i / fours, d = i % fours * 4;
       const int64_t src = s_src[k];
-      float kx = 0.f, vx = 0.f;
-      if (d < D && src >= 0) {
-        kx = to_f32(pool[src + d]);
-        vx = to_f32(pool[src + p.page_size * row_elems + d]);
-      } else if (d < D && src < -1) {
-        kx = to_f32(key[(-2 - src) * p.kv_node_stride + d]);
-        vx = to_f32(value[(-2 - src) * p.kv_node_stride + d]);
+      float4 kx = make_float4(0.f, 0.f, 0.f, 0.f), vx = kx;
+      if (src != -1) {
+        const T *kp = src >= 0 ? pool + src : key + (-2 - src) * p.kv_node_stride;
+        const T *vp = src >= 0 ? kp + p.page_size * row_elems : value + (-2 - src) * p.kv_node_stride;
+        kx = load_four(kp, d, D, four);
+        vx = load_four(vp, d, D, four);
       }
-      sk[k * pitch + d] = kx;
-      sv[k * pitch + d] = vx;
+      *reinterpret_cast<float4 *>(&sk[k * pitch + d]) = kx;
+      *reinterpret_cast<float4 *>(&sv[k * pitch + d]) = vx;
     }
     __syncthreads();
     float s[4][4];  // rows 4 ty + i, keys tx + 16 j
@@ -334,7 +350,15 @@ template <typename T, int NJ> int launch_simt(const TreeParams &p, cudaStream_t 
   if (int e = reserve_smem(reinterpret_cast<const void *>(kernel), bytes, "attend_tree")) return e;
   const int64_t tiles = ceil_div((int64_t)p.nodes * p.groups, kSimtRows);
   const dim3 grid((unsigned)p.splits, (unsigned)(p.kv_heads * tiles), (unsigned)p.batch);
-  kernel<<<grid, kSimtThreads, bytes, s>>>(p);
+  // one vector of four elements has an address of its own size
+  const uintptr_t addresses =
+      reinterpret_cast<uintptr_t>(p.query) | reinterpret_cast<uintptr_t>(p.key) |
+      reinterpret_cast<uintptr_t>(p.value) | reinterpret_cast<uintptr_t>(p.pool);
+  const int64_t strides =
+      p.q_batch_stride | p.q_node_stride | p.kv_batch_stride | p.kv_node_stride;
+  const bool four =
+      p.head_dim % 4 == 0 && addresses % (4 * sizeof(T)) == 0 && strides % 4 == 0;
+  kernel<<<grid, kSimtThreads, bytes, s>>>(p, four);
   return check_launch("tree_simt_kernel");
 }
 
