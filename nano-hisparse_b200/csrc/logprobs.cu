@@ -9,7 +9,7 @@
 // The alternatives come out of the same pass: every thread keeps its best entry. At
 // least `top` entries of the block's part reach the top-th best of the threads' best
 // values, so every one of its `top` largest entries does. Threads whose own best reaches
-// it (`top` of them, and equals) read their entries again and collect those that do; the
+// it (`top` of them, and equals) have their entries read again for those that do; the
 // collected keys are ranked by counting. (A looser bound, the smallest of the warps'
 // best, is found in half the time, but made a fifth of the threads read again: half as
 // much traffic again on rows that L2 does not hold.)
@@ -83,8 +83,8 @@ template <typename T> struct Vector {
     widen(raw, x);
     float m = x[0];
 #pragma unroll
-    for (int i = 1; i < n; ++i) m = max_nan(m, x[i]);
-    return m;
+    for (int i = 1; i + 1 < n; i += 2) m = max3_nan(m, x[i], x[i + 1]);
+    return max_nan(m, x[n - 1]);
   }
 };
 // the 16-bit types in pairs
@@ -100,6 +100,12 @@ template <> __device__ __forceinline__ float Vector<__nv_bfloat16>::largest(cons
   return pair_largest<__nv_bfloat162>(raw);
 }
 
+__device__ __forceinline__ float exp2_flush(float x) {  // below 2^-126: 0
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 // Differences are held above kFar where they multiply: a masked entry of -inf or
 // of the type's lowest value then adds 0 to t, not 0 * -inf. What that takes from
 // NaN and +inf comes back through s, whose own terms stay NaN.
@@ -107,16 +113,27 @@ struct Softmax {
   float m, s, t;  // maximum, sum exp(x - m), sum (x - m) exp(x - m)
   __device__ __forceinline__ void raise(float to) {
     if (m != -INFINITY) {
-      const float d = fmaxf(m - to, kFar), f = exp2f(d * kLog2e);
+      const float d = fmaxf(m - to, kFar), f = exp2_flush(d * kLog2e);
       t = f * fmaf(d, s, t);
       s *= f;
     }
     m = to;
   }
   __device__ __forceinline__ void add(float x) {  // x <= m
-    const float d = x - m, e = exp2f(d * kLog2e);
+    const float d = x - m, e = exp2_flush(d * kLog2e);
     s += e;
     t = fmaf(e, fmaxf(d, kFar), t);
+  }
+  // n entries, none above m: two sums of each kind, two products an instruction
+  template <int n> __device__ __forceinline__ void add(const float (&x)[n], float2 &s2, float2 &t2) const {
+    const float2 below = make_float2(-m, -m), log2e = make_float2(kLog2e, kLog2e);
+#pragma unroll
+    for (int i = 0; i < n; i += 2) {
+      const float2 d = pack_add(make_float2(x[i], x[i + 1]), below), y = pack_mul(d, log2e);
+      const float2 e = make_float2(exp2_flush(y.x), exp2_flush(y.y));
+      s2 = pack_add(s2, e);
+      t2 = pack_fma(e, make_float2(fmaxf(d.x, kFar), fmaxf(d.y, kFar)), t2);
+    }
   }
   // the sums over the warp's lanes, in every lane
   __device__ __forceinline__ void join_warp() {
@@ -124,7 +141,7 @@ struct Softmax {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(kFullMask, top, o));
     if (m != -INFINITY) {
-      const float d = fmaxf(m - top, kFar), f = exp2f(d * kLog2e);
+      const float d = fmaxf(m - top, kFar), f = exp2_flush(d * kLog2e);
       t = f * fmaf(d, s, t);
       s *= f;
     }
@@ -183,20 +200,20 @@ template <typename T> struct RowPart {
   __device__ __forceinline__ uint32_t index(int v, int i) const {
     return (uint32_t)(head + (first + v) * n + i);
   }
-  // this thread's kAhead vectors from number v0 on
-  __device__ __forceinline__ void load(int v0, uint4 (&raw)[kAhead]) const {
+  // kAhead vectors: v0, v0 + step, ...
+  __device__ __forceinline__ void load(int v0, int step, uint4 (&raw)[kAhead]) const {
 #pragma unroll
     for (int u = 0; u < kAhead; ++u)
-      if (v0 + u * kLogprobThreads < count) raw[u] = vector(v0 + u * kLogprobThreads);
+      if (v0 + u * step < count) raw[u] = vector(v0 + u * step);
   }
-  // f(vector, its number) for this thread's vectors, kAhead loads at a time
-  template <typename F> __device__ __forceinline__ void each(F f) const {
-    for (int v0 = threadIdx.x; v0 < count; v0 += kAhead * kLogprobThreads) {
+  // f(vector, its number) for vectors v0, v0 + step, ..., kAhead loads at a time
+  template <typename F> __device__ __forceinline__ void each(int v0, int step, F f) const {
+    for (; v0 < count; v0 += kAhead * step) {
       uint4 raw[kAhead];
-      load(v0, raw);
+      load(v0, step, raw);
 #pragma unroll
       for (int u = 0; u < kAhead; ++u)
-        if (v0 + u * kLogprobThreads < count) f(raw[u], v0 + u * kLogprobThreads);
+        if (v0 + u * step < count) f(raw[u], v0 + u * step);
     }
   }
 };
@@ -209,22 +226,27 @@ __device__ __forceinline__ int collect(LogprobShared &sh, const RowPart<T> &part
                                        uint64_t threshold) {
   if (threadIdx.x == 0) sh.found = 0;
   __syncthreads();
-  if (mine >= threshold) {
-    auto take = [&](uint64_t key) {
-      if (key < threshold) return;
-      const int at = atomicAdd(&sh.found, 1);
-      if (at < kCandidates) sh.candidates[at] = key;
-    };
-    const uint32_t least = (uint32_t)(threshold >> 32);
-    part.each([&](const uint4 &raw, int v) {
+  const auto take = [&](uint64_t key) {
+    if (key < threshold) return;
+    const int at = atomicAdd(&sh.found, 1);
+    if (at < kCandidates) sh.candidates[at] = key;
+  };
+  const uint32_t least = (uint32_t)(threshold >> 32);
+  // The whole warp reads the entries of each of its threads that pass, 32 vectors at a
+  // time: one thread alone would wait for memory once for every kAhead of them.
+  const int lane = threadIdx.x & 31, first = threadIdx.x - lane;
+  for (unsigned todo = __ballot_sync(kFullMask, mine >= threshold); todo != 0; todo &= todo - 1) {
+    const int owner = first + __ffs(todo) - 1;
+    part.each(owner + lane * kLogprobThreads, 32 * kLogprobThreads, [&](const uint4 &raw, int v) {
       if (value_order(Vector<T>::largest(raw)) < least) return;
       float x[Vector<T>::n];
       Vector<T>::widen(raw, x);
 #pragma unroll
       for (int i = 0; i < Vector<T>::n; ++i) take(entry_order(x[i], part.index(v, i)));
     });
-    if (part.edge >= 0) take(entry_order(to_f32(part.x[part.edge]), (uint32_t)part.edge));
   }
+  if (mine >= threshold && part.edge >= 0)
+    take(entry_order(to_f32(part.x[part.edge]), (uint32_t)part.edge));
   __syncthreads();
   return sh.found;
 }
@@ -270,7 +292,7 @@ __device__ __forceinline__ void block_best(LogprobShared &sh, const RowPart<T> &
       auto take = [&](uint64_t key) {
         if (key < below && key > next) next = key;
       };
-      part.each([&](const uint4 &raw, int v) {
+      part.each(threadIdx.x, kLogprobThreads, [&](const uint4 &raw, int v) {
         float x[Vector<T>::n];
         Vector<T>::widen(raw, x);
 #pragma unroll
@@ -305,11 +327,11 @@ __global__ void __launch_bounds__(kLogprobThreads, kLogprobBlocks)
   Softmax acc{-INFINITY, 0.f, 0.f};
   int at = -1;  // the vector that first held this thread's maximum
   uint4 raw[kAhead], next[kAhead];
-  part.load(threadIdx.x, next);
+  part.load(threadIdx.x, kLogprobThreads, next);
   for (int v0 = threadIdx.x; v0 < part.count; v0 += kAhead * kLogprobThreads) {
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) raw[u] = next[u];
-    part.load(v0 + kAhead * kLogprobThreads, next);  // while these are summed
+    part.load(v0 + kAhead * kLogprobThreads, kLogprobThreads, next);  // while these are summed
     float largest = -INFINITY;
     int where = v0;
 #pragma unroll
@@ -326,14 +348,16 @@ __global__ void __launch_bounds__(kLogprobThreads, kLogprobBlocks)
       acc.raise(largest);
     }
     if (acc.m == -INFINITY) continue;
+    float2 s2 = make_float2(acc.s, 0.f), t2 = make_float2(acc.t, 0.f);
 #pragma unroll
     for (int u = 0; u < kAhead; ++u)
       if (v0 + u * kLogprobThreads < part.count) {
         float e[Vector<T>::n];
         Vector<T>::widen(raw[u], e);
-#pragma unroll
-        for (int i = 0; i < Vector<T>::n; ++i) acc.add(e[i]);
+        acc.add(e, s2, t2);
       }
+    acc.s = s2.x + s2.y;
+    acc.t = t2.x + t2.y;
   }
   // This thread's best entry is at most `bound` and at least `mine` in the order:
   // the vector is known, the place in it is not.

@@ -99,22 +99,6 @@ __global__ void __launch_bounds__(kRopeThreads) norm_rope_any_kernel(RopeParams 
 // are issued before the set before it is worked on, the first before the angles. Products
 // are packed, two fp32 an instruction: a plain copy in this form takes 111 us at 32,768
 // tokens of 40 heads, so the instructions are what costs beyond the bytes.
-__device__ __forceinline__ float2 pack_fma(float2 a, float2 b, float2 c) {
-  float2 r;
-  asm("{\n .reg .b64 a, b, c, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n"
-      " mov.b64 c, {%6, %7};\n fma.rn.f32x2 d, a, b, c;\n mov.b64 {%0, %1}, d;\n}\n"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return r;
-}
-__device__ __forceinline__ float2 pack_mul(float2 a, float2 b) {
-  float2 r;
-  asm("{\n .reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n"
-      " mul.rn.f32x2 d, a, b;\n mov.b64 {%0, %1}, d;\n}\n"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return r;
-}
 template <typename T, int kPairs>  // 16 bytes as pairs of fp32
 __device__ __forceinline__ void unpack(const uint4 &raw, float2 (&x)[kPairs]) {
   const T *e = reinterpret_cast<const T *>(&raw);

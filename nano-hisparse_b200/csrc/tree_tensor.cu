@@ -144,28 +144,6 @@ __device__ __forceinline__ void fence_after() {
 __device__ __forceinline__ void fence_async_proxy() {
   asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
 }
-// fp32 pairs: one instruction for two products or sums
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 r;
-  asm("{\n .reg .b64 a, b, c, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n"
-      " mov.b64 c, {%6, %7};\n fma.rn.f32x2 d, a, b, c;\n mov.b64 {%0, %1}, d;\n}\n"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return r;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 r;
-  asm("{\n .reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n"
-      " add.rn.f32x2 d, a, b;\n mov.b64 {%0, %1}, d;\n}\n"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return r;
-}
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
 // Scores of keys that are not seen become -inf.
 __device__ __forceinline__ void hide(uint32_t (&s)[32], uint32_t seen) {
 #pragma unroll
@@ -592,14 +570,14 @@ __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreePara
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const float2 e =
-                fma2(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), scale2,
+                pack_fma(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), scale2,
                      make_float2(base, base));
             const float2 w2 = make_float2(tree_exp2(e.x), tree_exp2(e.y));
-            sums[i % 2] = add2(sums[i % 2], w2);
+            sums[i % 2] = pack_add(sums[i % 2], w2);
             packed[i] = pack2<T>(w2.x, w2.y);
           }
           tmem_store16(weights + h * 16, packed);
-          sums[0] = add2(sums[0], sums[1]);
+          sums[0] = pack_add(sums[0], sums[1]);
           l += sums[0].x + sums[0].y;
         }
         tmem_store_wait();
