@@ -266,13 +266,15 @@ __device__ __forceinline__ void block_best(LogprobShared &sh, const RowPart<T> &
     }
     return known;
   };
-  uint64_t threshold = search(0, 63, 32);
+  // to 16 bits of the value (8 of its fraction in fp32): a few entries more pass than
+  // with all of them, for half the steps
+  uint64_t threshold = search(0, 63, 48);
   if (threshold == 0) threshold = 1;  // fewer threads with entries than `top`: all of them
   int found = collect(sh, part, bound, threshold);
   if (found > kCandidates) {
-    // Many entries have that value: those of lower index go first, which the rest of
-    // the key says.
-    const uint64_t exact = search(threshold >> 32 << 32, 31, 0);
+    // Many entries are near that value or equal to it: the rest of the key tells them
+    // apart, equal ones by their index.
+    const uint64_t exact = search(threshold >> 48 << 48, 47, 0);
     if (exact > threshold) {
       threshold = exact;
       found = collect(sh, part, bound, threshold);
