@@ -59,8 +59,8 @@ HS_API int hs_qk_norm_rope(int64_t tokens, const void *query, int64_t query_toke
  * requests), mask int64 [batch, nodes], counts and node_counts int32 [batch];
  * counts below 0 or above their limit are clamped. out is contiguous
  * [batch, nodes, q_heads, head_dim]. A row beyond the pool is skipped and
- * raises HS_DEV_ROW_OUT_OF_RANGE. The workspace needs no initialisation; calls
- * that may overlap on the GPU need separate ones.
+ * raises HS_DEV_ROW_OUT_OF_RANGE. The workspace is 16-byte aligned and
+ * needs no initialisation; calls that may overlap on the GPU need separate ones.
  */
 HS_API size_t hs_attend_tree_workspace_bytes(int batch, int nodes, int q_heads, int kv_heads,
                                              int head_dim, int64_t count, int dtype);

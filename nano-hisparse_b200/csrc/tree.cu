@@ -56,8 +56,11 @@ __global__ void __launch_bounds__(kSimtThreads) tree_simt_kernel(TreeParams p, b
   extern __shared__ __align__(16) float smem[];
   float *sq = smem, *sk = sq + kSimtRows * pitch, *sv = sk + kSimtKeys * pitch;
   float *sp = sv + kSimtKeys * pitch;
-  __shared__ int64_t s_src[kSimtKeys];  // element offset of a key's K; see below
+  // where each key of this tile and the next lives: >= 0 an element offset in the pool,
+  // -1 nowhere, -2 - j node j
+  __shared__ int64_t s_places[2][kSimtKeys];
   __shared__ uint64_t s_mask[kSimtRows];
+  __shared__ unsigned long long s_bad;  // nodes whose V held a non-finite element
   const int tid = threadIdx.x, split = blockIdx.x;
   const int tiles = (int)ceil_div(p.nodes * p.groups, kSimtRows);
   const int kh = blockIdx.y / tiles, r0 = blockIdx.y % tiles * kSimtRows, b = blockIdx.z;
@@ -96,16 +99,17 @@ __global__ void __launch_bounds__(kSimtThreads) tree_simt_kernel(TreeParams p, b
   const T *value = static_cast<const T *>(p.value) + b * p.kv_batch_stride + (int64_t)kh * D;
   const int64_t *rows = p.rows + b * p.rows_batch_stride;
 
+  const auto look = [&](int64_t k0) {  // the places of the keys from k0 on, by 64 threads
+    const int64_t i = k0 + tid;
+    s_places[(k0 - begin) / kSimtKeys & 1][tid] =
+        i >= end ? -1 : i < valid ? row_offset(p, rows[i], row_elems) : -2 - (i - valid);
+  };
+  if (tid == 0) s_bad = 0;
+  if (tid < kSimtKeys && begin < end) look(begin);
+  const int used = (D + 3) / 4 * 4;  // elements that are not padding, in fours
   for (int64_t k0 = begin; k0 < end; k0 += kSimtKeys) {
     __syncthreads();
-    // where each key lives: >= 0 in the pool, -1 nowhere, -2 - j node j
-    if (tid < kSimtKeys) {
-      const int64_t i = k0 + tid;
-      s_src[tid] = i >= end ? -1
-                   : i < valid ? row_offset(p, rows[i], row_elems)
-                               : -2 - (i - valid);
-    }
-    __syncthreads();
+    const int64_t *s_src = s_places[(k0 - begin) / kSimtKeys & 1];
 #pragma unroll 4
     for (int i = tid; i < kSimtKeys * fours; i += kSimtThreads) {
       const int k = i / fours, d = i % fours * 4;
@@ -116,17 +120,29 @@ __global__ void __launch_bounds__(kSimtThreads) tree_simt_kernel(TreeParams p, b
         const T *vp = src >= 0 ? kp + p.page_size * row_elems : value + (-2 - src) * p.kv_node_stride;
         kx = load_four(kp, d, D, four);
         vx = load_four(vp, d, D, four);
+        // A node's V element that is not finite becomes 0 here: nodes that do not see
+        // it would meet 0 * NaN. Those that do get it added at the end.
+        if (src < -1 && !(fabsf(vx.x) < INFINITY && fabsf(vx.y) < INFINITY &&
+                          fabsf(vx.z) < INFINITY && fabsf(vx.w) < INFINITY)) {
+          atomicOr(&s_bad, 1ull << (-2 - src));
+          vx.x = fabsf(vx.x) < INFINITY ? vx.x : 0.f;
+          vx.y = fabsf(vx.y) < INFINITY ? vx.y : 0.f;
+          vx.z = fabsf(vx.z) < INFINITY ? vx.z : 0.f;
+          vx.w = fabsf(vx.w) < INFINITY ? vx.w : 0.f;
+        }
       }
       *reinterpret_cast<float4 *>(&sk[k * pitch + d]) = kx;
       *reinterpret_cast<float4 *>(&sv[k * pitch + d]) = vx;
     }
+    if (tid < kSimtKeys && k0 + kSimtKeys < end) look(k0 + kSimtKeys);
     __syncthreads();
     float s[4][4];  // rows 4 ty + i, keys tx + 16 j
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
-    for (int d = 0; d < dim; d += 4) {
+#pragma unroll 2
+    for (int d = 0; d < used; d += 4) {
       float4 q4[4], k4[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i)
@@ -170,26 +186,43 @@ __global__ void __launch_bounds__(kSimtThreads) tree_simt_kernel(TreeParams p, b
       for (int j = 0; j < 4 * NJ; ++j) acc[i][j] *= alpha;
     }
     __syncwarp();  // a row's probabilities are written and read by the same half warp
-    for (int k = 0; k < kSimtKeys; ++k) {
-      float w[4];
+#pragma unroll 2
+    for (int k = 0; k < kSimtKeys; k += 4) {
+      float4 w4[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = sp[(4 * ty + i) * kSimtPPitch + k];
+      for (int i = 0; i < 4; ++i)
+        w4[i] = *reinterpret_cast<const float4 *>(&sp[(4 * ty + i) * kSimtPPitch + k]);
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        const float4 v4 = *reinterpret_cast<const float4 *>(&sv[k * pitch + 4 * tx + 64 * j]);
+      for (int e = 0; e < 4; ++e)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          // a pair that is not seen takes no part even where its value is NaN or infinite
-          if (w[i] != 0.f) {
-            acc[i][4 * j] = fmaf(w[i], v4.x, acc[i][4 * j]);
-            acc[i][4 * j + 1] = fmaf(w[i], v4.y, acc[i][4 * j + 1]);
-            acc[i][4 * j + 2] = fmaf(w[i], v4.z, acc[i][4 * j + 2]);
-            acc[i][4 * j + 3] = fmaf(w[i], v4.w, acc[i][4 * j + 3]);
+        for (int j = 0; j < NJ; ++j) {
+          const float4 v4 =
+              *reinterpret_cast<const float4 *>(&sv[(k + e) * pitch + 4 * tx + 64 * j]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float w = e == 0 ? w4[i].x : e == 1 ? w4[i].y : e == 2 ? w4[i].z : w4[i].w;
+            acc[i][4 * j] = fmaf(w, v4.x, acc[i][4 * j]);
+            acc[i][4 * j + 1] = fmaf(w, v4.y, acc[i][4 * j + 1]);
+            acc[i][4 * j + 2] = fmaf(w, v4.z, acc[i][4 * j + 2]);
+            acc[i][4 * j + 3] = fmaf(w, v4.w, acc[i][4 * j + 3]);
           }
         }
-      }
     }
   }
+  __syncthreads();
+  const uint64_t bad = s_bad;
+  if (bad != 0)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint64_t seen = bad & s_mask[4 * ty + i];
+#pragma unroll 1
+      for (int j = 0; seen != 0 && j < 4 * NJ; ++j) {
+        const int d = 4 * tx + 64 * (j / 4) + j % 4;
+        const float x = d < D ? nonfinite_sum<T>(p, b, kh, d, seen) : 0.f;
+#pragma unroll
+        for (int e = 0; e < 4 * NJ; ++e) acc[i][e] += e == j ? x : 0.f;
+      }
+    }
   // rows of padded nodes: one split writes their zeros
   const int rows_all = p.nodes * G;
   T *out = static_cast<T *>(p.out) + (int64_t)b * p.nodes * p.q_heads * D;
@@ -300,6 +333,10 @@ template <typename T> int launch_merge(const TreeParams &p, cudaStream_t s) {
 
 // ---- layout of a call ----------------------------------------------------------------------
 enum class TreePath { simt, mma, tensor };
+// Bytes of `parts` (maximum, sum) pairs before the outputs, which are read and written 16
+// bytes at a time.
+size_t tree_stats_bytes(size_t parts) { return (parts * sizeof(float2) + 15) / 16 * 16; }
+
 // How a call is laid out: query rows of a block's tile, blocks on an SM, keys of a
 // step, splits of the key list.
 struct TreeShape {
@@ -326,15 +363,15 @@ TreeShape tree_shape(int batch, int nodes, int q_heads, int kv_heads, int head_d
   }
   s.keys = 64;
   // The split count with the least (rounds of blocks) x (keys of a block and what a
-  // block costs besides, as much as about 384 keys); more splits than two tiles each are not
-  // worth joining.
+  // block costs besides, as much as about 384 keys); splits of less than
+  // two tiles are not worth joining, but for the fp32 kernel, whose tiles take longest.
   const int64_t blocks = (int64_t)batch * kv_heads * ceil_div(queries, s.rows);
   const int64_t places = (int64_t)s.resident * sm_count(), total = count + nodes;
   int64_t least = 0;
   s.splits = 1;
   for (int n = 1; n <= kTreeMaxSplits; ++n) {
     const int64_t part = ceil_div(ceil_div(total, n), s.keys) * s.keys;
-    if (n > 1 && part < 2 * s.keys) break;
+    if (n > 1 && part < (s.path == TreePath::simt ? 1 : 2) * s.keys) break;
     const int64_t cost = ceil_div(blocks * n, places) * (part + 384) + (n > 1 ? 64 : 0);
     if (n == 1 || cost < least) {
       least = cost;
@@ -399,7 +436,7 @@ extern "C" size_t hs_attend_tree_workspace_bytes(int batch, int nodes, int q_hea
       tree_shape(batch, nodes, q_heads, kv_heads, head_dim, count, dtype).splits;
   if (splits == 1) return 0;
   const size_t parts = (size_t)batch * nodes * q_heads * splits;
-  return parts * sizeof(float2) + parts * head_dim * sizeof(float);
+  return tree_stats_bytes(parts) + parts * head_dim * sizeof(float);
 }
 
 extern "C" int hs_attend_tree(int batch, int nodes, const void *query, int64_t query_batch_stride,
@@ -462,12 +499,16 @@ extern "C" int hs_attend_tree(int batch, int nodes, const void *query, int64_t q
   p.scale_log2 = (float)(1.4426950408889634 / sqrt((double)head_dim));
   const size_t need =
       hs_attend_tree_workspace_bytes(batch, nodes, q_heads, kv_heads, head_dim, count, dtype);
+  if (need > 0 && (reinterpret_cast<uintptr_t>(workspace) & 15) != 0)
+    return set_error(HS_ERR_WORKSPACE, "attend_tree: the workspace must be 16-byte aligned");
   if (need > 0 && (!workspace || workspace_bytes < need))
     return set_error(HS_ERR_WORKSPACE, "attend_tree: workspace of %zu bytes < required %zu",
                      workspace_bytes, need);
   p.tile_rows = shape.rows;
   p.stats = static_cast<float2 *>(workspace);
-  p.partials = reinterpret_cast<float *>(p.stats + (size_t)batch * nodes * q_heads * p.splits);
+  p.partials = reinterpret_cast<float *>(
+      static_cast<char *>(workspace) +
+      tree_stats_bytes((size_t)batch * nodes * q_heads * p.splits));
   p.status = device_status;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (dtype) {

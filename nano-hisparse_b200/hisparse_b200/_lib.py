@@ -133,13 +133,20 @@ def require_cuda(*tensors):
 
 
 def one_device(first, *others) -> int:
-    """Index of the CUDA device that holds every given tensor (None is skipped)."""
+    """Index of the CUDA device that holds every given tensor (None is skipped).
+    Tensors that a gradient is asked of are refused: these operators have no
+    backward pass, and a result without one would drop it silently."""
     try:
         index = first.get_device()
-        same = index >= 0
+        same, grad = index >= 0, first.requires_grad
         for t in others:
-            if t is not None and t.get_device() != index:
-                same = False
+            if t is not None:
+                if t.get_device() != index:
+                    same = False
+                grad = grad or t.requires_grad
+        if grad and torch.is_grad_enabled():
+            raise ValueError("the operator has no backward pass: call it under "
+                             "torch.no_grad() or on detached tensors")
     except AttributeError:
         same = False
     if not same:

@@ -48,11 +48,10 @@ def token_logprobs(logits, tokens=None, top=0) -> TokenLogprobs:
         tokens = tokens.contiguous()
     if logits.stride(1) != 1:
         logits = logits.contiguous()
-    device = logits.device
-    logprobs = torch.empty(shape, dtype=torch.float32, device=device)
-    entropy = torch.empty(rows, dtype=torch.float32, device=device)
-    top_logprobs = torch.empty((rows, top), dtype=torch.float32, device=device)
-    top_tokens = torch.empty((rows, top), dtype=torch.int64, device=device)
+    logprobs = logits.new_empty(shape, dtype=torch.float32)
+    entropy = logits.new_empty(rows, dtype=torch.float32)
+    top_logprobs = logits.new_empty((rows, top), dtype=torch.float32)
+    top_tokens = logits.new_empty((rows, top), dtype=torch.int64)
     with _lib.on_device(index):
         _lib.check(_lib.load().hs_token_logprobs(
             rows, logits.data_ptr(), logits.stride(0), _lib.dtype_code(logits.dtype), vocab,

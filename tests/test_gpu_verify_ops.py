@@ -331,6 +331,25 @@ def test_logprobs_strides_and_tokens():
     assert [tuple(t.shape) for t in none] == [(0, 3), (0,), (0, 2), (0, 2)]
 
 
+def test_logprobs_rows_past_32_bits():
+    """The last rows of logits with more than 2^32 elements."""
+    from hisparse_b200 import token_logprobs
+
+    if torch.cuda.mem_get_info()[0] < 12 << 30:
+        pytest.skip("needs 12 GB")
+    rows, vocab = 34000, 128256
+    logits = torch.zeros((rows, vocab), dtype=BF16, device=DEV)
+    tail = (3 * torch.randn(3, vocab, generator=torch.Generator().manual_seed(9))).to(BF16).to(DEV)
+    logits[-3:] = tail
+    tokens = torch.full((rows,), 70000, device=DEV)
+    got = token_logprobs(logits, tokens, top=4)
+    # (few rows are split over blocks and many are not: their sums' order differs, so
+    # the last rows are held against the formula, not against a call of their own)
+    logprobs_check(type(got)(*(t[-3:] for t in got)), tail, tokens[-3:], 4)
+    assert got.top_tokens[0].tolist() == [0, 1, 2, 3]
+    assert abs(got.entropy[0].item() - math.log(vocab)) < 1e-4
+
+
 def test_logprobs_refusals():
     from hisparse_b200 import token_logprobs
 
@@ -427,7 +446,10 @@ SHAPES = [
     (2, 8, 32, 8, 128, 16, 513), (1, 17, 10, 2, 80, 12, 97), (2, 2, 12, 1, 256, 16, 130),
     (1, 33, 6, 6, 96, 5, 64), (1, 1, 16, 1, 200, 16, 257), (1, 4, 32, 8, 128, 16, 5000),
     (4, 16, 16, 4, 64, 16, 63), (2, 64, 16, 2, 128, 16, 190), (1, 5, 5, 1, 33, 3, 40),
-    (1, 12, 8, 1, 128, 1, 129), (17, 3, 4, 4, 16, 16, 33)]
+    (1, 12, 8, 1, 128, 1, 129), (17, 3, 4, 4, 16, 16, 33),
+    # an odd number of (row, split) pairs before the outputs of the splits
+    (1, 1, 1, 1, 128, 16, 5000), (1, 3, 5, 1, 64, 16, 3000), (1, 1, 3, 3, 32, 16, 900),
+    (1, 5, 1, 1, 256, 16, 2000), (1, 7, 3, 1, 20, 16, 700)]
 
 
 @pytest.mark.parametrize("dtype", [FP32, FP16, BF16])
@@ -478,13 +500,14 @@ def test_tree_empty_rows_and_masks(dtype, dim):
 
 @pytest.mark.parametrize("dtype", [FP32, FP16, BF16])
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
-def test_tree_nonfinite_values_out_of_sight(dtype, bad):
+@pytest.mark.parametrize("dim", [128, 64, 36, 256])
+def test_tree_nonfinite_values_out_of_sight(dtype, bad, dim):
     """What a node does not see takes no part, whatever it holds: other branches,
     padded nodes, rows behind counts and blocks that no row names. A node that
     sees a non-finite value gets it, in its own elements only."""
     from hisparse_b200 import attend_tree, tree_mask
 
-    inputs, _, pool, rows, config = tree_inputs(2, 12, 8, 2, 128, 16, 96, dtype, 12)
+    inputs, _, pool, rows, config = tree_inputs(2, 12, 8, 2, dim, 16, 96, dtype, 12)
     q, k, v = inputs
     parents = [[-1, 0, 1, 0, 3, 3, 0, 6, 7, 6, 6, 10]] * 2
     mask = tree_mask(parents, DEV)
@@ -537,6 +560,47 @@ def test_tree_strided_inputs_and_bad_rows():
         broken[2, 3] = 1 << 60
         tree_check(attend_tree(*inputs, mask, pool, broken, config), inputs, mask, pool, broken)
         assert flags() == [_lib.DEVICE_FLAGS[1]]
+
+
+def test_tree_rows_far_into_a_long_pool():
+    """Rows of blocks whose elements lie past 2^31 (and bytes past 2^32) give what the
+    same rows give at the start of a short pool, in runs and one by one."""
+    from hisparse_b200 import CacheConfig, attend_tree, tree_mask
+
+    if torch.cuda.mem_get_info()[0] < 12 << 30:
+        pytest.skip("needs 12 GB")
+    for dtype, dim in ((BF16, 128), (FP16, 256), (FP32, 64)):
+        inputs, parents, pool, rows, config = tree_inputs(2, 5, 8, 4, dim, 16, 200, dtype, 16)
+        mask = tree_mask(parents, DEV)
+        want = attend_tree(*inputs, mask, pool, rows, config)
+        first = 2 ** 31 // pool[0].numel() + 11
+        long_pool = torch.empty((first + pool.shape[0], *pool.shape[1:]), dtype=dtype, device=DEV)
+        long_pool[first:] = pool
+        far = CacheConfig(gpu_pages=long_pool.shape[0], page_size=16, kv_heads=4, head_dim=dim,
+                          device=DEV, dtype=dtype)
+        got = attend_tree(*inputs, mask, long_pool, rows + first * 16, far)
+        assert torch.equal(got, want)
+        mixed = torch.randperm(200, generator=torch.Generator().manual_seed(1)).to(DEV)
+        want = attend_tree(*inputs, mask, pool, rows[:, mixed].contiguous(), config)
+        got = attend_tree(*inputs, mask, long_pool, (rows + first * 16)[:, mixed].contiguous(), far)
+        assert torch.equal(got, want)
+        del long_pool
+    assert not flags()
+
+
+def test_tree_runs_equal_single_rows():
+    """Rows in page order (tiled copies) and the same rows shuffled are the same set:
+    equal within the bound of their sums."""
+    from hisparse_b200 import attend_tree, tree_mask
+
+    for dtype, dim in ((BF16, 128), (FP16, 64)):
+        inputs, parents, pool, rows, config = tree_inputs(3, 40, 8, 2, dim, 64, 1000, dtype, 18)
+        mask = tree_mask(parents, DEV)
+        rows[1, 100:300] = -1
+        rows[2, 5::7] = -1
+        order = torch.randperm(1000, generator=torch.Generator().manual_seed(2)).to(DEV)
+        for r in (rows, rows[:, order].contiguous(), rows[:, 3:].contiguous()):
+            tree_check(attend_tree(*inputs, mask, pool, r, config), inputs, mask, pool, r)
 
 
 def test_tree_peaked_scores():
@@ -643,6 +707,67 @@ def test_operators_together(dtype):
     from hisparse_b200 import TokenLogprobs
 
     logprobs_check(TokenLogprobs(*scores), logits, s["tokens"], 5)
+
+
+def test_operators_refuse_tensors_that_want_gradients():
+    from hisparse_b200 import attend_tree, qk_norm_rope, token_logprobs
+
+    s = _verify_inputs(FP32, 24)
+    x = s["fused"].requires_grad_()
+    with pytest.raises(ValueError, match="no backward"):
+        _verify_step(s)
+    with torch.no_grad():
+        (out, *scores), (q, k, v, logits) = _verify_step(s)
+    heads = [t.unflatten(0, (3, 6)) for t in (q, k, v.detach())]
+    with pytest.raises(ValueError, match="no backward"):
+        attend_tree(heads[0].requires_grad_(), *heads[1:], s["mask"], s["pool"], s["rows"],
+                    s["config"])
+    with pytest.raises(ValueError, match="no backward"):
+        token_logprobs(logits.requires_grad_())
+    with pytest.raises(ValueError, match="no backward"):
+        qk_norm_rope(q.detach(), k.detach(), s["positions"], s["freq"],
+                     s["w"].clone().requires_grad_(), s["w"])
+    assert x.grad is None
+
+
+def test_first_call_inside_a_capture(monkeypatch):
+    """The device's status word is made outside graphs only: a first call inside one
+    records no flags and works."""
+    from hisparse_b200 import _lib, token_logprobs
+
+    monkeypatch.setattr(_lib, "_status_words", {})
+    monkeypatch.setattr(_lib, "_status_pointers", {})
+    x = torch.randn(4, 100, device=DEV)
+    tokens = torch.tensor([1, 2, 100, 3], device=DEV)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = token_logprobs(x, tokens, top=2)
+    graph.replay()
+    assert _lib._status_words == {} and out.logprobs.isnan().tolist() == [False] * 2 + [True, False]
+    want = token_logprobs(x, tokens, top=2)
+    assert torch.equal(out.top_tokens, want.top_tokens)
+    assert flags() == [_lib.DEVICE_FLAGS[64]]
+
+
+def test_calls_on_two_streams_at_once():
+    """Calls that overlap have workspaces of their own."""
+    from hisparse_b200 import attend_tree, tree_mask
+
+    cases = []
+    for seed in (31, 32):
+        inputs, parents, pool, rows, config = tree_inputs(2, 20, 8, 2, 128, 16, 4000, BF16, seed)
+        cases.append((*inputs, tree_mask(parents, DEV), pool, rows, config))
+    want = [attend_tree(*c) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = [[], []]
+    for _ in range(8):
+        for i, (stream, case) in enumerate(zip(streams, cases)):
+            with torch.cuda.stream(stream):
+                got[i].append(attend_tree(*case))
+    torch.cuda.synchronize()
+    for outs, w in zip(got, want):
+        assert all(torch.equal(o, w) for o in outs)
 
 
 def test_operators_captured_and_on_another_stream():

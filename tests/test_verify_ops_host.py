@@ -85,6 +85,9 @@ def test_tree_validation():
     assert tree(batch=1, nodes=8, hq=32, hkv=8, dim=128, count=32768) == _lib.HS_ERR_WORKSPACE
     assert tree(batch=1, nodes=8, hq=32, hkv=8, dim=128, count=32768, ws=D,
                 ws_bytes=need - 1) == _lib.HS_ERR_WORKSPACE
+    assert tree(batch=1, nodes=8, hq=32, hkv=8, dim=128, count=32768, ws=D + 8,
+                ws_bytes=need) == _lib.HS_ERR_WORKSPACE
+    assert b"16-byte" in lib.hs_last_error()
     assert tree(batch=0, q=None) == _lib.HS_OK
 
 
