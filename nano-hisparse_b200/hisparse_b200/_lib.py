@@ -137,13 +137,14 @@ def one_device(first, *others) -> int:
     Tensors that a gradient is asked of are refused: these operators have no
     backward pass, and a result without one would drop it silently."""
     try:
-        index = first.get_device()
-        same, grad = index >= 0, first.requires_grad
+        index, grad = first.get_device(), first.requires_grad
+        same = index >= 0
         for t in others:
             if t is not None:
                 if t.get_device() != index:
                     same = False
-                grad = grad or t.requires_grad
+                if t.requires_grad:
+                    grad = True
         if grad and torch.is_grad_enabled():
             raise ValueError("the operator has no backward pass: call it under "
                              "torch.no_grad() or on detached tensors")

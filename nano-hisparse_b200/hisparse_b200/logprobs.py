@@ -33,29 +33,33 @@ def token_logprobs(logits, tokens=None, top=0) -> TokenLogprobs:
     above -inf has log probabilities -inf and entropy 0. Runs on the current
     stream."""
     index = _lib.one_device(logits, tokens)
-    if logits.ndim != 2 or logits.shape[1] < 1:
+    shape = logits.shape
+    if len(shape) != 2 or shape[1] < 1:
         raise ValueError("logits must be [rows, vocab]")
-    rows, vocab = logits.shape
+    rows, vocab = shape
     if not 0 <= top <= vocab:
         raise ValueError("top must be between 0 and the vocabulary size")
-    shape, given, code = (rows, 0), 0, _lib.HS_INT64
+    shape, given, code, address = (rows, 0), 0, _lib.HS_INT64, None
     if tokens is not None:
-        shape = tokens.shape
-        if tokens.dtype not in _TOKENS or len(shape) not in (1, 2) or shape[0] != rows:
+        shape, code = tokens.shape, _TOKENS.get(tokens.dtype)
+        if code is None or len(shape) not in (1, 2) or shape[0] != rows:
             raise ValueError("tokens must be int32 or int64 [rows] or [rows, given]")
         given = 1 if len(shape) == 1 else shape[1]
-        code = _TOKENS[tokens.dtype]
         tokens = tokens.contiguous()
-    if logits.stride(1) != 1:
+        address = tokens.data_ptr()
+    row_stride, inner = logits.stride()
+    if inner != 1:
         logits = logits.contiguous()
+        row_stride = vocab
     logprobs = logits.new_empty(shape, dtype=torch.float32)
     entropy = logits.new_empty(rows, dtype=torch.float32)
     top_logprobs = logits.new_empty((rows, top), dtype=torch.float32)
     top_tokens = logits.new_empty((rows, top), dtype=torch.int64)
     with _lib.on_device(index):
-        _lib.check(_lib.load().hs_token_logprobs(
-            rows, logits.data_ptr(), logits.stride(0), _lib.dtype_code(logits.dtype), vocab,
-            _lib.ptr(tokens), code, given, logprobs.data_ptr(), entropy.data_ptr(), top,
-            top_logprobs.data_ptr(), top_tokens.data_ptr(), _lib.status_pointer(index),
-            _lib.raw_stream(index)))
+        status = _lib.load().hs_token_logprobs(
+            rows, logits.data_ptr(), row_stride, _lib.dtype_code(logits.dtype), vocab, address,
+            code, given, logprobs.data_ptr(), entropy.data_ptr(), top, top_logprobs.data_ptr(),
+            top_tokens.data_ptr(), _lib.status_pointer(index), _lib.raw_stream(index))
+    if status:
+        _lib.check(status)
     return TokenLogprobs(logprobs, entropy, top_logprobs, top_tokens)

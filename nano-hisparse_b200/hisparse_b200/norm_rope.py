@@ -25,15 +25,6 @@ def rope_frequencies(head_dim: int, theta: float, device="cuda") -> torch.Tensor
     return float(theta) ** -exponent
 
 
-def _check_heads(name, x, tokens, head_dim, dtype):
-    if x.ndim != 3 or x.shape[0] != tokens or x.shape[2] != head_dim or x.shape[1] < 1:
-        raise ValueError(f"{name} must be [tokens, heads, head_dim]")
-    if x.dtype != dtype:
-        raise ValueError("query, key and weights must have one dtype")
-    # an inner stride other than 1 is laid out anew; any other stride is read in place
-    return x if x.stride(2) == 1 else x.contiguous()
-
-
 def qk_norm_rope(query, key, positions, inv_freq, query_weight=None, key_weight=None, eps=1e-6):
     """RMS-normalise every query and key head (with a weight; without one the
     norm is left out), then rotate the pairs (i, i + head_dim / 2) by
@@ -47,34 +38,50 @@ def qk_norm_rope(query, key, positions, inv_freq, query_weight=None, key_weight=
     rounding. Runs on the current stream.
     """
     index = _lib.one_device(query, key, positions, inv_freq, query_weight, key_weight)
-    if query.ndim != 3:
+    dtype, shape, key_shape = query.dtype, query.shape, key.shape
+    if len(shape) != 3 or shape[1] < 1:
         raise ValueError("query must be [tokens, heads, head_dim]")
-    tokens, q_heads, dim = query.shape
-    dtype = query.dtype
-    query = _check_heads("query", query, tokens, dim, dtype)
-    key = _check_heads("key", key, tokens, dim, dtype)
+    tokens, q_heads, dim = shape
+    if len(key_shape) != 3 or key_shape[0] != tokens or key_shape[2] != dim or key_shape[1] < 1:
+        raise ValueError("key must be [tokens, heads, head_dim]")
+    if key.dtype != dtype:
+        raise ValueError("query, key and weights must have one dtype")
     if dim < 2 or dim % 2:
         raise ValueError("head_dim must be even")
-    if positions.shape != (tokens,) or positions.dtype not in _POSITIONS:
+    code = _POSITIONS.get(positions.dtype)
+    if code is None or positions.shape != (tokens,):
         raise ValueError("positions must be int32 or int64 [tokens]")
-    if inv_freq.shape != (dim // 2,) or inv_freq.dtype != torch.float64:
+    if inv_freq.dtype != torch.float64 or inv_freq.shape != (dim // 2,):
         raise ValueError("inv_freq must be float64 [head_dim / 2]")
-    weights = [None, None]
-    for i, w in enumerate((query_weight, key_weight)):
-        if w is not None:
-            if w.shape != (dim,) or w.dtype != dtype:
-                raise ValueError("norm weights must be [head_dim] of the query's dtype")
-            weights[i] = w = w.contiguous()
+    q_weight = k_weight = None  # addresses
+    if query_weight is not None:
+        if query_weight.dtype != dtype or query_weight.shape != (dim,):
+            raise ValueError("norm weights must be [head_dim] of the query's dtype")
+        query_weight = query_weight.contiguous()
+        q_weight = query_weight.data_ptr()
+    if key_weight is not None:
+        if key_weight.dtype != dtype or key_weight.shape != (dim,):
+            raise ValueError("norm weights must be [head_dim] of the query's dtype")
+        key_weight = key_weight.contiguous()
+        k_weight = key_weight.data_ptr()
+    # an inner stride other than 1 is laid out anew; any other stride is read in place
+    q_token, q_head, inner = query.stride()
+    if inner != 1:
+        query = query.contiguous()
+        q_token, q_head, _ = query.stride()
+    k_token, k_head, inner = key.stride()
+    if inner != 1:
+        key = key.contiguous()
+        k_token, k_head, _ = key.stride()
     positions, inv_freq = positions.contiguous(), inv_freq.contiguous()
     query_out = torch.empty_like(query, memory_format=torch.contiguous_format)
     key_out = torch.empty_like(key, memory_format=torch.contiguous_format)
-    q_token, q_head, _ = query.stride()
-    k_token, k_head, _ = key.stride()
     with _lib.on_device(index):
-        _lib.check(_lib.load().hs_qk_norm_rope(
+        status = _lib.load().hs_qk_norm_rope(
             tokens, query.data_ptr(), q_token, q_head, q_heads, key.data_ptr(), k_token, k_head,
-            key.shape[1], dim, _lib.dtype_code(dtype), positions.data_ptr(),
-            _POSITIONS[positions.dtype], inv_freq.data_ptr(), _lib.ptr(weights[0]),
-            _lib.ptr(weights[1]), eps, query_out.data_ptr(), key_out.data_ptr(),
-            _lib.raw_stream(index)))
+            key_shape[1], dim, _lib.dtype_code(dtype), positions.data_ptr(), code,
+            inv_freq.data_ptr(), q_weight, k_weight, eps, query_out.data_ptr(),
+            key_out.data_ptr(), _lib.raw_stream(index))
+    if status:
+        _lib.check(status)
     return query_out, key_out

@@ -38,11 +38,6 @@ def tree_mask(parents, device="cuda") -> torch.Tensor:
     return torch.tensor(out, dtype=torch.int64).view(len(out), width).to(device)
 
 
-def _heads_adjacent(x):
-    """x [B, T, H, D] with the heads of a node adjacent (copied when they are not)."""
-    return x if x.stride(3) == 1 and x.stride(2) == x.shape[3] else x.contiguous()
-
-
 def attend_tree(query, key, value, mask, pool, rows, config, counts=None, nodes=None):
     """Attention of query [B, T, Hq, D] over pool rows and the nodes' key/value
     [B, T, Hkv, D]; T <= 64.
@@ -57,47 +52,61 @@ def attend_tree(query, key, value, mask, pool, rows, config, counts=None, nodes=
     heads. Returns a new [B, T, Hq, D]. Runs on the current stream.
     """
     index = _lib.one_device(query, key, value, mask, pool, rows, counts, nodes)
-    if query.ndim != 4 or query.shape[3] != config.head_dim:
+    shape, dtype, kv_heads = query.shape, query.dtype, config.kv_heads
+    if len(shape) != 4 or shape[3] != config.head_dim:
         raise ValueError("query must be [batch, nodes, heads, head_dim]")
-    batch, width, q_heads, dim = query.shape
-    if q_heads < 1 or q_heads % config.kv_heads:
+    batch, width, q_heads, dim = shape
+    if q_heads < 1 or q_heads % kv_heads:
         raise ValueError("query GQA/device mismatch")
     if width > MAX_NODES:
         raise ValueError(f"at most {MAX_NODES} nodes are supported")
-    kv_shape = (batch, width, config.kv_heads, dim)
+    kv_shape = (batch, width, kv_heads, dim)
     if key.shape != kv_shape or value.shape != kv_shape:
         raise ValueError("key and value must be [batch, nodes, kv_heads, head_dim]")
-    if pool.ndim != 5 or pool.shape[1:] != (2, config.page_size, config.kv_heads, dim) \
-            or not pool.is_contiguous():
+    blocks, *block = pool.shape
+    if block != [2, config.page_size, kv_heads, dim] or not pool.is_contiguous():
         raise ValueError("pool must be contiguous [blocks, 2, page_size, kv_heads, head_dim]")
-    if not query.dtype == key.dtype == value.dtype == pool.dtype:
+    if not dtype == key.dtype == value.dtype == pool.dtype:
         raise ValueError("query, key, value and pool must have one dtype")
     if mask.shape != (batch, width) or mask.dtype != torch.int64:
         raise ValueError("mask must be int64 [batch, nodes]")
-    if rows.ndim != 2 or rows.shape[0] != batch or rows.dtype != torch.int64:
+    rows_shape = rows.shape
+    if len(rows_shape) != 2 or rows_shape[0] != batch or rows.dtype != torch.int64:
         raise ValueError("rows must be int64 [batch, rows]")
+    limits = []  # addresses of counts and nodes
     for name, t in (("counts", counts), ("nodes", nodes)):
-        if t is not None and (t.shape != (batch,) or t.dtype != torch.int32
-                              or not t.is_contiguous()):
+        if t is None:
+            limits.append(None)
+            continue
+        if t.dtype != torch.int32 or t.shape != (batch,) or not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous int32 [batch]")
-    query, key, value, mask = (_heads_adjacent(query), _heads_adjacent(key),
-                               _heads_adjacent(value), mask.contiguous())
-    if key.stride() != value.stride():
+        limits.append(t.data_ptr())
+    # heads of a node adjacent (copied when they are not); batch and node strides as they are
+    q_batch, q_node, head, inner = query.stride()
+    if inner != 1 or head != dim:
+        query = query.contiguous()
+        q_batch, q_node, _, _ = query.stride()
+    strides = key.stride()
+    if strides != value.stride() or strides[3] != 1 or strides[2] != dim:
         key, value = key.contiguous(), value.contiguous()
-    if rows.stride(1) != 1 and rows.shape[1] > 1:
+        strides = (width * kv_heads * dim, kv_heads * dim)
+    mask, count = mask.contiguous(), rows_shape[1]
+    row_stride, inner = rows.stride()
+    if inner != 1 and count > 1:
         rows = rows.contiguous()
+        row_stride = count
     out = torch.empty_like(query, memory_format=torch.contiguous_format)
-    lib, code, count = _lib.load(), _lib.dtype_code(query.dtype), rows.shape[1]
-    q_batch, q_node, _, _ = query.stride()
-    kv_batch, kv_node, _, _ = key.stride()
+    lib, code = _lib.load(), _lib.dtype_code(dtype)
     with _lib.on_device(index):
-        nbytes = lib.hs_attend_tree_workspace_bytes(batch, width, q_heads, config.kv_heads, dim,
-                                                    count, code)
+        nbytes = lib.hs_attend_tree_workspace_bytes(batch, width, q_heads, kv_heads, dim, count,
+                                                    code)
         ws = _lib.workspace(nbytes, query.device)
-        _lib.check(lib.hs_attend_tree(
+        status = lib.hs_attend_tree(
             batch, width, query.data_ptr(), q_batch, q_node, key.data_ptr(), value.data_ptr(),
-            kv_batch, kv_node, code, mask.data_ptr(), _lib.ptr(nodes), pool.data_ptr(),
-            pool.shape[0], rows.data_ptr(), rows.stride(0), count, _lib.ptr(counts),
-            out.data_ptr(), q_heads, config.kv_heads, dim, config.page_size, _lib.ptr(ws), nbytes,
-            _lib.status_pointer(index), _lib.raw_stream(index)))
+            strides[0], strides[1], code, mask.data_ptr(), limits[1], pool.data_ptr(), blocks,
+            rows.data_ptr(), row_stride, count, limits[0], out.data_ptr(), q_heads, kv_heads, dim,
+            config.page_size, _lib.ptr(ws), nbytes, _lib.status_pointer(index),
+            _lib.raw_stream(index))
+    if status:
+        _lib.check(status)
     return out
