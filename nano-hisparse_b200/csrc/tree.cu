@@ -354,8 +354,8 @@ TreeShape tree_shape(int batch, int nodes, int q_heads, int kv_heads, int head_d
     s.resident = 2;
   } else if (head_dim <= 128) {
     s.path = TreePath::tensor;
-    s.rows = queries <= 128 ? 128 : 256;
-    s.resident = 1;
+    s.rows = 128;
+    s.resident = 2;
   } else {
     s.path = TreePath::mma;
     s.rows = queries <= 32 ? 32 : 64;

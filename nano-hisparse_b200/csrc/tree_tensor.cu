@@ -1,29 +1,27 @@
 // Tree attention on the fifth-generation tensor cores: 16-bit types, head_dim <= 128.
 //
-// A block has one SM and up to 256 query rows as two streams of 128 (a stream is
-// the M = 128 tile of tcgen05.mma, its rows the TMEM lanes). With more than 128
-// rows stream w owns rows 128 w .. and both work on every block of 64 keys; with
-// fewer, both own the same rows and take the key blocks in turn, so that one
-// stream's softmax runs beside the other's products, and join at the end. 18 warps:
-//   warps 0-3, 4-7  softmax of stream 0, 1: a thread has one query row. Scores
-//                   from TMEM, P = exp2(s - m) rounded to the 16-bit type back to
-//                   TMEM. The maximum is raised only when a score passes it by
-//                   more than 8 (a factor of 256, inside fp16's range), so the
-//                   output, which stays in TMEM, is rescaled rarely.
-//   warps 8-15      copy key blocks (four warps K, four V), 16 bytes a thread with
-//                   cp.async, into rings of stages in the 128-byte-swizzled layout of
-//                   the descriptors: rows are scattered over the pool, so there is no
-//                   tile for the TMA engine, and its gather of four rows of 128 bytes
-//                   was measured at 73 clocks each, a third of this path's rate.
-//   warp 16         issues S = Q K^T, both operands in shared memory, K-major
-//   warp 17         issues O += P V, P in TMEM, V in shared memory, MN-major (as
+// A block serves 128 query rows (the M = 128 tile of tcgen05.mma, its rows the TMEM
+// lanes) of a request and KV head over a split of the key list, in blocks of 64 keys.
+// Two blocks share an SM, so that one's softmax runs beside the other's products, and
+// one's start and end beside the other's middle. 10 warps:
+//   warps 0-3       softmax: a thread has one query row. Scores from TMEM, P =
+//                   exp2(s - m) rounded to the 16-bit type back to TMEM. The maximum is
+//                   raised only when a score passes it by more than 8 (a factor of 256,
+//                   inside fp16's range), so the output, which stays in TMEM, is rescaled
+//                   rarely.
+//   warps 4-7       copy key blocks (two warps K, two V) into rings of stages in the
+//                   128-byte-swizzled layout of the descriptors: 16 rows that follow one
+//                   another in the pool with one tiled copy, others with cp.async, 16
+//                   bytes a thread. (The copy engine's gather of four rows of 128 bytes
+//                   was measured at 73 clocks each, a third of this rate.)
+//   warp 8          issues S = Q K^T, both operands in shared memory, K-major
+//   warp 9          issues O += P V, P in TMEM, V in shared memory, MN-major (as
 //                   stored: a key's elements are adjacent)
-// The next block's scores do not wait for this one's output, so the tensor pipe and
-// the softmax overlap. What bounds it: up to about 50 nodes the
-// reads of K and V, beyond that the exponentials (16 a clock on an SM).
+// A block's scores do not wait for the one before it, so the tensor pipe and the
+// softmax overlap. What bounds it: up to about 50 nodes the reads of K and V, beyond
+// that the exponentials (16 a clock on an SM); with few keys the chain of its start.
 //
-// TMEM columns of a stream: O 0..127, two buffers of S from 128 on; P takes the
-// second half of its S.
+// TMEM columns: O 0..127, two buffers of S from 128 on; P takes the second half of its S.
 // Every wait is bounded; one that runs out sets HS_DEV_WAIT_TIMEOUT, ends its
 // warp's loop, and so lets every other wait run out.
 #include <cuda.h>
@@ -36,38 +34,45 @@
 namespace hs {
 namespace {
 
-constexpr int kSoftmaxWarps = 8, kLoadWarps = 8;  // half of the latter for K, half for V
-constexpr int kMaxStages = 8;
+constexpr int kSoftmaxWarps = 4, kLoadWarps = 4;  // half of the latter for K, half for V
+constexpr int kMaxStages = 5;
 constexpr int kPanel = 1024;   // bytes of 8 rows x 64 elements
 constexpr int kRun = 16;       // rows of a tiled copy
 constexpr int kMarks = 16;     // blocks whose marks (which keys are cache rows) are kept
 constexpr int kScoreWarp = kSoftmaxWarps + kLoadWarps, kOutputWarp = kScoreWarp + 1;
 constexpr int kTensorThreads = 32 * (kOutputWarp + 1);
-constexpr int kTile = 128;     // query rows of a stream
+constexpr int kTile = 128;     // query rows
 constexpr int kKeys = 64;      // keys of a block
 constexpr int kLook = 6;       // blocks that row numbers are read ahead
 constexpr unsigned long long kWaitNanoseconds = 4000000000ull;  // then a wait gives up
-constexpr int kColumnsS = 128, kStreamColumns = 256;
+constexpr int kColumnsS = 128, kColumns = 256;
+
+struct TensorShared {
+  uint64_t k_full[kMaxStages], k_free[kMaxStages], v_full[kMaxStages], v_free[kMaxStages];
+  uint64_t s_full[2], p_full[2], pv_done[2];  // by buffer
+  unsigned long long bad;                     // nodes whose V held a non-finite element
+  uint32_t cached[kMarks][kLoadWarps / 2];    // by block: its keys that are cache rows
+  uint32_t tmem;
+};
 
 // Shared memory of a block. kDim: head_dim rounded up to 64 or 128, the rest zero.
 // An operand is a list of 8-row groups, each of one or two panels of 64 elements
 // (128 bytes) a row: a panel of a group is a swizzle atom, and a run of rows in the
 // pool lands in it with one tiled copy.
 // K and V have rings of their own: a stage of K is free when its scores are done, a
-// stage of V only when its output is. Streams of the same rows need one tile of Q and
-// take the other's place for two more stages.
+// stage of V only when its output is.
 template <int kDim> struct TensorShape {
   static constexpr int atom = kDim / 64 * kPanel;        // bytes of an 8-row group
-  static constexpr int q_bytes = kTile * kDim * 2;       // of one stream
+  static constexpr int q_bytes = kTile * kDim * 2;
   static constexpr int plane_bytes = kKeys * kDim * 2;   // a stage: K or V of a block
-  static constexpr int k_stages = kDim == 64 ? 8 : 4, v_stages = kDim == 64 ? 8 : 5;
-  static constexpr int more = kDim == 64 ? 0 : 1;        // of each, with one tile of Q
-  static constexpr int bytes = 2 * q_bytes + (k_stages + v_stages) * plane_bytes;
-  static constexpr size_t dynamic = bytes + 1024;        // alignment to a swizzle atom
-  static constexpr int join_pitch = kDim + 4;            // floats of a result's row in the rings
-  static_assert(k_stages + more <= kMaxStages && v_stages + more <= kMaxStages, "barriers");
-  static_assert(2 * more * plane_bytes <= q_bytes, "the second tile of Q makes room for them");
-  static_assert(2 * kTile * join_pitch * 4 <= (k_stages + v_stages) * plane_bytes,
+  static constexpr int k_stages = kDim == 64 ? 4 : 2, v_stages = kDim == 64 ? 5 : 3;
+  static constexpr int bytes = q_bytes + (k_stages + v_stages) * plane_bytes;
+  static constexpr size_t dynamic = bytes + 1024;        // and TensorShared
+  static constexpr int result_pitch = kDim + 4;          // floats of a result's row in the rings
+  static_assert(k_stages <= kMaxStages && v_stages <= kMaxStages, "barriers");
+  static_assert(sizeof(TensorShared) <= 1024, "TensorShared has its place");
+  static_assert(2 * (dynamic + 1024) <= 228 * 1024, "two blocks on an SM");
+  static_assert(kTile * result_pitch * 4 <= (k_stages + v_stages) * plane_bytes,
                 "results fit the rings");
 };
 
@@ -118,17 +123,6 @@ __device__ __forceinline__ void tmem_load16_done(uint32_t (&a)[16]) {
                : "+r"(a[0]), "+r"(a[1]), "+r"(a[2]), "+r"(a[3]), "+r"(a[4]), "+r"(a[5]),
                  "+r"(a[6]), "+r"(a[7]), "+r"(a[8]), "+r"(a[9]), "+r"(a[10]), "+r"(a[11]),
                  "+r"(a[12]), "+r"(a[13]), "+r"(a[14]), "+r"(a[15])
-               :
-               : "memory");
-}
-__device__ __forceinline__ void tmem_load16_done(uint32_t (&a)[16], uint32_t (&b)[16]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;\n"
-               : "+r"(a[0]), "+r"(a[1]), "+r"(a[2]), "+r"(a[3]), "+r"(a[4]), "+r"(a[5]),
-                 "+r"(a[6]), "+r"(a[7]), "+r"(a[8]), "+r"(a[9]), "+r"(a[10]), "+r"(a[11]),
-                 "+r"(a[12]), "+r"(a[13]), "+r"(a[14]), "+r"(a[15]),
-                 "+r"(b[0]), "+r"(b[1]), "+r"(b[2]), "+r"(b[3]), "+r"(b[4]), "+r"(b[5]),
-                 "+r"(b[6]), "+r"(b[7]), "+r"(b[8]), "+r"(b[9]), "+r"(b[10]), "+r"(b[11]),
-                 "+r"(b[12]), "+r"(b[13]), "+r"(b[14]), "+r"(b[15])
                :
                : "memory");
 }
@@ -254,11 +248,6 @@ template <int kDim> __device__ __forceinline__ uint32_t place(int r, int c) {
                     (((c & 7) ^ (r & 7)) << 4));
 }
 
-struct TensorBarriers {
-  uint64_t k_full[kMaxStages], k_free[kMaxStages], v_full[kMaxStages], v_free[kMaxStages];
-  uint64_t s_full[2][2], p_full[2][2], pv_done[2][2];  // by stream and buffer
-};
-
 // This thread's 16-byte chunks of the 128 rows from row r0 of Q into a tile,
 // kThreads threads taking part; rows past the last live one become zero. One division:
 // from row to row the pointer moves by a constant, but for a node's last head.
@@ -292,37 +281,31 @@ __device__ __forceinline__ void copy_q(const TreeParams &p, int b, int kh, int r
 }
 
 template <typename T, int kDim>
-__global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreeParams p, const __grid_constant__ CUtensorMap map, bool tiled) {
+__global__ void __launch_bounds__(kTensorThreads, 2)
+    tree_tensor_kernel(TreeParams p, const __grid_constant__ CUtensorMap map, bool tiled) {
   using Shape = TensorShape<kDim>;
-  extern __shared__ unsigned char tensor_smem[];
-  __shared__ TensorBarriers bar;
-  __shared__ __align__(8) uint16_t s_cached[kMarks][kLoadWarps / 2];  // keys that are cache rows
-  __shared__ uint32_t s_tmem;
-  __shared__ unsigned long long s_bad;  // nodes whose V held a non-finite element
-  __shared__ float2 s_stats[2][kTile];
+  extern __shared__ __align__(1024) unsigned char smem[];
+  unsigned char *k_ring = smem + Shape::q_bytes;
+  unsigned char *v_ring = k_ring + Shape::k_stages * Shape::plane_bytes;
+  TensorShared &sh = *reinterpret_cast<TensorShared *>(smem + Shape::bytes);
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
-  unsigned char *smem = reinterpret_cast<unsigned char *>(
-      (reinterpret_cast<uintptr_t>(tensor_smem) + 1023) & ~(uintptr_t)1023);
   const int tid = threadIdx.x, lane = tid & 31, split = blockIdx.y;
   const int warp = __shfl_sync(kFullMask, tid >> 5, 0);  // the same for every lane, to the compiler too
   const int D = p.head_dim, G = p.groups, all = p.nodes * G, b = blockIdx.z;
   const int n_nodes = nodes_of(p, b), valid = (int)rows_of(p, b), live = n_nodes * G;
-  const int tiles = (all + p.tile_rows - 1) / p.tile_rows;
-  const int kh = blockIdx.x / tiles, r0 = blockIdx.x % tiles * p.tile_rows;
-  const bool apart = p.tile_rows > kTile;  // the streams own different rows
-  const int k_stages = Shape::k_stages + (apart ? 0 : Shape::more);
-  const int v_stages = Shape::v_stages + (apart ? 0 : Shape::more);
-  unsigned char *k_ring = smem + (apart ? 2 : 1) * Shape::q_bytes;
-  unsigned char *v_ring = k_ring + k_stages * Shape::plane_bytes;
+  const int tiles = (all + kTile - 1) / kTile;
+  const int kh = blockIdx.x / tiles, r0 = blockIdx.x % tiles * kTile;
   // the keys of this split: begin .. end - 1
   const unsigned total = r0 < live ? (unsigned)(valid + n_nodes) : 0;
   const unsigned share = ((total + p.splits - 1) / p.splits + kKeys - 1) / kKeys * kKeys;
   const int begin = (int)min((unsigned long long)total, (unsigned long long)split * share);
   const int end = (int)min(total, begin + share);
-  const int blocks = (end - begin + kKeys - 1) / kKeys, items = apart ? 2 * blocks : blocks;
+  const int blocks = (end - begin + kKeys - 1) / kKeys;
 
-  if (blocks == 0) {  // nothing is seen here: zeros, or a split without weight
-    for (int i = warp; i < p.tile_rows && r0 + i < all; i += kTensorThreads / 32) {
+  const bool placed = (smem_addr(smem) & 1023) == 0;  // the swizzle counts on it
+  if (!placed && tid == 0) flag(p.status, HS_DEV_MISALIGNED);
+  if (blocks == 0 || !placed) {  // nothing is seen here: zeros, or a split without weight
+    for (int i = warp; i < kTile && r0 + i < all; i += kTensorThreads / 32) {
       if (p.splits > 1) {
         if (lane == 0)
           p.stats[partial_number(p, b, kh, r0 + i, split)] = make_float2(-INFINITY, 0.f);
@@ -334,33 +317,32 @@ __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreePara
     return;
   }
 
-  // live rows of each stream's tile; a warp without any only takes part in barriers
-  const int live0 = min(kTile, live - r0);
-  const int live1 = apart ? max(0, min(kTile, live - r0 - kTile)) : live0;
+  // A softmax warp without a live row takes no part in the blocks.
+  const int live_here = min(kTile, live - r0), live_warps = (live_here + 31) / 32;
   if (tid == 32 * kSoftmaxWarps)
     asm volatile("prefetch.tensormap [%0];\n" ::"l"(&map) : "memory");
   if (tid == 32 * kScoreWarp) {
     for (int i = 0; i < kMaxStages; ++i) {
-      mbar_init(&bar.k_full[i], kLoadWarps / 2 * (32 + 1));
-      mbar_init(&bar.v_full[i], kLoadWarps / 2 * (32 + 1));
-      mbar_init(&bar.k_free[i], apart ? 2 : 1);
-      mbar_init(&bar.v_free[i], apart ? 2 : 1);
+      mbar_init(&sh.k_full[i], kLoadWarps / 2 * (32 + 1));
+      mbar_init(&sh.v_full[i], kLoadWarps / 2 * (32 + 1));
+      mbar_init(&sh.k_free[i], 1);
+      mbar_init(&sh.v_free[i], 1);
     }
-    for (int w = 0; w < 2; ++w)
-      for (int i = 0; i < 2; ++i) {
-        mbar_init(&bar.s_full[w][i], 2);  // the products, and the marks that came with their keys
-        mbar_init(&bar.p_full[w][i], max(1, ((w ? live1 : live0) + 31) / 32));
-        mbar_init(&bar.pv_done[w][i], 1);
-      }
-    s_bad = 0;
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sh.s_full[i], 2);  // the products, and the marks that came with their keys
+      mbar_init(&sh.p_full[i], live_warps);
+      mbar_init(&sh.pv_done[i], 1);
+    }
+    sh.bad = 0;
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
   __syncthreads();
 
   if (warp >= kSoftmaxWarps && warp < kSoftmaxWarps + kLoadWarps) {
     // ---- K or V of the key blocks into its ring -------------------------------------
-    constexpr int warps = kLoadWarps / 2, mine = kKeys / warps;  // keys of a block a warp copies
-    constexpr int chunks = kDim / 8, together = 32 / chunks, steps = mine / together;
+    constexpr int warps = kLoadWarps / 2;
+    constexpr int chunks = kDim / 8, together = 32 / chunks, steps = kRun / together;
+    static_assert(kKeys / warps == 32, "a lane for each key that a warp copies");
     const bool values = warp >= kSoftmaxWarps + warps;
     const int lw = (warp - kSoftmaxWarps) % warps, c = lane % chunks;
     const bool in_dim = c * 8 < D;
@@ -370,23 +352,23 @@ __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreePara
     const T *drafted = static_cast<const T *>(values ? p.value : p.key) +
                        (int64_t)b * p.kv_batch_stride + (int64_t)kh * D + c * 8;
     const int64_t *rows = p.rows + b * p.rows_batch_stride;
-    uint64_t *full = values ? bar.v_full : bar.k_full, *free = values ? bar.v_free : bar.k_free;
-    const int stages = values ? v_stages : k_stages;
-    const uint32_t ring_addr = smem_addr(values ? v_ring : k_ring);
+    uint64_t *full = values ? sh.v_full : sh.k_full, *free = values ? sh.v_free : sh.k_free;
+    const int stages = values ? Shape::v_stages : Shape::k_stages;
     unsigned char *ring = values ? v_ring : k_ring;
-    // lane i < mine reads the row number of the warp's i-th key, kLook blocks ahead:
-    // a block's time is shorter than the read's
+    const uint32_t ring_addr = smem_addr(ring);
+    // a lane reads the row number of one key of the warp's 32, kLook blocks ahead: a
+    // block's time is shorter than the read's
     const int last = min(end, valid);
     auto look = [&](int block) -> int64_t {
-      const int at = begin + block * kKeys + lw * mine + lane;
-      return lane < mine && at < last ? __ldg(rows + at) : -1;
+      const int at = begin + block * kKeys + lw * 32 + lane;
+      return at < last ? __ldg(rows + at) : -1;
     };
     int64_t next[kLook];
 #pragma unroll
     for (int i = 0; i < kLook; ++i) next[i] = i < blocks ? look(i) : -1;
     // Where this lane's first chunk goes; i keys further it is i rows down, and the
     // row's part of the swizzle differs by i (the lane's own part is below `together`).
-    const uint32_t to0 = place<kDim>(lw * mine + lane / chunks, c);
+    const uint32_t to0 = place<kDim>(lw * 32 + lane / chunks, c);
     int slot = 0, turn = 1;
     for (int block = 0; block < blocks; ++block) {
       if (block >= stages) {
@@ -397,346 +379,323 @@ __global__ void __launch_bounds__(kTensorThreads, 1) tree_tensor_kernel(TreePara
           break;
         }
       }
-      const int64_t now = next[0], offset = row_offset(p, now, row_elems);
+      const int64_t row = next[0], offset = row_offset(p, row, row_elems);
 #pragma unroll
       for (int i = 0; i + 1 < kLook; ++i) next[i] = next[i + 1];
       next[kLook - 1] = block + kLook < blocks ? look(block + kLook) : -1;
       if (!values) {
         const unsigned cached = __ballot_sync(kFullMask, offset >= 0);
-        if (lane == 0) s_cached[block % kMarks][lw] = (uint16_t)cached;
+        if (lane == 0) sh.cached[block % kMarks][lw] = cached;
       }
       const uint32_t stage_addr = ring_addr + slot * Shape::plane_bytes;
-      const int at0 = begin + block * kKeys + lw * mine;
-      // Rows that follow one another from a multiple of 8 on, as those of a page do: one
-      // tiled copy. The copy engine keeps more reads in flight than cp.async does.
-      const int64_t row = now, row0 = __shfl_sync(kFullMask, row, 0);
+      // Either half of the warp's rows: rows that follow one another from a multiple of 8
+      // on, as those of a page do, take one tiled copy. The copy engine keeps more reads
+      // in flight than cp.async does.
+      const int64_t row0 = __shfl_sync(kFullMask, row, lane & 16);
       const bool run = tiled && (row0 & 7) == 0 &&
-                       (row0 & (p.page_size - 1)) + kRun <= p.page_size;
-      if (__all_sync(kFullMask, run && (lane >= mine || (offset >= 0 && row == row0 + lane)))) {
+                       (row0 & (p.page_size - 1)) + kRun <= p.page_size && offset >= 0 &&
+                       row == row0 + (lane & 15);
+      const unsigned runs = __ballot_sync(kFullMask, run);
+      const bool first_run = (runs & 0xffff) == 0xffff, second_run = runs >> 16 == 0xffff;
+      if (first_run || second_run) {
+        const int64_t row1 = __shfl_sync(kFullMask, row, 16);
         if (lane == 0) {
-          const int group = (int)(((row0 >> p.page_shift) * 2 * p.page_size +
-                                   (values ? p.page_size : 0) + (row0 & (p.page_size - 1))) >> 3);
-          mbar_arrive_many(&full[slot], 32);
-          mbar_expect_tx(&full[slot], mine * kDim * 2);
-          tile_copy(stage_addr + lw * mine * kDim * 2, &map, kh * (kDim / 64), group, &full[slot]);
+          mbar_add_tx(&full[slot], ((int)first_run + (int)second_run) * kRun * kDim * 2);
+          const auto copy = [&](int64_t from, int half) {
+            const int group = (int)(((from >> p.page_shift) * 2 * p.page_size +
+                                     (values ? p.page_size : 0) + (from & (p.page_size - 1))) >> 3);
+            tile_copy(stage_addr + (lw * 32 + half * kRun) * kDim * 2, &map, kh * (kDim / 64),
+                      group, &full[slot]);
+          };
+          if (first_run) copy(row0, 0);
+          if (second_run) copy(row1, 1);
+          if (first_run && second_run) mbar_arrive_many(&full[slot], 32 + 1);
         }
-        __syncwarp();
-        if (++slot == stages) {
-          slot = 0;
-          turn ^= 1;
-        }
-        continue;
       }
-      int64_t off[steps];
+      if (!first_run || !second_run) {
+        bool written = false;
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+          if (half == 0 ? first_run : second_run) continue;
+          const int first = begin + block * kKeys + lw * 32 + half * kRun;  // its first key
+          if (first + kRun <= valid) {
 #pragma unroll
-      for (int i = 0; i < steps; ++i)
-        off[i] = __shfl_sync(kFullMask, offset, i * together + lane / chunks);
-      if (at0 + mine <= valid) {
-#pragma unroll
-        for (int i = 0; i < steps; ++i) {
-          const int key = i * together;
-          tree_cp_async16(stage_addr + (to0 ^ ((key & 7) << 4)) + (key >> 3) * Shape::atom +
-                              (key & 7) * 128,
-                          off[i] >= 0 ? pool + off[i] : pool, off[i] >= 0 && in_dim);
-        }
-      } else {
-        uint4 raw[steps];  // all loads before the first use
-        const auto node = [&](int i) {
-          const int at = at0 + i * together + lane / chunks;
-          return at >= valid && at < end ? at - valid : -1;
-        };
-#pragma unroll
-        for (int i = 0; i < steps; ++i) {
-          raw[i] = make_uint4(0, 0, 0, 0);
-          if (node(i) >= 0 && in_dim)
-            raw[i] = *reinterpret_cast<const uint4 *>(drafted + node(i) * p.kv_node_stride);
-        }
-#pragma unroll
-        for (int i = 0; i < steps; ++i) {
-          const uint32_t to = place<kDim>(lw * mine + i * together + lane / chunks, c);
-          if (node(i) >= 0) {
-            if (values && clear_nonfinite<T>(raw[i])) atomicOr(&s_bad, 1ull << node(i));
-            *reinterpret_cast<uint4 *>(ring + slot * Shape::plane_bytes + to) = raw[i];
+            for (int i = 0; i < steps; ++i) {
+              const int key = i * together;
+              const int64_t off = __shfl_sync(kFullMask, offset, half * kRun + key + lane / chunks);
+              tree_cp_async16(stage_addr + half * (kRun / 8 * Shape::atom) +
+                                  (to0 ^ ((key & 7) << 4)) + (key >> 3) * Shape::atom +
+                                  (key & 7) * 128,
+                              off >= 0 ? pool + off : pool, off >= 0 && in_dim);
+            }
           } else {
-            tree_cp_async16(stage_addr + to, off[i] >= 0 ? pool + off[i] : pool,
-                            off[i] >= 0 && in_dim);
+            written = true;
+            constexpr int some = steps < 4 ? steps : 4;  // loads in flight
+#pragma unroll 1
+            for (int i0 = 0; i0 < steps; i0 += some) {
+              const auto key = [&](int i) { return (i0 + i) * together + lane / chunks; };
+              const auto node = [&](int i) {  // this lane's key as a node, or -1
+                const int at = first + key(i);
+                return at >= valid && at < end ? at - valid : -1;
+              };
+              uint4 raw[some];
+#pragma unroll
+              for (int i = 0; i < some; ++i) {
+                raw[i] = make_uint4(0, 0, 0, 0);
+                if (node(i) >= 0 && in_dim)
+                  raw[i] = *reinterpret_cast<const uint4 *>(drafted + node(i) * p.kv_node_stride);
+              }
+#pragma unroll
+              for (int i = 0; i < some; ++i) {
+                const uint32_t to = place<kDim>(lw * 32 + half * kRun + key(i), c);
+                const int64_t off = __shfl_sync(kFullMask, offset, half * kRun + key(i));
+                if (node(i) >= 0) {
+                  if (values && clear_nonfinite<T>(raw[i])) atomicOr(&sh.bad, 1ull << node(i));
+                  *reinterpret_cast<uint4 *>(ring + slot * Shape::plane_bytes + to) = raw[i];
+                } else {
+                  tree_cp_async16(stage_addr + to, off >= 0 ? pool + off : pool,
+                                  off >= 0 && in_dim);
+                }
+              }
+            }
           }
         }
-        fence_async_proxy();
+        // Every lane's copies announce themselves when they land; lane 0's arrival
+        // carries what was written with plain stores.
+        if (written) fence_async_proxy();
+        __syncwarp();
+        copies_arrive(&full[slot]);
+        if (lane == 0) mbar_arrive(&full[slot]);
       }
-      // Every lane's copies announce themselves when they land; lane 0's arrival
-      // carries what was written with plain stores.
       __syncwarp();
-      copies_arrive(&full[slot]);
-      if (lane == 0) mbar_arrive(&full[slot]);
       if (++slot == stages) {
         slot = 0;
         turn ^= 1;
       }
     }
     asm volatile("cp.async.wait_all;\n" ::: "memory");
-  } else {
-    if (warp < kSoftmaxWarps) {
-      // Q into both streams' tiles (one tile when they share it)
-      if (apart)
-        copy_q<T, kDim, kTile>(p, b, kh, r0 + tid / kTile * kTile, live,
-                               smem + tid / kTile * Shape::q_bytes, tid % kTile);
-      else
-        copy_q<T, kDim, 2 * kTile>(p, b, kh, r0, live, smem, tid);
-      asm volatile("cp.async.wait_all;\n" ::: "memory");
-      fence_async_proxy();
-    } else if (warp == kOutputWarp) {
-      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(
-                       smem_addr(&s_tmem)),
-                   "r"(2 * kStreamColumns)
-                   : "memory");
-      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n");
-    }
-    fence_before();
-    __syncwarp();
-    asm volatile("bar.sync 2, %0;\n" ::"n"(32 * (kSoftmaxWarps + 2)) : "memory");
-    fence_after();
-    const uint32_t tmem = __shfl_sync(kFullMask, s_tmem, 0);
+    return;
+  }
 
-    if (warp < kSoftmaxWarps) {
-      // ---- softmax of stream w ------------------------------------------------------
-      const int w = warp / 4, quarter = warp % 4;
-      const int mine = apart ? blocks : (blocks + 1 - w) / 2;
-      const int live_here = w ? live1 : live0;
-      const int r = quarter * 32 + lane;  // row of the tile
-      const int row = r0 + (apart ? w * kTile : 0) + r;
-      const uint32_t lanes = tmem + w * kStreamColumns + ((uint32_t)(quarter * 32) << 16);
-      const bool here = quarter < max(1, (live_here + 31) / 32);
-      const uint64_t see = r < live_here ? (uint64_t)p.mask[(int64_t)b * p.nodes + row / G] : 0;
-      const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
-      float m = -INFINITY, l = 0.f;
-      bool ok = true;
-      for (int k = 0; here && k < mine; ++k) {
-        const int block = apart ? k : 2 * k + w, buffer = k & 1;
-        const uint32_t scores = lanes + kColumnsS + buffer * kKeys, weights = scores + kKeys / 2;
-        ok = wait_phase(&bar.s_full[w][buffer], k >> 1 & 1, p.status);
-        if (!__all_sync(kFullMask, ok)) break;
-        fence_after();
-        uint32_t s[32];
-        tmem_load32(s, scores);
-        // keys this row sees: cache rows, then nodes from position n0 on
-        uint64_t seen = *reinterpret_cast<const uint64_t *>(s_cached[block % kMarks]);
-        const int k0 = begin + block * kKeys;
-        if (k0 + kKeys > valid) {
-          const int n0 = max(valid - k0, 0), j0 = k0 + n0 - valid;
-          const int n = min(end, k0 + kKeys) - (k0 + n0);  // nodes in the block
-          const uint64_t nodes = n >= 64 ? ~0ull : (1ull << n) - 1;
-          seen |= (see >> j0 & nodes) << n0;
-        }
-        const bool plain = __all_sync(kFullMask, seen == ~0ull);
-        tmem_load_wait(s);
-        float top = largest(s, plain, (uint32_t)seen);
-        tmem_load32(s, scores + 32);
-        tmem_load_wait(s);
-        top = fmaxf(top, largest(s, plain, (uint32_t)(seen >> 32))) * p.scale_log2;
-        if (__any_sync(kFullMask, top > m + kLazy)) {
-          const float to = fmaxf(m, top);
-          const float f = m == -INFINITY ? 0.f : tree_exp2(m - to);
-          if (k > 0) {  // the output so far
-            ok = wait_phase(&bar.pv_done[w][buffer ^ 1], (k - 1) >> 1 & 1, p.status);
-            if (!__all_sync(kFullMask, ok)) break;
-            fence_after();
-#pragma unroll 1
-            for (int c = 0; c < kDim; c += 16) {
-              uint32_t o[16];
-              tmem_load16(o, lanes + c);
-              tmem_load16_done(o);
-#pragma unroll
-              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-              tmem_store16(lanes + c, o);
-            }
-          }
-          l *= f;
-          m = to;
-        }
-        // a row that has seen nothing keeps m = -inf: its weights are exp2(-inf) = 0
-        const float base = m == -INFINITY ? 0.f : kLift<T> - m;
-        // P takes the columns of the second half of S, which is in registers; the
-        // first half is read again (64 scores at once cost too many registers)
-#pragma unroll
-        for (int h = 1; h >= 0; --h) {
-          if (h == 0) {
-            tmem_load32(s, scores);
-            tmem_load_wait(s);
-            if (!plain) hide(s, (uint32_t)seen);
-          }
-          float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-          uint32_t packed[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float2 e =
-                pack_fma(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), scale2,
-                     make_float2(base, base));
-            const float2 w2 = make_float2(tree_exp2(e.x), tree_exp2(e.y));
-            sums[i % 2] = pack_add(sums[i % 2], w2);
-            packed[i] = pack2<T>(w2.x, w2.y);
-          }
-          tmem_store16(weights + h * 16, packed);
-          sums[0] = pack_add(sums[0], sums[1]);
-          l += sums[0].x + sums[0].y;
-        }
-        tmem_store_wait();
-        fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bar.p_full[w][buffer]);
-      }
-      // ---- the result -----------------------------------------------------------------
-      if (ok && mine > 0)
-        wait_phase(&bar.pv_done[w][(mine - 1) & 1], (mine - 1) >> 1 & 1, p.status);
-      __syncwarp();
+  if (warp < kSoftmaxWarps) {
+    copy_q<T, kDim, kTile>(p, b, kh, r0, live, smem, tid);
+    asm volatile("cp.async.wait_all;\n" ::: "memory");
+    fence_async_proxy();
+  } else if (warp == kOutputWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(
+                     smem_addr(&sh.tmem)),
+                 "r"(kColumns)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n");
+  }
+  fence_before();
+  __syncwarp();
+  asm volatile("bar.sync 2, %0;\n" ::"n"(32 * (kSoftmaxWarps + 2)) : "memory");
+  fence_after();
+  const uint32_t tmem = __shfl_sync(kFullMask, sh.tmem, 0);
+
+  if (warp < kSoftmaxWarps) {
+    // ---- softmax --------------------------------------------------------------------
+    const int r = tid, row = r0 + r;  // this thread's row, of the tile and of all
+    const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
+    const bool here = warp < live_warps, alive = r < live_here;
+    const uint64_t see = alive ? (uint64_t)p.mask[(int64_t)b * p.nodes + row / G] : 0;
+    const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int k = 0; here && k < blocks; ++k) {
+      const int buffer = k & 1;
+      const uint32_t scores = lanes + kColumnsS + buffer * kKeys, weights = scores + kKeys / 2;
+      ok = wait_phase(&sh.s_full[buffer], k >> 1 & 1, p.status);
+      if (!__all_sync(kFullMask, ok)) break;
       fence_after();
-      // With both streams' last products done the rings' memory is free: a row of
-      // fp32 for each query row, so that rows leave in whole lines. Streams of the same
-      // rows have the other's output in their own lanes, and write half the elements each.
-      s_stats[w][r] = here && mine > 0 ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
-      asm volatile("bar.sync 1, %0;\n" ::"n"(32 * kSoftmaxWarps) : "memory");
-      constexpr int pitch = Shape::join_pitch;
-      float *stage = reinterpret_cast<float *>(k_ring) +
-                     ((apart ? w * kTile : 0) + quarter * 32) * pitch;
-      const int d0 = apart ? 0 : w * (kDim / 2), dn = apart ? kDim : kDim / 2;
-      const bool other_mine = !apart && (w == 0 ? blocks > 1 : true);  // it had a block
-      const bool alive = here && r < live_here;
-      float f = 1.f, g = 0.f;  // weights of this stream's output and the other's
-      if (!apart) {
-        const float2 other = s_stats[w ^ 1][r];
-        const float to = fmaxf(m, other.x);
-        f = m == -INFINITY ? 0.f : tree_exp2(m - to);
-        g = other.x == -INFINITY ? 0.f : tree_exp2(other.x - to);
-        // a sum of NaN scores has no maximum: let it through
-        l = (m == -INFINITY ? l : l * f) + (other.x == -INFINITY ? other.y : other.y * g);
+      uint32_t s[32];
+      tmem_load32(s, scores);
+      // keys this row sees: cache rows, then nodes from position n0 on
+      const uint2 cached = *reinterpret_cast<const uint2 *>(sh.cached[k % kMarks]);
+      uint64_t seen = (uint64_t)cached.y << 32 | cached.x;
+      const int k0 = begin + k * kKeys;
+      if (k0 + kKeys > valid) {
+        const int n0 = max(valid - k0, 0), j0 = k0 + n0 - valid;
+        const int n = min(end, k0 + kKeys) - (k0 + n0);  // nodes in the block
+        const uint64_t nodes = n >= 64 ? ~0ull : (1ull << n) - 1;
+        seen |= (see >> j0 & nodes) << n0;
+      }
+      const bool plain = __all_sync(kFullMask, seen == ~0ull);
+      tmem_load_wait(s);
+      float top = largest(s, plain, (uint32_t)seen);
+      tmem_load32(s, scores + 32);
+      tmem_load_wait(s);
+      top = fmaxf(top, largest(s, plain, (uint32_t)(seen >> 32))) * p.scale_log2;
+      if (__any_sync(kFullMask, top > m + kLazy)) {
+        const float to = fmaxf(m, top);
+        const float f = m == -INFINITY ? 0.f : tree_exp2(m - to);
+        if (k > 0) {  // the output so far
+          ok = wait_phase(&sh.pv_done[buffer ^ 1], (k - 1) >> 1 & 1, p.status);
+          if (!__all_sync(kFullMask, ok)) break;
+          fence_after();
+#pragma unroll 1
+          for (int c = 0; c < kDim; c += 16) {
+            uint32_t o[16];
+            tmem_load16(o, lanes + c);
+            tmem_load16_done(o);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+            tmem_store16(lanes + c, o);
+          }
+        }
+        l *= f;
         m = to;
       }
-      if (!alive) l = 0.f;
-      if (p.splits == 1) {  // the result itself; otherwise the unnormalised output
-        const float scale = l > 0.f || l != l ? 1.f / l : 0.f;
-        f *= scale;
-        g *= scale;
-      }
-      if (here) {
-        const uint64_t bad = alive ? s_bad & see : 0;
-        float *own = stage + lane * pitch;
-#pragma unroll 2
-        for (int c = d0; c < d0 + dn; c += 16) {
-          uint32_t x[16], y[16];
-          __syncwarp();
-          tmem_load16(x, lanes + c);
-          tmem_load16(y, (apart ? lanes : lanes ^ kStreamColumns) + c);
-          tmem_load16_done(x, y);
+      // a row that has seen nothing keeps m = -inf: its weights are exp2(-inf) = 0
+      const float base = m == -INFINITY ? 0.f : kLift<T> - m;
+      // P takes the columns of the second half of S, which is in registers; the
+      // first half is read again (64 scores at once cost too many registers)
 #pragma unroll
-          for (int i = 0; i < 16; i += 4) {
-            float v[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              // a stream without a block left nothing in its columns
-              v[e] = mine > 0 ? __uint_as_float(x[i + e]) * f : 0.f;
-              if (other_mine) v[e] = fmaf(g, __uint_as_float(y[i + e]), v[e]);
-            }
-            *reinterpret_cast<float4 *>(own + c + i) = make_float4(v[0], v[1], v[2], v[3]);
-          }
+      for (int h = 1; h >= 0; --h) {
+        if (h == 0) {
+          tmem_load32(s, scores);
+          tmem_load_wait(s);
+          if (!plain) hide(s, (uint32_t)seen);
         }
-        if (bad != 0)
-          for (int d = d0; d < min(D, d0 + dn); ++d)
-            own[d] += nonfinite_sum<T>(p, b, kh, d, bad);
+        float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        uint32_t packed[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float2 e =
+              pack_fma(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])),
+                       scale2, make_float2(base, base));
+          const float2 w2 = make_float2(tree_exp2(e.x), tree_exp2(e.y));
+          sums[i % 2] = pack_add(sums[i % 2], w2);
+          packed[i] = pack2<T>(w2.x, w2.y);
+        }
+        tmem_store16(weights + h * 16, packed);
+        sums[0] = pack_add(sums[0], sums[1]);
+        l += sums[0].x + sums[0].y;
       }
+      tmem_store_wait();
+      fence_before();
       __syncwarp();
-      // The warp's 32 rows, four elements a lane, several rows at once. Lane i knows where
-      // row i goes: its partial number or its offset in `out`.
-      const int first = row - lane, rows_here = max(0, min(32, all - first));
-      const unsigned alive_rows = __ballot_sync(kFullMask, alive);
-      const int64_t number = row < all ? partial_number(p, b, kh, row, split) : 0;
-      const int64_t place_of = p.splits > 1 ? number * D : row < all ? out_offset(p, b, kh, row) : 0;
-      const int lanes_of = dn / 4, d = d0 + lane % lanes_of * 4;
-#pragma unroll 4
-      for (int i = lane / lanes_of; i < 32; i += 32 / lanes_of) {
-        const int64_t to = __shfl_sync(kFullMask, place_of, i) + d;
-        if (i >= rows_here || d >= D) continue;
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (alive_rows >> i & 1) x = *reinterpret_cast<const float4 *>(stage + i * pitch + d);
-        if (p.splits > 1)
-          *reinterpret_cast<float4 *>(p.partials + to) = x;
-        else
-          *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + to) =
-              make_uint2(pack2<T>(x.x, x.y), pack2<T>(x.z, x.w));
-      }
-      if (p.splits > 1 && row < all && (apart || w == 0))
-        p.stats[number] = make_float2(alive ? m : -INFINITY, l);
-    } else if (warp == kScoreWarp) {
-      // ---- S = Q K^T ------------------------------------------------------------------
-      // The whole warp walks the items, so that addresses stay in uniform registers;
-      // one lane issues.
-      const uint32_t idesc = instruction<T>(kKeys, false);
-      const uint32_t q0 = descriptor(smem_addr(smem));
-      const uint32_t k0 = descriptor(smem_addr(k_ring));
-      int slot = 0, turn = 0;
-      for (int n = 0; n < items; ++n) {
-        const int w = n & 1, k = n >> 1, buffer = k & 1;
-        // the products that read this buffer's P, then the keys
-        bool ready = k < 2 || wait_phase(&bar.pv_done[w][buffer], (k - 2) >> 1 & 1, p.status);
-        ready = ready && wait_phase(&bar.k_full[slot], turn, p.status);
-        if (!__all_sync(kFullMask, ready)) break;
-        fence_after();
-        fence_async_proxy();  // the copies are visible to this thread; now to its products
-        const uint32_t q = q0 + (apart ? w * (Shape::q_bytes >> 4) : 0);
-        const uint32_t kd = k0 + slot * (Shape::plane_bytes >> 4);
-        const uint32_t d = tmem + w * kStreamColumns + kColumnsS + buffer * kKeys;
-        if (elect_one()) {
+      if (lane == 0) mbar_arrive(&sh.p_full[buffer]);
+    }
+    // ---- the result -----------------------------------------------------------------
+    if (ok) wait_phase(&sh.pv_done[(blocks - 1) & 1], (blocks - 1) >> 1 & 1, p.status);
+    __syncwarp();
+    fence_after();
+    // With the last products done the rings' memory is free: a row of fp32 for each
+    // query row, so that rows leave in whole lines.
+    constexpr int pitch = Shape::result_pitch;
+    float *stage = reinterpret_cast<float *>(k_ring) + warp * 32 * pitch;
+    if (!alive) l = 0.f;
+    // with one split the result itself, with more the unnormalised output
+    const float scale = p.splits > 1 ? 1.f : l > 0.f || l != l ? 1.f / l : 0.f;
+    if (here) {
+      const uint64_t bad = alive ? sh.bad & see : 0;
+      float *own = stage + lane * pitch;
+#pragma unroll 2
+      for (int c = 0; c < kDim; c += 16) {
+        uint32_t x[16];
+        tmem_load16(x, lanes + c);
+        tmem_load16_done(x);
 #pragma unroll
-          for (int kk = 0; kk < kDim / 16; ++kk)
-            mma_shared<kDim>(d, q + ((kk / 4 * kPanel + kk % 4 * 32) >> 4),
-                             kd + ((kk / 4 * kPanel + kk % 4 * 32) >> 4), idesc, kk > 0);
-          commit(&bar.s_full[w][buffer]);
-          mbar_arrive(&bar.s_full[w][buffer]);
-          commit(&bar.k_free[slot]);
-        }
-        __syncwarp();
-        if ((!apart || w == 1) && ++slot == k_stages) {
-          slot = 0;
-          turn ^= 1;
-        }
+        for (int i = 0; i < 16; i += 4)
+          *reinterpret_cast<float4 *>(own + c + i) =
+              make_float4(__uint_as_float(x[i]) * scale, __uint_as_float(x[i + 1]) * scale,
+                          __uint_as_float(x[i + 2]) * scale, __uint_as_float(x[i + 3]) * scale);
       }
-    } else {
-      // ---- O += P V -------------------------------------------------------------------
-      const uint32_t idesc = instruction<T>(kDim, true);
-      const uint32_t v0 = descriptor(smem_addr(v_ring));
-      int slot = 0, turn = 0;
-      for (int n = 0; n < items; ++n) {
-        const int w = n & 1, k = n >> 1, buffer = k & 1;
-        bool ready = wait_phase(&bar.v_full[slot], turn, p.status);
-        ready = ready && wait_phase(&bar.p_full[w][buffer], k >> 1 & 1, p.status);
-        if (!__all_sync(kFullMask, ready)) break;
-        fence_after();
-        fence_async_proxy();
-        const uint32_t vd = v0 + slot * (Shape::plane_bytes >> 4);
-        const uint32_t d = tmem + w * kStreamColumns;
-        const uint32_t weights = d + kColumnsS + buffer * kKeys + kKeys / 2;
-        if (elect_one()) {
-#pragma unroll
-          for (int kk = 0; kk < kKeys / 16; ++kk)
-            mma_tmem<kDim>(d, weights + kk * 8, vd + (kk * 2 * Shape::atom >> 4), idesc,
-                           k > 0 || kk > 0);
-          commit(&bar.pv_done[w][buffer]);
-          commit(&bar.v_free[slot]);
-        }
-        __syncwarp();
-        if ((!apart || w == 1) && ++slot == v_stages) {
-          slot = 0;
-          turn ^= 1;
-        }
-      }
+      if (bad != 0)
+        for (int d = 0; d < D; ++d) own[d] += nonfinite_sum<T>(p, b, kh, d, bad);
     }
     __syncwarp();
-    fence_before();
-    asm volatile("bar.sync 2, %0;\n" ::"n"(32 * (kSoftmaxWarps + 2)) : "memory");
-    if (warp == kOutputWarp) {
-      fence_after();
-      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem),
-                   "r"(2 * kStreamColumns));
+    // The warp's 32 rows, four elements a lane. Lane i knows where row i goes: its
+    // partial number or its offset in `out`.
+    constexpr int lanes_of = kDim / 4;
+    const int first = row - lane, rows_here = max(0, min(32, all - first));
+    const unsigned alive_rows = __ballot_sync(kFullMask, alive);
+    const int64_t number = row < all ? partial_number(p, b, kh, row, split) : 0;
+    const int64_t place_of = p.splits > 1 ? number * D : row < all ? out_offset(p, b, kh, row) : 0;
+    const int d = lane % lanes_of * 4;
+#pragma unroll 4
+    for (int i = lane / lanes_of; i < 32; i += 32 / lanes_of) {
+      const int64_t to = __shfl_sync(kFullMask, place_of, i) + d;
+      if (i >= rows_here || d >= D) continue;
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (alive_rows >> i & 1) x = *reinterpret_cast<const float4 *>(stage + i * pitch + d);
+      if (p.splits > 1)
+        *reinterpret_cast<float4 *>(p.partials + to) = x;
+      else
+        *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + to) =
+            make_uint2(pack2<T>(x.x, x.y), pack2<T>(x.z, x.w));
     }
+    if (p.splits > 1 && row < all)
+      p.stats[number] = make_float2(alive ? m : -INFINITY, l);
+  } else if (warp == kScoreWarp) {
+    // ---- S = Q K^T ------------------------------------------------------------------
+    // The whole warp walks the blocks, so that addresses stay in uniform registers;
+    // one lane issues.
+    const uint32_t idesc = instruction<T>(kKeys, false);
+    const uint32_t q = descriptor(smem_addr(smem)), k0 = descriptor(smem_addr(k_ring));
+    int slot = 0, turn = 0;
+    for (int k = 0; k < blocks; ++k) {
+      const int buffer = k & 1;
+      // the products that read this buffer's P, then the keys
+      bool ready = k < 2 || wait_phase(&sh.pv_done[buffer], (k - 2) >> 1 & 1, p.status);
+      ready = ready && wait_phase(&sh.k_full[slot], turn, p.status);
+      if (!__all_sync(kFullMask, ready)) break;
+      fence_after();
+      fence_async_proxy();  // the copies are visible to this thread; now to its products
+      const uint32_t kd = k0 + slot * (Shape::plane_bytes >> 4);
+      const uint32_t d = tmem + kColumnsS + buffer * kKeys;
+      if (elect_one()) {
+#pragma unroll
+        for (int kk = 0; kk < kDim / 16; ++kk)
+          mma_shared<kDim>(d, q + ((kk / 4 * kPanel + kk % 4 * 32) >> 4),
+                           kd + ((kk / 4 * kPanel + kk % 4 * 32) >> 4), idesc, kk > 0);
+        commit(&sh.s_full[buffer]);
+        mbar_arrive(&sh.s_full[buffer]);
+        commit(&sh.k_free[slot]);
+      }
+      __syncwarp();
+      if (++slot == Shape::k_stages) {
+        slot = 0;
+        turn ^= 1;
+      }
+    }
+  } else {
+    // ---- O += P V -------------------------------------------------------------------
+    const uint32_t idesc = instruction<T>(kDim, true), v0 = descriptor(smem_addr(v_ring));
+    int slot = 0, turn = 0;
+    for (int k = 0; k < blocks; ++k) {
+      const int buffer = k & 1;
+      bool ready = wait_phase(&sh.v_full[slot], turn, p.status);
+      ready = ready && wait_phase(&sh.p_full[buffer], k >> 1 & 1, p.status);
+      if (!__all_sync(kFullMask, ready)) break;
+      fence_after();
+      fence_async_proxy();
+      const uint32_t vd = v0 + slot * (Shape::plane_bytes >> 4);
+      const uint32_t weights = tmem + kColumnsS + buffer * kKeys + kKeys / 2;
+      if (elect_one()) {
+#pragma unroll
+        for (int kk = 0; kk < kKeys / 16; ++kk)
+          mma_tmem<kDim>(tmem, weights + kk * 8, vd + (kk * 2 * Shape::atom >> 4), idesc,
+                         k > 0 || kk > 0);
+        commit(&sh.pv_done[buffer]);
+        commit(&sh.v_free[slot]);
+      }
+      __syncwarp();
+      if (++slot == Shape::v_stages) {
+        slot = 0;
+        turn ^= 1;
+      }
+    }
+  }
+  __syncwarp();
+  fence_before();
+  asm volatile("bar.sync 2, %0;\n" ::"n"(32 * (kSoftmaxWarps + 2)) : "memory");
+  if (warp == kOutputWarp) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem),
+                 "r"(kColumns));
   }
 }
 
@@ -779,7 +738,7 @@ template <typename T, int kDim> int launch(const TreeParams &p, int dtype, cudaS
   auto kernel = tree_tensor_kernel<T, kDim>;
   const size_t bytes = TensorShape<kDim>::dynamic;
   if (int e = reserve_smem(reinterpret_cast<const void *>(kernel), bytes, "attend_tree")) return e;
-  const int64_t tiles = ceil_div((int64_t)p.nodes * p.groups, p.tile_rows);
+  const int64_t tiles = ceil_div((int64_t)p.nodes * p.groups, kTile);
   // heads side by side: their slices of a cache row are neighbours in memory
   const dim3 grid((unsigned)(p.kv_heads * tiles), (unsigned)p.splits, (unsigned)p.batch);
   CUtensorMap map{};
