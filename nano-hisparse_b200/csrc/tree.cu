@@ -264,12 +264,14 @@ __global__ void __launch_bounds__(32 * kMergeWarps) tree_merge_kernel(TreeParams
   if (item >= p.nodes * p.q_heads) return;
   const int t = item / p.q_heads, h = item % p.q_heads;
   T *out = static_cast<T *>(p.out) + ((int64_t)b * p.nodes * p.q_heads + item) * D;
+  const int64_t first = partial_number(p, b, h / p.groups, t * p.groups + h % p.groups, 0);
+  // The splits are written. Warps of padded nodes wait too: this kernel must not end
+  // before the one that writes the workspace.
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
   if (t >= nodes_of(p, b)) {
     for (int d = lane; d < D; d += 32) out[d] = from_f32<T>(0.f);
     return;
   }
-  const int64_t first = partial_number(p, b, h / p.groups, t * p.groups + h % p.groups, 0);
-  asm volatile("griddepcontrol.wait;\n" ::: "memory");  // the splits are written
   static_assert(kTreeMaxSplits <= 64, "two splits a lane");
   float2 part[2];
 #pragma unroll
