@@ -239,97 +239,124 @@ __global__ void __launch_bounds__(kSimtThreads) tree_simt_kernel(TreeParams p, b
         if (d < D) o[d] = from_f32<T>(row < live ? acc[i][j] * inv : 0.f);
       }
     } else {
-      const int64_t at = partial_number(p, b, kh, row, split);
-      float *o = p.partials + at * D;
+      const int64_t part = part_of(p, b, kh, split);
 #pragma unroll
-      for (int j = 0; j < 4 * NJ; ++j) {
-        const int d = 4 * tx + 64 * (j / 4) + j % 4;
-        if (d < D) o[d] = acc[i][j];
-      }
-      if (tx == 0) p.stats[at] = make_float2(m[i], l[i]);
+      for (int j = 0; j < NJ; ++j)
+        if (4 * tx + 64 * j < D)
+          *quad_of(p, part, row, tx + 16 * j) = make_float4(
+              acc[i][4 * j], acc[i][4 * j + 1], acc[i][4 * j + 2], acc[i][4 * j + 3]);
+      if (tx == 0) *stat_of(p, part, row) = make_float2(m[i], l[i]);
     }
   }
 }
 
 // ---- joining the splits ------------------------------------------------------------------
-// One warp for each (request, node, query head): lane i takes the maxima and sums
-// of splits i and i + 32 to the row's weights exp2(m_i - m), then the warp sums the
-// weighted outputs, a lane 4 neighbouring elements (kFour) or every 32nd one.
-constexpr int kMergeWarps = 4;
+// A block joins 32 elements of 8 query rows of a KV head. Warp i takes row i's maxima and
+// sums, two splits a lane, to the row's weights exp2(m_s - m); then a thread sums the
+// weighted outputs of every fourth split for four neighbouring elements of a row, the
+// loads of four splits in flight (the first before the weights are known), and the four
+// threads' sums are added through shared memory. What bounds it is the chain of those
+// reads, so it wants many threads with few loads each.
+constexpr int kMergeRows = 8, kMergeQuads = 8, kMergeGroups = 4, kMergeAhead = 4;
+constexpr int kMergeThreads = kMergeRows * kMergeQuads * kMergeGroups;
 
-template <typename T, bool kFour>
-__global__ void __launch_bounds__(32 * kMergeWarps) tree_merge_kernel(TreeParams p) {
-  const int lane = threadIdx.x & 31, D = p.head_dim, b = blockIdx.y;
-  const int item = blockIdx.x * kMergeWarps + (threadIdx.x >> 5);
-  if (item >= p.nodes * p.q_heads) return;
-  const int t = item / p.q_heads, h = item % p.q_heads;
-  T *out = static_cast<T *>(p.out) + ((int64_t)b * p.nodes * p.q_heads + item) * D;
-  const int64_t first = partial_number(p, b, h / p.groups, t * p.groups + h % p.groups, 0);
-  // The splits are written. Warps of padded nodes wait too: this kernel must not end
-  // before the one that writes the workspace.
-  asm volatile("griddepcontrol.wait;\n" ::: "memory");
-  if (t >= nodes_of(p, b)) {
-    for (int d = lane; d < D; d += 32) out[d] = from_f32<T>(0.f);
-    return;
-  }
+template <typename T>
+__global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(TreeParams p, bool wide) {
+  static_assert(kMergeThreads == 32 * kMergeRows, "a warp for each row's weights");
   static_assert(kTreeMaxSplits <= 64, "two splits a lane");
-  float2 part[2];
+  __shared__ float weights[kMergeRows][kTreeMaxSplits + 1];  // the last: 1 / sum
+  __shared__ float4 sums[kMergeGroups - 1][kMergeRows * kMergeQuads];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, D = p.head_dim;
+  const int quads = (D + 3) / 4, slices = (quads + kMergeQuads - 1) / kMergeQuads;
+  const int b = blockIdx.z, kh = blockIdx.y, r0 = blockIdx.x / slices * kMergeRows;
+  const int all = p.nodes * p.groups, live = nodes_of(p, b) * p.groups;
+  const int group = threadIdx.x / (kMergeRows * kMergeQuads);
+  const int place = threadIdx.x % (kMergeRows * kMergeQuads);
+  const int r = r0 + place % kMergeRows;
+  const int quad = blockIdx.x % slices * kMergeQuads + place / kMergeRows;
+  const int64_t part = part_of(p, b, kh, 0);
+  // The splits are written. Every thread waits, also where there is nothing to read:
+  // this kernel must not end before the one that writes the workspace.
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  float2 stat[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int s = lane + 32 * i;
-    part[i] = s < p.splits ? p.stats[first + s] : make_float2(-INFINITY, 0.f);
+    stat[i] = s < p.splits && r0 + warp < live ? *stat_of(p, part + s, r0 + warp)
+                                               : make_float2(-INFINITY, 0.f);
   }
-  const float m = warp_max(fmaxf(part[0].x, part[1].x));
+  const bool here = r < live && quad < quads;
+  float4 x[kMergeAhead];
+  const auto load = [&](int s0) {
+#pragma unroll
+    for (int i = 0; i < kMergeAhead; ++i)
+      if (here && s0 + i * kMergeGroups < p.splits)
+        x[i] = *quad_of(p, part + s0 + i * kMergeGroups, r, quad);
+  };
+  load(group);
+  const float m = warp_max(fmaxf(stat[0].x, stat[1].x));
   float weight[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i)  // a split that saw nothing left no output
-    weight[i] = part[i].y == 0.f ? 0.f : tree_exp2(part[i].x - m);
-  const float l = warp_xor_tree_sum(part[0].y * weight[0] + part[1].y * weight[1]);
-  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-  const float *o = p.partials + first * D;
-  for (int d0 = 0; d0 < D; d0 += kFour ? 128 : 32) {
-    const int d = d0 + (kFour ? 4 * lane : lane);
-    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int s = 0; s < p.splits; ++s) {
-      const float w = __shfl_sync(kFullMask, s < 32 ? weight[0] : weight[1], s & 31);
-      if (w == 0.f || d >= D) continue;
-      if constexpr (kFour) {
-        const float4 x = *reinterpret_cast<const float4 *>(o + (int64_t)s * D + d);
-        sum.x = fmaf(w, x.x, sum.x);
-        sum.y = fmaf(w, x.y, sum.y);
-        sum.z = fmaf(w, x.z, sum.z);
-        sum.w = fmaf(w, x.w, sum.w);
-      } else {
-        sum.x = fmaf(w, o[(int64_t)s * D + d], sum.x);
-      }
-    }
-    if (d >= D) continue;
-    out[d] = from_f32<T>(sum.x * inv);
-    if constexpr (kFour) {
-      out[d + 1] = from_f32<T>(sum.y * inv);
-      out[d + 2] = from_f32<T>(sum.z * inv);
-      out[d + 3] = from_f32<T>(sum.w * inv);
+    weight[i] = stat[i].y == 0.f ? 0.f : tree_exp2(stat[i].x - m);
+  const float l = warp_xor_tree_sum(stat[0].y * weight[0] + stat[1].y * weight[1]);
+  weights[warp][lane] = weight[0];
+  weights[warp][lane + 32] = weight[1];
+  if (lane == 0) weights[warp][kTreeMaxSplits] = l > 0.f || l != l ? 1.f / l : 0.f;
+  __syncthreads();
+  const float *w = weights[place % kMergeRows];
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s0 = group; here && s0 < p.splits; s0 += kMergeAhead * kMergeGroups) {
+    if (s0 != group) load(s0);
+#pragma unroll
+    for (int i = 0; i < kMergeAhead; ++i) {
+      const int s = s0 + i * kMergeGroups;
+      if (s >= p.splits || w[s] == 0.f) continue;
+      sum.x = fmaf(w[s], x[i].x, sum.x);
+      sum.y = fmaf(w[s], x[i].y, sum.y);
+      sum.z = fmaf(w[s], x[i].z, sum.z);
+      sum.w = fmaf(w[s], x[i].w, sum.w);
     }
   }
+  if (group > 0) sums[group - 1][place] = sum;
+  __syncthreads();
+  if (group > 0 || r >= all || quad >= quads) return;
+#pragma unroll
+  for (int g = 0; g < kMergeGroups - 1; ++g) {
+    const float4 other = sums[g][place];
+    sum = make_float4(sum.x + other.x, sum.y + other.y, sum.z + other.z, sum.w + other.w);
+  }
+  const float inv = w[kTreeMaxSplits];
+  const float y[4] = {sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv};
+  T *out = static_cast<T *>(p.out) + out_offset(p, b, kh, r) + 4 * quad;
+  if constexpr (sizeof(T) == 2) {
+    if (wide) {  // rows of whole quads, on 8 bytes
+      *reinterpret_cast<uint2 *>(out) = make_uint2(pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]));
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (4 * quad + i < D) out[i] = from_f32<T>(y[i]);
 }
 
 template <typename T> int launch_merge(const TreeParams &p, cudaStream_t s) {
   if (p.splits == 1) return HS_OK;
-  const dim3 grid((unsigned)ceil_div((int64_t)p.nodes * p.q_heads, kMergeWarps),
-                  (unsigned)p.batch);
+  const int64_t slices = ceil_div(p.head_dim, 4 * kMergeQuads);
+  const dim3 grid((unsigned)(ceil_div((int64_t)p.nodes * p.groups, kMergeRows) * slices),
+                  (unsigned)p.kv_heads, (unsigned)p.batch);
   // its launch overlaps the end of the kernel before it, which it waits for itself
   cudaLaunchConfig_t config{};
   config.gridDim = grid;
-  config.blockDim = dim3(32 * kMergeWarps);
+  config.blockDim = dim3(kMergeThreads);
   config.stream = s;
   cudaLaunchAttribute attribute{};
   attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attribute.val.programmaticStreamSerializationAllowed = 1;
   config.attrs = &attribute;
   config.numAttrs = 1;
-  cudaLaunchKernelEx(&config, p.head_dim % 4 == 0 ? tree_merge_kernel<T, true>
-                                                  : tree_merge_kernel<T, false>, p);
+  const bool wide = p.head_dim % 4 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 7) == 0;
+  cudaLaunchKernelEx(&config, tree_merge_kernel<T>, p, wide);
   return check_launch("tree_merge_kernel");
 }
 
@@ -438,7 +465,7 @@ extern "C" size_t hs_attend_tree_workspace_bytes(int batch, int nodes, int q_hea
       tree_shape(batch, nodes, q_heads, kv_heads, head_dim, count, dtype).splits;
   if (splits == 1) return 0;
   const size_t parts = (size_t)batch * nodes * q_heads * splits;
-  return tree_stats_bytes(parts) + parts * head_dim * sizeof(float);
+  return tree_stats_bytes(parts) + parts * ((head_dim + 3) / 4) * sizeof(float4);
 }
 
 extern "C" int hs_attend_tree(int batch, int nodes, const void *query, int64_t query_batch_stride,

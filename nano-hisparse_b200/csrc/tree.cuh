@@ -29,8 +29,10 @@ struct TreeParams {
   int splits;
   float scale_log2;     // log2(e) / sqrt(head_dim): scores are kept in powers of two
   int tile_rows;        // query rows of a block
-  float *partials;      // [batch][kv_heads][nodes * groups][splits][head_dim], unnormalised
-  float2 *stats;        // [batch][kv_heads][nodes * groups][splits]: maximum, sum
+  // unnormalised outputs, four elements of a row together:
+  // [batch][kv_heads][splits][ceil(head_dim / 4)][nodes * groups][4]
+  float *partials;
+  float2 *stats;        // [batch][kv_heads][splits][nodes * groups]: maximum, sum
   int32_t *status;
 };
 
@@ -64,11 +66,18 @@ __device__ __forceinline__ int64_t row_offset(const TreeParams &p, int64_t row, 
   return (block * 2 * p.page_size + within) * row_elems;
 }
 
-// What split `split` leaves for query row r: the unnormalised output's place in
-// `partials` is its number times head_dim, (maximum, sum) is stats[number].
-__device__ __forceinline__ int64_t partial_number(const TreeParams &p, int b, int kh, int r,
-                                                  int split) {
-  return (((int64_t)b * p.kv_heads + kh) * (p.nodes * p.groups) + r) * p.splits + split;
+// What a split leaves: (maximum, sum) of query row r is stat_of(...), elements
+// 4 i .. 4 i + 3 of its unnormalised output are quad_of(..., i). The threads of the
+// tcgen05 kernel and of the joining one have a row each: theirs are neighbours.
+__device__ __forceinline__ int64_t part_of(const TreeParams &p, int b, int kh, int split) {
+  return ((int64_t)b * p.kv_heads + kh) * p.splits + split;
+}
+__device__ __forceinline__ float2 *stat_of(const TreeParams &p, int64_t part, int r) {
+  return p.stats + part * (p.nodes * p.groups) + r;
+}
+__device__ __forceinline__ float4 *quad_of(const TreeParams &p, int64_t part, int r, int i) {
+  return reinterpret_cast<float4 *>(p.partials) +
+         (part * ((p.head_dim + 3) / 4) + i) * (p.nodes * p.groups) + r;
 }
 
 // Where query row r of KV head kh starts in the output.

@@ -361,10 +361,10 @@ __global__ void __launch_bounds__(kMmaThreads, (MmaTile<kDim, kWarpsM>::resident
         out[(int64_t)(row / G) * p.q_heads * D + (int64_t)(kh * G + row % G) * D + d] =
             from_f32<T>(row < live ? x * inv : 0.f);
       else
-        p.partials[partial_number(p, b, kh, row, split) * D + d] = x;
+        reinterpret_cast<float *>(quad_of(p, part_of(p, b, kh, split), row, d / 4))[d % 4] = x;
     }
     if (p.splits > 1 && lane == 0)
-      p.stats[partial_number(p, b, kh, row, split)] = make_float2(m, l);
+      *stat_of(p, part_of(p, b, kh, split), row) = make_float2(m, l);
   }
 }
 

@@ -68,12 +68,9 @@ template <int kDim> struct TensorShape {
   static constexpr int k_stages = kDim == 64 ? 4 : 2, v_stages = kDim == 64 ? 5 : 3;
   static constexpr int bytes = q_bytes + (k_stages + v_stages) * plane_bytes;
   static constexpr size_t dynamic = bytes + 1024;        // and TensorShared
-  static constexpr int result_pitch = kDim + 4;          // floats of a result's row in the rings
   static_assert(k_stages <= kMaxStages && v_stages <= kMaxStages, "barriers");
   static_assert(sizeof(TensorShared) <= 1024, "TensorShared has its place");
   static_assert(2 * (dynamic + 1024) <= 228 * 1024, "two blocks on an SM");
-  static_assert(kTile * result_pitch * 4 <= (k_stages + v_stages) * plane_bytes,
-                "results fit the rings");
 };
 
 // 32 columns of this thread's TMEM lane
@@ -308,7 +305,7 @@ __global__ void __launch_bounds__(kTensorThreads, 2)
     for (int i = warp; i < kTile && r0 + i < all; i += kTensorThreads / 32) {
       if (p.splits > 1) {
         if (lane == 0)
-          p.stats[partial_number(p, b, kh, r0 + i, split)] = make_float2(-INFINITY, 0.f);
+          *stat_of(p, part_of(p, b, kh, split), r0 + i) = make_float2(-INFINITY, 0.f);
       } else {
         T *out = static_cast<T *>(p.out) + out_offset(p, b, kh, r0 + i);
         for (int d = lane; d < D; d += 32) out[d] = from_f32<T>(0.f);
@@ -582,53 +579,55 @@ __global__ void __launch_bounds__(kTensorThreads, 2)
     if (ok) wait_phase(&sh.pv_done[(blocks - 1) & 1], (blocks - 1) >> 1 & 1, p.status);
     __syncwarp();
     fence_after();
-    // With the last products done the rings' memory is free: a row of fp32 for each
-    // query row, so that rows leave in whole lines.
-    constexpr int pitch = Shape::result_pitch;
-    float *stage = reinterpret_cast<float *>(k_ring) + warp * 32 * pitch;
     if (!alive) l = 0.f;
-    // with one split the result itself, with more the unnormalised output
-    const float scale = p.splits > 1 ? 1.f : l > 0.f || l != l ? 1.f / l : 0.f;
-    if (here) {
-      const uint64_t bad = alive ? sh.bad & see : 0;
-      float *own = stage + lane * pitch;
-#pragma unroll 2
-      for (int c = 0; c < kDim; c += 16) {
-        uint32_t x[16];
-        tmem_load16(x, lanes + c);
-        tmem_load16_done(x);
+    const uint64_t bad = alive ? sh.bad & see : 0;
+    if (p.splits > 1) {  // the unnormalised output; rows past the last live one have none
+      const int64_t part = part_of(p, b, kh, split);
+      if (here) {
+        float4 *to = quad_of(p, part, row, 0);
+#pragma unroll 1
+        for (int c = 0; c < kDim; c += 32, to += 8 * all) {
+          uint32_t x[32];
+          tmem_load32(x, lanes + c);
+          tmem_load_wait(x);
 #pragma unroll
-        for (int i = 0; i < 16; i += 4)
-          *reinterpret_cast<float4 *>(own + c + i) =
-              make_float4(__uint_as_float(x[i]) * scale, __uint_as_float(x[i + 1]) * scale,
-                          __uint_as_float(x[i + 2]) * scale, __uint_as_float(x[i + 3]) * scale);
+          for (int i = 0; i < 32; i += 4)
+            if (alive && c + i < D)
+              to[i / 4 * all] = make_float4(__uint_as_float(x[i]), __uint_as_float(x[i + 1]),
+                                            __uint_as_float(x[i + 2]), __uint_as_float(x[i + 3]));
+        }
+      }
+      if (row < all) *stat_of(p, part, row) = make_float2(alive ? m : -INFINITY, l);
+      if (bad != 0)
+        for (int d = 0; d < D; ++d)
+          reinterpret_cast<float *>(quad_of(p, part, row, d / 4))[d % 4] +=
+              nonfinite_sum<T>(p, b, kh, d, bad);
+    } else if (row - lane < all) {  // the result, zeros past the last live row
+      T *out = static_cast<T *>(p.out) + out_offset(p, b, kh, min(row, all - 1));
+      const float scale = l > 0.f || l != l ? 1.f / l : 0.f;
+#pragma unroll 1
+      for (int c = 0; c < kDim; c += 32) {
+        uint32_t x[32];
+        if (here) {
+          tmem_load32(x, lanes + c);
+          tmem_load_wait(x);
+        }
+#pragma unroll
+        for (int i = 0; i < 32; i += 8) {
+          uint4 y = make_uint4(0, 0, 0, 0);
+          if (alive) {
+            const auto two = [&](int j) {
+              return pack2<T>(__uint_as_float(x[i + j]) * scale, __uint_as_float(x[i + j + 1]) * scale);
+            };
+            y = make_uint4(two(0), two(2), two(4), two(6));
+          }
+          if (row < all && c + i < D) *reinterpret_cast<uint4 *>(out + c + i) = y;
+        }
       }
       if (bad != 0)
-        for (int d = 0; d < D; ++d) own[d] += nonfinite_sum<T>(p, b, kh, d, bad);
+        for (int d = 0; d < D; ++d)
+          out[d] = from_f32<T>(to_f32(out[d]) + nonfinite_sum<T>(p, b, kh, d, bad));
     }
-    __syncwarp();
-    // The warp's 32 rows, four elements a lane. Lane i knows where row i goes: its
-    // partial number or its offset in `out`.
-    constexpr int lanes_of = kDim / 4;
-    const int first = row - lane, rows_here = max(0, min(32, all - first));
-    const unsigned alive_rows = __ballot_sync(kFullMask, alive);
-    const int64_t number = row < all ? partial_number(p, b, kh, row, split) : 0;
-    const int64_t place_of = p.splits > 1 ? number * D : row < all ? out_offset(p, b, kh, row) : 0;
-    const int d = lane % lanes_of * 4;
-#pragma unroll 4
-    for (int i = lane / lanes_of; i < 32; i += 32 / lanes_of) {
-      const int64_t to = __shfl_sync(kFullMask, place_of, i) + d;
-      if (i >= rows_here || d >= D) continue;
-      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (alive_rows >> i & 1) x = *reinterpret_cast<const float4 *>(stage + i * pitch + d);
-      if (p.splits > 1)
-        *reinterpret_cast<float4 *>(p.partials + to) = x;
-      else
-        *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + to) =
-            make_uint2(pack2<T>(x.x, x.y), pack2<T>(x.z, x.w));
-    }
-    if (p.splits > 1 && row < all)
-      p.stats[number] = make_float2(alive ? m : -INFINITY, l);
   } else if (warp == kScoreWarp) {
     // ---- S = Q K^T ------------------------------------------------------------------
     // The whole warp walks the blocks, so that addresses stay in uniform registers;
