@@ -361,7 +361,7 @@ template <typename T> int launch_merge(const TreeParams &p, cudaStream_t s) {
 }
 
 // ---- layout of a call ----------------------------------------------------------------------
-enum class TreePath { simt, mma, tensor };
+enum class TreePath { simt, tensor };
 // Bytes of `parts` (maximum, sum) pairs before the outputs, which are read and written 16
 // bytes at a time.
 size_t tree_stats_bytes(size_t parts) { return (parts * sizeof(float2) + 15) / 16 * 16; }
@@ -381,14 +381,10 @@ TreeShape tree_shape(int batch, int nodes, int q_heads, int kv_heads, int head_d
     s.path = TreePath::simt;
     s.rows = kSimtRows;
     s.resident = 2;
-  } else if (head_dim <= 128) {
+  } else {
     s.path = TreePath::tensor;
     s.rows = 128;
-    s.resident = 2;
-  } else {
-    s.path = TreePath::mma;
-    s.rows = queries <= 32 ? 32 : 64;
-    s.resident = 1;
+    s.resident = head_dim <= 128 ? 2 : 1;
   }
   s.keys = 64;
   // The split count with the least (rounds of blocks) x (keys of a block and what a
@@ -430,7 +426,7 @@ template <typename T, int NJ> int launch_simt(const TreeParams &p, cudaStream_t 
 
 template <typename T>
 int launch(const TreeParams &p, TreePath path, int dtype, cudaStream_t s) {
-  // the tensor-core paths copy 16 bytes: every address and stride has to be a multiple
+  // the tensor-core kernel copies 16 bytes: every address and stride has to be a multiple
   const uintptr_t addresses =
       reinterpret_cast<uintptr_t>(p.query) | reinterpret_cast<uintptr_t>(p.key) |
       reinterpret_cast<uintptr_t>(p.value) | reinterpret_cast<uintptr_t>(p.pool);
@@ -440,8 +436,6 @@ int launch(const TreeParams &p, TreePath path, int dtype, cudaStream_t s) {
   int status;
   if (path == TreePath::tensor) {
     status = launch_tree_tensor(p, dtype, s);
-  } else if (path == TreePath::mma) {
-    status = launch_tree_mma(p, dtype, s);
   } else {
     switch (ceil_div(p.head_dim, 64)) {
       case 1: status = launch_simt<T, 1>(p, s); break;
@@ -533,7 +527,6 @@ extern "C" int hs_attend_tree(int batch, int nodes, const void *query, int64_t q
   if (need > 0 && (!workspace || workspace_bytes < need))
     return set_error(HS_ERR_WORKSPACE, "attend_tree: workspace of %zu bytes < required %zu",
                      workspace_bytes, need);
-  p.tile_rows = shape.rows;
   p.stats = static_cast<float2 *>(workspace);
   p.partials = reinterpret_cast<float *>(
       static_cast<char *>(workspace) +

@@ -28,7 +28,6 @@ struct TreeParams {
   int groups;           // query heads of a KV head
   int splits;
   float scale_log2;     // log2(e) / sqrt(head_dim): scores are kept in powers of two
-  int tile_rows;        // query rows of a block
   // unnormalised outputs, four elements of a row together:
   // [batch][kv_heads][splits][ceil(head_dim / 4)][nodes * groups][4]
   float *partials;
@@ -142,9 +141,7 @@ __device__ __forceinline__ float nonfinite_sum(const TreeParams &p, int b, int k
   return x;
 }
 
-// tree_tensor.cu: the tcgen05 kernels; head_dim <= 128, a multiple of 8, 16-bit types
+// tree_tensor.cu: 16-bit types, head_dim a multiple of 8
 int launch_tree_tensor(const TreeParams &p, int dtype, cudaStream_t s);
-int launch_tree_mma(const TreeParams &p, int dtype, cudaStream_t s);
-
 
 }  // namespace hs

@@ -45,7 +45,6 @@ constexpr int kTile = 128;     // query rows
 constexpr int kKeys = 64;      // keys of a block
 constexpr int kLook = 6;       // blocks that row numbers are read ahead
 constexpr unsigned long long kWaitNanoseconds = 4000000000ull;  // then a wait gives up
-constexpr int kColumnsS = 128, kColumns = 256;
 
 struct TensorShared {
   uint64_t k_full[kMaxStages], k_free[kMaxStages], v_full[kMaxStages], v_free[kMaxStages];
@@ -55,8 +54,8 @@ struct TensorShared {
   uint32_t tmem;
 };
 
-// Shared memory of a block. kDim: head_dim rounded up to 64 or 128, the rest zero.
-// An operand is a list of 8-row groups, each of one or two panels of 64 elements
+// Shared memory and TMEM of a block. kDim: head_dim rounded up to 64, 128 or 256, the rest
+// zero. An operand is a list of 8-row groups, each of kDim / 64 panels of 64 elements
 // (128 bytes) a row: a panel of a group is a swizzle atom, and a run of rows in the
 // pool lands in it with one tiled copy.
 // K and V have rings of their own: a stage of K is free when its scores are done, a
@@ -65,12 +64,17 @@ template <int kDim> struct TensorShape {
   static constexpr int atom = kDim / 64 * kPanel;        // bytes of an 8-row group
   static constexpr int q_bytes = kTile * kDim * 2;
   static constexpr int plane_bytes = kKeys * kDim * 2;   // a stage: K or V of a block
-  static constexpr int k_stages = kDim == 64 ? 4 : 2, v_stages = kDim == 64 ? 5 : 3;
+  static constexpr int resident = kDim <= 128 ? 2 : 1;   // blocks on an SM
+  static constexpr int k_stages = kDim == 64 ? 4 : 2;
+  static constexpr int v_stages = kDim == 64 ? 5 : kDim == 128 ? 3 : 2;
+  static constexpr int column_s = kDim <= 128 ? 128 : 256;  // O before it
+  static constexpr int columns = 2 * column_s;
   static constexpr int bytes = q_bytes + (k_stages + v_stages) * plane_bytes;
   static constexpr size_t dynamic = bytes + 1024;        // and TensorShared
   static_assert(k_stages <= kMaxStages && v_stages <= kMaxStages, "barriers");
   static_assert(sizeof(TensorShared) <= 1024, "TensorShared has its place");
-  static_assert(2 * (dynamic + 1024) <= 228 * 1024, "two blocks on an SM");
+  static_assert(resident * (dynamic + 1024) <= 228 * 1024 && resident * columns <= 512,
+                "the blocks fit an SM");
 };
 
 // 32 columns of this thread's TMEM lane
@@ -252,7 +256,7 @@ template <typename T, int kDim, int kThreads>
 __device__ __forceinline__ void copy_q(const TreeParams &p, int b, int kh, int r0, int live,
                                        unsigned char *tile, int thread) {
   constexpr int chunks = kDim / 8, step = kThreads / chunks;
-  static_assert(step % 8 == 0, "a thread's rows have one place in the swizzle");
+  static_assert(step % 4 == 0, "a thread's rows have one or two places in the swizzle");
   const int D = p.head_dim, G = p.groups, c = thread % chunks, r = thread / chunks;
   int left = c * 8 < D ? live - (r0 + r) : 0;  // rows to the last live one
   const int t = (r0 + r) / G, skip = step / G;
@@ -262,12 +266,14 @@ __device__ __forceinline__ void copy_q(const TreeParams &p, int b, int kh, int r
   const int64_t stride = skip * p.q_node_stride + (int64_t)(step - skip * G) * D;
   const int64_t wrap = p.q_node_stride - (int64_t)G * D;
   const int rest = step - skip * G;
-  uint32_t to = smem_addr(tile + place<kDim>(r, c));
+  const uint32_t even = smem_addr(tile) + place<kDim>(r, c);
+  const uint32_t odd = smem_addr(tile) + place<kDim>(r + step, c);
 #pragma unroll
   for (int i = 0; i < kTile / step; ++i) {
+    // two steps are whole groups of 8 rows
+    const uint32_t to = (i % 2 ? odd : even) + i / 2 * (2 * step / 8) * TensorShape<kDim>::atom;
     tree_cp_async16(to, left > 0 ? from : static_cast<const T *>(p.query), left > 0);
     left -= step;
-    to += step / 8 * TensorShape<kDim>::atom;
     from += stride;
     g += rest;
     if (g >= G) {
@@ -278,7 +284,7 @@ __device__ __forceinline__ void copy_q(const TreeParams &p, int b, int kh, int r
 }
 
 template <typename T, int kDim>
-__global__ void __launch_bounds__(kTensorThreads, 2)
+__global__ void __launch_bounds__(kTensorThreads, TensorShape<kDim>::resident)
     tree_tensor_kernel(TreeParams p, const __grid_constant__ CUtensorMap map, bool tiled) {
   using Shape = TensorShape<kDim>;
   extern __shared__ __align__(1024) unsigned char smem[];
@@ -481,7 +487,7 @@ __global__ void __launch_bounds__(kTensorThreads, 2)
   } else if (warp == kOutputWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(
                      smem_addr(&sh.tmem)),
-                 "r"(kColumns)
+                 "r"(Shape::columns)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n");
   }
@@ -502,7 +508,7 @@ __global__ void __launch_bounds__(kTensorThreads, 2)
     bool ok = true;
     for (int k = 0; here && k < blocks; ++k) {
       const int buffer = k & 1;
-      const uint32_t scores = lanes + kColumnsS + buffer * kKeys, weights = scores + kKeys / 2;
+      const uint32_t scores = lanes + Shape::column_s + buffer * kKeys, weights = scores + kKeys / 2;
       ok = wait_phase(&sh.s_full[buffer], k >> 1 & 1, p.status);
       if (!__all_sync(kFullMask, ok)) break;
       fence_after();
@@ -644,7 +650,7 @@ __global__ void __launch_bounds__(kTensorThreads, 2)
       fence_after();
       fence_async_proxy();  // the copies are visible to this thread; now to its products
       const uint32_t kd = k0 + slot * (Shape::plane_bytes >> 4);
-      const uint32_t d = tmem + kColumnsS + buffer * kKeys;
+      const uint32_t d = tmem + Shape::column_s + buffer * kKeys;
       if (elect_one()) {
 #pragma unroll
         for (int kk = 0; kk < kDim / 16; ++kk)
@@ -672,7 +678,7 @@ __global__ void __launch_bounds__(kTensorThreads, 2)
       fence_after();
       fence_async_proxy();
       const uint32_t vd = v0 + slot * (Shape::plane_bytes >> 4);
-      const uint32_t weights = tmem + kColumnsS + buffer * kKeys + kKeys / 2;
+      const uint32_t weights = tmem + Shape::column_s + buffer * kKeys + kKeys / 2;
       if (elect_one()) {
 #pragma unroll
         for (int kk = 0; kk < kKeys / 16; ++kk)
@@ -694,7 +700,7 @@ __global__ void __launch_bounds__(kTensorThreads, 2)
   if (warp == kOutputWarp) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem),
-                 "r"(kColumns));
+                 "r"(Shape::columns));
   }
 }
 
@@ -747,13 +753,15 @@ template <typename T, int kDim> int launch(const TreeParams &p, int dtype, cudaS
   return check_launch("tree_tensor_kernel");
 }
 
+template <typename T> int launch(const TreeParams &p, int dtype, cudaStream_t s) {
+  if (p.head_dim <= 64) return launch<T, 64>(p, dtype, s);
+  return p.head_dim <= 128 ? launch<T, 128>(p, dtype, s) : launch<T, 256>(p, dtype, s);
+}
+
 }  // namespace
 
 int launch_tree_tensor(const TreeParams &p, int dtype, cudaStream_t s) {
-  if (dtype == HS_FLOAT16)
-    return p.head_dim <= 64 ? launch<__half, 64>(p, dtype, s) : launch<__half, 128>(p, dtype, s);
-  return p.head_dim <= 64 ? launch<__nv_bfloat16, 64>(p, dtype, s)
-                          : launch<__nv_bfloat16, 128>(p, dtype, s);
+  return dtype == HS_FLOAT16 ? launch<__half>(p, dtype, s) : launch<__nv_bfloat16>(p, dtype, s);
 }
 
 }  // namespace hs
