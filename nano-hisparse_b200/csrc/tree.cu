@@ -99,63 +99,89 @@ __global__ void __launch_bounds__(kSimtThreads) tree_simt_kernel(TreeParams p, b
   const T *value = static_cast<const T *>(p.value) + b * p.kv_batch_stride + (int64_t)kh * D;
   const int64_t *rows = p.rows + b * p.rows_batch_stride;
 
-  const auto look = [&](int64_t k0) {  // the places of the keys from k0 on, by 64 threads
+  const auto look = [&](int64_t k0) -> int64_t {  // the place of key k0 + tid
     const int64_t i = k0 + tid;
-    s_places[(k0 - begin) / kSimtKeys & 1][tid] =
-        i >= end ? -1 : i < valid ? row_offset(p, rows[i], row_elems) : -2 - (i - valid);
+    return i >= end ? -1 : i < valid ? row_offset(p, rows[i], row_elems) : -2 - (i - valid);
   };
-  if (tid == 0) s_bad = 0;
-  if (tid < kSimtKeys && begin < end) look(begin);
-  const int used = (D + 3) / 4 * 4;  // elements that are not padding, in fours
-  for (int64_t k0 = begin; k0 < end; k0 += kSimtKeys) {
-    __syncthreads();
-    const int64_t *s_src = s_places[(k0 - begin) / kSimtKeys & 1];
+  // K or V of the keys from k0 on. fp32 rows are copied without registers, but for V
+  // of nodes, whose elements that are not finite become 0: nodes that do not see them
+  // would meet 0 * NaN. Those that do get them added at the end.
+  const auto fill = [&](float *plane, bool values, int64_t k0) {
+    const int64_t *places = s_places[(k0 - begin) / kSimtKeys & 1];
+    const bool direct = sizeof(T) == 4 && four && (!values || k0 + kSimtKeys <= valid);
 #pragma unroll 4
     for (int i = tid; i < kSimtKeys * fours; i += kSimtThreads) {
       const int k = i / fours, d = i % fours * 4;
-      const int64_t src = s_src[k];
-      float4 kx = make_float4(0.f, 0.f, 0.f, 0.f), vx = kx;
-      if (src != -1) {
-        const T *kp = src >= 0 ? pool + src : key + (-2 - src) * p.kv_node_stride;
-        const T *vp = src >= 0 ? kp + p.page_size * row_elems : value + (-2 - src) * p.kv_node_stride;
-        kx = load_four(kp, d, D, four);
-        vx = load_four(vp, d, D, four);
-        // A node's V element that is not finite becomes 0 here: nodes that do not see
-        // it would meet 0 * NaN. Those that do get it added at the end.
-        if (src < -1 && !(fabsf(vx.x) < INFINITY && fabsf(vx.y) < INFINITY &&
-                          fabsf(vx.z) < INFINITY && fabsf(vx.w) < INFINITY)) {
-          atomicOr(&s_bad, 1ull << (-2 - src));
-          vx.x = fabsf(vx.x) < INFINITY ? vx.x : 0.f;
-          vx.y = fabsf(vx.y) < INFINITY ? vx.y : 0.f;
-          vx.z = fabsf(vx.z) < INFINITY ? vx.z : 0.f;
-          vx.w = fabsf(vx.w) < INFINITY ? vx.w : 0.f;
-        }
+      const int64_t src = places[k];
+      const T *from = src >= 0    ? pool + src + (values ? p.page_size * row_elems : 0)
+                      : src < -1 ? (values ? value : key) + (-2 - src) * p.kv_node_stride
+                                  : pool;
+      float *to = &plane[k * pitch + d];
+      if (direct) {
+        if (d < D) tree_cp_async16(smem_addr(to), from + d, src != -1);
+        continue;
       }
-      *reinterpret_cast<float4 *>(&sk[k * pitch + d]) = kx;
-      *reinterpret_cast<float4 *>(&sv[k * pitch + d]) = vx;
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (src != -1) x = load_four(from, d, D, four);
+      if (values && src < -1 &&
+          !(fabsf(x.x) < INFINITY && fabsf(x.y) < INFINITY && fabsf(x.z) < INFINITY &&
+            fabsf(x.w) < INFINITY)) {
+        atomicOr(&s_bad, 1ull << (-2 - src));
+        x.x = fabsf(x.x) < INFINITY ? x.x : 0.f;
+        x.y = fabsf(x.y) < INFINITY ? x.y : 0.f;
+        x.z = fabsf(x.z) < INFINITY ? x.z : 0.f;
+        x.w = fabsf(x.w) < INFINITY ? x.w : 0.f;
+      }
+      *reinterpret_cast<float4 *>(to) = x;
     }
-    if (tid < kSimtKeys && k0 + kSimtKeys < end) look(k0 + kSimtKeys);
+  };
+  if (tid == 0) s_bad = 0;
+  int64_t ahead = -1;  // the place of key tid of the tile after the next
+  if (tid < kSimtKeys && begin < end) {
+    s_places[0][tid] = look(begin);
+    ahead = look(begin + kSimtKeys);
+  }
+  __syncthreads();
+  if (begin < end) fill(sk, false, begin);
+  const int used = (D + 3) / 4 * 4;  // elements that are not padding, in fours
+  // V of a tile lands while its scores are computed, K of the next one while the output is
+  for (int64_t k0 = begin; k0 < end; k0 += kSimtKeys) {
+    asm volatile("cp.async.wait_all;\n" ::: "memory");
     __syncthreads();
+    fill(sv, true, k0);
+    const int64_t *s_src = s_places[(k0 - begin) / kSimtKeys & 1];
+    if (tid < kSimtKeys) {
+      s_places[((k0 - begin) / kSimtKeys + 1) & 1][tid] = ahead;
+      ahead = look(k0 + 2 * kSimtKeys);
+    }
     float s[4][4];  // rows 4 ty + i, keys tx + 16 j
+    {
+      float2 s2[4][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
+        for (int j = 0; j < 4; ++j) s2[i][j] = make_float2(0.f, 0.f);
 #pragma unroll 2
-    for (int d = 0; d < used; d += 4) {
-      float4 q4[4], k4[4];
+      for (int d = 0; d < used; d += 4) {
+        float4 q4[4], k4[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        q4[i] = *reinterpret_cast<const float4 *>(&sq[(4 * ty + i) * pitch + d]);
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        k4[j] = *reinterpret_cast<const float4 *>(&sk[(tx + 16 * j) * pitch + d]);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i)
+          q4[i] = *reinterpret_cast<const float4 *>(&sq[(4 * ty + i) * pitch + d]);
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          s[i][j] = fmaf(q4[i].x, k4[j].x, fmaf(q4[i].y, k4[j].y,
-                    fmaf(q4[i].z, k4[j].z, fmaf(q4[i].w, k4[j].w, s[i][j]))));
+          k4[j] = *reinterpret_cast<const float4 *>(&sk[(tx + 16 * j) * pitch + d]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            s2[i][j] = pack_fma(make_float2(q4[i].z, q4[i].w), make_float2(k4[j].z, k4[j].w),
+                                pack_fma(make_float2(q4[i].x, q4[i].y),
+                                         make_float2(k4[j].x, k4[j].y), s2[i][j]));
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[i][j] = s2[i][j].x + s2[i][j].y;
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -185,7 +211,9 @@ __global__ void __launch_bounds__(kSimtThreads) tree_simt_kernel(TreeParams p, b
 #pragma unroll
       for (int j = 0; j < 4 * NJ; ++j) acc[i][j] *= alpha;
     }
-    __syncwarp();  // a row's probabilities are written and read by the same half warp
+    asm volatile("cp.async.wait_all;\n" ::: "memory");
+    __syncthreads();
+    if (k0 + kSimtKeys < end) fill(sk, false, k0 + kSimtKeys);
 #pragma unroll 2
     for (int k = 0; k < kSimtKeys; k += 4) {
       float4 w4[4];
@@ -201,10 +229,12 @@ __global__ void __launch_bounds__(kSimtThreads) tree_simt_kernel(TreeParams p, b
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float w = e == 0 ? w4[i].x : e == 1 ? w4[i].y : e == 2 ? w4[i].z : w4[i].w;
-            acc[i][4 * j] = fmaf(w, v4.x, acc[i][4 * j]);
-            acc[i][4 * j + 1] = fmaf(w, v4.y, acc[i][4 * j + 1]);
-            acc[i][4 * j + 2] = fmaf(w, v4.z, acc[i][4 * j + 2]);
-            acc[i][4 * j + 3] = fmaf(w, v4.w, acc[i][4 * j + 3]);
+            float *o = &acc[i][4 * j];
+            const float2 lo = pack_fma(make_float2(w, w), make_float2(v4.x, v4.y),
+                                       make_float2(o[0], o[1]));
+            const float2 hi = pack_fma(make_float2(w, w), make_float2(v4.z, v4.w),
+                                       make_float2(o[2], o[3]));
+            o[0] = lo.x, o[1] = lo.y, o[2] = hi.x, o[3] = hi.y;
           }
         }
     }
