@@ -19,19 +19,23 @@ namespace hs {
 namespace {
 
 // ---- fp32 arithmetic: every type, head_dim and alignment -------------------------------
-// 128 threads over a tile of 32 query rows and 64 keys, operands widened to fp32
-// in shared memory. For the scores a thread holds 4 rows x 4 keys, for the output
-// 4 rows x 4 NJ elements, so that four products follow each shared-memory word.
+// 128 threads over a tile of 32 query rows and 32 to 64 keys, operands widened to fp32
+// in shared memory. For the scores a thread holds 4 rows x 2 to 4 keys, for the output
+// 4 rows x 4 NJ elements, so that four products follow each shared-memory word. A warp
+// issues every fifth clock (its products wait for shared memory and for each other), so
+// the tile is as small as it takes for two to four blocks on an SM.
 constexpr int kSimtThreads = 128;
 constexpr int kSimtRows = 32;
-constexpr int kSimtKeys = 64;
-constexpr int kSimtPPitch = kSimtKeys + 4;
 
 template <int NJ> struct SimtShape {
-  static constexpr int dim = 64 * NJ;     // head_dim rounded up, the rest zero
+  static constexpr int keys = NJ == 1 ? 64 : NJ == 2 ? 48 : 32;
+  static constexpr int resident = NJ == 1 ? 4 : NJ == 2 ? 3 : 2;  // blocks on an SM
+  static constexpr int p_pitch = keys + 4;
+  static constexpr int dim = 64 * NJ;     // head_dim rounded up
   static constexpr int pitch = dim + 4;   // floats between rows
   static constexpr size_t bytes =
-      sizeof(float) * ((kSimtRows + 2 * kSimtKeys) * pitch + kSimtRows * kSimtPPitch);
+      sizeof(float) * ((kSimtRows + 2 * keys) * pitch + kSimtRows * p_pitch);
+  static_assert(resident * (bytes + 1024 + 2048) <= 228 * 1024, "the blocks fit an SM");
 };
 
 // Elements d .. d + 3 of a row of head_dim D as fp32, zero past its end. `four`: one
@@ -50,15 +54,16 @@ __device__ __forceinline__ float4 load_four(const T *row, int d, int D, bool fou
 }
 
 template <typename T, int NJ>
-__global__ void __launch_bounds__(kSimtThreads) tree_simt_kernel(TreeParams p, bool four) {
+__global__ void __launch_bounds__(kSimtThreads, SimtShape<NJ>::resident) tree_simt_kernel(TreeParams p, bool four) {
   using Shape = SimtShape<NJ>;
   constexpr int dim = Shape::dim, pitch = Shape::pitch;
+  constexpr int keys = Shape::keys, p_pitch = Shape::p_pitch, KJ = keys / 16;
   extern __shared__ __align__(16) float smem[];
-  float *sq = smem, *sk = sq + kSimtRows * pitch, *sv = sk + kSimtKeys * pitch;
-  float *sp = sv + kSimtKeys * pitch;
+  float *sq = smem, *sk = sq + kSimtRows * pitch, *sv = sk + keys * pitch;
+  float *sp = sv + keys * pitch;
   // where each key of this tile and the next lives: >= 0 an element offset in the pool,
   // -1 nowhere, -2 - j node j
-  __shared__ int64_t s_places[2][kSimtKeys];
+  __shared__ int64_t s_places[2][keys];
   __shared__ uint64_t s_mask[kSimtRows];
   __shared__ unsigned long long s_bad;  // nodes whose V held a non-finite element
   const int tid = threadIdx.x, split = blockIdx.x;
@@ -67,7 +72,7 @@ __global__ void __launch_bounds__(kSimtThreads) tree_simt_kernel(TreeParams p, b
   const int D = p.head_dim, G = p.groups;
   const int n_nodes = nodes_of(p, b), live = n_nodes * G;  // query rows with a result
   const int64_t valid = rows_of(p, b), total = valid + n_nodes;
-  const int64_t chunk = ceil_div(ceil_div(total, p.splits), kSimtKeys) * kSimtKeys;
+  const int64_t chunk = ceil_div(ceil_div(total, p.splits), keys) * keys;
   const int64_t begin = split * chunk, end = min(total, begin + chunk);
   const int tx = tid & 15, ty = tid >> 4;  // keys / elements; rows 4 ty .. 4 ty + 3
 
@@ -107,10 +112,10 @@ __global__ void __launch_bounds__(kSimtThreads) tree_simt_kernel(TreeParams p, b
   // of nodes, whose elements that are not finite become 0: nodes that do not see them
   // would meet 0 * NaN. Those that do get them added at the end.
   const auto fill = [&](float *plane, bool values, int64_t k0) {
-    const int64_t *places = s_places[(k0 - begin) / kSimtKeys & 1];
-    const bool direct = sizeof(T) == 4 && four && (!values || k0 + kSimtKeys <= valid);
+    const int64_t *places = s_places[(k0 - begin) / keys & 1];
+    const bool direct = sizeof(T) == 4 && four && (!values || k0 + keys <= valid);
 #pragma unroll 4
-    for (int i = tid; i < kSimtKeys * fours; i += kSimtThreads) {
+    for (int i = tid; i < keys * fours; i += kSimtThreads) {
       const int k = i / fours, d = i % fours * 4;
       const int64_t src = places[k];
       const T *from = src >= 0    ? pool + src + (values ? p.page_size * row_elems : 0)
@@ -137,43 +142,43 @@ __global__ void __launch_bounds__(kSimtThreads) tree_simt_kernel(TreeParams p, b
   };
   if (tid == 0) s_bad = 0;
   int64_t ahead = -1;  // the place of key tid of the tile after the next
-  if (tid < kSimtKeys && begin < end) {
+  if (tid < keys && begin < end) {
     s_places[0][tid] = look(begin);
-    ahead = look(begin + kSimtKeys);
+    ahead = look(begin + keys);
   }
   __syncthreads();
   if (begin < end) fill(sk, false, begin);
   const int used = (D + 3) / 4 * 4;  // elements that are not padding, in fours
   // V of a tile lands while its scores are computed, K of the next one while the output is
-  for (int64_t k0 = begin; k0 < end; k0 += kSimtKeys) {
+  for (int64_t k0 = begin; k0 < end; k0 += keys) {
     asm volatile("cp.async.wait_all;\n" ::: "memory");
     __syncthreads();
     fill(sv, true, k0);
-    const int64_t *s_src = s_places[(k0 - begin) / kSimtKeys & 1];
-    if (tid < kSimtKeys) {
-      s_places[((k0 - begin) / kSimtKeys + 1) & 1][tid] = ahead;
-      ahead = look(k0 + 2 * kSimtKeys);
+    const int64_t *s_src = s_places[(k0 - begin) / keys & 1];
+    if (tid < keys) {
+      s_places[((k0 - begin) / keys + 1) & 1][tid] = ahead;
+      ahead = look(k0 + 2 * keys);
     }
-    float s[4][4];  // rows 4 ty + i, keys tx + 16 j
+    float s[4][KJ];  // rows 4 ty + i, keys tx + 16 j
     {
-      float2 s2[4][4];
+      float2 s2[4][KJ];
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s2[i][j] = make_float2(0.f, 0.f);
+        for (int j = 0; j < KJ; ++j) s2[i][j] = make_float2(0.f, 0.f);
 #pragma unroll 2
       for (int d = 0; d < used; d += 4) {
-        float4 q4[4], k4[4];
+        float4 q4[4], k4[KJ];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           q4[i] = *reinterpret_cast<const float4 *>(&sq[(4 * ty + i) * pitch + d]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < KJ; ++j)
           k4[j] = *reinterpret_cast<const float4 *>(&sk[(tx + 16 * j) * pitch + d]);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
+          for (int j = 0; j < KJ; ++j)
             s2[i][j] = pack_fma(make_float2(q4[i].z, q4[i].w), make_float2(k4[j].z, k4[j].w),
                                 pack_fma(make_float2(q4[i].x, q4[i].y),
                                          make_float2(k4[j].x, k4[j].y), s2[i][j]));
@@ -181,13 +186,13 @@ __global__ void __launch_bounds__(kSimtThreads) tree_simt_kernel(TreeParams p, b
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[i][j] = s2[i][j].x + s2[i][j].y;
+        for (int j = 0; j < KJ; ++j) s[i][j] = s2[i][j].x + s2[i][j].y;
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       float top = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < KJ; ++j) {
         const int64_t src = s_src[tx + 16 * j];
         const bool seen = src >= 0 || (src < -1 && (s_mask[4 * ty + i] >> (-2 - src) & 1));
         s[i][j] = seen ? s[i][j] * p.scale_log2 : -INFINITY;
@@ -199,10 +204,10 @@ __global__ void __launch_bounds__(kSimtThreads) tree_simt_kernel(TreeParams p, b
       const float alpha = m[i] == -INFINITY ? 0.f : exp2f(m[i] - m_new);
       float sum = 0.f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < KJ; ++j) {
         const float w = s[i][j] == -INFINITY ? 0.f : exp2f(s[i][j] - m_new);
         sum += w;
-        sp[(4 * ty + i) * kSimtPPitch + tx + 16 * j] = w;
+        sp[(4 * ty + i) * p_pitch + tx + 16 * j] = w;
       }
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(kFullMask, sum, o);
@@ -213,13 +218,13 @@ __global__ void __launch_bounds__(kSimtThreads) tree_simt_kernel(TreeParams p, b
     }
     asm volatile("cp.async.wait_all;\n" ::: "memory");
     __syncthreads();
-    if (k0 + kSimtKeys < end) fill(sk, false, k0 + kSimtKeys);
+    if (k0 + keys < end) fill(sk, false, k0 + keys);
 #pragma unroll 2
-    for (int k = 0; k < kSimtKeys; k += 4) {
+    for (int k = 0; k < keys; k += 4) {
       float4 w4[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        w4[i] = *reinterpret_cast<const float4 *>(&sp[(4 * ty + i) * kSimtPPitch + k]);
+        w4[i] = *reinterpret_cast<const float4 *>(&sp[(4 * ty + i) * p_pitch + k]);
 #pragma unroll
       for (int e = 0; e < 4; ++e)
 #pragma unroll
@@ -410,13 +415,13 @@ TreeShape tree_shape(int batch, int nodes, int q_heads, int kv_heads, int head_d
   if (dtype == HS_FLOAT32 || head_dim % 8 != 0) {
     s.path = TreePath::simt;
     s.rows = kSimtRows;
-    s.resident = 2;
+    s.resident = head_dim <= 64 ? 4 : head_dim <= 128 ? 3 : 2;
   } else {
     s.path = TreePath::tensor;
     s.rows = 128;
     s.resident = head_dim <= 128 ? 2 : 1;
   }
-  s.keys = 64;
+  s.keys = s.path == TreePath::tensor || head_dim <= 64 ? 64 : head_dim <= 128 ? 48 : 32;
   // The split count with the least (rounds of blocks) x (keys of a block and what a
   // block costs besides, as much as about 384 keys); splits of less than
   // two tiles are not worth joining, but for the fp32 kernel, whose tiles take longest.
