@@ -14,6 +14,11 @@
 // best, is found in half the time, but made a fifth of the threads read again: half as
 // much traffic again on rows that L2 does not hold.)
 //
+// 2,048 rows of 128,256 take 191 us in fp32 with 5 alternatives (5.5 TB/s, 0.84 of a
+// measured copy; 184 us without alternatives, 279 with 32) and 125 us in bf16 (4.2 TB/s,
+// bound by widening and summing: 114 without alternatives). Rows whose entries are all
+// equal take one pass for each alternative (64 rows in bf16, 32 alternatives: 94 us).
+//
 // A row is split over a cluster of 1 to 8 blocks, which join their sums and their
 // best keys in the first block's shared memory: few rows reach many SMs without
 // a workspace or a second launch.

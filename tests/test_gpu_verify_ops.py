@@ -534,6 +534,29 @@ def test_tree_nonfinite_values_out_of_sight(dtype, bad, dim):
     assert not flags()
 
 
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+def test_tree_nonfinite_value_of_a_vanishing_weight(dtype):
+    """A value that is not finite makes the result not finite however small its
+    weight is, also when the splits are joined: 4,096 cache rows score 128, the
+    node -128, so that its weight exp(-256) is 0 in fp32."""
+    from hisparse_b200 import attend_tree, tree_mask
+
+    (q, k, v), _, pool, rows, config = tree_inputs(1, 1, 2, 1, 64, 16, 4096, dtype, 21)
+    q.fill_(8.0)
+    pool[:, 0] = 2.0
+    k.fill_(-2.0)
+    v[..., 5] = math.inf
+    got = attend_tree(q, k, v, tree_mask([[-1]], DEV), pool, rows, config)
+    assert not got[..., 5].isfinite().any()
+    rest = torch.arange(64, device=DEV) != 5
+    assert got[..., rest].isfinite().all()
+    want = pool[:, 1].double()[rows[0] // 16, rows[0] % 16].mean(0)  # equal scores
+    # equal weights (exponents of up to 185 in fp32: 1 + 185 F each), an addition each of a
+    # term of at most max |v| in fp32, one rounding
+    bound = half_step(dtype) * want.abs() + 4400 * F * pool[:, 1].double().abs().max()
+    assert_within(got[0, 0][:, rest], want[:, rest].expand(2, -1), bound[:, rest].expand(2, -1))
+
+
 def test_tree_strided_inputs_and_bad_rows():
     """Views of a fused projection, an expanded row list, heads that are not
     adjacent; a row beyond the pool is skipped and flagged."""
