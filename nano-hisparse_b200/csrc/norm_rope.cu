@@ -27,6 +27,7 @@ namespace {
 constexpr int kRopeThreads = 256;
 constexpr int kRopeWarps = kRopeThreads / 32;
 constexpr int kRopeMaxDim = 256;
+constexpr int kRopeResident = 3;  // blocks on an SM
 
 struct RopeParams {
   int64_t tokens;
@@ -134,8 +135,8 @@ __device__ __forceinline__ uint4 choose(bool first, const uint4 &a, const uint4 
 }
 
 template <typename T, int kGroup>
-__global__ void __launch_bounds__(kRopeThreads, 3) norm_rope_kernel(RopeParams p, int spans,
-                                                                 int span) {
+__global__ void __launch_bounds__(kRopeThreads, kRopeResident)
+    norm_rope_kernel(RopeParams p, int spans, int span) {
   constexpr int kVec = 16 / sizeof(T), kHeads = 32 / kGroup;
   const int lane = threadIdx.x & 31, j = lane % kGroup;
   const int all = p.heads[0] + p.heads[1], half = p.head_dim / 2;
@@ -235,12 +236,22 @@ __global__ void __launch_bounds__(kRopeThreads, 3) norm_rope_kernel(RopeParams p
 }
 
 template <typename T, int kGroup> int launch_vector(const RopeParams &p, cudaStream_t s) {
-  // One token's heads are split over warps until every SM has 16 of them: few
-  // tokens spread out, many tokens compute their angles once.
+  // One token's heads are split over `spans` warps so that (rounds of blocks) x (head
+  // sets of a warp and its angles, as much as about two) is least: few tokens spread out,
+  // many compute their angles once, and the last round is not a nearly empty one.
   const int sets = (int)ceil_div(p.heads[0] + p.heads[1], 32 / kGroup);
-  const int64_t want = ceil_div((int64_t)16 * sm_count(), p.tokens);
-  const int spans0 = (int)(want < 1 ? 1 : (want > sets ? sets : want));
-  const int span = (int)ceil_div(sets, spans0), spans = (int)ceil_div(sets, span);
+  int span = sets, spans = 1;
+  int64_t least = 0;
+  for (int n = 1; n <= sets; ++n) {
+    const int each = (int)ceil_div(sets, n), warps = (int)ceil_div(sets, each);
+    const int64_t rounds = ceil_div(ceil_div(p.tokens * warps, kRopeWarps),
+                                    (int64_t)kRopeResident * sm_count());
+    if (n == 1 || rounds * (each + 2) < least) {
+      least = rounds * (each + 2);
+      span = each;
+      spans = warps;
+    }
+  }
   const int64_t blocks = ceil_div(p.tokens * spans, kRopeWarps);
   if (blocks > 0x7fffffff)
     return set_error(HS_ERR_UNSUPPORTED, "norm_rope: too many tokens");
