@@ -562,7 +562,7 @@ def test_tree_strided_inputs_and_bad_rows():
     adjacent; a row beyond the pool is skipped and flagged."""
     from hisparse_b200 import _lib, attend_tree, tree_mask
 
-    for dtype, dim in ((FP32, 32), (BF16, 128), (BF16, 64), (FP16, 40)):
+    for dtype, dim in ((FP32, 32), (BF16, 128), (BF16, 64), (FP16, 40), (BF16, 256)):
         inputs, parents, pool, rows, config = tree_inputs(3, 6, 8, 2, dim, 16, 100, dtype, 13)
         mask = tree_mask(parents, DEV)
         fused = torch.cat([x.flatten(2) for x in inputs], -1)
@@ -616,7 +616,7 @@ def test_tree_runs_equal_single_rows():
     equal within the bound of their sums."""
     from hisparse_b200 import attend_tree, tree_mask
 
-    for dtype, dim in ((BF16, 128), (FP16, 64)):
+    for dtype, dim in ((BF16, 128), (FP16, 64), (BF16, 256), (FP16, 192)):
         inputs, parents, pool, rows, config = tree_inputs(3, 40, 8, 2, dim, 64, 1000, dtype, 18)
         mask = tree_mask(parents, DEV)
         rows[1, 100:300] = -1
