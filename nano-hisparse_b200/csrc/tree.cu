@@ -293,30 +293,31 @@ __global__ void __launch_bounds__(kSimtThreads, SimtShape<NJ>::resident) tree_si
 }
 
 // ---- joining the splits ------------------------------------------------------------------
-// A block joins 32 elements of 8 query rows of a KV head. Warp i takes row i's maxima and
+// A block joins elements of 8 query rows of a KV head. Warp i takes row i's maxima and
 // sums, two splits a lane, to the row's weights exp2(m_s - m); then a thread sums the
-// weighted outputs of every fourth split for four neighbouring elements of a row, the
-// loads of four splits in flight (the first before the weights are known), and the four
-// threads' sums are added through shared memory. What bounds it is the chain of those
-// reads, so it wants many threads with few loads each.
-constexpr int kMergeRows = 8, kMergeQuads = 8, kMergeGroups = 4, kMergeAhead = 4;
-constexpr int kMergeThreads = kMergeRows * kMergeQuads * kMergeGroups;
+// weighted outputs of every kGroups-th split for four neighbouring elements of a row, the
+// loads of four splits in flight (the first before the weights are known), and the
+// kGroups threads' sums are added through shared memory. With few rows the chain of those
+// reads bounds it, so four threads share the splits; with many, or few splits, its
+// instructions do, and one thread takes all (4,096 rows of two splits: 2 us of 43 less; 8,192 rows of nine: 4 of 186).
+constexpr int kMergeRows = 8, kMergeThreads = 32 * kMergeRows, kMergeAhead = 4;
+constexpr int kMergeGroups = 4;
 
-template <typename T>
-__global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(TreeParams p, bool wide) {
-  static_assert(kMergeThreads == 32 * kMergeRows, "a warp for each row's weights");
+template <typename T, int kGroups>
+__global__ void __launch_bounds__(kMergeThreads, 6) tree_merge_kernel(TreeParams p, bool wide) {
   static_assert(kTreeMaxSplits <= 64, "two splits a lane");
+  constexpr int kQuads = kMergeThreads / kMergeRows / kGroups, kPlaces = kMergeRows * kQuads;
   __shared__ float weights[kMergeRows][kTreeMaxSplits + 1];  // the last: 1 / sum
-  __shared__ float4 sums[kMergeGroups - 1][kMergeRows * kMergeQuads];
+  __shared__ float4 sums[kGroups > 1 ? kGroups - 1 : 1][kPlaces];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, D = p.head_dim;
-  const int quads = (D + 3) / 4, slices = (quads + kMergeQuads - 1) / kMergeQuads;
+  const int quads = (D + 3) / 4, slices = (quads + kQuads - 1) / kQuads;
   const int b = blockIdx.z, kh = blockIdx.y, r0 = blockIdx.x / slices * kMergeRows;
   const int all = p.nodes * p.groups, live = nodes_of(p, b) * p.groups;
-  const int group = threadIdx.x / (kMergeRows * kMergeQuads);
-  const int place = threadIdx.x % (kMergeRows * kMergeQuads);
+  const int group = threadIdx.x / kPlaces, place = threadIdx.x % kPlaces;
   const int r = r0 + place % kMergeRows;
-  const int quad = blockIdx.x % slices * kMergeQuads + place / kMergeRows;
-  const int64_t part = part_of(p, b, kh, 0);
+  const int quad = blockIdx.x % slices * kQuads + place / kMergeRows;
+  const int64_t part = part_of(p, b, kh, 0), step = (int64_t)quads * all;
+  const float4 *from = quad_of(p, part, r, quad) + group * step;  // of this thread's first split
   // The splits are written. Every thread waits, also where there is nothing to read:
   // this kernel must not end before the one that writes the workspace.
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
@@ -331,9 +332,8 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(TreeParams p,
   float4 x[kMergeAhead];
   const auto load = [&](int s0) {
 #pragma unroll
-    for (int i = 0; i < kMergeAhead; ++i)
-      if (here && s0 + i * kMergeGroups < p.splits)
-        x[i] = *quad_of(p, part + s0 + i * kMergeGroups, r, quad);
+    for (int i = 0; i < kMergeAhead; ++i, from += kGroups * step)
+      if (here && s0 + i * kGroups < p.splits) x[i] = *from;
   };
   load(group);
   const float m = warp_max(fmaxf(stat[0].x, stat[1].x));
@@ -348,11 +348,11 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(TreeParams p,
   __syncthreads();
   const float *w = weights[place % kMergeRows];
   float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int s0 = group; here && s0 < p.splits; s0 += kMergeAhead * kMergeGroups) {
+  for (int s0 = group; here && s0 < p.splits; s0 += kMergeAhead * kGroups) {
     if (s0 != group) load(s0);
 #pragma unroll
     for (int i = 0; i < kMergeAhead; ++i) {
-      const int s = s0 + i * kMergeGroups;
+      const int s = s0 + i * kGroups;
       if (s >= p.splits || w[s] < 0.f) continue;
       sum.x = fmaf(w[s], x[i].x, sum.x);
       sum.y = fmaf(w[s], x[i].y, sum.y);
@@ -360,11 +360,13 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(TreeParams p,
       sum.w = fmaf(w[s], x[i].w, sum.w);
     }
   }
-  if (group > 0) sums[group - 1][place] = sum;
-  __syncthreads();
+  if constexpr (kGroups > 1) {
+    if (group > 0) sums[group - 1][place] = sum;
+    __syncthreads();
+  }
   if (group > 0 || r >= all || quad >= quads) return;
 #pragma unroll
-  for (int g = 0; g < kMergeGroups - 1; ++g) {
+  for (int g = 0; g < kGroups - 1; ++g) {
     const float4 other = sums[g][place];
     sum = make_float4(sum.x + other.x, sum.y + other.y, sum.z + other.z, sum.w + other.w);
   }
@@ -384,9 +386,14 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(TreeParams p,
 
 template <typename T> int launch_merge(const TreeParams &p, cudaStream_t s) {
   if (p.splits == 1) return HS_OK;
-  const int64_t slices = ceil_div(p.head_dim, 4 * kMergeQuads);
-  const dim3 grid((unsigned)(ceil_div((int64_t)p.nodes * p.groups, kMergeRows) * slices),
-                  (unsigned)p.kv_heads, (unsigned)p.batch);
+  // threads when one takes all splits of four elements
+  const int64_t quads = ceil_div(p.head_dim, 4), rows = (int64_t)p.nodes * p.groups;
+  const int64_t threads = quads * rows * p.kv_heads * p.batch;
+  const int groups = p.splits > kMergeAhead && threads * kMergeGroups <= (int64_t)2048 * sm_count()
+                         ? kMergeGroups : 1;
+  const int64_t slices = ceil_div(quads, kMergeThreads / kMergeRows / groups);
+  const dim3 grid((unsigned)(ceil_div(rows, kMergeRows) * slices), (unsigned)p.kv_heads,
+                  (unsigned)p.batch);
   // its launch overlaps the end of the kernel before it, which it waits for itself
   cudaLaunchConfig_t config{};
   config.gridDim = grid;
@@ -398,7 +405,8 @@ template <typename T> int launch_merge(const TreeParams &p, cudaStream_t s) {
   config.attrs = &attribute;
   config.numAttrs = 1;
   const bool wide = p.head_dim % 4 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 7) == 0;
-  cudaLaunchKernelEx(&config, tree_merge_kernel<T>, p, wide);
+  cudaLaunchKernelEx(&config, groups == 1 ? tree_merge_kernel<T, 1>
+                                          : tree_merge_kernel<T, kMergeGroups>, p, wide);
   return check_launch("tree_merge_kernel");
 }
 

@@ -23,8 +23,8 @@
 // softmax overlap. What bounds it: up to about 50 nodes the reads of K and V, beyond
 // that the chain score, softmax, product (special functions 41 %, tensor pipe 60 %);
 // with few keys the chain of its start (counts, row numbers, keys: 4 us).
-// 8 requests of 32 nodes, 32,768 rows, 32 query and 8 KV heads of 128 in bf16: 186 us with
-// the join, 5.2 TB/s (6.7 in the steady part); 213 with one block of two tiles on an SM,
+// 8 requests of 32 nodes, 32,768 rows, 32 query and 8 KV heads of 128 in bf16: 182 us with
+// the join, 5.3 TB/s (6.7 in the steady part); 213 with one block of two tiles on an SM,
 // 217 with pages of 8 rows, whose copies all go through cp.async, where pages of 16 take
 // 203 (every node and row present). 8 requests of 63 nodes, 8,192 rows, 28 query and 4 KV
 // heads: 78 us, 757 TFLOP/s. 8 requests of 8 nodes, 8,192 rows, 16 query and 4 KV heads of
