@@ -240,13 +240,16 @@ template <typename T, int kGroup> int launch_vector(const RopeParams &p, cudaStr
   // sets of a warp and its angles, as much as about two) is least: few tokens spread out,
   // many compute their angles once, and the last round is not a nearly empty one.
   const int sets = (int)ceil_div(p.heads[0] + p.heads[1], 32 / kGroup);
+  const int64_t places = (int64_t)kRopeResident * sm_count();
   int span = sets, spans = 1;
   int64_t least = 0;
-  for (int n = 1; n <= sets; ++n) {
+  // a warp for every set where one round holds them
+  const bool one_round = p.tokens * sets <= places * kRopeWarps;
+  const int from = one_round ? sets : 1, to = one_round ? sets : sets < 64 ? sets : 64;
+  for (int n = from; n <= to; ++n) {
     const int each = (int)ceil_div(sets, n), warps = (int)ceil_div(sets, each);
-    const int64_t rounds = ceil_div(ceil_div(p.tokens * warps, kRopeWarps),
-                                    (int64_t)kRopeResident * sm_count());
-    if (n == 1 || rounds * (each + 2) < least) {
+    const int64_t rounds = ceil_div(ceil_div(p.tokens * warps, kRopeWarps), places);
+    if (n == from || rounds * (each + 2) < least) {
       least = rounds * (each + 2);
       span = each;
       spans = warps;

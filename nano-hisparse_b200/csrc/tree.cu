@@ -416,6 +416,12 @@ enum class TreePath { simt, tensor };
 // bytes at a time.
 size_t tree_stats_bytes(size_t parts) { return (parts * sizeof(float2) + 15) / 16 * 16; }
 
+size_t tree_workspace(int64_t rows, int splits, int head_dim) {
+  if (splits == 1) return 0;
+  const size_t parts = (size_t)rows * splits;
+  return tree_stats_bytes(parts) + parts * ((head_dim + 3) / 4) * sizeof(float4);
+}
+
 // How a call is laid out: query rows of a block's tile, blocks on an SM, keys of a
 // step, splits of the key list.
 struct TreeShape {
@@ -505,11 +511,9 @@ extern "C" size_t hs_attend_tree_workspace_bytes(int batch, int nodes, int q_hea
   using namespace hs;
   if (batch < 1 || nodes < 1 || kv_heads < 1 || q_heads < kv_heads || head_dim < 1 || count < 0)
     return 0;
-  const int splits =
-      tree_shape(batch, nodes, q_heads, kv_heads, head_dim, count, dtype).splits;
-  if (splits == 1) return 0;
-  const size_t parts = (size_t)batch * nodes * q_heads * splits;
-  return tree_stats_bytes(parts) + parts * ((head_dim + 3) / 4) * sizeof(float4);
+  return tree_workspace((int64_t)batch * nodes * q_heads,
+                        tree_shape(batch, nodes, q_heads, kv_heads, head_dim, count, dtype).splits,
+                        head_dim);
 }
 
 extern "C" int hs_attend_tree(int batch, int nodes, const void *query, int64_t query_batch_stride,
@@ -570,8 +574,7 @@ extern "C" int hs_attend_tree(int batch, int nodes, const void *query, int64_t q
   const TreeShape shape = tree_shape(batch, nodes, q_heads, kv_heads, head_dim, count, dtype);
   p.splits = shape.splits;
   p.scale_log2 = (float)(1.4426950408889634 / sqrt((double)head_dim));
-  const size_t need =
-      hs_attend_tree_workspace_bytes(batch, nodes, q_heads, kv_heads, head_dim, count, dtype);
+  const size_t need = tree_workspace((int64_t)batch * nodes * q_heads, p.splits, head_dim);
   if (need > 0 && (reinterpret_cast<uintptr_t>(workspace) & 15) != 0)
     return set_error(HS_ERR_WORKSPACE, "attend_tree: the workspace must be 16-byte aligned");
   if (need > 0 && (!workspace || workspace_bytes < need))

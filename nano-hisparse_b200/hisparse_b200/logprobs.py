@@ -51,10 +51,15 @@ def token_logprobs(logits, tokens=None, top=0) -> TokenLogprobs:
     if inner != 1:
         logits = logits.contiguous()
         row_stride = vocab
-    logprobs = logits.new_empty(shape, dtype=torch.float32)
-    entropy = logits.new_empty(rows, dtype=torch.float32)
-    top_logprobs = logits.new_empty((rows, top), dtype=torch.float32)
+    # like one another where the shapes agree: that is made faster than a new shape
+    if tokens is None:
+        logprobs = logits.new_empty(shape, dtype=torch.float32)
+    else:
+        logprobs = torch.empty_like(tokens, dtype=torch.float32)
+    entropy = torch.empty_like(logprobs) if len(shape) == 1 else \
+        logits.new_empty(rows, dtype=torch.float32)
     top_tokens = logits.new_empty((rows, top), dtype=torch.int64)
+    top_logprobs = torch.empty_like(top_tokens, dtype=torch.float32)
     with _lib.on_device(index):
         status = _lib.load().hs_token_logprobs(
             rows, logits.data_ptr(), row_stride, _lib.dtype_code(logits.dtype), vocab, address,

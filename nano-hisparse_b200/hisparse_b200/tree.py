@@ -100,7 +100,7 @@ def attend_tree(query, key, value, mask, pool, rows, config, counts=None, nodes=
     with _lib.on_device(index):
         nbytes = lib.hs_attend_tree_workspace_bytes(batch, width, q_heads, kv_heads, dim, count,
                                                     code)
-        ws = _lib.workspace(nbytes, query.device)
+        ws = query.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
         status = lib.hs_attend_tree(
             batch, width, query.data_ptr(), q_batch, q_node, key.data_ptr(), value.data_ptr(),
             strides[0], strides[1], code, mask.data_ptr(), limits[1], pool.data_ptr(), blocks,
