@@ -14,7 +14,7 @@
 // best, is found in half the time, but made a fifth of the threads read again: half as
 // much traffic again on rows that L2 does not hold.)
 //
-// 2,048 rows of 128,256 take 191 us in fp32 with 5 alternatives (5.5 TB/s, 0.84 of a
+// 2,048 rows of 128,256 take 190 us in fp32 with 5 alternatives (5.5 TB/s, 0.84 of a
 // measured copy; 184 us without alternatives, 279 with 32) and 125 us in bf16 (4.2 TB/s,
 // bound by widening and summing: 114 without alternatives). Rows whose entries are all
 // equal take one pass for each alternative (64 rows in bf16, 32 alternatives: 94 us).
@@ -30,9 +30,9 @@
 namespace hs {
 namespace {
 
-constexpr int kLogprobThreads = 256;
+constexpr int kLogprobThreads = 256;  // of a block, or half as many
 constexpr int kLogprobWarps = kLogprobThreads / 32;
-constexpr int kLogprobBlocks = 4;   // blocks resident on an SM
+constexpr int kLogprobBlocks = 4;   // blocks resident on an SM, and twice as many of those
 constexpr int kMaxTop = 32;
 constexpr int kMaxCluster = 8;
 constexpr int kAhead = 4;           // 16-byte vectors in flight per thread
@@ -226,7 +226,7 @@ template <typename T> struct RowPart {
 // Collects the block's entries with a key of at least `threshold`; returns their
 // number, of which the first kCandidates are kept. `mine`: a key that no entry of
 // this thread passes.
-template <typename T>
+template <int kThreads, typename T>
 __device__ __forceinline__ int collect(LogprobShared &sh, const RowPart<T> &part, uint64_t mine,
                                        uint64_t threshold) {
   if (threadIdx.x == 0) sh.found = 0;
@@ -242,7 +242,7 @@ __device__ __forceinline__ int collect(LogprobShared &sh, const RowPart<T> &part
   const int lane = threadIdx.x & 31, first = threadIdx.x - lane;
   for (unsigned todo = __ballot_sync(kFullMask, mine >= threshold); todo != 0; todo &= todo - 1) {
     const int owner = first + __ffs(todo) - 1;
-    part.each(owner + lane * kLogprobThreads, 32 * kLogprobThreads, [&](const uint4 &raw, int v) {
+    part.each(owner + lane * kThreads, 32 * kThreads, [&](const uint4 &raw, int v) {
       if (value_order(Vector<T>::largest(raw)) < least) return;
       float x[Vector<T>::n];
       Vector<T>::widen(raw, x);
@@ -258,7 +258,7 @@ __device__ __forceinline__ int collect(LogprobShared &sh, const RowPart<T> &part
 
 // The block's `top` largest keys into sh.best (0 where it has fewer entries).
 // `mine` is this thread's best key, `bound` one that no entry of it passes.
-template <typename T>
+template <int kThreads, typename T>
 __device__ __forceinline__ void block_best(LogprobShared &sh, const RowPart<T> &part, int top,
                                            uint64_t mine, uint64_t bound) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -275,18 +275,18 @@ __device__ __forceinline__ void block_best(LogprobShared &sh, const RowPart<T> &
   // with all of them, for half the steps
   uint64_t threshold = search(0, 63, 48);
   if (threshold == 0) threshold = 1;  // fewer threads with entries than `top`: all of them
-  int found = collect(sh, part, bound, threshold);
+  int found = collect<kThreads>(sh, part, bound, threshold);
   if (found > kCandidates) {
     // Many entries are near that value or equal to it: the rest of the key tells them
     // apart, equal ones by their index.
     const uint64_t exact = search(threshold >> 48 << 48, 47, 0);
     if (exact > threshold) {
       threshold = exact;
-      found = collect(sh, part, bound, threshold);
+      found = collect<kThreads>(sh, part, bound, threshold);
     }
   }
   if (found <= kCandidates) {
-    for (int i = threadIdx.x; i < found; i += kLogprobThreads) {
+    for (int i = threadIdx.x; i < found; i += kThreads) {
       const uint64_t key = sh.candidates[i];
       int rank = 0;
       for (int j = 0; j < found; ++j) rank += sh.candidates[j] > key;
@@ -299,7 +299,7 @@ __device__ __forceinline__ void block_best(LogprobShared &sh, const RowPart<T> &
       auto take = [&](uint64_t key) {
         if (key < below && key > next) next = key;
       };
-      part.each(threadIdx.x, kLogprobThreads, [&](const uint4 &raw, int v) {
+      part.each(threadIdx.x, kThreads, [&](const uint4 &raw, int v) {
         float x[Vector<T>::n];
         Vector<T>::widen(raw, x);
 #pragma unroll
@@ -311,7 +311,7 @@ __device__ __forceinline__ void block_best(LogprobShared &sh, const RowPart<T> &
       if (lane == 0) sh.warp_best[warp] = next;
       __syncthreads();
       below = sh.warp_best[0];
-      for (int w = 1; w < kLogprobWarps; ++w)
+      for (int w = 1; w < kThreads / 32; ++w)
         if (sh.warp_best[w] > below) below = sh.warp_best[w];
       if (threadIdx.x == 0) sh.best[k] = below;
     }
@@ -319,9 +319,10 @@ __device__ __forceinline__ void block_best(LogprobShared &sh, const RowPart<T> &
   __syncthreads();
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kLogprobThreads, kLogprobBlocks)
+template <typename T, int kThreads>
+__global__ void __launch_bounds__(kThreads, kLogprobBlocks *kLogprobThreads / kThreads)
     logprobs_kernel(LogprobParams p) {
+  constexpr int kWarps = kThreads / 32;
   __shared__ LogprobShared sh;
   const int rank = (int)cluster_rank(), cluster = p.cluster;
   const int64_t row = blockIdx.x / cluster;
@@ -334,20 +335,20 @@ __global__ void __launch_bounds__(kLogprobThreads, kLogprobBlocks)
   Softmax acc{-INFINITY, 0.f, 0.f};
   int at = -1;  // the vector that first held this thread's maximum
   uint4 raw[kAhead], next[kAhead];
-  part.load(threadIdx.x, kLogprobThreads, next);
-  for (int v0 = threadIdx.x; v0 < part.count; v0 += kAhead * kLogprobThreads) {
+  part.load(threadIdx.x, kThreads, next);
+  for (int v0 = threadIdx.x; v0 < part.count; v0 += kAhead * kThreads) {
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) raw[u] = next[u];
-    part.load(v0 + kAhead * kLogprobThreads, kLogprobThreads, next);  // while these are summed
+    part.load(v0 + kAhead * kThreads, kThreads, next);  // while these are summed
     float largest = -INFINITY;
     int where = v0;
 #pragma unroll
     for (int u = 0; u < kAhead; ++u)
-      if (v0 + u * kLogprobThreads < part.count) {
+      if (v0 + u * kThreads < part.count) {
         const float m = Vector<T>::largest(raw[u]);
         if (m > largest || (m != m && largest == largest)) {
           largest = m;
-          where = v0 + u * kLogprobThreads;
+          where = v0 + u * kThreads;
         }
       }
     if (at < 0 || largest > acc.m || (largest != largest && acc.m == acc.m)) {
@@ -358,7 +359,7 @@ __global__ void __launch_bounds__(kLogprobThreads, kLogprobBlocks)
     float2 s2 = make_float2(acc.s, 0.f), t2 = make_float2(acc.t, 0.f);
 #pragma unroll
     for (int u = 0; u < kAhead; ++u)
-      if (v0 + u * kLogprobThreads < part.count) {
+      if (v0 + u * kThreads < part.count) {
         float e[Vector<T>::n];
         Vector<T>::widen(raw[u], e);
         acc.add(e, s2, t2);
@@ -389,13 +390,13 @@ __global__ void __launch_bounds__(kLogprobThreads, kLogprobBlocks)
     sh.parts[warp][1] = acc.s;
     sh.parts[warp][2] = acc.t;
   }
-  if (p.top > 0) block_best(sh, part, p.top, mine, bound);
+  if (p.top > 0) block_best<kThreads>(sh, part, p.top, mine, bound);
   else __syncthreads();
 
   if (cluster > 1) asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
   LogprobShared &out = *(cluster > 1 ? map_rank(&sh, 0) : &sh);
   if (warp == 0) {
-    acc = Softmax::part(sh.parts[lane % kLogprobWarps], lane < kLogprobWarps);
+    acc = Softmax::part(sh.parts[lane % kWarps], lane < kWarps);
     acc.join_warp();
     if (lane < 3) out.joined[rank][lane] = lane == 0 ? acc.m : lane == 1 ? acc.s : acc.t;
   }
@@ -413,7 +414,7 @@ __global__ void __launch_bounds__(kLogprobThreads, kLogprobBlocks)
   const float log_s = logf(acc.s);
   // (x - m) - log s: one rounding less than x - lse for entries near the maximum
   auto logprob = [&](float v) { return empty ? -INFINITY : (v - acc.m) - log_s; };
-  for (int c = threadIdx.x; c < p.given; c += kLogprobThreads) {
+  for (int c = threadIdx.x; c < p.given; c += kThreads) {
     const int64_t where = row * p.given + c;
     const int64_t token = p.tokens64 ? static_cast<const int64_t *>(p.tokens)[where]
                                      : static_cast<const int32_t *>(p.tokens)[where];
@@ -451,13 +452,23 @@ int logprob_cluster(int64_t rows, int64_t row_bytes) {
 }
 
 template <typename T> int launch(LogprobParams &p, int64_t rows, cudaStream_t s) {
-  static_assert(kMaxCluster * kMaxTop <= kLogprobThreads, "one thread for each joined key");
+  static_assert(kMaxCluster * kMaxTop <= kLogprobThreads && kMaxTop <= kLogprobThreads / 2,
+                "one thread for each joined key");
   p.cluster = logprob_cluster(rows, (int64_t)p.vocab * sizeof(T));
   if (rows * p.cluster > 0x7fffffff)
     return set_error(HS_ERR_UNSUPPORTED, "logprobs: too many rows");
+  // More rows than places: blocks of half the threads, twice as many of them on an SM, let
+  // what a block costs besides its reads overlap that of more others. Better for rows of up
+  // to 64 KB (2,048 rows of 4,000 in bf16, 5 alternatives: 31 -> 23 us, of 32,000: even) and
+  // where it makes one round of two (700 rows of 128,256 in bf16: 66 -> 59); longer rows in
+  // more rounds are read faster by large blocks (2,048 of 128,256 in fp32: 204, else 233).
+  const int64_t places = (int64_t)kLogprobBlocks * sm_count();
+  const bool small = p.cluster == 1 && rows > places &&
+                     ((int64_t)p.vocab * sizeof(T) <= 64 * 1024 || rows <= 2 * places);
+  const int threads = small ? kLogprobThreads / 2 : kLogprobThreads;
   cudaLaunchConfig_t config{};
   config.gridDim = dim3((unsigned)(rows * p.cluster));
-  config.blockDim = dim3(kLogprobThreads);
+  config.blockDim = dim3((unsigned)threads);
   config.stream = s;
   cudaLaunchAttribute attribute{};
   attribute.id = cudaLaunchAttributeClusterDimension;
@@ -465,7 +476,9 @@ template <typename T> int launch(LogprobParams &p, int64_t rows, cudaStream_t s)
   attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
   config.attrs = &attribute;
   config.numAttrs = p.cluster > 1 ? 1 : 0;
-  cudaLaunchKernelEx(&config, logprobs_kernel<T>, p);
+  cudaLaunchKernelEx(&config, threads == kLogprobThreads
+                                  ? logprobs_kernel<T, kLogprobThreads>
+                                  : logprobs_kernel<T, kLogprobThreads / 2>, p);
   return check_launch("logprobs_kernel");
 }
 

@@ -259,6 +259,28 @@ def test_logprobs(dtype, rows, vocab, given, top):
     assert not flags()
 
 
+@pytest.mark.parametrize("dtype", [FP32, FP16, BF16])
+@pytest.mark.parametrize("rows,vocab,given,top", [
+    (700, 4099, 3, 5), (1300, 4104, 1, 32), (650, 8190, 200, 1), (640, 30011, 1, 20)])
+def test_logprobs_more_rows_than_places(dtype, rows, vocab, given, top):
+    """More rows than the GPU holds blocks for: blocks of half the threads, also with
+    more given tokens than those, odd row strides and every row twice."""
+    from hisparse_b200 import token_logprobs
+
+    gen = torch.Generator().manual_seed(rows * vocab)
+    logits = (3 * torch.randn(rows // 2, vocab, generator=gen)).to(dtype)
+    logits[1] = 0.5                       # all equal
+    logits[2, ::2] = -math.inf
+    logits[3] = torch.finfo(dtype).min
+    logits[4] = (torch.arange(vocab) % 2).to(dtype)
+    tokens = torch.randint(-1, vocab, (rows // 2, given), generator=gen)
+    logits, tokens = logits.to(DEV), tokens.to(DEV)
+    got = token_logprobs(logits.repeat(2, 1), tokens.repeat(2, 1), top=top)
+    for half in (slice(0, rows // 2), slice(rows // 2, None)):
+        logprobs_check(type(got)(*(x[half] for x in got)), logits, tokens, top)
+    assert not flags()
+
+
 @pytest.mark.parametrize("dtype", [FP32, BF16])
 def test_logprobs_ties_and_orders(dtype):
     """Equal logits go to the lower token, in constant, ascending, descending and
