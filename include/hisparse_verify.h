@@ -61,6 +61,8 @@ HS_API int hs_qk_norm_rope(int64_t tokens, const void *query, int64_t query_toke
  * [batch, nodes, q_heads, head_dim]. A row beyond the pool is skipped and
  * raises HS_DEV_ROW_OUT_OF_RANGE. The workspace is 16-byte aligned and
  * needs no initialisation; calls that may overlap on the GPU need separate ones.
+ * Every other address has its element's alignment; 16-bit calls are an order of
+ * magnitude faster where all of them, out included, are multiples of 16 bytes.
  */
 HS_API size_t hs_attend_tree_workspace_bytes(int batch, int nodes, int q_heads, int kv_heads,
                                              int head_dim, int64_t count, int dtype);

@@ -482,10 +482,12 @@ template <typename T, int NJ> int launch_simt(const TreeParams &p, cudaStream_t 
 
 template <typename T>
 int launch(const TreeParams &p, TreePath path, int dtype, cudaStream_t s) {
-  // the tensor-core kernel copies 16 bytes: every address and stride has to be a multiple
+  // the tensor-core kernel copies 16 bytes: every address and stride has to be a multiple,
+  // that of the result too where it writes it itself (the join looks at it on its own)
   const uintptr_t addresses =
       reinterpret_cast<uintptr_t>(p.query) | reinterpret_cast<uintptr_t>(p.key) |
-      reinterpret_cast<uintptr_t>(p.value) | reinterpret_cast<uintptr_t>(p.pool);
+      reinterpret_cast<uintptr_t>(p.value) | reinterpret_cast<uintptr_t>(p.pool) |
+      (p.splits == 1 ? reinterpret_cast<uintptr_t>(p.out) : 0);
   const int64_t strides =
       p.q_batch_stride | p.q_node_stride | p.kv_batch_stride | p.kv_node_stride;
   if ((addresses & 15) != 0 || (strides & 7) != 0) path = TreePath::simt;
