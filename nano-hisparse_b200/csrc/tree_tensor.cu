@@ -343,7 +343,7 @@ __global__ void __launch_bounds__(kTensorThreads, TensorShape<kDim>::resident)
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sh.s_full[i], 2);  // the products, and the marks that came with their keys
       mbar_init(&sh.p_full[i], live_warps);
-      mbar_init(&sh.pv_done[i], 1);
+      mbar_init(&sh.pv_done[i], 2);  // the products, and the marks that came with their values
     }
     sh.bad = 0;
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
@@ -694,6 +694,7 @@ __global__ void __launch_bounds__(kTensorThreads, TensorShape<kDim>::resident)
           mma_tmem<kDim>(tmem, weights + kk * 8, vd + (kk * 2 * Shape::atom >> 4), idesc,
                          k > 0 || kk > 0);
         commit(&sh.pv_done[buffer]);
+        mbar_arrive(&sh.pv_done[buffer]);  // sh.bad reaches the softmax warps by this one
         commit(&sh.v_free[slot]);
       }
       __syncwarp();
