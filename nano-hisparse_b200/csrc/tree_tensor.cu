@@ -650,10 +650,11 @@ __global__ void __launch_bounds__(kTensorThreads, TensorShape<kDim>::resident)
     const uint32_t idesc = instruction<T>(kKeys, false);
     const uint32_t q = descriptor(smem_addr(smem)), k0 = descriptor(smem_addr(k_ring));
     int slot = 0, turn = 0;
+    bool ready = true;
     for (int k = 0; k < blocks; ++k) {
       const int buffer = k & 1;
       // the products that read this buffer's P, then the keys
-      bool ready = k < 2 || wait_phase(&sh.pv_done[buffer], (k - 2) >> 1 & 1, p.status);
+      ready = k < 2 || wait_phase(&sh.pv_done[buffer], (k - 2) >> 1 & 1, p.status);
       ready = ready && wait_phase(&sh.k_full[slot], turn, p.status);
       if (!__all_sync(kFullMask, ready)) break;
       fence_after();
@@ -667,7 +668,7 @@ __global__ void __launch_bounds__(kTensorThreads, TensorShape<kDim>::resident)
                            kd + ((kk / 4 * kPanel + kk % 4 * 32) >> 4), idesc, kk > 0);
         commit(&sh.s_full[buffer]);
         mbar_arrive(&sh.s_full[buffer]);
-        commit(&sh.k_free[slot]);
+        if (k + Shape::k_stages < blocks) commit(&sh.k_free[slot]);  // else nobody waits for it
       }
       __syncwarp();
       if (++slot == Shape::k_stages) {
@@ -675,6 +676,10 @@ __global__ void __launch_bounds__(kTensorThreads, TensorShape<kDim>::resident)
         turn ^= 1;
       }
     }
+    // The softmax warps see the last block's products done; with the one before it, too, no
+    // arrival of a product is left that could come after the block has ended.
+    if (blocks > 1 && __all_sync(kFullMask, ready))
+      wait_phase(&sh.pv_done[blocks & 1], (blocks - 2) >> 1 & 1, p.status);
   } else {
     // ---- O += P V -------------------------------------------------------------------
     const uint32_t idesc = instruction<T>(kDim, true), v0 = descriptor(smem_addr(v_ring));
@@ -695,7 +700,7 @@ __global__ void __launch_bounds__(kTensorThreads, TensorShape<kDim>::resident)
                          k > 0 || kk > 0);
         commit(&sh.pv_done[buffer]);
         mbar_arrive(&sh.pv_done[buffer]);  // sh.bad reaches the softmax warps by this one
-        commit(&sh.v_free[slot]);
+        if (k + Shape::v_stages < blocks) commit(&sh.v_free[slot]);
       }
       __syncwarp();
       if (++slot == Shape::v_stages) {
