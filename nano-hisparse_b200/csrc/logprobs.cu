@@ -197,7 +197,7 @@ template <typename T> struct RowPart {
     first = min(vectors, rank * share);
     count = min(vectors, first + share) - first;
     const int i = threadIdx.x;
-    edge = rank != 0 ? -1 : i < head ? i : tail + i - head < p.vocab ? tail + i - head : -1;
+    edge = rank != 0 ? -1 : i < head ? i : i - head < p.vocab - tail ? tail + (i - head) : -1;
   }
   __device__ __forceinline__ uint4 vector(int v) const {
     return __ldg(reinterpret_cast<const uint4 *>(x + head) + first + v);

@@ -43,3 +43,37 @@ def test_tree_marks_of_values_that_are_not_finite(dtype, dim, width):
         same[:, :, 2:4, 0] = False
         assert torch.equal(got[same], clean[same])
     assert not flags()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("offset", [0, 1, 3])
+def test_logprobs_of_the_longest_row(dtype, offset):
+    """2^31 - 1 entries, the most that is accepted, from a 16-byte boundary and off it:
+    few entries above -inf, at both ends and in the middle, so that every sum is short."""
+    from hisparse_b200 import token_logprobs
+
+    v = 2 ** 31 - 1
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 24 GB")
+    buffer = torch.full((v + offset,), -math.inf, dtype=dtype, device=DEV)
+    logits = buffer[offset:].view(1, v)
+    at = {0: 1.0, 1: 0.5, v // 2: 0.25, v - 2: 1.5, v - 1: 2.0}
+    for index, value in at.items():
+        logits[0, index] = value
+    tokens = torch.tensor([[*at, 7, v, -1]], device=DEV)
+    got = token_logprobs(logits, tokens, top=6)
+    lse = math.log(sum(math.exp(x) for x in at.values()))
+    want = [x - lse for x in at.values()]
+    # five exps (2 f each and f of an exponent of at most 1.75), their sums, a logarithm and
+    # two differences of at most 2: under 32 f
+    bound = 32 * 2.0 ** -24
+    have = got.logprobs[0].tolist()
+    assert all(abs(a - b) < bound for a, b in zip(have, want))
+    assert have[5] == -math.inf and math.isnan(have[6]) and have[7] == 0
+    entropy = -sum(math.exp(x) * x for x in want)
+    assert abs(got.entropy.item() - entropy) < bound
+    order = sorted(at, key=lambda i: -at[i])
+    assert got.top_tokens[0].tolist() == order + [2]
+    top = got.top_logprobs[0].tolist()
+    assert all(abs(a - (at[i] - lse)) < bound for a, i in zip(top, order)) and top[5] == -math.inf
+    assert flags()  # the token past the vocabulary
