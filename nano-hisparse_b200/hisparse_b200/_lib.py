@@ -14,6 +14,7 @@ import threading
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 LIB_PATH = Path(__file__).resolve().parent.parent / "libhisparse.so"
 ABI_VERSION = 1
@@ -132,10 +133,15 @@ def require_cuda(*tensors):
             raise ValueError("hisparse_b200 operators take CUDA tensors; there is no CPU path")
 
 
+def _has_tangent(*tensors) -> bool:
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def one_device(first, *others) -> int:
     """Index of the CUDA device that holds every given tensor (None is skipped).
-    Tensors that a gradient is asked of are refused: these operators have no
-    backward pass, and a result without one would drop it silently."""
+    Tensors that a gradient is asked of, or that carry a forward-mode tangent, are
+    refused: these operators have no derivative, and a result without one would
+    drop it silently."""
     try:
         index, grad = first.get_device(), first.requires_grad
         same = index >= 0
@@ -148,6 +154,10 @@ def one_device(first, *others) -> int:
         if grad and torch.is_grad_enabled():
             raise ValueError("the operator has no backward pass: call it under "
                              "torch.no_grad() or on detached tensors")
+        # (the level spares unpack_dual's cost outside of forward-mode differentiation)
+        if getattr(forward_ad, "_current_level", 0) >= 0 and _has_tangent(first, *others):
+            raise ValueError("the operator has no derivative: call it on tensors without a "
+                             "forward-mode tangent")
     except AttributeError:
         same = False
     if not same:

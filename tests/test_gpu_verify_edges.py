@@ -77,3 +77,24 @@ def test_logprobs_of_the_longest_row(dtype, offset):
     top = got.top_logprobs[0].tolist()
     assert all(abs(a - (at[i] - lse)) < bound for a, i in zip(top, order)) and top[5] == -math.inf
     assert flags()  # the token past the vocabulary
+
+
+def test_operators_refuse_forward_mode_tangents():
+    from torch.autograd import forward_ad
+
+    from hisparse_b200 import attend_tree, qk_norm_rope, rope_frequencies, token_logprobs, tree_mask
+    from test_gpu_verify_ops import tree_inputs
+
+    (q, k, v), parents, pool, rows, config = tree_inputs(1, 3, 4, 2, 32, 16, 20, torch.float32, 52)
+    mask, positions = tree_mask(parents, DEV), torch.arange(3, device=DEV)
+    freq = rope_frequencies(32, 1e4, DEV)
+    want = attend_tree(q, k, v, mask, pool, rows, config)
+    with forward_ad.dual_level():
+        tangent = forward_ad.make_dual(v, torch.ones_like(v))
+        for call in (lambda: attend_tree(q, k, tangent, mask, pool, rows, config),
+                     lambda: qk_norm_rope(q[0], tangent[0], positions, freq),
+                     lambda: token_logprobs(tangent[0, :, 0], positions, top=1)):
+            with pytest.raises(ValueError, match="no derivative"):
+                call()
+        # inside a level, tensors without a tangent are taken as ever
+        assert torch.equal(attend_tree(q, k, v, mask, pool, rows, config), want)
