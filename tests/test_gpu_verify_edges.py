@@ -98,3 +98,33 @@ def test_operators_refuse_forward_mode_tangents():
                 call()
         # inside a level, tensors without a tangent are taken as ever
         assert torch.equal(attend_tree(q, k, v, mask, pool, rows, config), want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows,kbytes,threads,top", [
+    (2, 512, 256, 32), (2, 512, 256, 7), (300, 60, 256, 32), (601, 60, 128, 32), (601, 60, 128, 2)])
+def test_logprobs_large_entries_of_few_threads(dtype, rows, kbytes, threads, top):
+    """Entries that pass the threshold are collected up to 1,024 a block. Rows whose large
+    entries all fall to fewer than `top` threads pass with more: the threshold is then a
+    small entry's, and the alternatives are found by one pass each. In 8 blocks a row (512
+    KB), in one block, and in one of half the threads."""
+    from hisparse_b200 import token_logprobs
+    from test_gpu_verify_ops import logprobs_check
+
+    size = torch.tensor([], dtype=dtype).element_size()
+    vocab, n = kbytes * 1024 // size, 16 // size
+    i = torch.arange(vocab)
+    large = i // n % threads < top - 1
+    values = torch.stack([(1 + r % 5) * 100 + (i * 7919 + r) % 601 for r in range(min(rows, 6))])
+    logits = torch.where(large, values, torch.randn(len(values), vocab)).to(dtype)
+    blocks = 8 if kbytes == 512 else 1
+    if top == 32:
+        assert all(part.sum() > 1024 for part in large.view(blocks, -1))
+    logits = logits.repeat(-(-rows // len(values)), 1)[:rows].contiguous().to(DEV)
+    tokens = torch.arange(rows, device=DEV) * 31 % vocab
+    got = token_logprobs(logits, tokens, top=top)
+    for part in (slice(0, 6), slice(rows - 6, rows)) if rows > 6 else (slice(0, rows),):
+        logprobs_check(type(got)(*(x[part] for x in got)), logits[part], tokens[part], top)
+    again = token_logprobs(logits, tokens, top=top)
+    assert all(torch.equal(x, y) for x, y in zip(got, again))
+    assert not flags()
