@@ -255,9 +255,12 @@ class DecodeBatch:
         st.last_use.record(compute)
         return out
 
-    def _resolve_and_gather(self, layer, positions, counts):
+    def _resolve_and_gather(self, layer, positions, counts, ready=None, mark=lambda *a: None):
         """The resolver on the compute stream, then the miss gather on the transfer
-        stream; st.ready is recorded behind the gather."""
+        stream, behind the resolver and behind the last readers of the layer's hot
+        rows; st.ready is recorded behind the gather. ready: address of the list of
+        rows that need no gather, or None. Returns `mark`'s events: the resolver's
+        end, the gather's start and end."""
         cache, cfg, st, lib = self.cache, self.config, self.layers[layer], _lib.load()
         compute, transfer, status = self.compute, self.transfer, self.status.data_ptr()
         b = self.batch
@@ -266,20 +269,24 @@ class DecodeBatch:
             st.table_pages, st.hot_ptrs.data_ptr(), cache.hot_blocks, st.tag_ptrs.data_ptr(),
             st.lru_ptrs.data_ptr(), self.hot_rows, st.lengths.data_ptr(), cfg.page_size,
             self.physical.data_ptr(), self.miss_host.data_ptr(), self.miss_device.data_ptr(),
-            counts.data_ptr(), None, _lib.ptr(self.resolve_ws), self.resolve_ws_bytes, status,
+            counts.data_ptr(), ready, _lib.ptr(self.resolve_ws), self.resolve_ws_bytes, status,
             compute.cuda_stream))
+        t2 = mark(compute, "resolve")
         resolved = torch.cuda.Event()
         resolved.record(compute)
         transfer.wait_event(resolved)
         if st.last_use is not None:
             transfer.wait_event(st.last_use)
+        t3 = mark(transfer, "gather")
         _lib.check(lib.hs_gather_rows(
             cache.mapped.data_ptr(), cache.host.shape[0], cache.pool.data_ptr(),
             cache.pool.shape[0], self.miss_host.data_ptr(), self.miss_device.data_ptr(),
             b * self.width, self.width, cfg.page_size, self._row_bytes, status,
             transfer.cuda_stream))
+        t4 = mark(transfer, "gather")
         st.ready = torch.cuda.Event()
         st.ready.record(transfer)
+        return t2, t3, t4
 
     def exchange(self):
         """All-gather of the partial scores over the group, on the current
@@ -327,30 +334,9 @@ class DecodeBatch:
         """Resolve, gather, both attention phases and the merge of `layer`."""
         cache, cfg, st, lib = self.cache, self.config, self.layers[layer], _lib.load()
         b, hq, d = query.shape
-        compute, transfer = self.compute, self.transfer
+        compute = self.compute
         stream, status = compute.cuda_stream, self.status.data_ptr()
-        _lib.check(lib.hs_resolve_rows_batched(
-            b, tokens, self.width, st.src_ptrs.data_ptr(), st.res_ptrs.data_ptr(),
-            st.table_pages, st.hot_ptrs.data_ptr(), cache.hot_blocks, st.tag_ptrs.data_ptr(),
-            st.lru_ptrs.data_ptr(), self.hot_rows, st.lengths.data_ptr(), cfg.page_size,
-            self.physical.data_ptr(), self.miss_host.data_ptr(), self.miss_device.data_ptr(),
-            counts.data_ptr(), self.ready.data_ptr(), _lib.ptr(self.resolve_ws),
-            self.resolve_ws_bytes, status, stream))
-        t2 = mark(compute, "resolve")
-        resolved = torch.cuda.Event()
-        resolved.record(compute)
-        transfer.wait_event(resolved)
-        if st.last_use is not None:
-            transfer.wait_event(st.last_use)
-        t3 = mark(transfer, "gather")
-        _lib.check(lib.hs_gather_rows(
-            cache.mapped.data_ptr(), cache.host.shape[0], cache.pool.data_ptr(),
-            cache.pool.shape[0], self.miss_host.data_ptr(), self.miss_device.data_ptr(),
-            b * self.width, self.width, cfg.page_size, self._row_bytes, status,
-            transfer.cuda_stream))
-        t4 = mark(transfer, "gather")
-        st.ready = torch.cuda.Event()
-        st.ready.record(transfer)
+        t2, t3, t4 = self._resolve_and_gather(layer, tokens, counts, self.ready.data_ptr(), mark)
         # phase 0: rows that need no gather, concurrently with the gather
         if serial:
             compute.wait_event(st.ready)
