@@ -672,8 +672,11 @@ class BatchedEngine:
     drafter: None, or an object whose ``propose(tokens, limit)`` returns a tree
     of likely continuations of a token list as (token, parent) pairs, parents
     first, -1 for a child of the last token, at most `limit` of them
-    (``hisparse_b200.PromptLookup`` drafts from the request's own text). A
-    request's turn then emits one or more tokens, those that greedy decoding
+    (``hisparse_b200.PromptLookup`` drafts from the request's own text). A drafter
+    may also have ``follow(tokens)``: the object that it returns is kept while the
+    request runs, told of new tokens with ``extend(tokens)`` and asked with
+    ``propose(limit)``, so that no turn hands over the whole text again (None: it is
+    asked with the text after all). A request's turn then emits one or more tokens, those that greedy decoding
     would emit one by one. Needs the full causal history (top_k=None): with a
     page budget every token selects its own pages."""
 
@@ -696,6 +699,7 @@ class BatchedEngine:
             raise ValueError("drafted decoding reads the full history: top_k must be None")
         self.logprobs, self.drafter = logprobs, drafter
         self.draft_stats = {"steps": 0, "drafted": 0, "accepted": 0}
+        self._texts: dict[str, list] = {}  # by request: drafter, what it follows, tokens told
         self.model, self.cache, self.top_k, self.backend = weights, cache, top_k, backend
         self.eos_token_id, self.selector = eos_token_id, selector
         self.requests: dict[str, Request] = {}
@@ -737,6 +741,7 @@ class BatchedEngine:
         request.generated.append(token)
         if token == self.eos_token_id or len(request.generated) >= request.max_new_tokens:
             request.finished = True
+            self._texts.pop(request.request_id, None)
             self.cache.release_request(request.request_id, wait=False)
         return token
 
@@ -792,6 +797,7 @@ class BatchedEngine:
             self.waiting.remove(request)
         else:
             self.running.remove(request)
+            self._texts.pop(request_id, None)
             self.cache.release_request(request_id, wait=False)
         request.finished = request.cancelled = True
 
@@ -847,8 +853,23 @@ class BatchedEngine:
         if left < 1:
             return []
         limit = MAX_NODES - 1
-        drafted = list(self.drafter.propose(request.prompt + request.generated, limit))
-        return tree_of(drafted, limit, left, self.model.config.vocab_size)
+        return tree_of(list(self._propose(request, limit)), limit, left,
+                       self.model.config.vocab_size)
+
+    def _propose(self, request, limit):
+        known = self._texts.get(request.request_id)
+        if known is None or known[0] is not self.drafter:
+            follow = getattr(self.drafter, "follow", None)
+            text = None if follow is None else follow(request.prompt + request.generated)
+            known = [self.drafter, text, len(request.generated)]
+            self._texts[request.request_id] = known
+        _, text, told = known
+        if text is None:
+            return self.drafter.propose(request.prompt + request.generated, limit)
+        if told < len(request.generated):
+            text.extend(request.generated[told:])
+            known[2] = len(request.generated)
+        return text.propose(limit)
 
     @torch.inference_mode()
     def _decode_drafted(self, requests, trees):
