@@ -15,12 +15,14 @@
 // much traffic again on rows that L2 does not hold.)
 //
 // 2,048 rows of 128,256 take 190 us in fp32 with 5 alternatives (5.5 TB/s, 0.84 of a
-// measured copy; 184 us without alternatives, 279 with 32) and 125 us in bf16 (4.2 TB/s,
-// bound by widening and summing: 114 without alternatives). Where more than kCandidates
-// entries of a block pass, the rest of the key tells them apart in a second collection
-// (64 rows of equal entries in bf16, 32 alternatives: 92 us; of random ones 23). Only where
-// the large entries all fall to fewer than `top` threads do more than that pass again: those
-// rows take one pass for each alternative (307 us).
+// measured copy; 184 us without alternatives, 279 with 32) and 125 us in bf16 (4.2 TB/s;
+// 114 without alternatives), bound by about eleven instructions an entry and lane (at 1,184
+// rows issue slots 67 % of the cycles, the heavy fp32 pipe 57 %, special functions 49 %, few
+// waits for memory). Where more than kCandidates entries of a block pass, the rest of the
+// key tells them apart in a second collection (64 rows of equal entries in bf16, 32
+// alternatives: 92 us; of random ones 23). Only where the large entries all fall to fewer
+// than `top` threads do more than that pass again: those rows take one pass for each
+// alternative (307 us).
 //
 // A row is split over a cluster of 1 to 8 blocks, which join their sums and their
 // best keys in the first block's shared memory: few rows reach many SMs without
