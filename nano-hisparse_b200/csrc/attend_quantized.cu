@@ -1,0 +1,384 @@
+// (11) Decode attention over the rows of an 8-bit cache.
+//
+// s_i = (q . k_i) 2^ek_i / sqrt(head_dim) with k_i the codes, in powers of two. A row's V
+// scale goes into its weight, so that the codes are multiplied as they are: with m the
+// running maximum of s_i + ev_i,
+//   o += 2^(s_i + ev_i - m) v_i     l += 2^(s_i - m + kSumLift)     out = o / l 2^kSumLift
+// The two powers are taken apart: a row with a small scale may weigh nothing in o and
+// most in l. As scales are 2^-100 to 2^120, the largest term of l lies between 2^-110 and
+// 2^110, and l stays inside fp32. The maximum is kept as its row's score and exponent,
+// whose rounded sum would cost digits of the weights.
+#include "attend_quantized.cuh"
+
+namespace hs {
+namespace {
+
+constexpr int kSimtThreads = 128;
+constexpr int kSimtWarps = kSimtThreads / 32;
+constexpr int kSimtHeads = 8;    // query heads of a block
+constexpr int kSimtAhead = 4;    // rows of a warp in flight
+
+// CUDA cores, every type and shape. A warp takes four rows at a time, a lane C
+// neighbouring elements of each.
+template <typename T, int C>
+__global__ void __launch_bounds__(kSimtThreads) quant_simt_kernel(QuantAttendParams p) {
+  __shared__ float4 red[kSimtWarps][kSimtHeads];  // a maximum's score, exponent; the sum
+  __shared__ float red_o[kSimtWarps][kSimtHeads][32 * C];
+  const int split = blockIdx.x, b = blockIdx.z, D = p.head_dim;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, d0 = lane * C;
+  int kh, h0, hn;
+  if (p.rows_head_stride == 0) {
+    const int chunks = (p.groups + kSimtHeads - 1) / kSimtHeads;
+    kh = blockIdx.y / chunks;
+    h0 = kh * p.groups + blockIdx.y % chunks * kSimtHeads;
+    hn = min(kSimtHeads, (kh + 1) * p.groups - h0);
+  } else {
+    h0 = blockIdx.y;
+    kh = h0 / p.groups;
+    hn = 1;
+  }
+  float q[kSimtHeads][C], ms[kSimtHeads], me[kSimtHeads], l[kSimtHeads], o[kSimtHeads][C];
+  const T *query = static_cast<const T *>(p.query) + (int64_t)b * p.q_batch_stride;
+#pragma unroll
+  for (int g = 0; g < kSimtHeads; ++g) {
+    ms[g] = -INFINITY;
+    me[g] = l[g] = 0.f;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      q[g][c] = g < hn && d0 + c < D ? to_f32(query[(int64_t)(h0 + g) * D + d0 + c]) : 0.f;
+      o[g][c] = 0.f;
+    }
+  }
+  const int64_t valid = quant_rows(p, b), share = ceil_div(valid, p.splits);
+  const int64_t begin = min(valid, split * share), end = min(valid, begin + share);
+  const int64_t *rows = p.rows + b * p.rows_batch_stride + h0 * p.rows_head_stride;
+  const int64_t E = (int64_t)p.kv_heads * D, plane = (int64_t)p.page_size * p.record;
+  for (int64_t i0 = begin + warp * kSimtAhead; i0 < end; i0 += kSimtWarps * kSimtAhead) {
+    float k[kSimtAhead][C], v[kSimtAhead][C], k_scale[kSimtAhead];
+    int v_exponent[kSimtAhead];
+    bool seen[kSimtAhead];
+#pragma unroll
+    for (int r = 0; r < kSimtAhead; ++r) {
+      const int64_t index = i0 + r < end ? record_index(rows[i0 + r], p.page_size, p.page_shift,
+                                                        p.pool_blocks, p.status) : -1;
+      seen[r] = index >= 0;
+      k_scale[r] = 0.f;
+      v_exponent[r] = 0;
+#pragma unroll
+      for (int c = 0; c < C; ++c) k[r][c] = v[r][c] = 0.f;
+      if (!seen[r]) continue;
+      const unsigned char *record = p.pool + index * p.record;
+      k_scale[r] = scale_of(record[E + kh]) * p.scale_log2;
+      v_exponent[r] = (int)record[plane + E + kh] - 127;
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+        if (d0 + c < D) {
+          k[r][c] = decode1(record[(int64_t)kh * D + d0 + c]);
+          v[r][c] = decode1(record[plane + (int64_t)kh * D + d0 + c]);
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < kSimtAhead; ++r) {
+      if (!seen[r]) continue;  // the same for the whole warp
+#pragma unroll
+      for (int g = 0; g < kSimtHeads; ++g) {
+        if (g >= hn) break;
+        float dot = 0.f;
+#pragma unroll
+        for (int c = 0; c < C; ++c) dot = fmaf(q[g][c], k[r][c], dot);
+        const float s = warp_xor_tree_sum(dot) * k_scale[r], e = (float)v_exponent[r];
+        if (ms[g] == -INFINITY || s + e > ms[g] + me[g]) {  // the new maximum (or NaN, kept)
+          const float f = ms[g] == -INFINITY ? 0.f : quant_share(ms[g], me[g], s, e);
+          l[g] *= f;
+#pragma unroll
+          for (int c = 0; c < C; ++c) o[g][c] *= f;
+          ms[g] = s;
+          me[g] = e;
+        }
+        const float w = quant_share(s, e, ms[g], me[g]);
+        l[g] += quant_share(s, kSumLift, ms[g], me[g]);
+#pragma unroll
+        for (int c = 0; c < C; ++c) o[g][c] = fmaf(w, v[r][c], o[g][c]);
+      }
+    }
+  }
+  // the warps' results
+#pragma unroll
+  for (int g = 0; g < kSimtHeads; ++g) {
+    if (g >= hn) break;
+    if (lane == 0) red[warp][g] = make_float4(ms[g], me[g], l[g], 0.f);
+#pragma unroll
+    for (int c = 0; c < C; ++c) red_o[warp][g][d0 + c] = o[g][c];
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < hn * 32 * C; i += kSimtThreads) {
+    const int g = i / (32 * C), d = i % (32 * C);
+    if (d >= D) continue;
+    float4 top = red[0][g];
+    float sum = 0.f, x = 0.f;
+    for (int w = 1; w < kSimtWarps; ++w) top = quant_larger(top, red[w][g]);
+    for (int w = 0; w < kSimtWarps; ++w) {
+      const float4 part = red[w][g];
+      if (part.z == 0.f) continue;  // saw nothing
+      const float f = quant_share(part.x, part.y, top.x, top.y);
+      sum = fmaf(part.z, f, sum);
+      x = fmaf(red_o[w][g][d], f, x);
+    }
+    if (p.out != nullptr) {
+      const float y = sum > 0.f || sum != sum ? x / sum * kSumScale : 0.f;
+      static_cast<T *>(p.out)[((int64_t)b * p.q_heads + h0 + g) * D + d] = from_f32<T>(y);
+    } else {
+      const int64_t part = quant_part(p, p.phase, b, h0 + g, split);
+      if (d == 0) p.stats[part] = make_float4(top.x, top.y, sum, 0.f);
+      p.partials[part * quant_pad(D) + d] = x;
+    }
+  }
+}
+
+// ---- the join of splits and phases ----------------------------------------------------------
+constexpr int kJoinWarps = 4;
+
+// One block a query head; a warp takes every fourth partial result, a lane four
+// elements of each.
+template <typename T>
+__global__ void __launch_bounds__(32 * kJoinWarps) quant_merge_kernel(QuantAttendParams p,
+                                                                      int phases, T *out) {
+  __shared__ float4 sums[kJoinWarps][kQuantMaxDim / 4];
+  const int h = blockIdx.x, b = blockIdx.y, D = p.head_dim, quads = quant_pad(D) / 4;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, all = phases * p.splits;
+  const auto part = [&](int i) { return quant_part(p, i / p.splits, b, h, i % p.splits); };
+  float4 top = make_float4(-INFINITY, 0.f, 0.f, 0.f);
+  float l = 0.f;
+  for (int i = lane; i < all; i += 32) top = quant_larger(top, p.stats[part(i)]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    top = quant_larger(top, make_float4(__shfl_xor_sync(kFullMask, top.x, o),
+                                        __shfl_xor_sync(kFullMask, top.y, o),
+                                        __shfl_xor_sync(kFullMask, top.z, o), 0.f));
+  for (int i = lane; i < all; i += 32) {
+    const float4 s = p.stats[part(i)];
+    if (s.z != 0.f) l = fmaf(s.z, quant_share(s.x, s.y, top.x, top.y), l);
+  }
+  l = warp_xor_tree_sum(l);
+  float4 x[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+  for (int i = warp; i < all; i += kJoinWarps) {
+    const float4 s = p.stats[part(i)];
+    if (s.z == 0.f) continue;  // saw nothing
+    const float f = quant_share(s.x, s.y, top.x, top.y);
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      if (lane + 32 * j < quads) {
+        const float4 y =
+            reinterpret_cast<const float4 *>(p.partials + part(i) * 4 * quads)[lane + 32 * j];
+        x[j].x = fmaf(f, y.x, x[j].x);
+        x[j].y = fmaf(f, y.y, x[j].y);
+        x[j].z = fmaf(f, y.z, x[j].z);
+        x[j].w = fmaf(f, y.w, x[j].w);
+      }
+  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+    if (lane + 32 * j < quads) sums[warp][lane + 32 * j] = x[j];
+  __syncthreads();
+  const float inv = l > 0.f || l != l ? kSumScale / l : 0.f;
+  for (int d = threadIdx.x; d < D; d += 32 * kJoinWarps) {
+    float y = 0.f;
+    for (int w = 0; w < kJoinWarps; ++w) y += reinterpret_cast<const float *>(sums[w])[d];
+    out[((int64_t)b * p.q_heads + h) * D + d] = from_f32<T>(y * inv);
+  }
+}
+
+// Splits of a request's rows: about eight blocks an SM, none under 32 rows.
+int quant_splits(int batch, int kv_heads, int64_t count) {
+  int64_t s = ceil_div((int64_t)sm_count() * 8, (int64_t)batch * kv_heads);
+  if (s > ceil_div(count, 32)) s = ceil_div(count, 32);
+  return (int)(s < 1 ? 1 : (s > kQuantMaxSplits ? kQuantMaxSplits : s));
+}
+int check_sizes(int batch, int dtype, int64_t pool_blocks, int64_t count, int q_heads,
+                int kv_heads, int head_dim, int page_size) {
+  if (batch < 0 || kv_heads < 1 || q_heads < 1 || head_dim < 1 || page_size < 1 ||
+      pool_blocks < 0 || count < 0)
+    return set_error(HS_ERR_INVALID_ARGUMENT, "attend_quantized: invalid sizes");
+  if (q_heads % kv_heads)
+    return set_error(HS_ERR_INVALID_ARGUMENT, "query GQA/device mismatch");
+  if (head_dim > kQuantMaxDim)
+    return set_error(HS_ERR_UNSUPPORTED, "attend_quantized: head_dim %d > %d is not supported",
+                     head_dim, kQuantMaxDim);
+  if (dtype != HS_FLOAT32 && dtype != HS_FLOAT16 && dtype != HS_BFLOAT16)
+    return set_error(HS_ERR_INVALID_ARGUMENT, "attend_quantized: invalid dtype %d", dtype);
+  if (batch > 65535 || q_heads > 32767 || count > 0x7fffff00)
+    return set_error(HS_ERR_UNSUPPORTED, "attend_quantized: batch, heads or rows too many");
+  return HS_OK;
+}
+
+// Puts the workspace's parts into p; `phases` phases have to fit.
+int place_workspace(QuantAttendParams &p, int phases, void *workspace, size_t bytes) {
+  const size_t need = hs_attend_quantized_workspace_bytes(p.batch, phases, p.q_heads, p.kv_heads,
+                                                          p.head_dim, p.count);
+  if (need == 0) return HS_OK;
+  if ((reinterpret_cast<uintptr_t>(workspace) & 15) != 0)
+    return set_error(HS_ERR_WORKSPACE, "attend_quantized: the workspace must be 16-byte aligned");
+  if (!workspace || bytes < need)
+    return set_error(HS_ERR_WORKSPACE, "attend_quantized: workspace of %zu bytes < required %zu",
+                     bytes, need);
+  return HS_OK;
+}
+
+template <typename T> int launch_rows(const QuantAttendParams &p, cudaStream_t s) {
+  const int per = (p.groups + kSimtHeads - 1) / kSimtHeads;
+  const dim3 grid((unsigned)p.splits,
+                  (unsigned)(p.rows_head_stride == 0 ? p.kv_heads * per : p.q_heads),
+                  (unsigned)p.batch);
+  switch (ceil_div(p.head_dim, 32)) {
+    case 1: quant_simt_kernel<T, 1><<<grid, kSimtThreads, 0, s>>>(p); break;
+    case 2: quant_simt_kernel<T, 2><<<grid, kSimtThreads, 0, s>>>(p); break;
+    case 3:
+    case 4: quant_simt_kernel<T, 4><<<grid, kSimtThreads, 0, s>>>(p); break;
+    default: quant_simt_kernel<T, 8><<<grid, kSimtThreads, 0, s>>>(p); break;
+  }
+  return check_launch("quant_simt_kernel");
+}
+template <typename T>
+int launch_merge(const QuantAttendParams &p, int phases, void *out, cudaStream_t s) {
+  const dim3 grid((unsigned)p.q_heads, (unsigned)p.batch);
+  quant_merge_kernel<T><<<grid, 32 * kJoinWarps, 0, s>>>(p, phases, static_cast<T *>(out));
+  return check_launch("quant_merge_kernel");
+}
+int launch_rows(const QuantAttendParams &p, int dtype, cudaStream_t s) {
+  switch (dtype) {
+    case HS_FLOAT32: return launch_rows<float>(p, s);
+    case HS_FLOAT16: return launch_rows<__half>(p, s);
+    default: return launch_rows<__nv_bfloat16>(p, s);
+  }
+}
+int launch_merge(const QuantAttendParams &p, int phases, void *out, int dtype, cudaStream_t s) {
+  switch (dtype) {
+    case HS_FLOAT32: return launch_merge<float>(p, phases, out, s);
+    case HS_FLOAT16: return launch_merge<__half>(p, phases, out, s);
+    default: return launch_merge<__nv_bfloat16>(p, phases, out, s);
+  }
+}
+
+// The parameters that every form has; the workspace holds `phases` phases.
+QuantAttendParams params_of(int batch, int phases, int q_heads, int kv_heads, int head_dim,
+                            int64_t count, void *workspace) {
+  QuantAttendParams p{};
+  p.batch = batch;
+  p.count = count;
+  p.q_heads = q_heads;
+  p.kv_heads = kv_heads;
+  p.head_dim = head_dim;
+  p.groups = q_heads / kv_heads;
+  p.splits = quant_splits(batch, kv_heads, count);
+  p.record = record_bytes(kv_heads, head_dim);
+  p.scale_log2 = (float)(1.4426950408889634 / sqrt((double)head_dim));
+  p.stats = static_cast<float4 *>(workspace);
+  p.partials = reinterpret_cast<float *>(p.stats + (int64_t)phases * batch * q_heads * p.splits);
+  return p;
+}
+
+}  // namespace
+}  // namespace hs
+
+extern "C" size_t hs_attend_quantized_workspace_bytes(int batch, int phases, int q_heads,
+                                                      int kv_heads, int head_dim,
+                                                      int64_t count) {
+  using namespace hs;
+  if (batch < 1 || phases < 1 || kv_heads < 1 || q_heads < kv_heads || head_dim < 1 || count < 0)
+    return 0;
+  const int splits = quant_splits(batch, kv_heads, count);
+  if (splits == 1 && phases == 1) return 0;
+  const int64_t parts = (int64_t)phases * batch * q_heads * splits;
+  return (size_t)parts * (sizeof(float4) + quant_pad(head_dim) * sizeof(float));
+}
+
+extern "C" int hs_attend_quantized(int batch, const void *query, int64_t query_batch_stride,
+                                   int dtype, const void *pool, int64_t pool_blocks,
+                                   const int64_t *rows, int64_t rows_batch_stride,
+                                   int64_t rows_head_stride, int64_t count, const int32_t *counts,
+                                   void *out, int q_heads, int kv_heads, int head_dim,
+                                   int page_size, void *workspace, size_t workspace_bytes,
+                                   int32_t *device_status, hs_stream stream) {
+  using namespace hs;
+  if (int e = check_sizes(batch, dtype, pool_blocks, count, q_heads, kv_heads, head_dim,
+                          page_size))
+    return e;
+  if (batch == 0) return HS_OK;
+  if (!query || !out || (count > 0 && (!rows || !pool)))
+    return set_error(HS_ERR_INVALID_ARGUMENT, "attend_quantized: null pointer");
+  if ((reinterpret_cast<uintptr_t>(pool) & 15) != 0)
+    return set_error(HS_ERR_INVALID_ARGUMENT,
+                     "attend_quantized: the pool must be 16-byte aligned");
+  QuantAttendParams p = params_of(batch, 1, q_heads, kv_heads, head_dim, count, workspace);
+  if (int e = place_workspace(p, 1, workspace, workspace_bytes)) return e;
+  p.query = query;
+  p.q_batch_stride = query_batch_stride;
+  p.pool = static_cast<const unsigned char *>(pool);
+  p.pool_blocks = pool_blocks;
+  p.rows = rows;
+  p.rows_batch_stride = rows_batch_stride;
+  p.rows_head_stride = rows_head_stride;
+  p.counts32 = counts;
+  p.out = p.splits == 1 ? out : nullptr;
+  p.page_size = page_size;
+  p.page_shift = page_shift_of(page_size);
+  p.status = device_status;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int status = launch_rows(p, dtype, s);
+  return status != HS_OK || p.splits == 1 ? status : launch_merge(p, 1, out, dtype, s);
+}
+
+extern "C" int hs_attend_quantized_phase(int batch, const void *query,
+                                         int64_t query_batch_stride, int dtype, const void *pool,
+                                         int64_t pool_blocks, const int64_t *rows,
+                                         int64_t rows_batch_stride, int64_t count,
+                                         const int64_t *counts, int counts_stride,
+                                         int counts_first, int counts_n, int phase, int q_heads,
+                                         int kv_heads, int head_dim, int page_size,
+                                         void *workspace, size_t workspace_bytes,
+                                         int32_t *device_status, hs_stream stream) {
+  using namespace hs;
+  if (int e = check_sizes(batch, dtype, pool_blocks, count, q_heads, kv_heads, head_dim,
+                          page_size))
+    return e;
+  if (phase < 0 || phase > 1 || counts_n < 0 || counts_first < 0 || counts_stride < 0)
+    return set_error(HS_ERR_INVALID_ARGUMENT, "attend_quantized: invalid phase or counts");
+  if (batch == 0) return HS_OK;
+  if (!query || (count > 0 && (!rows || !pool)))
+    return set_error(HS_ERR_INVALID_ARGUMENT, "attend_quantized: null pointer");
+  if ((reinterpret_cast<uintptr_t>(pool) & 15) != 0)
+    return set_error(HS_ERR_INVALID_ARGUMENT,
+                     "attend_quantized: the pool must be 16-byte aligned");
+  QuantAttendParams p = params_of(batch, 2, q_heads, kv_heads, head_dim, count, workspace);
+  if (int e = place_workspace(p, 2, workspace, workspace_bytes)) return e;
+  p.query = query;
+  p.q_batch_stride = query_batch_stride;
+  p.pool = static_cast<const unsigned char *>(pool);
+  p.pool_blocks = pool_blocks;
+  p.rows = rows;
+  p.rows_batch_stride = rows_batch_stride;
+  p.counts64 = counts;
+  p.counts_stride = counts_stride;
+  p.counts_first = counts_first;
+  p.counts_n = counts_n;
+  p.phase = phase;
+  p.page_size = page_size;
+  p.page_shift = page_shift_of(page_size);
+  p.status = device_status;
+  return launch_rows(p, dtype, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int hs_attend_quantized_merge(int batch, int phases, void *out, int dtype, int q_heads,
+                                         int kv_heads, int head_dim, int64_t count,
+                                         void *workspace, size_t workspace_bytes,
+                                         hs_stream stream) {
+  using namespace hs;
+  if (int e = check_sizes(batch, dtype, 0, count, q_heads, kv_heads, head_dim, 1)) return e;
+  if (phases < 1 || phases > 2)
+    return set_error(HS_ERR_INVALID_ARGUMENT, "attend_quantized: invalid number of phases");
+  if (batch == 0) return HS_OK;
+  if (!out) return set_error(HS_ERR_INVALID_ARGUMENT, "attend_quantized: null pointer");
+  QuantAttendParams p = params_of(batch, 2, q_heads, kv_heads, head_dim, count, workspace);
+  if (int e = place_workspace(p, 2, workspace, workspace_bytes)) return e;
+  return launch_merge(p, phases, out, dtype, static_cast<cudaStream_t>(stream));
+}

@@ -1,5 +1,5 @@
-"""ctypes binding of libhisparse.so, whose C ABI is declared in include/hisparse.h
-and include/hisparse_verify.h.
+"""ctypes binding of libhisparse.so, whose C ABI is declared in include/hisparse.h,
+include/hisparse_verify.h and include/hisparse_quantized.h.
 
 The shared library is built in-tree (nano-hisparse_b200/libhisparse.so) by
 ``make -C nano-hisparse_b200/csrc`` or ``__graft_entry__.build()``. There is no
@@ -79,6 +79,21 @@ _VERIFY_SIGNATURES = {
                            _P], _INT),
 }
 
+# include/hisparse_quantized.h
+_QUANTIZED_SIGNATURES = {
+    "hs_quantized_row_bytes": ([_INT, _INT], _I64),
+    "hs_append_quantized": ([_INT, _P, _P, _I64, _INT, _P, _P, _P, _P, _I64, _P, _P, _I64, _P, _P,
+                             _P, _INT, _INT, _INT, _P, _P], _INT),
+    "hs_read_quantized": ([_P, _I64, _P, _I64, _P, _INT, _INT, _INT, _INT, _P, _P], _INT),
+    "hs_attend_quantized_workspace_bytes": ([_INT, _INT, _INT, _INT, _INT, _I64], _SZ),
+    "hs_attend_quantized": ([_INT, _P, _I64, _INT, _P, _I64, _P, _I64, _I64, _I64, _P, _P, _INT,
+                             _INT, _INT, _INT, _P, _SZ, _P, _P], _INT),
+    "hs_attend_quantized_phase": ([_INT, _P, _I64, _INT, _P, _I64, _P, _I64, _I64, _P, _INT, _INT,
+                                   _INT, _INT, _INT, _INT, _INT, _INT, _P, _SZ, _P, _P], _INT),
+    "hs_attend_quantized_merge": ([_INT, _INT, _P, _INT, _INT, _INT, _INT, _I64, _P, _SZ, _P],
+                                  _INT),
+}
+
 _lib = None
 _lock = threading.Lock()
 
@@ -96,7 +111,8 @@ def load():
                 f"{LIB_PATH} is missing: build it with `make -C nano-hisparse_b200/csrc` "
                 "(the sm_100a kernels have no fallback)")
         lib = ctypes.CDLL(str(LIB_PATH))
-        for name, (argtypes, restype) in {**_SIGNATURES, **_VERIFY_SIGNATURES}.items():
+        for name, (argtypes, restype) in {**_SIGNATURES, **_VERIFY_SIGNATURES,
+                                              **_QUANTIZED_SIGNATURES}.items():
             fn = getattr(lib, name)
             fn.argtypes, fn.restype = argtypes, restype
         if lib.hs_version() != ABI_VERSION:

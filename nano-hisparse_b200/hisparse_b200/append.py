@@ -22,6 +22,8 @@ import importlib
 import torch
 
 from . import _lib
+from .config import held_in_8_bits
+from .quantized import append_quantized
 from .row_kernels import MappedHost
 
 
@@ -34,8 +36,12 @@ def append_chunks(k, v, within, count, pool_block, pool, minimum_ptrs, maximum_p
     minimum_ptrs / maximum_ptrs / summary_ptrs: int64 [B] device pointers to
     the page's [Hkv, D] bounds (KV dtype) and fp32 summary; host: MappedHost
     of the pinned store (or None) and host_block int64 [B] (-1: no mirror).
-    Chunks of one call must touch distinct pages.
+    Chunks of one call must touch distinct pages. A pool held in 8 bits takes
+    any of the three KV dtypes and bfloat16 bounds (``append_quantized``).
     """
+    if held_in_8_bits(config):
+        return append_quantized(k, v, within, count, pool_block, pool, minimum_ptrs,
+                                maximum_ptrs, summary_ptrs, config, host, host_block)
     _lib.require_cuda(k, v, within, count, pool_block, pool, minimum_ptrs, maximum_ptrs,
                       summary_ptrs, host_block)
     if k.shape != v.shape or k.ndim != 4 or tuple(k.shape[2:]) != (config.kv_heads,
@@ -69,7 +75,8 @@ def append_chunks(k, v, within, count, pool_block, pool, minimum_ptrs, maximum_p
 def append_page(pool, k, v, slot, within, minimum, maximum, summary, config, host=None,
                 host_slot=-1):
     """One page chunk: rows within..within+len(k)-1 of pool block `slot` take
-    k/v [count, Hkv, D]; minimum/maximum [Hkv, D] (KV dtype) and summary
+    k/v [count, Hkv, D]; minimum/maximum [Hkv, D] (KV dtype; bfloat16 for a pool
+    held in 8 bits) and summary
     [Hkv, D] (fp32) are the page's metadata entries, updated in place; with a
     MappedHost `host`, host block `host_slot` receives the same rows."""
     _lib.require_cuda(pool, k, v, minimum, maximum, summary)
@@ -78,7 +85,8 @@ def append_page(pool, k, v, slot, within, minimum, maximum, summary, config, hos
         return
     if not (0 <= within and within + count <= config.page_size):
         raise ValueError("append chunk leaves its page")
-    for name, t, dt in (("minimum", minimum, pool.dtype), ("maximum", maximum, pool.dtype),
+    bounds = torch.bfloat16 if held_in_8_bits(config) else pool.dtype
+    for name, t, dt in (("minimum", minimum, bounds), ("maximum", maximum, bounds),
                         ("summary", summary, torch.float32)):
         if (t.dtype != dt or tuple(t.shape) != (config.kv_heads, config.head_dim)
                 or not t.is_contiguous()):

@@ -85,10 +85,10 @@ class RowCache:
             raise ValueError("RowCache lives on a CUDA device; there is no CPU path")
         if config.host_pages * config.page_size >= 2**31:
             raise ValueError("host row tags require int32 addresses")
-        shape = (2, config.page_size, config.kv_heads, config.head_dim)
-        self.pool = torch.empty((config.gpu_pages, *shape), dtype=config.dtype, device=self.device)
+        shape, dtype = config.page_shape, config.storage_dtype
+        self.pool = torch.empty((config.gpu_pages, *shape), dtype=dtype, device=self.device)
         self.host = host if host is not None else torch.empty(
-            (config.host_pages, *shape), dtype=config.dtype, pin_memory=True)
+            (config.host_pages, *shape), dtype=dtype, pin_memory=True)
         self.mapped = MappedHost(self.host)
         self.compute = torch.cuda.current_stream(self.device)
         self.transfer = torch.cuda.Stream(device=self.device)

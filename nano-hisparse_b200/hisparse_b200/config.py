@@ -5,11 +5,18 @@ configuration objects and call sites carry over unchanged."""
 from __future__ import annotations
 
 from dataclasses import dataclass
+from functools import cached_property
 from math import ceil
 
 import torch
 
+QUANTIZED = torch.float8_e4m3fn  # the KV dtype of a cache held in 8 bits
 ACTIVE_TAIL_PAGES = 2  # pages at the write tail that always stay resident (hybrid.py:19)
+
+
+def held_in_8_bits(config) -> bool:
+    """Whether `config`, which may be the reference's own class, is of an 8-bit cache."""
+    return getattr(config, "quantized", False)
 
 
 class CapacityError(RuntimeError):
@@ -18,6 +25,11 @@ class CapacityError(RuntimeError):
 
 @dataclass(frozen=True)
 class CacheConfig:
+    """Storage dimensions. dtype torch.float8_e4m3fn (no counterpart in the
+    reference) holds every row in 8 bits: pool and host store are then uint8
+    [pages, 2, page_size, row_bytes], records of e4m3 codes with a scale a KV
+    head (include/hisparse_quantized.h), and the Quest metadata is bfloat16."""
+
     gpu_pages: int = 16
     host_pages: int = 1024
     page_size: int = 16
@@ -31,15 +43,40 @@ class CacheConfig:
         for name in ("gpu_pages", "host_pages", "page_size", "kv_heads", "head_dim"):
             if getattr(self, name) < 1:
                 raise ValueError(f"{name} must be positive")
-        if self.dtype not in (torch.float32, torch.float16, torch.bfloat16):
-            raise ValueError("KV dtype must be float32, float16 or bfloat16")
+        if self.dtype not in (torch.float32, torch.float16, torch.bfloat16, QUANTIZED):
+            raise ValueError("KV dtype must be float32, float16 or bfloat16, or float8_e4m3fn "
+                             "for a cache held in 8 bits")
+        if self.quantized and self.head_dim > 256:
+            raise ValueError("a cache held in 8 bits supports head_dim up to 256")
         if self.index_budget_bytes < 1:
             raise ValueError("index budget must be positive")
 
-    @property
+    @cached_property
     def row_bytes(self) -> int:
-        """Bytes of one token's K (or V) across all KV heads."""
+        """Bytes of one token's K (or V) across all KV heads (8 bits: of its record)."""
+        if self.quantized:
+            return -(-self.kv_heads * (self.head_dim + 1) // 32) * 32
         return self.kv_heads * self.head_dim * torch.empty((), dtype=self.dtype).element_size()
+
+    @cached_property
+    def quantized(self) -> bool:
+        return self.dtype == QUANTIZED
+
+    @cached_property
+    def page_shape(self) -> tuple:
+        """Shape of a page of the pool or the host store."""
+        row = (self.row_bytes,) if self.quantized else (self.kv_heads, self.head_dim)
+        return (2, self.page_size, *row)
+
+    @property
+    def storage_dtype(self) -> torch.dtype:
+        """Element type of the pool and the host store."""
+        return torch.uint8 if self.quantized else self.dtype
+
+    @property
+    def metadata_dtype(self) -> torch.dtype:
+        """Element type of the Quest bounds: bfloat16 holds those of an 8-bit cache exactly."""
+        return torch.bfloat16 if self.quantized else self.dtype
 
 
 @dataclass(frozen=True)

@@ -15,6 +15,7 @@ import ctypes
 import torch
 
 from . import _lib
+from .config import held_in_8_bits
 
 
 class MappedHost:
@@ -64,7 +65,8 @@ def gather_rows(host, pool, plan, config):
     if miss_host.dtype != torch.int64 or miss_device.dtype != torch.int64:
         miss_host, miss_device = miss_host.long(), miss_device.long()
     n = miss_host.numel()
-    row_bytes = config.kv_heads * config.head_dim * pool.element_size()
+    row_bytes = config.row_bytes if held_in_8_bits(config) else \
+        config.kv_heads * config.head_dim * pool.element_size()
     _lib.check(lib.hs_gather_rows(
         mapped.data_ptr(), mapped.tensor.shape[0], pool.data_ptr(), pool.shape[0],
         miss_host.data_ptr(), miss_device.data_ptr(), n, n, config.page_size, row_bytes,
@@ -74,13 +76,17 @@ def gather_rows(host, pool, plan, config):
 def attend_rows(query, pool, rows, config):
     """Decode attention of query [Hq, D] over physical rows of the pool.
 
-    rows: int64 [Hq, K] (a stride-0 expansion of a shared [K] vector is read
+    On a pool held in 8 bits this is ``attend_quantized``. rows: int64 [Hq, K] (a stride-0 expansion of a shared [K] vector is read
     once per GQA group) or [K]; -1 entries are masked; a head with no valid row
     gets zeros. Output has the query's dtype.
     """
     _lib.require_cuda(query, pool, rows)
     if rows.ndim == 1:
         rows = rows[None, :].expand(query.shape[0], -1)
+    if held_in_8_bits(config):
+        from .quantized import attend_quantized
+
+        return attend_quantized(query[None], pool, rows[None], config)[0]
     query = query.contiguous()
     output = torch.empty_like(query)
     attend_into(output, query, pool, rows, config)
