@@ -61,7 +61,7 @@ __global__ void __launch_bounds__(kSimtThreads) quant_simt_kernel(QuantAttendPar
     for (int r = 0; r < kSimtAhead; ++r) {
       const int64_t index = i0 + r < end ? record_index(rows[i0 + r], p.page_size, p.page_shift,
                                                         p.pool_blocks, p.status) : -1;
-      seen[r] = index >= 0;
+      seen[r] = index >= 0 && p.pool[index * p.record + E + kh] != 0;
       k_scale[r] = 0.f;
       v_exponent[r] = 0;
 #pragma unroll
@@ -188,11 +188,25 @@ __global__ void __launch_bounds__(32 * kJoinWarps) quant_merge_kernel(QuantAtten
   }
 }
 
-// Splits of a request's rows: about eight blocks an SM, none under 32 rows.
-int quant_splits(int batch, int kv_heads, int64_t count) {
-  int64_t s = ceil_div((int64_t)sm_count() * 8, (int64_t)batch * kv_heads);
-  if (s > ceil_div(count, 32)) s = ceil_div(count, 32);
-  return (int)(s < 1 ? 1 : (s > kQuantMaxSplits ? kQuantMaxSplits : s));
+// Splits of a request's rows: those with the least (rounds of blocks) x (tiles of 16 rows
+// of a warp, and what a block costs besides, as much as about eight). One number for
+// every type, so that the workspace depends on the sizes alone.
+int quant_splits(int batch, int q_heads, int kv_heads, int head_dim, int64_t count) {
+  const QuantMmaGrid g = quant_mma_grid(q_heads, kv_heads, head_dim);
+  const int64_t blocks = (int64_t)batch * g.groups * g.chunks;
+  const int64_t places = (int64_t)g.resident * sm_count(), tiles = ceil_div(count, 16);
+  int64_t least = 0;
+  int splits = 1;
+  for (int n = 1; n <= kQuantMaxSplits && (n == 1 || n * g.slices <= tiles); ++n) {
+    const int64_t cost = ceil_div(blocks * n, places) *
+                             (ceil_div(ceil_div(tiles, n), g.slices) + 8) +
+                         (n > 1 ? 4 : 0);
+    if (n == 1 || cost < least) {
+      least = cost;
+      splits = n;
+    }
+  }
+  return splits;
 }
 int check_sizes(int batch, int dtype, int64_t pool_blocks, int64_t count, int q_heads,
                 int kv_heads, int head_dim, int page_size) {
@@ -245,6 +259,9 @@ int launch_merge(const QuantAttendParams &p, int phases, void *out, cudaStream_t
   return check_launch("quant_merge_kernel");
 }
 int launch_rows(const QuantAttendParams &p, int dtype, cudaStream_t s) {
+  if (dtype != HS_FLOAT32 && p.head_dim % 16 == 0 && p.rows_head_stride == 0 &&
+      reinterpret_cast<uintptr_t>(p.query) % 8 == 0 && p.q_batch_stride % 4 == 0)
+    return launch_quant_mma(p, dtype, s);
   switch (dtype) {
     case HS_FLOAT32: return launch_rows<float>(p, s);
     case HS_FLOAT16: return launch_rows<__half>(p, s);
@@ -269,7 +286,7 @@ QuantAttendParams params_of(int batch, int phases, int q_heads, int kv_heads, in
   p.kv_heads = kv_heads;
   p.head_dim = head_dim;
   p.groups = q_heads / kv_heads;
-  p.splits = quant_splits(batch, kv_heads, count);
+  p.splits = quant_splits(batch, q_heads, kv_heads, head_dim, count);
   p.record = record_bytes(kv_heads, head_dim);
   p.scale_log2 = (float)(1.4426950408889634 / sqrt((double)head_dim));
   p.stats = static_cast<float4 *>(workspace);
@@ -286,7 +303,7 @@ extern "C" size_t hs_attend_quantized_workspace_bytes(int batch, int phases, int
   using namespace hs;
   if (batch < 1 || phases < 1 || kv_heads < 1 || q_heads < kv_heads || head_dim < 1 || count < 0)
     return 0;
-  const int splits = quant_splits(batch, kv_heads, count);
+  const int splits = quant_splits(batch, q_heads, kv_heads, head_dim, count);
   if (splits == 1 && phases == 1) return 0;
   const int64_t parts = (int64_t)phases * batch * q_heads * splits;
   return (size_t)parts * (sizeof(float4) + quant_pad(head_dim) * sizeof(float));

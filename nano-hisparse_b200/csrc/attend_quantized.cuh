@@ -8,7 +8,7 @@
 
 namespace hs {
 
-constexpr int kQuantMaxSplits = 64;
+constexpr int kQuantMaxSplits = 128;
 constexpr float kSumLift = 10.f, kSumScale = 1024.f;  // 2^kSumLift
 
 struct QuantAttendParams {
@@ -69,5 +69,16 @@ __device__ __forceinline__ float4 quant_larger(float4 a, float4 b) {
 __device__ __forceinline__ float quant_share(float s, float e, float top_s, float top_e) {
   return quant_exp2((s - top_s) + (e - top_e));
 }
+
+// attend_quantized_mma.cu: 16-bit queries, head_dim a multiple of 16, shared rows, query
+// and its stride multiples of 8 bytes
+struct QuantMmaGrid {
+  int queries, chunks;         // query heads of a warp, such parts of a KV head's
+  int heads, groups, places;   // KV heads of a block, such blocks, warps side by side
+  int slices;                  // warps that share a head's rows
+  int resident;                // blocks on an SM
+};
+QuantMmaGrid quant_mma_grid(int q_heads, int kv_heads, int head_dim);
+int launch_quant_mma(const QuantAttendParams &p, int dtype, cudaStream_t s);
 
 }  // namespace hs

@@ -67,7 +67,7 @@ def test_host_side_validation_needs_no_device():
     assert read(count=-1) == read(dtype=5) == read(pool=None) == read(pool=8) == bad
     assert read(dim=257) == unsupported
 
-    def attend(batch=1, q_heads=4, dim=32, count=64, dtype=_lib.HS_FLOAT32, ws=16, nbytes=1 << 30,
+    def attend(batch=1, q_heads=4, dim=32, count=4096, dtype=_lib.HS_FLOAT32, ws=16, nbytes=1 << 30,
                pool=16):
         return lib.hs_attend_quantized(batch, 16, 128, dtype, pool, 4, 16, count, 0, count, None,
                                        16, q_heads, 2, dim, 16, ws, nbytes, None, None)
@@ -76,7 +76,7 @@ def test_host_side_validation_needs_no_device():
     assert attend(q_heads=5) == attend(count=-1) == attend(dtype=9) == attend(pool=None) == bad
     assert attend(pool=24) == bad
     assert attend(dim=257) == attend(batch=65536) == unsupported
-    assert lib.hs_attend_quantized_workspace_bytes(1, 1, 4, 2, 32, 64) > 0
+    assert lib.hs_attend_quantized_workspace_bytes(1, 1, 4, 2, 32, 4096) > 0
     assert attend(ws=None) == attend(nbytes=8) == attend(ws=8) == workspace
 
     def phase(phase=0, counts_n=1, nbytes=1 << 30):
@@ -89,8 +89,8 @@ def test_host_side_validation_needs_no_device():
     assert lib.hs_attend_quantized_merge(1, 3, 16, 0, 4, 2, 32, 64, 16, 1 << 30, None) == bad
     assert lib.hs_attend_quantized_merge(1, 2, None, 0, 4, 2, 32, 64, 16, 1 << 30, None) == bad
     assert lib.hs_attend_quantized_merge(1, 2, 16, 0, 4, 2, 32, 64, 16, 8, None) == workspace
-    assert lib.hs_attend_quantized_workspace_bytes(2, 2, 4, 2, 32, 64) >= \
-        2 * lib.hs_attend_quantized_workspace_bytes(2, 1, 4, 2, 32, 64) > 0
+    assert lib.hs_attend_quantized_workspace_bytes(2, 2, 4, 2, 32, 4096) >= \
+        2 * lib.hs_attend_quantized_workspace_bytes(2, 1, 4, 2, 32, 4096) > 0
 
 
 def test_operators_refuse_cpu_tensors():
