@@ -49,7 +49,7 @@ HS_API int64_t hs_quantized_row_bytes(int kv_heads, int head_dim);
  * their way into pool and host records, and with the metadata taken from the
  * values that are held: minimum_ptrs / maximum_ptrs point to bf16 bounds
  * (torch.minimum / torch.maximum semantics), summary_ptrs to the fp32 mean of the
- * page's rows so far. A row of k or v is kv_heads * head_dim adjacent elements,
+ * page's rows so far; all three NULL: no metadata. A row of k or v is kv_heads * head_dim adjacent elements,
  * rows of a chunk follow one another, chunks are kv_batch_stride elements apart.
  */
 HS_API int hs_append_quantized(int batch, const void *k, const void *v, int64_t kv_batch_stride,

@@ -118,7 +118,8 @@ __global__ void __launch_bounds__(32 * kAppendWarps) append_quantized_kernel(Qua
     high[i] = -INFINITY;
     sum[i] = 0.f;
   }
-  if (plane == 0 && here) {  // rows 0 .. w-1 of the page, for the mean
+  const bool metadata = plane == 0 && p.minimum_ptrs != nullptr;
+  if (metadata && here) {  // rows 0 .. w-1 of the page, for the mean
     const unsigned char *page = pool != nullptr ? pool : host;
 #pragma unroll 4
     for (int r = first; r < w; r += step) {
@@ -158,7 +159,7 @@ __global__ void __launch_bounds__(32 * kAppendWarps) append_quantized_kernel(Qua
       if (pool != nullptr) store8<kWide>(pool + to, n, codes);
       if (host != nullptr) store8<kWide>(host + to, n, codes);
       if (lane % lanes == 0) scales[r][head] = (unsigned char)(e + 127);
-      if (plane == 0) {
+      if (metadata) {
         decode8(codes, power_of_two(e), x);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -179,7 +180,7 @@ __global__ void __launch_bounds__(32 * kAppendWarps) append_quantized_kernel(Qua
     }
     __syncthreads();
   }
-  if (plane != 0) return;
+  if (!metadata) return;
   // ---- metadata: the lanes that share columns meet in shuffles, the slices in shared memory
   for (int o = lanes; o < 32; o <<= 1) {
 #pragma unroll
@@ -337,8 +338,8 @@ extern "C" int hs_append_quantized(int batch, const void *k, const void *v,
     return set_error(HS_ERR_UNSUPPORTED, "append: head_dim %d > %d is not supported", head_dim,
                      kQuantMaxDim);
   if (batch == 0) return HS_OK;
-  if (!k || !v || !within || !count || !pool_block || !pool || !host_block || !minimum_ptrs ||
-      !maximum_ptrs || !summary_ptrs)
+  if (!k || !v || !within || !count || !pool_block || !pool || !host_block ||
+      !minimum_ptrs != !maximum_ptrs || !minimum_ptrs != !summary_ptrs)
     return set_error(HS_ERR_INVALID_ARGUMENT, "append: null pointer");
   if (batch > 65535) return set_error(HS_ERR_UNSUPPORTED, "append: batch %d > 65535", batch);
   QuantAppendParams p{batch, k, v, kv_batch_stride, within, count, pool_block, host_block,

@@ -22,6 +22,7 @@ import torch
 
 from . import _lib
 from .cache import RowCache
+from .config import CacheConfig, held_in_8_bits
 
 
 def _pointers(tensors, device):
@@ -63,6 +64,8 @@ class DecodeBatch:
     """Decode hot path for a fixed set of requests of a RowCache.
 
     minimum / maximum: {request_id: [layers, pages, Hkv, D]} Quest metadata.
+    Queries have the cache's dtype; those over a cache held in 8 bits may be
+    float32, float16 or bfloat16.
     """
 
     def __init__(self, cache: RowCache, request_ids, layers, minimum, maximum, top_pages,
@@ -106,8 +109,12 @@ class DecodeBatch:
         self.quest_ws = _lib.workspace(self.quest_ws_bytes, dev, zeroed=True)
         self.resolve_ws_bytes = lib.hs_resolve_workspace_bytes(b, self.width, self.hot_rows)
         self.resolve_ws = _lib.workspace(self.resolve_ws_bytes, dev)
-        self.attend_ws_bytes = lib.hs_attend_workspace_bytes(b, q_heads, cfg.kv_heads,
-                                                             cfg.head_dim, self.width)
+        if held_in_8_bits(cfg):
+            self.attend_ws_bytes = lib.hs_attend_quantized_workspace_bytes(
+                b, 2, q_heads, cfg.kv_heads, cfg.head_dim, self.width)
+        else:
+            self.attend_ws_bytes = lib.hs_attend_workspace_bytes(b, q_heads, cfg.kv_heads,
+                                                                 cfg.head_dim, self.width)
         self.attend_ws = _lib.workspace(self.attend_ws_bytes, dev)
         self.group, self.shards = group, 1
         if group is not None:
@@ -125,7 +132,7 @@ class DecodeBatch:
             self.partials = torch.empty((self.shards, b * self.max_pages), dtype=torch.float32,
                                         device=dev)
         self.status = _lib.status_word(dev)
-        self._dtype = _lib.dtype_code(cfg.dtype)
+        self._dtype = _lib.dtype_code(cfg.metadata_dtype)
         self._row_bytes = cfg.row_bytes
 
     def set_lengths(self, layer: int, lengths: torch.Tensor):
@@ -233,7 +240,10 @@ class DecodeBatch:
         over the physical rows and the nodes' own key/value, on the batch's compute
         stream. query [B, T, Hq, D], key/value [B, T, Hkv, D], mask int64 [B, T],
         nodes int32 [B] (see attend_tree); positions int32 [B, width], -1 padded
-        behind row_counts int32 [B] leading ones. Returns [B, T, Hq, D]."""
+        behind row_counts int32 [B] leading ones. Returns [B, T, Hq, D]. Rows held
+        in 8 bits are read back in the query's dtype first (``read_quantized``), and
+        the nodes' own are taken as they will be held."""
+        from .quantized import held_values, read_quantized
         from .tree import attend_tree
 
         cfg, st, compute = self.config, self.layers[layer], self.compute
@@ -249,8 +259,19 @@ class DecodeBatch:
             compute.wait_event(st.ready)
         self._resolve_and_gather(layer, positions.data_ptr(), st.counts)
         compute.wait_event(st.ready)
-        out = attend_tree(query, key, value, mask, self.cache.pool, self.physical, cfg,
-                          counts=row_counts, nodes=nodes)
+        pool, rows = self.cache.pool, self.physical
+        if held_in_8_bits(cfg):
+            # one page of all rows, in the order of the requests; padding has none
+            page = self.batch * self.width
+            order = torch.arange(page, device=self.device).view(self.batch, self.width)
+            pool = read_quantized(pool, rows, cfg, query.dtype).view(
+                1, 2, page, cfg.kv_heads, cfg.head_dim)
+            rows = torch.where(rows >= 0, order, rows)
+            key, value = held_values(key, value, cfg)
+            cfg = CacheConfig(gpu_pages=1, page_size=page, kv_heads=cfg.kv_heads,
+                              head_dim=cfg.head_dim, device=cfg.device, dtype=query.dtype)
+        out = attend_tree(query, key, value, mask, pool, rows, cfg, counts=row_counts,
+                          nodes=nodes)
         st.last_use = torch.cuda.Event()
         st.last_use.record(compute)
         return out
@@ -341,9 +362,17 @@ class DecodeBatch:
         if serial:
             compute.wait_event(st.ready)
         t5 = mark(compute, "attend_ready")
-        common = (b, query.data_ptr(), hq * d, _lib.dtype_code(query.dtype), cache.pool.data_ptr(),
-                  cache.pool.shape[0], self._dtype)
-        _lib.check(lib.hs_attend_rows_phase(
+        common = [b, query.data_ptr(), hq * d, _lib.dtype_code(query.dtype), cache.pool.data_ptr(),
+                  cache.pool.shape[0]]
+        merge = [b, 2, out.data_ptr(), hq * d, _lib.dtype_code(query.dtype), hq, cfg.kv_heads, d,
+                 self.width, _lib.ptr(self.attend_ws), self.attend_ws_bytes, status, stream]
+        if held_in_8_bits(cfg):
+            attend_phase, attend_merge = lib.hs_attend_quantized_phase, lib.hs_attend_quantized_merge
+            del merge[3], merge[-2]  # the output is contiguous; the merge meets no rows
+        else:
+            attend_phase, attend_merge = lib.hs_attend_rows_phase, lib.hs_attend_merge
+            common.append(self._dtype)
+        _lib.check(attend_phase(
             *common, self.ready.data_ptr(), self.width, self.width, counts.data_ptr(), 3, 0, 2, 0,
             hq, cfg.kv_heads, d, cfg.page_size, _lib.ptr(self.attend_ws), self.attend_ws_bytes,
             status, stream))
@@ -351,14 +380,12 @@ class DecodeBatch:
         # phase 1: the gathered rows, then the merge
         compute.wait_event(st.ready)
         t7 = mark(compute, "attend_gathered")
-        _lib.check(lib.hs_attend_rows_phase(
+        _lib.check(attend_phase(
             *common, self.miss_device.data_ptr(), self.width, self.width, counts.data_ptr(), 3, 2,
             1, 1, hq, cfg.kv_heads, d, cfg.page_size, _lib.ptr(self.attend_ws),
             self.attend_ws_bytes, status, stream))
         t8 = mark(compute, "attend_gathered", "merge")
-        _lib.check(lib.hs_attend_merge(
-            b, 2, out.data_ptr(), hq * d, _lib.dtype_code(query.dtype), hq, cfg.kv_heads, d,
-            self.width, _lib.ptr(self.attend_ws), self.attend_ws_bytes, status, stream))
+        _lib.check(attend_merge(*merge))
         if timing is not None:
             t9 = mark(compute, "merge")
             for name, a, b_ in (("quest", t0, t1), ("resolve", t1, t2), ("gather", t3, t4),
@@ -388,7 +415,7 @@ class DecodeGraph:
     previous step's readers of its hot rows.
     """
 
-    def __init__(self, batches, layers: int, timing=False, segmented=None):
+    def __init__(self, batches, layers: int, timing=False, segmented=None, dtype=None):
         """timing: False, True (every stage) or an iterable of stage names of
         DecodeBatch.layer; the captured step then records timing events, and
         after a replay ``self.timing`` holds that replay's (name, start, end)
@@ -399,7 +426,10 @@ class DecodeGraph:
         all-gathers between them at replay, so no collective is captured.
         Default: when a batch has a process group (head-sharded selection).
         A replay then costs the host two graph launches and one all-gather
-        per layer."""
+        per layer.
+
+        dtype: of the queries and outputs over a cache held in 8 bits (bfloat16
+        without); otherwise the cache's."""
         self.batches, self.layers = list(batches), layers
         if segmented is None:
             segmented = any(bt.group is not None for bt in self.batches)
@@ -413,6 +443,10 @@ class DecodeGraph:
         b0 = self.batches[0]
         self.device = b0.device
         dt = b0.config.dtype
+        if held_in_8_bits(b0.config):
+            dt = torch.bfloat16 if dtype is None else dtype
+        elif dtype not in (None, dt):
+            raise ValueError("queries must have the cache's dtype")
         self.queries = [torch.zeros((layers, bt.batch, bt.q_heads, bt.config.head_dim),
                                     dtype=dt, device=self.device) for bt in self.batches]
         self.outputs = [torch.empty_like(q) for q in self.queries]

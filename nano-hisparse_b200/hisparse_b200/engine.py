@@ -339,7 +339,7 @@ class ServingCache:
         self.free_pool = list(range(config.gpu_pages))[::-1]  # pop() takes the lowest
         self.free_host = list(range(config.host_pages))[::-1]
         self.requests: dict[str, _Reservation] = {}
-        elt = torch.empty((), dtype=config.dtype).element_size()
+        elt = config.metadata_dtype.itemsize
         self._meta_row = config.kv_heads * config.head_dim
         self._meta_bytes = self._meta_row * elt
         self.stats = {"borrowed": 0, "revoked": 0, "host_only_pages": 0}
@@ -400,8 +400,9 @@ class ServingCache:
             tags = torch.full((layers, h), -1, dtype=torch.int32, device=dev)
             lru = torch.arange(h, dtype=torch.int64, device=dev).repeat(layers, 1)
             shape = (layers, pages, cfg.kv_heads, cfg.head_dim)
-            res.minimum = torch.full(shape, float("inf"), dtype=cfg.dtype, device=dev)
-            res.maximum = torch.full(shape, float("-inf"), dtype=cfg.dtype, device=dev)
+            bounds = cfg.metadata_dtype
+            res.minimum = torch.full(shape, float("inf"), dtype=bounds, device=dev)
+            res.maximum = torch.full(shape, float("-inf"), dtype=bounds, device=dev)
             res.summary = torch.zeros(shape, dtype=torch.float32, device=dev)
         res.tables = (source, resident, hot, tags, lru)
         for layer in range(layers):
@@ -678,7 +679,11 @@ class BatchedEngine:
     ``propose(limit)``, so that no turn hands over the whole text again (None: it is
     asked with the text after all). A request's turn then emits one or more tokens, those that greedy decoding
     would emit one by one. Needs the full causal history (top_k=None): with a
-    page budget every token selects its own pages."""
+    page budget every token selects its own pages.
+
+    A cache held in 8 bits (CacheConfig(dtype=torch.float8_e4m3fn)) serves a model
+    of any dtype: rows are quantised as they are appended, and decode turns attend
+    to the values held. A prompt attends to its own exact rows."""
 
     def __init__(self, model, cache: ServingCache, top_k=None, backend="auto",
                  eos_token_id: int | None = None, selector: str = "quest",
@@ -687,7 +692,8 @@ class BatchedEngine:
         cfg, kv = weights.config, cache.config
         if (cfg.num_key_value_heads, cfg.head_dim) != (kv.kv_heads, kv.head_dim):
             raise ValueError("model/cache head dimensions differ")
-        if weights.device != cache.pool.device or weights.dtype != cache.pool.dtype:
+        if weights.device != cache.pool.device or (weights.dtype != kv.dtype
+                                                   and not kv.quantized):
             raise ValueError("model/cache dtype or device differ")
         if top_k is not None and top_k < 1:
             raise ValueError("top_k must be positive or None")

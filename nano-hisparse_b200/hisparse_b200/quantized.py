@@ -16,6 +16,8 @@ formulas stand in include/hisparse_quantized.h.
 
 from __future__ import annotations
 
+from dataclasses import replace
+
 import torch
 
 from . import _lib
@@ -40,7 +42,8 @@ def append_quantized(k, v, within, count, pool_block, pool, minimum_ptrs, maximu
     k, v: [B, T, Hkv, D] of one of the three value dtypes (chunk b uses rows
     0..count[b]-1); within, count: int32 [B]; pool_block: int64 [B];
     minimum_ptrs / maximum_ptrs / summary_ptrs: int64 [B] device pointers to the
-    page's [Hkv, D] bounds (bfloat16) and fp32 mean, both of the values held;
+    page's [Hkv, D] bounds (bfloat16) and fp32 mean, both of the values held
+    (all three None: no metadata);
     host: MappedHost of the pinned store (uint8, of the pool's page shape) and
     host_block int64 [B] (-1: no mirror; pool_block -1: host only). Chunks of one
     call must touch distinct pages. Runs on the current stream.
@@ -60,12 +63,17 @@ def append_quantized(k, v, within, count, pool_block, pool, minimum_ptrs, maximu
     batch, tokens = shape[:2]
     if host_block is None:
         host_block = torch.full_like(pool_block, -1)
+    metadata = (minimum_ptrs, maximum_ptrs, summary_ptrs)
+    if any(t is None for t in metadata) and any(t is not None for t in metadata):
+        raise ValueError("bounds and mean go together: all three addresses or none")
     for name, t, dt in (("within", within, torch.int32), ("count", count, torch.int32),
                         ("pool_block", pool_block, torch.int64),
                         ("host_block", host_block, torch.int64),
                         ("minimum_ptrs", minimum_ptrs, torch.int64),
                         ("maximum_ptrs", maximum_ptrs, torch.int64),
                         ("summary_ptrs", summary_ptrs, torch.int64)):
+        if t is None:
+            continue
         if t.dtype != dt or t.numel() != batch or not t.is_contiguous():
             raise ValueError(f"{name} must be a contiguous {dt} tensor of {batch} entries")
     # rows of a chunk adjacent (copied when they are not); any distance between chunks
@@ -80,11 +88,26 @@ def append_quantized(k, v, within, count, pool_block, pool, minimum_ptrs, maximu
             batch, k.data_ptr(), v.data_ptr(), strides[0], _lib.dtype_code(k.dtype),
             within.data_ptr(), count.data_ptr(), pool_block.data_ptr(), pool.data_ptr(), blocks,
             host_block.data_ptr(), None if host is None else host.data_ptr(),
-            0 if host is None else host.tensor.shape[0], minimum_ptrs.data_ptr(),
-            maximum_ptrs.data_ptr(), summary_ptrs.data_ptr(), config.kv_heads, config.head_dim,
-            config.page_size, _lib.status_pointer(index), _lib.raw_stream(index))
+            0 if host is None else host.tensor.shape[0], *map(_lib.ptr, metadata),
+            config.kv_heads, config.head_dim, config.page_size, _lib.status_pointer(index),
+            _lib.raw_stream(index))
     if status:
         _lib.check(status)
+
+
+def held_values(k, v, config):
+    """The values that K and V rows [B, T, Hkv, D] will be held as, in their own dtype:
+    [2, B, T, Hkv, D]. Drafted rows that are not appended yet are attended to as those,
+    so that a drafted turn computes what the plain turns after it will."""
+    batch, tokens = k.shape[:2]
+    page = replace(config, gpu_pages=max(1, batch), page_size=max(1, tokens))
+    pool = k.new_empty((batch, *page.page_shape), dtype=torch.uint8)
+    within = torch.zeros(batch, dtype=torch.int32, device=k.device)
+    blocks = torch.arange(batch, device=k.device)
+    append_quantized(k, v, within, torch.full_like(within, tokens), blocks, pool, None, None,
+                     None, page)
+    rows = torch.arange(batch * tokens, device=k.device).view(batch, tokens)
+    return read_quantized(pool, rows, page, k.dtype)
 
 
 def read_quantized(pool, rows, config, dtype=torch.bfloat16):
