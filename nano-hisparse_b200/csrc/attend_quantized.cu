@@ -22,6 +22,7 @@ constexpr int kSimtAhead = 4;    // rows of a warp in flight
 // neighbouring elements of each.
 template <typename T, int C>
 __global__ void __launch_bounds__(kSimtThreads) quant_simt_kernel(QuantAttendParams p) {
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
   __shared__ float4 red[kSimtWarps][kSimtHeads];  // a maximum's score, exponent; the sum
   __shared__ float red_o[kSimtWarps][kSimtHeads][32 * C];
   const int split = blockIdx.x, b = blockIdx.z, D = p.head_dim;
@@ -136,56 +137,80 @@ __global__ void __launch_bounds__(kSimtThreads) quant_simt_kernel(QuantAttendPar
 }
 
 // ---- the join of splits and phases ----------------------------------------------------------
-constexpr int kJoinWarps = 4;
+constexpr int kJoinThreads = 256, kJoinAhead = 4;
 
-// One block a query head; a warp takes every fourth partial result, a lane four
-// elements of each.
-template <typename T>
-__global__ void __launch_bounds__(32 * kJoinWarps) quant_merge_kernel(QuantAttendParams p,
-                                                                      int phases, T *out) {
-  __shared__ float4 sums[kJoinWarps][kQuantMaxDim / 4];
+// One block a query head. A thread reads the statistics of one partial result (at most two
+// phases of kQuantMaxSplits), whose weights meet in shared memory; then kLanes threads
+// have four elements each, and kJoinThreads / kLanes groups of them a share of the
+// results, kJoinAhead loads in flight.
+template <typename T, int kLanes>
+__global__ void __launch_bounds__(kJoinThreads) quant_merge_kernel(QuantAttendParams p, int phases,
+                                                                   T *out) {
+  constexpr int kGroups = kJoinThreads / kLanes, kWarps = kJoinThreads / 32;
+  static_assert(2 * kQuantMaxSplits <= kJoinThreads, "a thread for each partial result");
+  __shared__ float weights[kJoinThreads];
+  __shared__ float4 tops[kWarps];
+  __shared__ float totals[kWarps];
+  __shared__ float4 sums[kGroups][kLanes];
   const int h = blockIdx.x, b = blockIdx.y, D = p.head_dim, quads = quant_pad(D) / 4;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, all = phases * p.splits;
-  const auto part = [&](int i) { return quant_part(p, i / p.splits, b, h, i % p.splits); };
-  float4 top = make_float4(-INFINITY, 0.f, 0.f, 0.f);
-  float l = 0.f;
-  for (int i = lane; i < all; i += 32) top = quant_larger(top, p.stats[part(i)]);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, all = phases * p.splits;
+  const int quad = tid % kLanes, group = tid / kLanes;
+  const auto part = [&](int i) {
+    const int phase = i >= p.splits;
+    return quant_part(p, phase, b, h, i - phase * p.splits);
+  };
+  const auto load = [&](int i, float4(&x)[kJoinAhead]) {
+#pragma unroll
+    for (int u = 0; u < kJoinAhead; ++u)
+      if (i + u * kGroups < all && quad < quads)
+        x[u] = reinterpret_cast<const float4 *>(p.partials)[part(i + u * kGroups) * quads + quad];
+  };
+  // Every thread waits: this kernel must not end before the one that writes the workspace.
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  float4 x[kJoinAhead];
+  const float4 mine = tid < all ? p.stats[part(tid)] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+  load(group, x);
+  float4 top = mine;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1)
     top = quant_larger(top, make_float4(__shfl_xor_sync(kFullMask, top.x, o),
                                         __shfl_xor_sync(kFullMask, top.y, o),
                                         __shfl_xor_sync(kFullMask, top.z, o), 0.f));
-  for (int i = lane; i < all; i += 32) {
-    const float4 s = p.stats[part(i)];
-    if (s.z != 0.f) l = fmaf(s.z, quant_share(s.x, s.y, top.x, top.y), l);
-  }
-  l = warp_xor_tree_sum(l);
-  float4 x[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
-  for (int i = warp; i < all; i += kJoinWarps) {
-    const float4 s = p.stats[part(i)];
-    if (s.z == 0.f) continue;  // saw nothing
-    const float f = quant_share(s.x, s.y, top.x, top.y);
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-      if (lane + 32 * j < quads) {
-        const float4 y =
-            reinterpret_cast<const float4 *>(p.partials + part(i) * 4 * quads)[lane + 32 * j];
-        x[j].x = fmaf(f, y.x, x[j].x);
-        x[j].y = fmaf(f, y.y, x[j].y);
-        x[j].z = fmaf(f, y.z, x[j].z);
-        x[j].w = fmaf(f, y.w, x[j].w);
-      }
-  }
-#pragma unroll
-  for (int j = 0; j < 2; ++j)
-    if (lane + 32 * j < quads) sums[warp][lane + 32 * j] = x[j];
+  if (lane == 0) tops[warp] = top;
   __syncthreads();
-  const float inv = l > 0.f || l != l ? kSumScale / l : 0.f;
-  for (int d = threadIdx.x; d < D; d += 32 * kJoinWarps) {
-    float y = 0.f;
-    for (int w = 0; w < kJoinWarps; ++w) y += reinterpret_cast<const float *>(sums[w])[d];
-    out[((int64_t)b * p.q_heads + h) * D + d] = from_f32<T>(y * inv);
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) top = quant_larger(top, tops[w]);
+  // one that saw nothing left no output: below 0
+  const float f = mine.z == 0.f ? -1.f : quant_share(mine.x, mine.y, top.x, top.y);
+  weights[tid] = f;
+  const float share = warp_xor_tree_sum(mine.z == 0.f ? 0.f : mine.z * f);
+  if (lane == 0) totals[warp] = share;
+  __syncthreads();
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = group; i < all; i += kJoinAhead * kGroups) {
+    if (i != group) load(i, x);
+#pragma unroll
+    for (int u = 0; u < kJoinAhead; ++u) {
+      if (i + u * kGroups >= all) break;
+      const float w = weights[i + u * kGroups];
+      if (w < 0.f || quad >= quads) continue;
+      sum.x = fmaf(w, x[u].x, sum.x);
+      sum.y = fmaf(w, x[u].y, sum.y);
+      sum.z = fmaf(w, x[u].z, sum.z);
+      sum.w = fmaf(w, x[u].w, sum.w);
+    }
   }
+  sums[group][quad] = sum;
+  __syncthreads();
+  float l = 0.f;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) l += totals[w];
+  const float inv = l > 0.f || l != l ? kSumScale / l : 0.f;
+  if (tid >= D) return;
+  float y = 0.f;
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g) y += reinterpret_cast<const float *>(sums[g])[tid];
+  out[((int64_t)b * p.q_heads + h) * D + tid] = from_f32<T>(y * inv);
 }
 
 // Splits of a request's rows: those with the least (rounds of blocks) x (tiles of 16 rows
@@ -252,15 +277,31 @@ template <typename T> int launch_rows(const QuantAttendParams &p, cudaStream_t s
   }
   return check_launch("quant_simt_kernel");
 }
+// beside: whether its launch may overlap the end of the kernel before it, which it waits
+// for itself
 template <typename T>
-int launch_merge(const QuantAttendParams &p, int phases, void *out, cudaStream_t s) {
-  const dim3 grid((unsigned)p.q_heads, (unsigned)p.batch);
-  quant_merge_kernel<T><<<grid, 32 * kJoinWarps, 0, s>>>(p, phases, static_cast<T *>(out));
+int launch_merge(const QuantAttendParams &p, int phases, void *out, bool beside, cudaStream_t s) {
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3((unsigned)p.q_heads, (unsigned)p.batch);
+  config.blockDim = dim3(kJoinThreads);
+  config.stream = s;
+  cudaLaunchAttribute attribute{};
+  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attribute;
+  config.numAttrs = beside ? 1 : 0;
+  T *to = static_cast<T *>(out);
+  if (p.head_dim <= 64) cudaLaunchKernelEx(&config, quant_merge_kernel<T, 16>, p, phases, to);
+  else if (p.head_dim <= 128) cudaLaunchKernelEx(&config, quant_merge_kernel<T, 32>, p, phases, to);
+  else cudaLaunchKernelEx(&config, quant_merge_kernel<T, 64>, p, phases, to);
   return check_launch("quant_merge_kernel");
 }
 int launch_rows(const QuantAttendParams &p, int dtype, cudaStream_t s) {
-  if (dtype != HS_FLOAT32 && p.head_dim % 16 == 0 && p.rows_head_stride == 0 &&
-      reinterpret_cast<uintptr_t>(p.query) % 8 == 0 && p.q_batch_stride % 4 == 0)
+  // the tensor-core kernel reads four query elements together and numbers records in 32 bits
+  const int four = dtype == HS_FLOAT32 ? 16 : 8;
+  if (p.head_dim % 16 == 0 && p.rows_head_stride == 0 &&
+      reinterpret_cast<uintptr_t>(p.query) % four == 0 && p.q_batch_stride % 4 == 0 &&
+      p.pool_blocks <= 0xfffffffell / 2 / p.page_size)
     return launch_quant_mma(p, dtype, s);
   switch (dtype) {
     case HS_FLOAT32: return launch_rows<float>(p, s);
@@ -268,11 +309,12 @@ int launch_rows(const QuantAttendParams &p, int dtype, cudaStream_t s) {
     default: return launch_rows<__nv_bfloat16>(p, s);
   }
 }
-int launch_merge(const QuantAttendParams &p, int phases, void *out, int dtype, cudaStream_t s) {
+int launch_merge(const QuantAttendParams &p, int phases, void *out, int dtype, bool beside,
+                 cudaStream_t s) {
   switch (dtype) {
-    case HS_FLOAT32: return launch_merge<float>(p, phases, out, s);
-    case HS_FLOAT16: return launch_merge<__half>(p, phases, out, s);
-    default: return launch_merge<__nv_bfloat16>(p, phases, out, s);
+    case HS_FLOAT32: return launch_merge<float>(p, phases, out, beside, s);
+    case HS_FLOAT16: return launch_merge<__half>(p, phases, out, beside, s);
+    default: return launch_merge<__nv_bfloat16>(p, phases, out, beside, s);
   }
 }
 
@@ -342,7 +384,7 @@ extern "C" int hs_attend_quantized(int batch, const void *query, int64_t query_b
   p.status = device_status;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int status = launch_rows(p, dtype, s);
-  return status != HS_OK || p.splits == 1 ? status : launch_merge(p, 1, out, dtype, s);
+  return status != HS_OK || p.splits == 1 ? status : launch_merge(p, 1, out, dtype, true, s);
 }
 
 extern "C" int hs_attend_quantized_phase(int batch, const void *query,
@@ -397,5 +439,5 @@ extern "C" int hs_attend_quantized_merge(int batch, int phases, void *out, int d
   if (!out) return set_error(HS_ERR_INVALID_ARGUMENT, "attend_quantized: null pointer");
   QuantAttendParams p = params_of(batch, 2, q_heads, kv_heads, head_dim, count, workspace);
   if (int e = place_workspace(p, 2, workspace, workspace_bytes)) return e;
-  return launch_merge(p, phases, out, dtype, static_cast<cudaStream_t>(stream));
+  return launch_merge(p, phases, out, dtype, false, static_cast<cudaStream_t>(stream));
 }

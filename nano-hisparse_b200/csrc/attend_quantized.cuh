@@ -70,8 +70,8 @@ __device__ __forceinline__ float quant_share(float s, float e, float top_s, floa
   return quant_exp2((s - top_s) + (e - top_e));
 }
 
-// attend_quantized_mma.cu: 16-bit queries, head_dim a multiple of 16, shared rows, query
-// and its stride multiples of 8 bytes
+// attend_quantized_mma.cu: head_dim a multiple of 16, shared rows, query and its stride
+// multiples of four elements, fewer than 2^32 records
 struct QuantMmaGrid {
   int queries, chunks;         // query heads of a warp, such parts of a KV head's
   int heads, groups, places;   // KV heads of a block, such blocks, warps side by side

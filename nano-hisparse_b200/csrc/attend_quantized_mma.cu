@@ -1,21 +1,26 @@
-// Decode attention over an 8-bit cache, 16-bit queries, head_dim a multiple of 16, heads
+// Decode attention over an 8-bit cache on tensor cores: head_dim a multiple of 16, heads
 // that share their rows.
 //
-// A warp serves one KV head and up to 8 * kTiles of its query heads over tiles of 16
-// rows, alone: it copies its own tiles (cp.async, 16 bytes a lane, into a ring of its
-// own) and keeps its own maximum, sum and output, so that nothing in the loop waits for
-// another warp. The heads of a block read neighbouring parts of the same rows. With
-// keys as the M side of m16n8k16 and the query heads as N,
-//   S^T = K Q^T     the codes of a lane's ldmatrix word are two fp16 pairs (every e4m3
-//                   number is one of fp16); which element of head_dim stands where in
-//                   the sum does not matter as long as Q is laid out alike. Q is fp16,
-//                   scaled by a power of two for each query, which keeps bf16 exact.
-//   O^T += V^T P^T  V through ldmatrix.trans, whose 16-bit unit is two neighbouring
-//                   elements of a row: a byte permutation makes pairs of rows of each.
-//                   P is rounded to fp16, times 2^7 at the current maximum, which is
-//                   raised only when a weight would pass it by more than 2^8. Half a step
-//                   of a weight (2^-11) is an eighth of a bf16 result's own rounding; for
-//                   fp16 results, which round by as much, what was lost is a second P.
+// A warp serves one KV head and up to 4 * kQuads of its query heads over units of 32
+// rows, alone: it copies its own rows (cp.async, 16 bytes a lane, into a ring of its own)
+// and keeps its own maximum, sum and output, so that nothing in the loop waits for
+// another warp. The heads of a block read neighbouring parts of the same rows. Keys are
+// the M side of the products, 16 at a time:
+//   S^T = K Q^T     m16n8k32 in e4m3: the codes go from ldmatrix to the tensor core as
+//                   they are. Q is taken apart into e4m3 numbers, each a sixteenth of the
+//                   one before it (q = q0 + q1 / 16 + ...): 2 parts hold bf16, 3 fp16 and
+//                   6 fp32 exactly, since each part leaves at most 2^-4 of what it takes.
+//                   Two parts of a query are neighbouring columns, whose sums meet in one
+//                   lane. The products are exact and added in fp32 (measured: within
+//                   2^-20 of the largest, as fp16 products are).
+//   O^T += V^T P^T  m16n8k16 in fp16, which holds every e4m3 number. V through
+//                   ldmatrix.trans, whose 16-bit unit is two neighbouring elements of a
+//                   row: a byte permutation makes pairs of rows of each. P is the weight
+//                   rounded to fp16 and, in the column beside it, what that left (22 bits
+//                   together). Two quads of bf16 queries share the columns instead: half
+//                   a step of a weight (2^-11) is an eighth of such a result's rounding.
+// A weight is kept times 2^7 of the current maximum's, which is raised only when one would
+// pass it by more than 2^8.
 #include <type_traits>
 
 #include "attend_quantized.cuh"
@@ -24,21 +29,32 @@ namespace hs {
 namespace {
 
 constexpr int kMmaWarps = 8, kMmaThreads = 32 * kMmaWarps;
-constexpr int kMmaRows = 16;     // rows of a tile
-constexpr float kRaise = 8.f;    // the maximum is raised past this
-constexpr float kWeightLift = 7.f;
+constexpr int kMmaRows = 16;     // rows of a tile, a stage of the ring
+constexpr int kUnitRows = 32;    // two tiles: a lane has the number of one of their rows
+constexpr int kStages = 3;       // the two tiles after the one that is worked on are on their way
+constexpr float kWeightLift = 7.f, kRaise = 15.f;  // lifted weights stay below 2^kRaise
+constexpr float kNothing = 1e38f;                  // base of a query that has seen nothing
 
-template <int kDim, int kTiles> struct MmaShape {
+// parts of a query element
+template <typename T> constexpr int kQueryParts = 2;
+template <> constexpr int kQueryParts<__half> = 3;
+template <> constexpr int kQueryParts<float> = 6;
+
+template <typename T, int kDim, int kQuads> struct MmaShape {
+  static constexpr int query_tiles = (kQueryParts<T> + 1) / 2;  // of 8 columns, for each quad
+  static constexpr bool paired = std::is_same<T, __nv_bfloat16>::value && kQuads > 1;
+  static constexpr int output_tiles = paired ? kQuads / 2 : kQuads;
   static constexpr int pitch = kDim + 16;  // of a row: an odd number of 16-byte chunks
   static constexpr int plane = kMmaRows * pitch;
   static constexpr int stage = 2 * plane + 2 * kMmaRows * 4;  // K, V, the words with their scales
-  static constexpr int stages = kDim == 64 ? 4 : 3;
-  static constexpr int resident = kDim <= 128 && kTiles == 1 ? 2 : 1;
-  static constexpr int queries = 8 * kTiles;
-  static constexpr int ring = stages * stage;
+  static constexpr int queries = 4 * kQuads;
+  static constexpr int ring = kStages * stage;
   // the warps' results at the end, in the place of the rings
   static constexpr int result = queries * (kDim + 4) * 4;
   static constexpr size_t bytes = (size_t)kMmaWarps * (ring > result ? ring : result);
+  // blocks on an SM: two where the output and the queries leave the registers for it
+  static constexpr int resident =
+      kDim / 4 * output_tiles + kDim / 16 * kQuads * query_tiles <= 64 && kDim <= 128 ? 2 : 1;
   static_assert(resident * (bytes + 1024) <= 228 * 1024, "the blocks fit an SM");
 };
 
@@ -51,6 +67,13 @@ __device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr)
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];\n"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(addr));
+}
+__device__ __forceinline__ void mma_e4m3(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0, %1, %2, %3}, "
+               "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};\n"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                         uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -77,16 +100,39 @@ __device__ __forceinline__ void copy4(uint32_t dst, const void *src, int bytes) 
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(dst), "l"(src), "r"(bytes)
                : "memory");
 }
+// This lane's part (of the two of a column pair: `odd`) in each tile of columns
+template <typename T, int kTiles>
+__device__ __forceinline__ void split_query(float4 x, bool odd, uint32_t (&codes)[kTiles]) {
+#pragma unroll
+  for (int part = 0; part < kQueryParts<T>; ++part) {
+    const uint32_t code = encode4(x.x, x.y, x.z, x.w);
+    if ((part & 1) == (int)odd) codes[part / 2] = code;
+    const float4 y = decode4_f32(code);
+    x = make_float4((x.x - y.x) * 16.f, (x.y - y.y) * 16.f, (x.z - y.z) * 16.f,
+                    (x.w - y.w) * 16.f);
+  }
+}
+__device__ __forceinline__ float4 load4(const float *from) {
+  return __ldg(reinterpret_cast<const float4 *>(from));
+}
+template <typename T> __device__ __forceinline__ float4 load4(const T *from) {
+  const uint2 raw = __ldg(reinterpret_cast<const uint2 *>(from));
+  const T *x = reinterpret_cast<const T *>(&raw);
+  return make_float4(to_f32(x[0]), to_f32(x[1]), to_f32(x[2]), to_f32(x[3]));
+}
 
-template <typename T, int kDim, int kTiles>
-__global__ void __launch_bounds__(kMmaThreads, MmaShape<kDim, kTiles>::resident)
+template <typename T, int kDim, int kQuads>
+__global__ void __launch_bounds__(kMmaThreads, MmaShape<T, kDim, kQuads>::resident)
     quant_mma_kernel(QuantAttendParams p, int heads_of_block, int head_places) {
-  using Shape = MmaShape<kDim, kTiles>;
-  constexpr int kParts = std::is_same<T, __half>::value ? 2 : 1;  // of P
-  constexpr int kChunks = kDim / 16, kQueries = Shape::queries, kStages = Shape::stages;
+  using Shape = MmaShape<T, kDim, kQuads>;
+  constexpr int kChunks = kDim / 16, kQueries = Shape::queries;
+  constexpr int kQueryTiles = Shape::query_tiles, kOutputTiles = Shape::output_tiles;
+  constexpr bool kPaired = Shape::paired;
+  constexpr uint32_t kNone = 0xffffffffu;
   extern __shared__ __align__(128) unsigned char smem[];
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, D = p.head_dim;
+  const int lane = threadIdx.x & 31, D = p.head_dim;
+  const int warp = __shfl_sync(kFullMask, threadIdx.x >> 5, 0);
   const int split = blockIdx.x, b = blockIdx.z;
   const int chunks = (p.groups + kQueries - 1) / kQueries;  // of a KV head's query heads
   const int group = blockIdx.y / chunks, chunk = blockIdx.y - group * chunks;
@@ -97,205 +143,237 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<kDim, kTiles>::resident)
   const int h0 = kh * p.groups + chunk * kQueries;
   const int hn = here ? min(kQueries, p.groups - chunk * kQueries) : 0;  // query heads
 
-  // this warp's tiles: first, first + slices, ... < last
-  const int valid = (int)quant_rows(p, b), tiles = (valid + kMmaRows - 1) / kMmaRows;
-  const int first = (int)((int64_t)tiles * split / p.splits) + slice;
-  const int last = here ? (int)((int64_t)tiles * (split + 1) / p.splits) : 0;
+  // this warp's units: first, first + slices, ... < last
+  const int valid = (int)quant_rows(p, b), units = (valid + kUnitRows - 1) / kUnitRows;
+  const int first = (int)((int64_t)units * split / p.splits) + slice;
+  const int last = here ? (int)((int64_t)units * (split + 1) / p.splits) : 0;
 
-  const unsigned char *pool = p.pool + (int64_t)kh * D;
-  const int64_t E = (int64_t)p.kv_heads * D, v_plane = (int64_t)p.page_size * p.record;
-  const int64_t scales = E - (int64_t)kh * D + (kh & ~3);  // of the scales' word, from `pool`
+  // A lane has the row number of one row of a unit, read one unit before its copies.
   const int64_t *rows = p.rows + b * p.rows_batch_stride;
-  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * Shape::ring;
-  const int c16 = lane % kChunks * 16;
-  // a lane has the row number of one row of a tile, read one tile before its copies
-  const auto look = [&](int tile) -> int64_t {
-    const int at = tile * kMmaRows + (lane & 15);
-    return tile < last && at < valid ? __ldg(rows + at) : -1;
+  const auto look = [&](int unit) -> int64_t {
+    const int at = unit * kUnitRows + lane;
+    return unit < last && at < valid ? __ldg(rows + at) : -1;
   };
-  int64_t next = look(first);
-  int issue = first, to = 0;  // the next tile to copy and its stage
-  const auto copy_tile = [&] {
-    if (issue < last) {
-      const int64_t index =
-          record_index(next, p.page_size, p.page_shift, p.pool_blocks, p.status);
-      const int64_t offset = index < 0 ? -1 : index * p.record;
-      next = look(issue + slices);
-      const uint32_t stage = ring + to * Shape::stage;
-      constexpr int together = 32 / kChunks;
-#pragma unroll
-      for (int i = 0; i < kMmaRows / together; ++i) {
-        const int r = i * together + lane / kChunks;
-        const int64_t from = __shfl_sync(kFullMask, offset, r);
-        const int bytes = from >= 0 && c16 < D ? 16 : 0;
-        const unsigned char *src = bytes ? pool + from + c16 : p.pool;
-        const uint32_t dst = stage + r * Shape::pitch + c16;
-        copy16(dst, src, bytes);
-        copy16(dst + Shape::plane, bytes ? src + v_plane : p.pool, bytes);
-      }
-      // lanes 0-15 the words with the K scales, 16-31 those of V
-      const unsigned char *src = pool + offset + scales + (lane < 16 ? 0 : v_plane);
-      copy4(stage + 2 * Shape::plane + lane * 4, offset >= 0 ? src : p.pool, offset >= 0 ? 4 : 0);
-      issue += slices;
-      if (++to == kStages) to = 0;
+  // The index of its K record; the launch has checked that all of them fit 32 bits.
+  const int64_t pool_rows = p.pool_blocks * p.page_size;
+  const auto record_of = [&](int64_t row) -> uint32_t {
+    if (row < 0) return kNone;
+    if (row >= pool_rows) {
+      flag(p.status, HS_DEV_ROW_OUT_OF_RANGE);
+      return kNone;
     }
+    const uint32_t r = (uint32_t)row, P = (uint32_t)p.page_size;
+    return r + (p.page_shift >= 0 ? r & ~(P - 1) : r / P * P);  // block * 2 P + within
+  };
+  const uint32_t record = (uint32_t)p.record, ring = smem_addr(smem) + warp * Shape::ring;
+  const int c16 = lane % kChunks * 16;
+  const int copied = c16 < D ? 16 : 0;  // chunks past head_dim are zeros
+  const int64_t v_plane = (int64_t)p.page_size * p.record;
+  const unsigned char *chunk_of = p.pool + (copied ? (int64_t)kh * D + c16 : 0);
+  // lanes 0-15 copy the words with a tile's K scales, 16-31 those of V
+  const unsigned char *scale_word =
+      p.pool + (int64_t)p.kv_heads * D + (kh & ~3) + (lane < 16 ? 0 : v_plane);
+  const uint32_t to_chunk = ring + lane / kChunks * Shape::pitch + c16;
+  const uint32_t to_scale = ring + 2 * Shape::plane + lane * 4;
+  const auto copy_tile = [&](uint32_t index, int half, int stage) {
+    constexpr int together = 32 / kChunks;  // rows of a step
+#pragma unroll
+    for (int i = 0; i < kMmaRows / together; ++i) {
+      const uint32_t at =
+          __shfl_sync(kFullMask, index, half * kMmaRows + i * together + lane / kChunks);
+      const int bytes = at != kNone ? copied : 0;
+      const unsigned char *src = chunk_of + (uint64_t)(at != kNone ? at : 0u) * record;
+      const uint32_t dst = to_chunk + stage * Shape::stage + i * (together * Shape::pitch);
+      copy16(dst, src, bytes);
+      copy16(dst + Shape::plane, src + v_plane, bytes);
+    }
+    const uint32_t at = __shfl_sync(kFullMask, index, half * kMmaRows + (lane & 15));
+    copy4(to_scale + stage * Shape::stage, scale_word + (uint64_t)(at != kNone ? at : 0u) * record,
+          at != kNone ? 4 : 0);
+  };
+  uint32_t index = kNone;   // of the unit whose tiles are copied next
+  int64_t next = look(first);
+  int to = 0;               // stage of the next copy
+  const auto copy_half = [&](int unit, int half) {
+    if (unit < last) {
+      if (half == 0) {
+        index = record_of(next);
+        next = look(unit + slices);
+      }
+      copy_tile(index, half, to);
+    }
+    to = to == kStages - 1 ? 0 : to + 1;
     asm volatile("cp.async.commit_group;\n" ::: "memory");
   };
-#pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) copy_tile();
+  copy_half(first, 0);
+  copy_half(first, 1);
 
-  // Q: query head lane / 4, of every 16 elements those at 4 * (lane % 4) on
-  uint32_t q[kTiles][kChunks][2];
-  float factor[kTiles][2];  // of the scores of the query heads 2 * (lane % 4) + 0, 1
+  // Q: column lane / 4 of a tile is query head lane / 8 of a quad, part lane / 4 % 2; of
+  // every 16 elements this lane has those at 4 * (lane % 4) on
+  uint32_t q[kQuads][kQueryTiles][kChunks];
+  float factor[kQuads];  // of the scores of query head lane % 4
 #pragma unroll
-  for (int n = 0; n < kTiles; ++n) {
-    const int g = n * 8 + lane / 4;
+  for (int n = 0; n < kQuads; ++n) {
+    const int g = n * 4 + lane / 8;
     const T *from = static_cast<const T *>(p.query) + (int64_t)b * p.q_batch_stride +
                     (int64_t)(h0 + g) * D + lane % 4 * 4;
     float largest = 0.f;
-    uint2 raw[kChunks];
+    float4 x[kChunks];
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
-      raw[c] = make_uint2(0, 0);
-      if (g < hn && c * 16 < D) raw[c] = __ldg(reinterpret_cast<const uint2 *>(from + c * 16));
-      const T *x = reinterpret_cast<const T *>(&raw[c]);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) largest = fmaxf(largest, fabsf(to_f32(x[i])));
+      x[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (g < hn && c * 16 < D) x[c] = load4(from + c * 16);
+      largest = fmaxf(fmaxf(largest, fmaxf(fabsf(x[c].x), fabsf(x[c].y))),
+                      fmaxf(fabsf(x[c].z), fabsf(x[c].w)));
     }
     largest = fmaxf(largest, __shfl_xor_sync(kFullMask, largest, 1));
     largest = fmaxf(largest, __shfl_xor_sync(kFullMask, largest, 2));
-    // to below 2^14: what is 2^27 times smaller is still a normal number of fp16
-    const int e = largest > 0.f ? (__float_as_int(largest) >> 23) - 127 - 13 : 0;
-    const float scale = power_of_two(max(-126, min(127, -e)));
+    // to between 128 and 256: what is 2^13 times smaller is still a normal e4m3 number. An
+    // infinity leaves NaN, as its scores are
+    const int e = (__float_as_int(largest) >> 23) - 127 - 7;
+    const float scale = largest > 0.f ? power_of_two(max(-126, min(127, -e))) : 1.f;
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
-      const T *x = reinterpret_cast<const T *>(&raw[c]);
-      q[n][c][0] = pack_half(to_f32(x[0]) * scale, to_f32(x[1]) * scale);
-      q[n][c][1] = pack_half(to_f32(x[2]) * scale, to_f32(x[3]) * scale);
+      uint32_t codes[kQueryTiles];
+      const float4 y = make_float4(x[c].x * scale, x[c].y * scale, x[c].z * scale,
+                                   x[c].w * scale);
+      for (int t = 0; t < kQueryTiles; ++t) codes[t] = 0;
+      split_query<T, kQueryTiles>(y, lane & 4, codes);
+      const bool finite = largest < INFINITY;
+#pragma unroll
+      for (int t = 0; t < kQueryTiles; ++t) q[n][t][c] = finite ? codes[t] : 0x7f7f7f7fu;
     }
-    const float back = p.scale_log2 / scale;
-    factor[n][0] = __shfl_sync(kFullMask, back, lane % 4 * 8);
-    factor[n][1] = __shfl_sync(kFullMask, back, lane % 4 * 8 + 4);
+    factor[n] = __shfl_sync(kFullMask, p.scale_log2 / scale, lane % 4 * 8);
   }
 
-  float m[kTiles][2], l[kTiles][2], o[kTiles][kChunks][4];
+  // base: lift less the maximum, added to a score before its power is taken
+  float base[kQuads], l[kQuads], o[kOutputTiles][kChunks][4];
 #pragma unroll
-  for (int n = 0; n < kTiles; ++n) {
+  for (int n = 0; n < kQuads; ++n) {
+    base[n] = kNothing;
+    l[n] = 0.f;
+  }
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      m[n][j] = -INFINITY;
-      l[n][j] = 0.f;
-    }
+  for (int n = 0; n < kOutputTiles; ++n)
 #pragma unroll
     for (int c = 0; c < kChunks; ++c)
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[n][c][i] = 0.f;
-  }
   // ldmatrix: matrix lane / 8 has rows (lane / 8 % 2) * 8 on, chunk lane / 16
-  const uint32_t matrix = (lane & 15) * Shape::pitch + lane / 16 * 16;
-  int slot = 0;
-  for (int tile = first; tile < last; tile += slices) {
-    asm volatile("cp.async.wait_group %0;\n" ::"n"(kStages - 2) : "memory");
-    __syncwarp();
-    copy_tile();
-    const uint32_t stage = ring + slot * Shape::stage;
-    const unsigned char *bytes = smem + warp * Shape::ring + slot * Shape::stage +
-                                 2 * Shape::plane + (kh & 3) + lane / 4 * 4;
-    if (++slot == kStages) slot = 0;
-    // ---- S^T: rows lane / 4 and lane / 4 + 8, query heads 2 * (lane % 4) + 0, 1
-    float s[kTiles][2][4];
+  const uint32_t matrix = ring + (lane & 15) * Shape::pitch + lane / 16 * 16;
+  const unsigned char *scale_byte =
+      smem + warp * Shape::ring + 2 * Shape::plane + (kh & 3) + lane / 4 * 4;
+  int stage = 0;
+  for (int unit = first; unit < last; unit += slices) {
 #pragma unroll
-    for (int n = 0; n < kTiles; ++n)
+    for (int half = 0; half < 2; ++half) {
+      asm volatile("cp.async.wait_group %0;\n" ::"n"(kStages - 2) : "memory");
+      __syncwarp();
+      copy_half(unit + slices, half);
+      const uint32_t tile = matrix + stage * Shape::stage;
+      const unsigned char *bytes = scale_byte + stage * Shape::stage;
+      stage = stage == kStages - 1 ? 0 : stage + 1;
+      if (unit * kUnitRows + half * kMmaRows >= valid) continue;  // the last unit's second half
+      // ---- S^T: rows lane / 4 and lane / 4 + 8, query head lane % 4 of each quad
+      float s[kQuads][kQueryTiles][4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[n][0][i] = s[n][1][i] = 0.f;
+      for (int n = 0; n < kQuads; ++n)
 #pragma unroll
-    for (int c = 0; c < kChunks; c += 2) {
-      uint32_t k[4];
-      ldmatrix4(k, stage + matrix + c * 16);
+        for (int t = 0; t < kQueryTiles; ++t)
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const uint2 lo = decode4(k[2 * u]), hi = decode4(k[2 * u + 1]);
+          for (int i = 0; i < 4; ++i) s[n][t][i] = 0.f;
 #pragma unroll
-        for (int n = 0; n < kTiles; ++n)
-          mma_f16(s[n][u], lo.x, hi.x, lo.y, hi.y, q[n][c + u][0], q[n][c + u][1]);
+      for (int c = 0; c < kChunks; c += 2) {
+        uint32_t k[4];
+        ldmatrix4(k, tile + c * 16);
+#pragma unroll
+        for (int n = 0; n < kQuads; ++n)
+#pragma unroll
+          for (int t = 0; t < kQueryTiles; ++t)
+            mma_e4m3(s[n][t], k, q[n][t][c], q[n][t][c + 1]);
       }
-    }
-    // a row that is not seen has zeros in the place of its scale, which is never 0
-    const unsigned ek[2] = {bytes[0], bytes[32]}, ev[2] = {bytes[64], bytes[96]};
-    const float k_scale[2] = {scale_of(ek[0]), scale_of(ek[1])};
-    const float v_exponent[2] = {(float)((int)ev[0] - 127), (float)((int)ev[1] - 127)};
-    float t[kTiles][4];  // s + exponent
-    bool raise = false;
-#pragma unroll
-    for (int n = 0; n < kTiles; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = i >> 1, j = i & 1;
-        const float x = (s[n][0][i] + s[n][1][i]) * (k_scale[r] * factor[n][j]);
-        s[n][0][i] = ek[r] != 0 ? x : -INFINITY;
-        t[n][i] = s[n][0][i] + v_exponent[r];
-        raise = raise || t[n][i] > m[n][j] + kRaise;
-      }
-    if (__any_sync(kFullMask, raise)) {
-#pragma unroll
-      for (int n = 0; n < kTiles; ++n)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          float top = fmaxf(t[n][j], t[n][2 + j]);
-#pragma unroll
-          for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, x));
-          top = fmaxf(top, m[n][j]);
-          const float f = m[n][j] == -INFINITY ? 0.f : quant_exp2(m[n][j] - top);
-          m[n][j] = top;
-          l[n][j] *= f;
-#pragma unroll
-          for (int c = 0; c < kChunks; ++c) {
-            o[n][c][j] *= f;
-            o[n][c][2 + j] *= f;
-          }
-        }
-    }
-    uint32_t w[kTiles][kParts][2];
-#pragma unroll
-    for (int n = 0; n < kTiles; ++n) {
-      // nothing seen so far: exp2(-inf) = 0
-      const float base[2] = {m[n][0] == -INFINITY ? 0.f : kWeightLift - m[n][0],
-                             m[n][1] == -INFINITY ? 0.f : kWeightLift - m[n][1]};
+      // a row that is not seen has zeros in the place of its scale, which is never 0
+      const unsigned ek[2] = {bytes[0], bytes[32]}, ev[2] = {bytes[64], bytes[96]};
+      float k_scale[2], hidden[2], v_exponent[2];
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const float2 x = make_float2(quant_exp2(t[n][2 * r] + base[0]),
-                                     quant_exp2(t[n][2 * r + 1] + base[1]));
-        const uint32_t rounded = pack_half(x.x, x.y);
-        w[n][0][r] = transpose8(rounded);
-        if constexpr (kParts == 2) {
-          const float2 y = __half22float2(*reinterpret_cast<const __half2 *>(&rounded));
-          w[n][1][r] = transpose8(pack_half(x.x - y.x, x.y - y.y));
+        k_scale[r] = scale_of(ek[r]);
+        hidden[r] = ek[r] != 0 ? 0.f : -INFINITY;
+        // byte - 127 as a float: the byte under 2^23's exponent
+        v_exponent[r] = __uint_as_float(0x4b000000u | ev[r]) - (8388608.f + 127.f);
+      }
+      float x[kQuads][2], y[kQuads][2];  // exponents of the weights in the sum and in the output
+      bool raise = false;
+#pragma unroll
+      for (int n = 0; n < kQuads; ++n)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          float dot = 0.f;
+#pragma unroll
+          for (int t = kQueryTiles - 1; t >= 0; --t)
+            dot = fmaf(dot, 1.f / 256.f, fmaf(s[n][t][2 * r + 1], 1.f / 16.f, s[n][t][2 * r]));
+          x[n][r] = fmaf(dot, k_scale[r] * factor[n], hidden[r]);
+          y[n][r] = x[n][r] + v_exponent[r];
+          raise = raise || y[n][r] + base[n] > kRaise;
+        }
+      if (__any_sync(kFullMask, raise)) {
+        float f[kQuads];
+#pragma unroll
+        for (int n = 0; n < kQuads; ++n) {
+          float top = fmaxf(y[n][0], y[n][1]);
+#pragma unroll
+          for (int i = 4; i < 32; i <<= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, i));
+          // (a base of kNothing makes f 0)
+          const float to_base = fminf(base[n], kWeightLift - top);
+          f[n] = quant_exp2(to_base - base[n]);
+          base[n] = to_base;
+          l[n] *= f[n];
         }
 #pragma unroll
-        for (int j = 0; j < 2; ++j) l[n][j] += quant_exp2(s[n][0][2 * r + j] + (base[j] + kSumLift));
+        for (int n = 0; n < kOutputTiles; ++n)
+#pragma unroll
+          for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[n][c][i] *= kPaired ? f[2 * n + (i & 1)] : f[n];
+      }
+#pragma unroll
+      for (int n = 0; n < kQuads; ++n)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          l[n] += quant_exp2(x[n][r] + base[n]);
+          y[n][r] = quant_exp2(y[n][r] + base[n]);
+        }
+      uint32_t w[kOutputTiles][2];
+#pragma unroll
+      for (int n = 0; n < kOutputTiles; ++n)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          if constexpr (kPaired) {
+            w[n][r] = transpose8(pack_half(y[2 * n][r], y[2 * n + 1][r]));
+          } else {
+            const __half rounded = __float2half_rn(y[n][r]);
+            w[n][r] = transpose8(pack_half(y[n][r], y[n][r] - __half2float(rounded)));
+          }
+        }
+      // ---- O^T: elements 16 c + 2 * (lane / 4) + 0, 1, columns 2 * (lane % 4) + 0, 1
+#pragma unroll
+      for (int c = 0; c < kChunks; c += 2) {
+        uint32_t v[4];
+        ldmatrix4_trans(v, tile + Shape::plane + c * 16);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const uint2 lo = decode4(__byte_perm(v[2 * u], 0, 0x3120));
+          const uint2 hi = decode4(__byte_perm(v[2 * u + 1], 0, 0x3120));
+#pragma unroll
+          for (int n = 0; n < kOutputTiles; ++n)
+            mma_f16(o[n][c + u], lo.x, lo.y, hi.x, hi.y, w[n][0], w[n][1]);
+        }
       }
     }
-    // ---- O^T: elements 16 c + 2 * (lane / 4) + 0, 1, query heads 2 * (lane % 4) + 0, 1
-#pragma unroll
-    for (int c = 0; c < kChunks; c += 2) {
-      uint32_t v[4];
-      ldmatrix4_trans(v, stage + Shape::plane + matrix + c * 16);
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const uint2 lo = decode4(__byte_perm(v[2 * u], 0, 0x3120));
-        const uint2 hi = decode4(__byte_perm(v[2 * u + 1], 0, 0x3120));
-#pragma unroll
-        for (int n = 0; n < kTiles; ++n)
-#pragma unroll
-          for (int part = 0; part < kParts; ++part)
-            mma_f16(o[n][c + u], lo.x, lo.y, hi.x, hi.y, w[n][part][0], w[n][part][1]);
-      }
-    }
-    __syncwarp();
   }
   asm volatile("cp.async.wait_all;\n" ::: "memory");
 
-  // ---- results --------------------------------------------------------------------------
+  // ---- results: out = o / l, in the join's terms o 2^-kSumLift / l 2^kSumLift ------------
   const auto write = [&](int g, int d, float top, float sum, float2 x) {
     const int h = h0 + g;
     if (p.out != nullptr) {
@@ -309,50 +387,46 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<kDim, kTiles>::resident)
       *reinterpret_cast<float2 *>(p.partials + part * quant_pad(D) + d) = x;
     }
   };
+  // elements 16 c + 2 * (lane / 4) + 0, 1 of query head lane % 4 of quad n
+  const auto result = [&](int n, int c) {
+    const float(&x)[4] = o[kPaired ? n / 2 : n][c];
+    const float2 sum = kPaired ? make_float2(x[n & 1], x[2 + (n & 1)])
+                               : make_float2(x[0] + x[1], x[2] + x[3]);
+    return make_float2(sum.x * (1.f / kSumScale), sum.y * (1.f / kSumScale));
+  };
 #pragma unroll
-  for (int n = 0; n < kTiles; ++n)
+  for (int n = 0; n < kQuads; ++n)
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-#pragma unroll
-      for (int x = 4; x < 32; x <<= 1) l[n][j] += __shfl_xor_sync(kFullMask, l[n][j], x);
-      m[n][j] -= kWeightLift;
-    }
+    for (int i = 4; i < 32; i <<= 1) l[n] += __shfl_xor_sync(kFullMask, l[n], i);
   if (slices == 1) {
 #pragma unroll
-    for (int n = 0; n < kTiles; ++n)
+    for (int n = 0; n < kQuads; ++n)
 #pragma unroll
-      for (int c = 0; c < kChunks; ++c)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int g = n * 8 + lane % 4 * 2 + j, d = c * 16 + lane / 4 * 2;
-          if (g < hn && d < D)
-            write(g, d, m[n][j], l[n][j], make_float2(o[n][c][j], o[n][c][2 + j]));
-        }
+      for (int c = 0; c < kChunks; ++c) {
+        const int g = n * 4 + lane % 4, d = c * 16 + lane / 4 * 2;
+        if (g < hn && d < D) write(g, d, -base[n], l[n], result(n, c));
+      }
     return;
   }
   // the slices' results meet in shared memory: a query's maximum and sum, then its elements
   __syncthreads();
   float *mine = reinterpret_cast<float *>(smem + (size_t)warp * Shape::result);
 #pragma unroll
-  for (int n = 0; n < kTiles; ++n)
+  for (int n = 0; n < kQuads; ++n) {
+    float *to_query = mine + (n * 4 + lane % 4) * (kDim + 4);
+    if (lane < 4) *reinterpret_cast<float2 *>(to_query) = make_float2(-base[n], l[n]);
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      float *to_query = mine + (n * 8 + lane % 4 * 2 + j) * (kDim + 4);
-      if (lane < 4) *reinterpret_cast<float2 *>(to_query) = make_float2(m[n][j], l[n][j]);
-#pragma unroll
-      for (int c = 0; c < kChunks; ++c)
-        *reinterpret_cast<float2 *>(to_query + 4 + c * 16 + lane / 4 * 2) =
-            make_float2(o[n][c][j], o[n][c][2 + j]);
-    }
+    for (int c = 0; c < kChunks; ++c)
+      *reinterpret_cast<float2 *>(to_query + 4 + c * 16 + lane / 4 * 2) = result(n, c);
+  }
   __syncthreads();
-  if (hn == 0) return;
   // warp (place, slice) takes every slices-th query of its head
   for (int g = slice; g < hn; g += slices) {
     const auto of = [&](int s) {
       return reinterpret_cast<const float *>(smem + (size_t)(s * head_places + place) *
                                                         Shape::result) + g * (kDim + 4);
     };
-    float top = -INFINITY, sum = 0.f;
+    float top = -kNothing, sum = 0.f;
     for (int s = 0; s < slices; ++s) top = fmaxf(top, of(s)[0]);
     for (int s = 0; s < slices; ++s)
       if (of(s)[1] != 0.f) sum = fmaf(of(s)[1], quant_exp2(of(s)[0] - top), sum);
@@ -370,22 +444,31 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<kDim, kTiles>::resident)
   }
 }
 
-template <typename T, int kDim, int kTiles>
+template <typename T, int kDim, int kQuads>
 int launch(const QuantAttendParams &p, cudaStream_t s) {
-  auto kernel = quant_mma_kernel<T, kDim, kTiles>;
-  const size_t bytes = MmaShape<kDim, kTiles>::bytes;
+  auto kernel = quant_mma_kernel<T, kDim, kQuads>;
+  const size_t bytes = MmaShape<T, kDim, kQuads>::bytes;
   if (int e = reserve_smem(reinterpret_cast<const void *>(kernel), bytes, "attend_quantized"))
     return e;
   const QuantMmaGrid g = quant_mma_grid(p.q_heads, p.kv_heads, p.head_dim);
-  const dim3 grid((unsigned)p.splits, (unsigned)(g.groups * g.chunks), (unsigned)p.batch);
+  const int chunks = (p.groups + 4 * kQuads - 1) / (4 * kQuads);
+  const dim3 grid((unsigned)p.splits, (unsigned)(g.groups * chunks), (unsigned)p.batch);
   kernel<<<grid, kMmaThreads, bytes, s>>>(p, g.heads, g.places);
   return check_launch("quant_mma_kernel");
 }
-template <typename T> int launch(const QuantAttendParams &p, cudaStream_t s) {
-  const bool two = quant_mma_grid(p.q_heads, p.kv_heads, p.head_dim).queries == 16;
-  if (p.head_dim <= 64) return two ? launch<T, 64, 2>(p, s) : launch<T, 64, 1>(p, s);
-  if (p.head_dim <= 128) return two ? launch<T, 128, 2>(p, s) : launch<T, 128, 1>(p, s);
-  return launch<T, 256, 1>(p, s);
+// Quads of a warp: as many as the query heads need and the registers hold.
+template <typename T, int kDim, int kMost>
+int launch_quads(const QuantAttendParams &p, cudaStream_t s) {
+  if constexpr (kMost >= 4)
+    if (p.groups > 8) return launch<T, kDim, 4>(p, s);
+  if constexpr (kMost >= 2)
+    if (p.groups > 4) return launch<T, kDim, 2>(p, s);
+  return launch<T, kDim, 1>(p, s);
+}
+template <typename T, int kWide> int launch(const QuantAttendParams &p, cudaStream_t s) {
+  if (p.head_dim <= 64) return launch_quads<T, 64, 4>(p, s);
+  if (p.head_dim <= 128) return launch_quads<T, 128, kWide>(p, s);
+  return launch_quads<T, 256, kWide / 2>(p, s);
 }
 
 }  // namespace
@@ -393,19 +476,23 @@ template <typename T> int launch(const QuantAttendParams &p, cudaStream_t s) {
 QuantMmaGrid quant_mma_grid(int q_heads, int kv_heads, int head_dim) {
   QuantMmaGrid g;
   const int per = q_heads / kv_heads;
-  g.queries = per > 8 && head_dim <= 128 ? 16 : 8;
-  g.chunks = (per + g.queries - 1) / g.queries;
+  const int queries = per <= 4 ? 4 : per <= 8 ? 8 : head_dim <= 128 ? 16 : 8;
+  g.chunks = (per + queries - 1) / queries;
   g.groups = (kv_heads + kMmaWarps - 1) / kMmaWarps;
   g.heads = (kv_heads + g.groups - 1) / g.groups;
   g.groups = (kv_heads + g.heads - 1) / g.heads;
   for (g.places = 1; g.places < g.heads; g.places <<= 1) {}
-  g.resident = head_dim <= 128 && g.queries == 8 ? 2 : 1;
+  g.resident = head_dim <= 128 && queries <= 8 ? 2 : 1;
   g.slices = kMmaWarps / g.places;
   return g;
 }
 
 int launch_quant_mma(const QuantAttendParams &p, int dtype, cudaStream_t s) {
-  return dtype == HS_FLOAT16 ? launch<__half>(p, s) : launch<__nv_bfloat16>(p, s);
+  switch (dtype) {
+    case HS_FLOAT32: return launch<float, 2>(p, s);
+    case HS_FLOAT16: return launch<__half, 2>(p, s);
+    default: return launch<__nv_bfloat16, 4>(p, s);
+  }
 }
 
 }  // namespace hs
