@@ -2,10 +2,14 @@
 // that share their rows.
 //
 // A warp serves one KV head and up to 4 * kQuads of its query heads over units of 32
-// rows, alone: it copies its own rows (cp.async, 16 bytes a lane, into a ring of its own)
-// and keeps its own maximum, sum and output, so that nothing in the loop waits for
-// another warp. The heads of a block read neighbouring parts of the same rows. Keys are
-// the M side of the products, 16 at a time:
+// rows: it copies its head's part of them (cp.async, 16 bytes a lane, into a ring of its
+// own, two tiles of 16 rows ahead) and keeps its own maximum, sum and output. The heads of a
+// block read neighbouring parts of the same rows and share one thing, the rows' scales: each
+// of the warps in turn copies those of a unit for all of them, since 32 rows' scales are
+// 32 requests of a few bytes for whoever reads them (a head's part of a row is one or
+// two), and the number of requests is what bounds the reads. The ring of scales is deep enough that the
+// warps hardly ever wait for one another. Keys are the M side of the products, 16 at a
+// time:
 //   S^T = K Q^T     m16n8k32 in e4m3: the codes go from ldmatrix to the tensor core as
 //                   they are. Q is taken apart into e4m3 numbers, each a sixteenth of the
 //                   one before it (q = q0 + q1 / 16 + ...): 2 parts hold bf16, 3 fp16 and
@@ -32,6 +36,11 @@ constexpr int kMmaWarps = 8, kMmaThreads = 32 * kMmaWarps;
 constexpr int kMmaRows = 16;     // rows of a tile, a stage of the ring
 constexpr int kUnitRows = 32;    // two tiles: a lane has the number of one of their rows
 constexpr int kStages = 3;       // the two tiles after the one that is worked on are on their way
+constexpr int kSlots = 8;        // units whose scales are kept
+constexpr int kAhead = 2;        // units that scales are copied ahead
+// A unit's scales of one plane: 4 bytes a row where all heads' are in one word, else the
+// one or two 16-byte chunks of a row that have the block's heads
+constexpr int kScaleRoom = 16 * 1024;  // of all rings of scales: 8 of words or 1 of two chunks
 constexpr float kWeightLift = 7.f, kRaise = 15.f;  // lifted weights stay below 2^kRaise
 constexpr float kNothing = 1e38f;                  // base of a query that has seen nothing
 
@@ -44,14 +53,15 @@ template <typename T, int kDim, int kQuads> struct MmaShape {
   static constexpr int query_tiles = (kQueryParts<T> + 1) / 2;  // of 8 columns, for each quad
   static constexpr bool paired = std::is_same<T, __nv_bfloat16>::value && kQuads > 1;
   static constexpr int output_tiles = paired ? kQuads / 2 : kQuads;
-  static constexpr int pitch = kDim + 16;  // of a row: an odd number of 16-byte chunks
-  static constexpr int plane = kMmaRows * pitch;
-  static constexpr int stage = 2 * plane + 2 * kMmaRows * 4;  // K, V, the words with their scales
+  static constexpr int plane = kMmaRows * kDim;
+  static constexpr int stage = 2 * plane;  // K, V
   static constexpr int queries = 4 * kQuads;
   static constexpr int ring = kStages * stage;
   // the warps' results at the end, in the place of the rings
   static constexpr int result = queries * (kDim + 4) * 4;
-  static constexpr size_t bytes = (size_t)kMmaWarps * (ring > result ? ring : result);
+  static constexpr int rings = kMmaWarps * (ring > result ? ring : result);
+  // the rings of scales, and their barriers: for each slice of the warps full and free
+  static constexpr size_t bytes = rings + kScaleRoom + kMmaWarps * 2 * kSlots * sizeof(uint64_t);
   // blocks on an SM: two where the output and the queries leave the registers for it
   static constexpr int resident =
       kDim / 4 * output_tiles + kDim / 16 * kQuads * query_tiles <= 64 && kDim <= 128 ? 2 : 1;
@@ -98,6 +108,22 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void *src, int bytes)
 }
 __device__ __forceinline__ void copy4(uint32_t dst, const void *src, int bytes) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(dst), "l"(src), "r"(bytes)
+               : "memory");
+}
+// Place of 16-byte chunk c of row r of a tile: rows of 128 bytes (64 where kDim is 64),
+// panel after panel, swizzled so that the eight rows of an ldmatrix are in different
+// banks. Chunk c + i of a row, c < 2 and i even, is at the place of c changed by
+// tile_chunk.
+template <int kDim> __device__ __forceinline__ uint32_t tile_place(int r, int c) {
+  if constexpr (kDim == 64) return r * 64 + ((c ^ (r >> 1 & 3)) << 4);
+  return (c >> 3) * (kMmaRows * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+}
+template <int kDim> __device__ __forceinline__ uint32_t tile_chunk(uint32_t place, int i) {
+  return (place ^ (i & 7) << 4) + (i >> 3) * (kMmaRows * 128);
+}
+// Arrives on `bar` once this thread's copies so far have landed.
+__device__ __forceinline__ void copies_arrive(uint64_t *bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];\n" ::"r"(smem_addr(bar))
                : "memory");
 }
 // This lane's part (of the two of a column pair: `odd`) in each tile of columns
@@ -165,16 +191,27 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<T, kDim, kQuads>::reside
     const uint32_t r = (uint32_t)row, P = (uint32_t)p.page_size;
     return r + (p.page_shift >= 0 ? r & ~(P - 1) : r / P * P);  // block * 2 P + within
   };
+  // scales: a ring for each slice of the warps
+  const int width = p.kv_heads <= 4 ? 4 : (group * heads_of_block & 15) + heads_of_block > 16 ? 32 : 16;
+  unsigned char *scales = smem + Shape::rings + slice * (kSlots * 2 * kUnitRows) * width;
+  uint64_t *full = reinterpret_cast<uint64_t *>(smem + Shape::rings + kScaleRoom) +
+                   slice * 2 * kSlots, *free = full + kSlots;
+  const int sharing = min(head_places, min(heads_of_block, p.kv_heads - group * heads_of_block));
+  if (place == 0 && lane == 0) {
+    for (int i = 0; i < kSlots; ++i) {
+      mbar_init(&full[i], 32);
+      mbar_init(&free[i], sharing);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  }
+  __syncthreads();
   const uint32_t record = (uint32_t)p.record, ring = smem_addr(smem) + warp * Shape::ring;
   const int c16 = lane % kChunks * 16;
   const int copied = c16 < D ? 16 : 0;  // chunks past head_dim are zeros
   const int64_t v_plane = (int64_t)p.page_size * p.record;
   const unsigned char *chunk_of = p.pool + (copied ? (int64_t)kh * D + c16 : 0);
-  // lanes 0-15 copy the words with a tile's K scales, 16-31 those of V
-  const unsigned char *scale_word =
-      p.pool + (int64_t)p.kv_heads * D + (kh & ~3) + (lane < 16 ? 0 : v_plane);
-  const uint32_t to_chunk = ring + lane / kChunks * Shape::pitch + c16;
-  const uint32_t to_scale = ring + 2 * Shape::plane + lane * 4;
+  const int scale0 = width == 4 ? 0 : group * heads_of_block & ~15;  // the first head's of a slot
+  const unsigned char *scale_of_row = p.pool + (int64_t)p.kv_heads * D + scale0;
   const auto copy_tile = [&](uint32_t index, int half, int stage) {
     constexpr int together = 32 / kChunks;  // rows of a step
 #pragma unroll
@@ -183,28 +220,53 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<T, kDim, kQuads>::reside
           __shfl_sync(kFullMask, index, half * kMmaRows + i * together + lane / kChunks);
       const int bytes = at != kNone ? copied : 0;
       const unsigned char *src = chunk_of + (uint64_t)(at != kNone ? at : 0u) * record;
-      const uint32_t dst = to_chunk + stage * Shape::stage + i * (together * Shape::pitch);
+      const uint32_t dst = ring + stage * Shape::stage +
+                           tile_place<kDim>(i * together + lane / kChunks, lane % kChunks);
       copy16(dst, src, bytes);
       copy16(dst + Shape::plane, src + v_plane, bytes);
     }
-    const uint32_t at = __shfl_sync(kFullMask, index, half * kMmaRows + (lane & 15));
-    copy4(to_scale + stage * Shape::stage, scale_word + (uint64_t)(at != kNone ? at : 0u) * record,
-          at != kNone ? 4 : 0);
+  };
+  // The scales of the i-th unit of this slice, a row a lane, into slot i % kSlots; i counts
+  // the units that the warps of the slice have in common.
+  bool ok = true;
+  const auto copy_scales = [&](int i, uint32_t at) {
+    if (i >= kSlots) {
+      ok = __all_sync(kFullMask, wait_phase(&free[i % kSlots], (i / kSlots - 1) & 1, p.status));
+      if (!ok) return;
+    }
+    const unsigned char *src = scale_of_row + (uint64_t)(at != kNone ? at : 0u) * record;
+    const uint32_t dst = smem_addr(scales) + ((i % kSlots) * 2 * kUnitRows + lane) * width;
+#pragma unroll
+    for (int plane = 0; plane < 2; ++plane) {
+      if (width == 4) {
+        copy4(dst + plane * kUnitRows * 4, src + plane * v_plane, at != kNone ? 4 : 0);
+      } else {
+        copy16(dst + plane * kUnitRows * width, src + plane * v_plane, at != kNone ? 16 : 0);
+        if (width == 32)
+          copy16(dst + plane * kUnitRows * width + 16, src + plane * v_plane + 16,
+                 at != kNone ? 16 : 0);
+      }
+    }
+    copies_arrive(&full[i % kSlots]);
   };
   uint32_t index = kNone;   // of the unit whose tiles are copied next
-  int64_t next = look(first);
+  int64_t next = look(first), later = look(first + slices);  // row numbers of the units after it
   int to = 0;               // stage of the next copy
   const auto copy_half = [&](int unit, int half) {
     if (unit < last) {
       if (half == 0) {
         index = record_of(next);
-        next = look(unit + slices);
+        next = later;
+        later = look(unit + 2 * slices);
       }
       copy_tile(index, half, to);
     }
     to = to == kStages - 1 ? 0 : to + 1;
     asm volatile("cp.async.commit_group;\n" ::: "memory");
   };
+  for (int i = 0; i < kAhead; ++i)
+    if (i % sharing == place && first + i * slices < last)
+      copy_scales(i, record_of(i == 0 ? next : later));
   copy_half(first, 0);
   copy_half(first, 1);
 
@@ -260,18 +322,25 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<T, kDim, kQuads>::reside
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[n][c][i] = 0.f;
   // ldmatrix: matrix lane / 8 has rows (lane / 8 % 2) * 8 on, chunk lane / 16
-  const uint32_t matrix = ring + (lane & 15) * Shape::pitch + lane / 16 * 16;
-  const unsigned char *scale_byte =
-      smem + warp * Shape::ring + 2 * Shape::plane + (kh & 3) + lane / 4 * 4;
-  int stage = 0;
-  for (int unit = first; unit < last; unit += slices) {
+  const uint32_t matrix = ring + tile_place<kDim>(lane & 15, lane / 16);
+  const unsigned char *scale_byte = scales + lane / 4 * width + (kh - scale0);
+  int stage = 0, count = 0;
+  for (int unit = first; unit < last && ok; unit += slices, ++count) {
+    // row numbers of unit + 2 * slices are in `next` until the copies below move on
+    if ((count + kAhead) % sharing == place && unit + kAhead * slices < last) {
+      copy_scales(count + kAhead, record_of(later));
+      if (!ok) break;
+    }
+    const int slot = count % kSlots;
+    ok = __all_sync(kFullMask, wait_phase(&full[slot], count / kSlots & 1, p.status));
+    if (!ok) break;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       asm volatile("cp.async.wait_group %0;\n" ::"n"(kStages - 2) : "memory");
       __syncwarp();
       copy_half(unit + slices, half);
       const uint32_t tile = matrix + stage * Shape::stage;
-      const unsigned char *bytes = scale_byte + stage * Shape::stage;
+      const unsigned char *bytes = scale_byte + (slot * 2 * kUnitRows + half * kMmaRows) * width;
       stage = stage == kStages - 1 ? 0 : stage + 1;
       if (unit * kUnitRows + half * kMmaRows >= valid) continue;  // the last unit's second half
       // ---- S^T: rows lane / 4 and lane / 4 + 8, query head lane % 4 of each quad
@@ -285,7 +354,7 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<T, kDim, kQuads>::reside
 #pragma unroll
       for (int c = 0; c < kChunks; c += 2) {
         uint32_t k[4];
-        ldmatrix4(k, tile + c * 16);
+        ldmatrix4(k, tile_chunk<kDim>(tile, c));
 #pragma unroll
         for (int n = 0; n < kQuads; ++n)
 #pragma unroll
@@ -293,7 +362,8 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<T, kDim, kQuads>::reside
             mma_e4m3(s[n][t], k, q[n][t][c], q[n][t][c + 1]);
       }
       // a row that is not seen has zeros in the place of its scale, which is never 0
-      const unsigned ek[2] = {bytes[0], bytes[32]}, ev[2] = {bytes[64], bytes[96]};
+      const unsigned ek[2] = {bytes[0], bytes[8 * width]};
+      const unsigned ev[2] = {bytes[kUnitRows * width], bytes[(kUnitRows + 8) * width]};
       float k_scale[2], hidden[2], v_exponent[2];
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
@@ -359,7 +429,7 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<T, kDim, kQuads>::reside
 #pragma unroll
       for (int c = 0; c < kChunks; c += 2) {
         uint32_t v[4];
-        ldmatrix4_trans(v, tile + Shape::plane + c * 16);
+        ldmatrix4_trans(v, tile_chunk<kDim>(tile + Shape::plane, c));
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const uint2 lo = decode4(__byte_perm(v[2 * u], 0, 0x3120));
@@ -370,6 +440,8 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<T, kDim, kQuads>::reside
         }
       }
     }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&free[slot]);
   }
   asm volatile("cp.async.wait_all;\n" ::: "memory");
 

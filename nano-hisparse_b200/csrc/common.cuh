@@ -291,4 +291,29 @@ __device__ __forceinline__ bool mbar_wait(uint64_t *bar, unsigned parity, int32_
   return false;
 }
 
+constexpr unsigned long long kWaitNanoseconds = 4000000000ull;  // then a wait gives up
+// As mbar_wait, without the hint to sleep: waits here are a few hundred clocks, and
+// waking from a hinted sleep was measured to take more than a thousand.
+__device__ __forceinline__ bool wait_phase(uint64_t *bar, unsigned parity, int32_t *status) {
+  unsigned long long first = 0;
+  for (unsigned i = 0;; ++i) {
+    unsigned done;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+        " selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(done)
+        : "r"(smem_addr(bar)), "r"(parity)
+        : "memory");
+    if (done) return true;
+    if ((i & 1023) == 1023) {
+      unsigned long long now;
+      asm volatile("mov.u64 %0, %%globaltimer;\n" : "=l"(now));
+      if (first == 0) first = now;
+      if (now - first > kWaitNanoseconds) break;
+    }
+  }
+  flag(status, HS_DEV_WAIT_TIMEOUT);
+  return false;
+}
+
 }  // namespace hs

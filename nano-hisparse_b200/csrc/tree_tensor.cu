@@ -53,7 +53,6 @@ constexpr int kTensorThreads = 32 * (kOutputWarp + 1);
 constexpr int kTile = 128;     // query rows
 constexpr int kKeys = 64;      // keys of a block
 constexpr int kLook = 6;       // blocks that row numbers are read ahead
-constexpr unsigned long long kWaitNanoseconds = 4000000000ull;  // then a wait gives up
 
 struct TensorShared {
   uint64_t k_full[kMaxStages], k_free[kMaxStages], v_full[kMaxStages], v_free[kMaxStages];
@@ -163,29 +162,6 @@ __device__ __forceinline__ float largest(uint32_t (&s)[32], bool plain, uint32_t
   return fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]);
 }
 
-// As mbar_wait, without the hint to sleep: waits here are a few hundred clocks, and
-// waking from a hinted sleep was measured to take more than a thousand.
-__device__ __forceinline__ bool wait_phase(uint64_t *bar, unsigned parity, int32_t *status) {
-  unsigned long long first = 0;
-  for (unsigned i = 0;; ++i) {
-    unsigned done;
-    asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
-        " selp.u32 %0, 1, 0, p;\n}\n"
-        : "=r"(done)
-        : "r"(smem_addr(bar)), "r"(parity)
-        : "memory");
-    if (done) return true;
-    if ((i & 1023) == 1023) {
-      unsigned long long now;
-      asm volatile("mov.u64 %0, %%globaltimer;\n" : "=l"(now));
-      if (first == 0) first = now;
-      if (now - first > kWaitNanoseconds) break;
-    }
-  }
-  flag(status, HS_DEV_WAIT_TIMEOUT);
-  return false;
-}
 __device__ __forceinline__ void mbar_arrive_many(uint64_t *bar, unsigned count) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;\n" ::"r"(smem_addr(bar)), "r"(count)
                : "memory");
