@@ -46,14 +46,17 @@ HS_API int64_t hs_quantized_row_bytes(int kv_heads, int head_dim);
 
 /* ---- (9) append ------------------------------------------------------------------
  * As hs_append_rows (hisparse.h), with k and v of dtype kv_dtype quantised on
- * their way into pool and host records, and with the metadata taken from the
+ * their way into pool and host records (host_block NULL: no host mirror), and with the metadata taken from the
  * values that are held: minimum_ptrs / maximum_ptrs point to bf16 bounds
  * (torch.minimum / torch.maximum semantics), summary_ptrs to the fp32 mean of the
  * page's rows so far; all three NULL: no metadata. A row of k or v is kv_heads * head_dim adjacent elements,
- * rows of a chunk follow one another, chunks are kv_batch_stride elements apart.
+ * rows of a chunk follow one another, chunks are kv_batch_stride elements apart
+ * and have `tokens` rows each; a count above that is refused like one that leaves
+ * its page.
  */
-HS_API int hs_append_quantized(int batch, const void *k, const void *v, int64_t kv_batch_stride,
-                               int kv_dtype, const int32_t *within, const int32_t *count,
+HS_API int hs_append_quantized(int batch, int64_t tokens, const void *k, const void *v,
+                               int64_t kv_batch_stride, int kv_dtype, const int32_t *within,
+                               const int32_t *count,
                                const int64_t *pool_block, void *pool, int64_t pool_blocks,
                                const int64_t *host_block, void *host_alias, int64_t host_blocks,
                                const uint64_t *minimum_ptrs, const uint64_t *maximum_ptrs,

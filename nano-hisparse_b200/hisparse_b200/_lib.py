@@ -82,7 +82,7 @@ _VERIFY_SIGNATURES = {
 # include/hisparse_quantized.h
 _QUANTIZED_SIGNATURES = {
     "hs_quantized_row_bytes": ([_INT, _INT], _I64),
-    "hs_append_quantized": ([_INT, _P, _P, _I64, _INT, _P, _P, _P, _P, _I64, _P, _P, _I64, _P, _P,
+    "hs_append_quantized": ([_INT, _I64, _P, _P, _I64, _INT, _P, _P, _P, _P, _I64, _P, _P, _I64, _P, _P,
                              _P, _INT, _INT, _INT, _P, _P], _INT),
     "hs_read_quantized": ([_P, _I64, _P, _I64, _P, _INT, _INT, _INT, _INT, _P, _P], _INT),
     "hs_attend_quantized_workspace_bytes": ([_INT, _INT, _INT, _INT, _INT, _I64], _SZ),

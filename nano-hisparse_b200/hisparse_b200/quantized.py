@@ -61,11 +61,10 @@ def append_quantized(k, v, within, count, pool_block, pool, minimum_ptrs, maximu
                              or not host.tensor.is_contiguous()):
         raise ValueError("host store and pool layouts differ")
     batch, tokens = shape[:2]
-    if host_block is None:
-        host_block = torch.full_like(pool_block, -1)
-    metadata = (minimum_ptrs, maximum_ptrs, summary_ptrs)
-    if any(t is None for t in metadata) and any(t is not None for t in metadata):
+    if (minimum_ptrs is None) != (maximum_ptrs is None) or \
+            (minimum_ptrs is None) != (summary_ptrs is None):
         raise ValueError("bounds and mean go together: all three addresses or none")
+    limits = []  # addresses
     for name, t, dt in (("within", within, torch.int32), ("count", count, torch.int32),
                         ("pool_block", pool_block, torch.int64),
                         ("host_block", host_block, torch.int64),
@@ -73,9 +72,11 @@ def append_quantized(k, v, within, count, pool_block, pool, minimum_ptrs, maximu
                         ("maximum_ptrs", maximum_ptrs, torch.int64),
                         ("summary_ptrs", summary_ptrs, torch.int64)):
         if t is None:
+            limits.append(None)
             continue
-        if t.dtype != dt or t.numel() != batch or not t.is_contiguous():
+        if t.dtype != dt or t.shape != (batch,) or not t.is_contiguous():
             raise ValueError(f"{name} must be a contiguous {dt} tensor of {batch} entries")
+        limits.append(t.data_ptr())
     # rows of a chunk adjacent (copied when they are not); any distance between chunks
     row = config.kv_heads * config.head_dim
     strides = k.stride()
@@ -85,11 +86,11 @@ def append_quantized(k, v, within, count, pool_block, pool, minimum_ptrs, maximu
         strides = (tokens * row,)
     with _lib.on_device(index):
         status = _lib.load().hs_append_quantized(
-            batch, k.data_ptr(), v.data_ptr(), strides[0], _lib.dtype_code(k.dtype),
-            within.data_ptr(), count.data_ptr(), pool_block.data_ptr(), pool.data_ptr(), blocks,
-            host_block.data_ptr(), None if host is None else host.data_ptr(),
-            0 if host is None else host.tensor.shape[0], *map(_lib.ptr, metadata),
-            config.kv_heads, config.head_dim, config.page_size, _lib.status_pointer(index),
+            batch, tokens, k.data_ptr(), v.data_ptr(), strides[0], _lib.dtype_code(k.dtype),
+            *limits[:3], pool.data_ptr(), blocks, limits[3],
+            None if host is None else host.data_ptr(),
+            0 if host is None else host.tensor.shape[0], *limits[4:], config.kv_heads,
+            config.head_dim, config.page_size, _lib.status_pointer(index),
             _lib.raw_stream(index))
     if status:
         _lib.check(status)

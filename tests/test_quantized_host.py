@@ -52,7 +52,7 @@ def test_host_side_validation_needs_no_device():
                                    _lib.HS_ERR_WORKSPACE)
 
     def append(batch=1, dtype=_lib.HS_BFLOAT16, heads=2, dim=32, page=16, k=16):
-        return lib.hs_append_quantized(batch, k, 16, 64, dtype, 16, 16, 16, 16, 4, 16, None, 0,
+        return lib.hs_append_quantized(batch, 1, k, 16, 64, dtype, 16, 16, 16, 16, 4, 16, None, 0,
                                        16, 16, 16, heads, dim, page, None, None)
 
     assert append(batch=0) == _lib.HS_OK
