@@ -1,6 +1,6 @@
 // (9) Append to an 8-bit cache, and (10) reading its rows back.
 //
-// append: one block serves a chunk's K or V of up to 16 KV heads. A head's row is spread
+// append: one block serves a chunk's K or V of up to 8 KV heads. A head's row is spread
 // over kLanes lanes, 8 elements a lane, so that a warp has 32 / kLanes rows of a head at
 // once and kBatch such groups of rows in flight: the reads are what bounds it, as long as
 // enough of them are on their way. The largest elements meet in shuffles, the exponent
@@ -15,8 +15,8 @@
 namespace hs {
 namespace {
 
-constexpr int kHeadGroup = 16;                  // heads of a block
-constexpr int kAppendWarps = 16;                // of a block at most
+constexpr int kHeadGroup = 8;                   // heads of a block
+constexpr int kAppendWarps = 8;                 // of a block at most
 constexpr int kTailRows = 64;                   // rows whose scales are kept in shared memory
 constexpr int kBatch = 4;                       // rows of a lane in flight
 
@@ -79,24 +79,27 @@ __device__ __forceinline__ uint2 load_codes(const unsigned char *from, int n) {
   }
   return codes;
 }
-__device__ __forceinline__ void decode8(uint2 codes, float scale, float (&x)[8]) {
+__device__ __forceinline__ void decode8(uint2 codes, float scale, float2 (&x)[4]) {
   const float4 lo = decode4_f32(codes.x), hi = decode4_f32(codes.y);
-  x[0] = lo.x * scale;
-  x[1] = lo.y * scale;
-  x[2] = lo.z * scale;
-  x[3] = lo.w * scale;
-  x[4] = hi.x * scale;
-  x[5] = hi.y * scale;
-  x[6] = hi.z * scale;
-  x[7] = hi.w * scale;
+  const float2 s = make_float2(scale, scale);
+  x[0] = pack_mul(make_float2(lo.x, lo.y), s);
+  x[1] = pack_mul(make_float2(lo.z, lo.w), s);
+  x[2] = pack_mul(make_float2(hi.x, hi.y), s);
+  x[3] = pack_mul(make_float2(hi.z, hi.w), s);
 }
+
+// A lane's part of the bounds and sums
+struct Columns {
+  __nv_bfloat162 low[4], high[4];
+  float2 sum[4];
+};
 
 // kWide: head_dim is a multiple of 8 and every address of its vector's size
 template <typename T, bool kWide, int kLanes>
-__global__ void __launch_bounds__(32 * kAppendWarps)
+__global__ void __launch_bounds__(32 * kAppendWarps, sizeof(T) == 2 ? 4 : 2)
     append_quantized_kernel(QuantAppendParams p, int slices) {
   __shared__ unsigned char scales[kTailRows][kHeadGroup];
-  __shared__ float columns[kAppendWarps][8 * kLanes];
+  __shared__ Columns columns[kAppendWarps][kLanes];
   constexpr int kTogether = 32 / kLanes;  // rows of a warp at once
   const int b = blockIdx.y, plane = blockIdx.x & 1, h0 = (blockIdx.x >> 1) * kHeadGroup;
   const int cnt = p.count[b], w = p.within[b];
@@ -128,25 +131,42 @@ __global__ void __launch_bounds__(32 * kAppendWarps)
   const T *from = static_cast<const T *>(plane ? p.v : p.k) + (int64_t)b * p.kv_batch_stride + at;
 
   Raw<T> raw[kBatch];
-  const auto load = [&](int i0) {
+  const int64_t from_step = (int64_t)step * E, to_step = (int64_t)step * p.record;
+  const T *load_at = from + (int64_t)first * E;  // of the next row to load
+  const auto load = [&](int r) {  // rows r, r + step, ..., below cnt
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      const int r = i0 + u * step + first;
-      raw[u].template load<kWide>(from + (int64_t)r * E, r < cnt ? n : 0);
-    }
+    for (int u = 0; u < kBatch; ++u, load_at += from_step)
+      raw[u].template load<kWide>(load_at, r + u * step < cnt ? n : 0);
   };
-  load(0);
+  load(first);
   // the bounds so far, by the lanes that will write them
   const bool writes = metadata && here && slice == 0 && lane < kLanes && n > 0;
   __nv_bfloat16 *minimum = reinterpret_cast<__nv_bfloat16 *>(entries[0]) + at;
   __nv_bfloat16 *maximum = reinterpret_cast<__nv_bfloat16 *>(entries[1]) + at;
-  float low[8], high[8], sum[8];
+  // two columns a word: a value held has 4 significant bits and is exact in bf16
+  alignas(16) __nv_bfloat162 low[4], high[4];
+  float2 sum[4];
+  const bool vectors = kWide && ((entries[0] | entries[1] | entries[2]) & 15) == 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    low[i] = writes && i < n ? __bfloat162float(minimum[i]) : INFINITY;
-    high[i] = writes && i < n ? __bfloat162float(maximum[i]) : -INFINITY;
-    sum[i] = 0.f;
+  for (int i = 0; i < 4; ++i) {
+    low[i] = __float2bfloat162_rn(INFINITY);
+    high[i] = __float2bfloat162_rn(-INFINITY);
   }
+  if (writes) {
+    if (vectors) {
+      *reinterpret_cast<uint4 *>(low) = *reinterpret_cast<const uint4 *>(minimum);
+      *reinterpret_cast<uint4 *>(high) = *reinterpret_cast<const uint4 *>(maximum);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < n) {
+          reinterpret_cast<__nv_bfloat16 *>(low)[i] = minimum[i];
+          reinterpret_cast<__nv_bfloat16 *>(high)[i] = maximum[i];
+        }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) sum[i] = make_float2(0.f, 0.f);
   if (metadata && here) {  // rows 0 .. w-1 of the page, for the mean
     const unsigned char *page = pool != nullptr ? pool : host;
     for (int r0 = first; r0 < w; r0 += kBatch * step) {
@@ -161,73 +181,81 @@ __global__ void __launch_bounds__(32 * kAppendWarps)
       }
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) {
-        float x[8];
+        float2 x[4];
         decode8(codes[u], scale_of(scale[u]), x);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum[i] += x[i];
+        for (int i = 0; i < 4; ++i) sum[i] = pack_add(sum[i], x[i]);
       }
     }
   }
   const int tail = (int)(p.record - E);  // bytes of a record behind its codes
   const bool last_group = h0 + heads == p.kv_heads;
   const int own = last_group ? tail - h0 : heads;  // those that this block writes
+  // where the next row goes
+  const int64_t place = (int64_t)(w + first) * p.record + at;
+  unsigned char *pool_at = pool != nullptr ? pool + place : nullptr;
+  unsigned char *host_at = host != nullptr ? host + place : nullptr;
   for (int r0 = 0; r0 < cnt; r0 += kTailRows) {
     const int rows = min(kTailRows, cnt - r0);
     for (int i0 = 0; i0 < rows; i0 += kBatch * step) {
-      if (r0 + i0 > 0) load(r0 + i0);
+      if (r0 + i0 > 0) load(r0 + i0 + first);
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u) {
+      for (int u = 0; u < kBatch; ++u, pool_at += to_step, host_at += to_step) {
+        if (i0 + u * step >= rows) continue;  // the same for the whole block
         const int r = i0 + u * step + first;
-        if (i0 + u * step >= rows) break;  // the same for the whole block
-        float x[8], largest = 0.f;
+        float2 x[4];
+        float largest = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = raw[u].at(i);
-#pragma unroll
-        for (int i = 0; i < 8; i += 2) largest = max3_nan(largest, fabsf(x[i]), fabsf(x[i + 1]));
+        for (int i = 0; i < 4; ++i) {
+          x[i] = make_float2(raw[u].at(2 * i), raw[u].at(2 * i + 1));
+          largest = max3_nan(largest, fabsf(x[i].x), fabsf(x[i].y));
+        }
 #pragma unroll
         for (int o = kLanes >> 1; o > 0; o >>= 1)
           largest = max_nan(largest, __shfl_xor_sync(kFullMask, largest, o));
         if (!__all_sync(kFullMask, largest < INFINITY)) {  // the largest of the finite ones
           largest = 0.f;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const bool finite = fabsf(x[i]) < INFINITY;
-            largest = fmaxf(largest, finite ? fabsf(x[i]) : 0.f);
-            x[i] = finite ? x[i] : __int_as_float(0x7fffffff);
+          for (int i = 0; i < 4; ++i) {
+            const float nan = __int_as_float(0x7fffffff);
+            if (!(fabsf(x[i].x) < INFINITY)) x[i].x = nan;
+            if (!(fabsf(x[i].y) < INFINITY)) x[i].y = nan;
+            largest = fmaxf(largest, fmaxf(fabsf(x[i].x), fabsf(x[i].y)));  // ignores NaN
           }
 #pragma unroll
           for (int o = kLanes >> 1; o > 0; o >>= 1)
             largest = fmaxf(largest, __shfl_xor_sync(kFullMask, largest, o));
         }
         const int e = exponent_of(largest);
-        const float inverse = power_of_two(-e);
-        const uint2 codes =
-            make_uint2(encode4(x[0] * inverse, x[1] * inverse, x[2] * inverse, x[3] * inverse),
-                       encode4(x[4] * inverse, x[5] * inverse, x[6] * inverse, x[7] * inverse));
+        const float2 inverse = make_float2(power_of_two(-e), power_of_two(-e));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = pack_mul(x[i], inverse);
+        const uint2 codes = make_uint2(encode4(x[0].x, x[0].y, x[1].x, x[1].y),
+                                       encode4(x[2].x, x[2].y, x[3].x, x[3].y));
         if (r >= rows || !here) continue;
-        const int64_t to = (int64_t)(w + r0 + r) * p.record + at;
-        if (pool != nullptr) store8<kWide>(pool + to, n, codes);
-        if (host != nullptr) store8<kWide>(host + to, n, codes);
+        if (pool != nullptr) store8<kWide>(pool_at, n, codes);
+        if (host != nullptr) store8<kWide>(host_at, n, codes);
         if (lane % kLanes == 0) scales[r][head] = (unsigned char)(e + 127);
         if (metadata) {
           decode8(codes, power_of_two(e), x);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            low[i] = min_nan(low[i], x[i]);
-            high[i] = max_nan(high[i], x[i]);
-            sum[i] += x[i];
+          for (int i = 0; i < 4; ++i) {
+            const __nv_bfloat162 y = __floats2bfloat162_rn(x[i].x, x[i].y);
+            low[i] = __hmin2_nan(low[i], y);
+            high[i] = __hmax2_nan(high[i], y);
+            sum[i] = pack_add(sum[i], x[i]);
           }
         }
       }
     }
     __syncthreads();
     // the scales and, by the last group, the padding
+    const int64_t row0 = (int64_t)(w + r0) * p.record + E + h0;
     for (int r = warp; r < rows; r += blockDim.x >> 5)
       for (int j = lane; j < own; j += 32) {
         const unsigned char byte = j < heads ? scales[r][j] : 0;
-        const int64_t to = (int64_t)(w + r0 + r) * p.record + E + h0 + j;
-        if (pool != nullptr) pool[to] = byte;
-        if (host != nullptr) host[to] = byte;
+        if (pool != nullptr) pool[row0 + r * p.record + j] = byte;
+        if (host != nullptr) host[row0 + r * p.record + j] = byte;
       }
     if (r0 + kTailRows < cnt) __syncthreads();
   }
@@ -236,37 +264,51 @@ __global__ void __launch_bounds__(32 * kAppendWarps)
 #pragma unroll
   for (int o = kLanes; o < 32; o <<= 1) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      low[i] = min_nan(low[i], __shfl_xor_sync(kFullMask, low[i], o));
-      high[i] = max_nan(high[i], __shfl_xor_sync(kFullMask, high[i], o));
-      sum[i] += __shfl_xor_sync(kFullMask, sum[i], o);
+    for (int i = 0; i < 4; ++i) {
+      low[i] = __hmin2_nan(low[i], __shfl_xor_sync(kFullMask, low[i], o));
+      high[i] = __hmax2_nan(high[i], __shfl_xor_sync(kFullMask, high[i], o));
+      sum[i].x += __shfl_xor_sync(kFullMask, sum[i].x, o);
+      sum[i].y += __shfl_xor_sync(kFullMask, sum[i].y, o);
     }
   }
-  const auto join = [&](float(&x)[8], auto op) {
-    if (slices == 1) return;
-    if (lane < kLanes)
+  if (slices > 1) {
+    Columns &mine = columns[warp][lane % kLanes];
+    if (slice > 0 && lane < kLanes)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) columns[warp][d0 + i] = x[i];
+      for (int i = 0; i < 4; ++i) {
+        mine.low[i] = low[i];
+        mine.high[i] = high[i];
+        mine.sum[i] = sum[i];
+      }
     __syncthreads();
     if (slice == 0)
-      for (int s = 1; s < slices; ++s)
+      for (int s = 1; s < slices; ++s) {
+        const Columns &other = columns[warp + s][lane % kLanes];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = op(x[i], columns[warp + s][d0 + i]);
-    __syncthreads();
-  };
-  join(low, [](float a, float c) { return min_nan(a, c); });
-  join(high, [](float a, float c) { return max_nan(a, c); });
-  join(sum, [](float a, float c) { return a + c; });
+        for (int i = 0; i < 4; ++i) {
+          low[i] = __hmin2_nan(low[i], other.low[i]);
+          high[i] = __hmax2_nan(high[i], other.high[i]);
+          sum[i] = pack_add(sum[i], other.sum[i]);
+        }
+      }
+  }
   if (!writes) return;
   float *summary = reinterpret_cast<float *>(entries[2]) + at;
-  const float rows = (float)(w + cnt);
+  const float share = 1.f / (float)(w + cnt);  // two roundings instead of a division's one
+  if (vectors) {
+    *reinterpret_cast<uint4 *>(minimum) = *reinterpret_cast<const uint4 *>(low);
+    *reinterpret_cast<uint4 *>(maximum) = *reinterpret_cast<const uint4 *>(high);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      reinterpret_cast<float2 *>(summary)[i] = make_float2(sum[i].x * share, sum[i].y * share);
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     if (i >= n) break;
-    // a value held has 4 significant bits: exact in bf16
-    minimum[i] = __float2bfloat16_rn(low[i]);
-    maximum[i] = __float2bfloat16_rn(high[i]);
-    summary[i] = sum[i] / rows;
+    minimum[i] = reinterpret_cast<const __nv_bfloat16 *>(low)[i];
+    maximum[i] = reinterpret_cast<const __nv_bfloat16 *>(high)[i];
+    summary[i] = (i % 2 ? sum[i / 2].y : sum[i / 2].x) * share;
   }
 }
 
@@ -352,16 +394,16 @@ __global__ void __launch_bounds__(kReadThreads) read_quantized_kernel(ReadParams
       for (int u = 0; u < kReadAhead; ++u) {
         const int i = i0 + u * kReadThreads;
         if (i >= all) break;
-        float x[8];
+        float2 x[4];
         decode8(codes[u], scale_of(scale[u]), x);
         T *to = out + ((int64_t)plane * p.count + row0) * E + (int64_t)i * kN;
         if constexpr (kN == 8) {
           Eight<T> y;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) y.x[j] = from_f32<T>(x[j]);
+          for (int j = 0; j < 8; ++j) y.x[j] = from_f32<T>(j % 2 ? x[j / 2].y : x[j / 2].x);
           *reinterpret_cast<Eight<T> *>(to) = y;
         } else {
-          *to = from_f32<T>(x[0]);
+          *to = from_f32<T>(x[0].x);
         }
       }
     }
