@@ -342,6 +342,12 @@ int launch_append(const QuantAppendParams &p, int64_t tokens, cudaStream_t s) {
 }
 
 // ---- (10) ---------------------------------------------------------------------------------
+// Reads and writes are what bounds it, and close behind them its instructions. A thread
+// takes as many codes at a time as make one vector of 16 bytes, so that neighbouring
+// threads write whole sectors (16 codes a thread, half a sector a store: 285 us where 8 take
+// 274, 262,144 rows of 8 heads of 128 in bf16; in fp32 half of them 293 and 4 codes 249).
+// Where the next codes are follows from the last ones by additions: the divisions of a
+// plain index took 339.
 constexpr int kReadThreads = 256;
 constexpr int kReadRows = 16;   // rows of a block
 constexpr int kReadAhead = 4;   // loads in flight
@@ -354,68 +360,107 @@ struct ReadParams {
   void *out;
   int kv_heads, head_dim, page_size, page_shift;
   int64_t record;
+  int units;                  // of kN codes, in a plane of a row
+  int step_rows, step_units;  // of kReadThreads units
+  uint32_t head_magic;  // unit * head_magic / 2^32 is its head; 0: the unit itself is
   int32_t *status;
 };
 
-template <typename T> struct alignas(8 * sizeof(T) < 16 ? 8 * sizeof(T) : 16) Eight { T x[8]; };
-
-// kN codes a thread and step: 8, or 1 where head_dim or an address does not allow it
 template <typename T, int kN>
-__global__ void __launch_bounds__(kReadThreads) read_quantized_kernel(ReadParams p) {
-  __shared__ int64_t records[kReadRows];  // index of the K record, or -1
-  const int64_t row0 = (int64_t)blockIdx.x * kReadRows;
-  const int rows = (int)min((int64_t)kReadRows, p.count - row0);
-  if (threadIdx.x < rows)
-    records[threadIdx.x] = record_index(p.rows[row0 + threadIdx.x], p.page_size, p.page_shift,
-                                        p.pool_blocks, p.status);
-  __syncthreads();
-  const int64_t E = (int64_t)p.kv_heads * p.head_dim;
-  const int units = (int)(E / kN), per_head = p.head_dim / kN;
-  T *out = static_cast<T *>(p.out);
-  for (int plane = 0; plane < 2; ++plane) {
-    const int all = rows * units;
-    for (int i0 = threadIdx.x; i0 < all; i0 += kReadThreads * kReadAhead) {
-      uint2 codes[kReadAhead];
-      unsigned scale[kReadAhead];
+__device__ __forceinline__ void write_values(T *to, const uint32_t (&codes)[(kN + 3) / 4],
+                                             float scale) {
+  if constexpr (kN == 1) {
+    *to = from_f32<T>(decode4_f32(codes[0]).x * scale);
+  } else {
+    const float2 s = make_float2(scale, scale);
+    alignas(16) T y[kN];
 #pragma unroll
-      for (int u = 0; u < kReadAhead; ++u) {
-        const int i = i0 + u * kReadThreads, r = i / units, c = i - r * units;
-        codes[u] = make_uint2(0, 0);
-        scale[u] = 127;
-        if (i < all && records[r] >= 0) {
-          const unsigned char *record =
-              p.pool + (records[r] + (int64_t)plane * p.page_size) * p.record;
-          if constexpr (kN == 8) codes[u] = __ldg(reinterpret_cast<const uint2 *>(record) + c);
-          else codes[u].x = record[c];
-          scale[u] = record[E + c / per_head];
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < kReadAhead; ++u) {
-        const int i = i0 + u * kReadThreads;
-        if (i >= all) break;
-        float2 x[4];
-        decode8(codes[u], scale_of(scale[u]), x);
-        T *to = out + ((int64_t)plane * p.count + row0) * E + (int64_t)i * kN;
-        if constexpr (kN == 8) {
-          Eight<T> y;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) y.x[j] = from_f32<T>(j % 2 ? x[j / 2].y : x[j / 2].x);
-          *reinterpret_cast<Eight<T> *>(to) = y;
-        } else {
-          *to = from_f32<T>(x[0].x);
-        }
-      }
+    for (int j = 0; j < kN; j += 4) {
+      const float4 x = decode4_f32(codes[j / 4]);
+      const float2 lo = pack_mul(make_float2(x.x, x.y), s);
+      const float2 hi = pack_mul(make_float2(x.z, x.w), s);
+      y[j] = from_f32<T>(lo.x);
+      y[j + 1] = from_f32<T>(lo.y);
+      y[j + 2] = from_f32<T>(hi.x);
+      y[j + 3] = from_f32<T>(hi.y);
     }
+    *reinterpret_cast<uint4 *>(to) = *reinterpret_cast<const uint4 *>(y);
   }
 }
 
-template <typename T> int launch_read(const ReadParams &p, cudaStream_t s) {
+template <typename T, int kN>
+__global__ void __launch_bounds__(kReadThreads) read_quantized_kernel(ReadParams p) {
+  constexpr int kWords = (kN + 3) / 4;
+  __shared__ const unsigned char *records[2 * kReadRows];  // K's, then V's; NULL: zeros
+  const int64_t row0 = (int64_t)blockIdx.x * kReadRows;
+  const int rows = (int)min((int64_t)kReadRows, p.count - row0);
+  if (threadIdx.x < rows) {
+    const int64_t index = record_index(p.rows[row0 + threadIdx.x], p.page_size, p.page_shift,
+                                       p.pool_blocks, p.status);
+    records[threadIdx.x] = index < 0 ? nullptr : p.pool + index * p.record;
+    records[rows + threadIdx.x] =
+        index < 0 ? nullptr : p.pool + (index + p.page_size) * p.record;
+  }
+  __syncthreads();
+  const int64_t E = (int64_t)p.kv_heads * p.head_dim;
+  // a plane's results follow one another like the units do
+  T *out = static_cast<T *>(p.out) + row0 * E + (int64_t)threadIdx.x * kN;
+  const int64_t plane = (p.count - rows) * E;  // from the block's K rows' end to its V rows
+  int r = threadIdx.x / p.units, c = threadIdx.x - r * p.units;
+  while (r < 2 * rows) {
+    uint32_t codes[kReadAhead][kWords];
+    unsigned scale[kReadAhead];
+    int rs[kReadAhead];
+#pragma unroll
+    for (int u = 0; u < kReadAhead; ++u) {
+      rs[u] = r;
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) codes[u][i] = 0;
+      scale[u] = 127;
+      const unsigned char *record = r < 2 * rows ? records[r] : nullptr;
+      if (record != nullptr) {
+        const unsigned char *from = record + (int64_t)c * kN;
+        if constexpr (kN == 8) {
+          const uint2 x = __ldg(reinterpret_cast<const uint2 *>(from));
+          codes[u][0] = x.x;
+          codes[u][1] = x.y;
+        } else if constexpr (kN == 4) {
+          codes[u][0] = __ldg(reinterpret_cast<const uint32_t *>(from));
+        } else {
+          codes[u][0] = __ldg(from);
+        }
+        const uint32_t head = p.head_magic ? __umulhi((uint32_t)c, p.head_magic) : (uint32_t)c;
+        scale[u] = __ldg(record + E + head);
+      }
+      r += p.step_rows;
+      c += p.step_units;
+      if (c >= p.units) {
+        c -= p.units;
+        ++r;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kReadAhead; ++u, out += kReadThreads * kN)
+      if (rs[u] < 2 * rows)
+        write_values<T, kN>(out + (rs[u] >= rows ? plane : 0), codes[u], scale_of(scale[u]));
+  }
+}
+
+template <typename T, int kN> int launch_read(ReadParams p, cudaStream_t s) {
+  p.units = (int)((int64_t)p.kv_heads * p.head_dim / kN);
+  p.step_rows = kReadThreads / p.units;
+  p.step_units = kReadThreads % p.units;
+  // exact while units * (units of a head) stays below 2^32
+  const uint32_t per_head = (uint32_t)(p.head_dim / kN);
+  p.head_magic = per_head == 1 ? 0 : (uint32_t)((0x100000000ull + per_head - 1) / per_head);
   const unsigned grid = (unsigned)ceil_div(p.count, kReadRows);
-  const bool wide = p.head_dim % 8 == 0 && reinterpret_cast<uintptr_t>(p.out) % 16 == 0;
-  if (wide) read_quantized_kernel<T, 8><<<grid, kReadThreads, 0, s>>>(p);
-  else read_quantized_kernel<T, 1><<<grid, kReadThreads, 0, s>>>(p);
+  read_quantized_kernel<T, kN><<<grid, kReadThreads, 0, s>>>(p);
   return check_launch("read_quantized_kernel");
+}
+template <typename T> int launch_read(const ReadParams &p, cudaStream_t s) {
+  const bool wide = reinterpret_cast<uintptr_t>(p.out) % 16 == 0;
+  constexpr int kN = 16 / sizeof(T);  // one vector of results
+  return wide && p.head_dim % kN == 0 ? launch_read<T, kN>(p, s) : launch_read<T, 1>(p, s);
 }
 
 }  // namespace
@@ -477,11 +522,20 @@ extern "C" int hs_read_quantized(const void *pool, int64_t pool_blocks, const in
     return set_error(HS_ERR_INVALID_ARGUMENT, "read_quantized: null pointer");
   if ((reinterpret_cast<uintptr_t>(pool) & 15) != 0)
     return set_error(HS_ERR_INVALID_ARGUMENT, "read_quantized: the pool must be 16-byte aligned");
-  if (count > (int64_t)0x7fffffff * kReadRows || (int64_t)kv_heads * head_dim > (1 << 26))
+  if (count > (int64_t)0x7fffffff * kReadRows || (int64_t)kv_heads * head_dim > (1 << 24))
     return set_error(HS_ERR_UNSUPPORTED, "read_quantized: rows or heads too many");
-  ReadParams p{static_cast<const unsigned char *>(pool), pool_blocks, rows, count, out, kv_heads,
-               head_dim, page_size, page_shift_of(page_size), record_bytes(kv_heads, head_dim),
-               device_status};
+  ReadParams p{};
+  p.pool = static_cast<const unsigned char *>(pool);
+  p.pool_blocks = pool_blocks;
+  p.rows = rows;
+  p.count = count;
+  p.out = out;
+  p.kv_heads = kv_heads;
+  p.head_dim = head_dim;
+  p.page_size = page_size;
+  p.page_shift = page_shift_of(page_size);
+  p.record = record_bytes(kv_heads, head_dim);
+  p.status = device_status;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (dtype) {
     case HS_FLOAT32: return launch_read<float>(p, s);
