@@ -213,26 +213,44 @@ __global__ void __launch_bounds__(kJoinThreads) quant_merge_kernel(QuantAttendPa
   out[((int64_t)b * p.q_heads + h) * D + tid] = from_f32<T>(y * inv);
 }
 
-// Splits of a request's rows: those with the least (rounds of blocks) x (tiles of 16 rows
-// of a warp, and what a block costs besides, as much as about eight). One number for
-// every type, so that the workspace depends on the sizes alone.
+// Splits of a request's rows, from what was measured of the tensor-core kernel: a warp takes
+// 1.45 us for a unit of 32 rows (2.5 above head_dim 128) while memory keeps up, the blocks
+// of an SM together 1.73 us for 67.6 KB of records; a block takes 3 us besides (half of it
+// beside another block's work), the join 2.5 and 0.02 for each split. More blocks than one an SM thus do not help large calls
+// (4 requests of 8,192 rows, 8 heads of 128: 37 splits 18.2 us, 74 splits 19.9), more rounds
+// of blocks do not hurt them (16 of 32,768: 18 splits 172, 37 splits 168), and small calls
+// want a unit a warp (1 of 2,048: 64 splits 9.5, 16 splits 12.5). One number for every
+// type, so that the workspace depends on the sizes alone. Times in ns.
 int quant_splits(int batch, int q_heads, int kv_heads, int head_dim, int64_t count) {
   const QuantMmaGrid g = quant_mma_grid(q_heads, kv_heads, head_dim);
-  const int64_t blocks = (int64_t)batch * g.groups * g.chunks;
-  const int64_t places = (int64_t)g.resident * sm_count(), tiles = ceil_div(count, 16);
-  int64_t least = 0;
-  int splits = 1;
-  for (int n = 1; n <= kQuantMaxSplits && (n == 1 || n * g.slices <= tiles); ++n) {
-    const int64_t cost = ceil_div(blocks * n, places) *
-                             (ceil_div(ceil_div(tiles, n), g.slices) + 8) +
-                         (n > 1 ? 4 : 0);
-    if (n == 1 || cost < least) {
-      least = cost;
-      splits = n;
+  const int64_t blocks = (int64_t)batch * g.groups * g.chunks, sms = sm_count();
+  const int64_t units = ceil_div(count, 32);
+  int64_t most = units / g.slices;  // a unit for each warp
+  if (most > kQuantMaxSplits) most = kQuantMaxSplits;
+  const int64_t compute = head_dim > 128 ? 2500 : 1450;
+  const int64_t share = (int64_t)64 * g.heads * (head_dim + 1) * 1730 / 67584;
+  int64_t best = 1, least = 0;
+  const auto consider = [&](int64_t n) {
+    if (n > most) n = most;
+    if (n < 1) n = 1;
+    const int64_t per = ceil_div(ceil_div(units, n), g.slices);
+    if (per > 0) n = ceil_div(units, per * g.slices);  // the fewest with as many units a warp
+    const int64_t all = blocks * n, beside = all > sms ? g.resident : 1;
+    const int64_t rounds = ceil_div(all, beside * sms);
+    const int64_t unit = compute > beside * share ? compute : beside * share;
+    const int64_t time =
+        rounds * (per * unit + 3000 / beside) + (n > 1 ? 2500 + 20 * n : 0);
+    if (least == 0 || time < least) {
+      least = time;
+      best = n;
     }
-  }
-  return splits;
+  };
+  consider(1);
+  for (int i = 1; i <= 4; ++i) consider(sms * i / blocks);
+  consider(most);
+  return (int)best;
 }
+
 int check_sizes(int batch, int dtype, int64_t pool_blocks, int64_t count, int q_heads,
                 int kv_heads, int head_dim, int page_size) {
   if (batch < 0 || kv_heads < 1 || q_heads < 1 || head_dim < 1 || page_size < 1 ||
