@@ -17,7 +17,9 @@
  * A floating-point code gains nothing from a scale between powers of two but up
  * to one bit of its smallest numbers, and these make every result exact: the
  * scaled element in fp32, the value held in bf16 and fp32. Rows have scales of
- * their own because the resolver moves them alone between host and pool.
+ * their own because the resolver moves them alone between host and pool. No scale is 0:
+ * a record of zeros, as in cleared memory, holds nothing; attention does not see
+ * such a row, and reading it gives zeros.
  *
  *   pool   [pool_blocks, 2 (K|V), page_size, record]   bytes, 16-byte aligned
  *   host   [host_blocks, 2 (K|V), page_size, record]
@@ -65,7 +67,8 @@ HS_API int hs_append_quantized(int batch, int64_t tokens, const void *k, const v
 
 /* ---- (10) reading rows back --------------------------------------------------------
  * out [2 (K|V), count, kv_heads, head_dim] of `dtype` takes the values of
- * physical rows rows[0 .. count-1], rounded to nearest once; zeros for a negative
+ * physical rows rows[0 .. count-1], rounded to nearest once (exact in bf16 and
+ * fp32; fp16 overflows to infinity as any conversion does); zeros for a negative
  * row (padding) and for one beyond the pool, which raises
  * HS_DEV_ROW_OUT_OF_RANGE.
  */

@@ -177,8 +177,8 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<T, kDim, kQuads>::reside
   // A lane has the row number of one row of a unit, read one unit before its copies.
   const int64_t *rows = p.rows + b * p.rows_batch_stride;
   const auto look = [&](int unit) -> int64_t {
-    const int at = unit * kUnitRows + lane;
-    return unit < last && at < valid ? __ldg(rows + at) : -1;
+    const unsigned at = (unsigned)unit * kUnitRows + lane;
+    return unit < last && at < (unsigned)valid ? __ldg(rows + at) : -1;
   };
   // The index of its K record; the launch has checked that all of them fit 32 bits.
   const int64_t pool_rows = p.pool_blocks * p.page_size;

@@ -89,6 +89,8 @@ class RowCache:
         self.pool = torch.empty((config.gpu_pages, *shape), dtype=dtype, device=self.device)
         self.host = host if host is not None else torch.empty(
             (config.host_pages, *shape), dtype=dtype, pin_memory=True)
+        if config.quantized and (self.host.dtype != dtype or self.host.shape[1:] != shape):
+            raise ValueError("host store must be uint8 [pages, 2, page_size, row_bytes]")
         self.mapped = MappedHost(self.host)
         self.compute = torch.cuda.current_stream(self.device)
         self.transfer = torch.cuda.Stream(device=self.device)

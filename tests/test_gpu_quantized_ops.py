@@ -227,6 +227,51 @@ def test_append_views_and_page_form():
     assert torch.equal(pool, pools[0])
 
 
+def test_append_without_metadata_and_too_many_rows():
+    config = make_config(3, 8, 2, 32)
+    pool = torch.full((3, *config.page_shape), 5, dtype=torch.uint8, device=DEV)
+    k = normal(3, 4, 2, 32, seed=14, dtype=torch.bfloat16).to(DEV)
+    # the second chunk claims more rows than K has, the third a host block without a host
+    append_quantized(k, k, ints([1, 0, 0]), ints([3, 5, 1]), ints([2, 1, 0], torch.int64), pool,
+                     None, None, None, config, host_block=ints([-1, -1, 0], torch.int64))
+    expected = np.full(tuple(pool.shape), 5, dtype=np.uint8)
+    expected[2, :, 1:4] = ref.records(k[0, :3].double().cpu().numpy())
+    assert np.array_equal(pool.cpu().numpy(), expected)
+    assert "beyond the pool" in _lib.device_flags(DEV)[0]
+    with pytest.raises(ValueError, match="go together"):
+        at = ints([0, 0, 0], torch.int64)
+        append_quantized(k, k, ints([0] * 3), ints([1] * 3), at, pool, at, None, at, config)
+
+
+def test_append_nothing():
+    config = make_config(2, 8, 2, 32)
+    pool = torch.full((2, *config.page_shape), 5, dtype=torch.uint8, device=DEV)
+    for shape in ((0, 3, 2, 32), (2, 0, 2, 32)):
+        k = torch.zeros(shape, device=DEV)
+        n = shape[0]
+        append_quantized(k, k, ints([0] * n), ints([0] * n), ints([0] * n, torch.int64), pool,
+                         None, None, None, config)
+    assert torch.all(pool == 5) and not _lib.device_flags(DEV)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_append_strided_chunks(dtype):
+    """Chunks a distance apart that vectors cannot step over, and expanded ones."""
+    heads, dim = 2, 64
+    config = make_config(4, 8, heads, dim)
+    flat = normal(2000, seed=15, dtype=dtype).to(DEV)
+    k = flat.as_strided((3, 2, heads, dim), (2 * heads * dim + 3, heads * dim, dim, 1))
+    for source in (k, k[:1].expand(3, 2, heads, dim)):
+        pool = torch.zeros((4, *config.page_shape), dtype=torch.uint8, device=DEV)
+        append_quantized(source, source, ints([0, 2, 6]), ints([2, 2, 2]),
+                         ints([3, 1, 0], torch.int64), pool, None, None, None, config)
+        got = pool.cpu().numpy()
+        for b, (block, w) in enumerate(((3, 0), (1, 2), (0, 6))):
+            want = ref.records(source[b].double().cpu().numpy())
+            for plane in range(2):
+                assert np.array_equal(got[block, plane, w:w + 2], want)
+
+
 # ---- reading back -----------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("heads,dim,page,count", [
@@ -344,6 +389,22 @@ def test_attend_unseen_rows_take_no_part(dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [128, 33])
+def test_attend_rows_never_written(dtype, dim):
+    """Records of zeros are not seen, wherever they are in the list."""
+    config = make_config(8, 16, 2, dim)
+    pool = make_pool(config, seed=62)
+    pool[2], pool[5, :, 3:] = 0, 0
+    rows = np.random.default_rng(63).permutation(128)[None].repeat(2, 0)
+    query = normal(2, 8, dim, seed=64, dtype=dtype)
+    written = pool[rows // 16, 0, rows % 16].any(-1)
+    got = check_attend(query, pool, np.where(written, rows, -1), config)
+    same = attend_quantized(query.to(DEV), torch.from_numpy(pool).to(DEV),
+                            torch.from_numpy(rows).to(DEV), config)
+    assert torch.equal(same, got)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_attend_nan_is_kept(dtype):
     """A NaN in a seen K makes its heads NaN, one in a seen V its element."""
     config = make_config(4, 16, 2, 128)
@@ -440,6 +501,35 @@ def test_attend_far_rows():
                      *pages.pointers(), config)
     assert np.array_equal(pool[-1, 0, 15].cpu().numpy(),
                           ref.records(k[0, 0].double().cpu().numpy()))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,group", [(8, 4), (4, 7), (17, 2), (1, 12), (3, 5)])
+def test_attend_many_units(dtype, heads, group):
+    """Enough rows that every warp goes around its rings of rows and of scales several
+    times, on one split and on many, with runs, single rows and masked ones."""
+    batch, count, dim, page = 40, 1200, 64, 16
+    blocks = 200
+    config = make_config(blocks, page, heads, dim)
+    pool = make_pool(config, seed=65)
+    rng = np.random.default_rng(66)
+    rows = rng.integers(0, blocks * page, (batch, count))
+    runs = rng.integers(0, blocks, (batch, count // 32))
+    for i in range(0, count // 32 - 1, 2):  # every other unit two runs
+        rows[:, 32 * i:32 * i + 16] = runs[:, i:i + 1] * page + np.arange(16)
+        rows[:, 32 * i + 16:32 * i + 32] = runs[:, i + 1:i + 2] * page + np.arange(16)
+    rows[:, 7::29] = -1
+    query = normal(batch, heads * group, dim, seed=67, dtype=dtype)
+    device = torch.from_numpy(pool).to(DEV)
+    got = attend_quantized(query.to(DEV), device, torch.from_numpy(rows).to(DEV), config)
+    for b in (0, 17, 39):
+        out, spread, size = ref.attend(query[b:b + 1].double().numpy(), pool, rows[b:b + 1], heads)
+        bound = ref.attend_tolerance(out, spread, size, dim, count, dtype)
+        assert np.all(np.abs(got[b:b + 1].double().cpu().numpy() - out) <= bound)
+        alone = attend_quantized(query[b:b + 1].to(DEV), device,
+                                 torch.from_numpy(rows[b:b + 1]).to(DEV), config)
+        assert np.all(np.abs(alone.double().cpu().numpy() - out) <= bound)
+    assert not _lib.device_flags(DEV)
 
 
 # ---- streams, graphs, refusals --------------------------------------------------------------------

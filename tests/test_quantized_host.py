@@ -58,6 +58,9 @@ def test_host_side_validation_needs_no_device():
     assert append(batch=0) == _lib.HS_OK
     assert append(batch=-1) == append(heads=0) == append(page=0) == append(dtype=7) == bad
     assert append(k=None) == bad
+    # bounds without the mean
+    assert lib.hs_append_quantized(1, 1, 16, 16, 64, 0, 16, 16, 16, 16, 4, 16, None, 0, 16, 16,
+                                   None, 2, 32, 16, None, None) == bad
     assert append(dim=257) == append(batch=65536) == unsupported
 
     def read(count=4, dtype=_lib.HS_FLOAT32, dim=32, pool=16):
