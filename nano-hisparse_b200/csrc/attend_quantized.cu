@@ -213,14 +213,24 @@ __global__ void __launch_bounds__(kJoinThreads) quant_merge_kernel(QuantAttendPa
   out[((int64_t)b * p.q_heads + h) * D + tid] = from_f32<T>(y * inv);
 }
 
+// Splits that a call in one phase may have without a join and without a workspace: those of
+// a cluster, for the tensor-core kernel's head_dims and two blocks an SM (with one, clusters
+// leave SMs idle: 4 requests of 4,096 rows, one head of 256: 22.7 us as a cluster of 8, 17.1
+// with a join). A call that cannot take that kernel all the same has one split.
+int splits_without_join(const QuantMmaGrid &g, int head_dim) {
+  return head_dim % 16 == 0 && g.resident == 2 ? kClusterSplits : 1;
+}
 // Splits of a request's rows, from what was measured of the tensor-core kernel: a warp takes
 // 1.45 us for a unit of 32 rows (2.5 above head_dim 128) while memory keeps up, the blocks
 // of an SM together 1.73 us for 67.6 KB of records; a block takes 3 us besides (half of it
 // beside another block's work), the join 2.5 and 0.02 for each split. More blocks than one an SM thus do not help large calls
 // (4 requests of 8,192 rows, 8 heads of 128: 37 splits 18.2 us, 74 splits 19.9), more rounds
 // of blocks do not hurt them (16 of 32,768: 18 splits 172, 37 splits 168), and small calls
-// want a unit a warp (1 of 2,048: 64 splits 9.5, 16 splits 12.5). One number for every
-// type, so that the workspace depends on the sizes alone. Times in ns.
+// want a unit a warp (1 of 2,048: 64 splits 9.5, 16 splits 12.5). A cluster saves the join's
+// launch and its traffic (4 requests of 1,000 rows: 8 splits 11.6, 14.5 with a join), but
+// those of more than 4 blocks crowd on some SMs while others idle (16 of 2,048: 8 splits
+// 23.8, 20.5 with a join): they count as two blocks an SM. One number for every type, so
+// that the workspace depends on the sizes alone. Times in ns.
 int quant_splits(int batch, int q_heads, int kv_heads, int head_dim, int64_t count) {
   const QuantMmaGrid g = quant_mma_grid(q_heads, kv_heads, head_dim);
   const int64_t blocks = (int64_t)batch * g.groups * g.chunks, sms = sm_count();
@@ -235,17 +245,20 @@ int quant_splits(int batch, int q_heads, int kv_heads, int head_dim, int64_t cou
     if (n < 1) n = 1;
     const int64_t per = ceil_div(ceil_div(units, n), g.slices);
     if (per > 0) n = ceil_div(units, per * g.slices);  // the fewest with as many units a warp
-    const int64_t all = blocks * n, beside = all > sms ? g.resident : 1;
+    const bool join = n > splits_without_join(g, head_dim);
+    const int64_t all = blocks * n, beside = all > sms || (!join && n > 4) ? g.resident : 1;
     const int64_t rounds = ceil_div(all, beside * sms);
     const int64_t unit = compute > beside * share ? compute : beside * share;
-    const int64_t time =
-        rounds * (per * unit + 3000 / beside) + (n > 1 ? 2500 + 20 * n : 0);
+    const int64_t time = rounds * (per * unit + 3000 / beside) +
+                         (n == 1 ? 0 : join ? 2500 + 20 * n : 1000);
     if (least == 0 || time < least) {
       least = time;
       best = n;
     }
   };
   consider(1);
+  consider(4);
+  consider(kClusterSplits);
   for (int i = 1; i <= 4; ++i) consider(sms * i / blocks);
   consider(most);
   return (int)best;
@@ -314,13 +327,16 @@ int launch_merge(const QuantAttendParams &p, int phases, void *out, bool beside,
   else cudaLaunchKernelEx(&config, quant_merge_kernel<T, 64>, p, phases, to);
   return check_launch("quant_merge_kernel");
 }
-int launch_rows(const QuantAttendParams &p, int dtype, cudaStream_t s) {
-  // the tensor-core kernel reads four query elements together and numbers records in 32 bits
+// Whether the tensor-core kernel takes a call: it reads four query elements together and
+// numbers records in 32 bits.
+bool on_tensor_cores(const QuantAttendParams &p, int dtype) {
   const int four = dtype == HS_FLOAT32 ? 16 : 8;
-  if (p.head_dim % 16 == 0 && p.rows_head_stride == 0 &&
-      reinterpret_cast<uintptr_t>(p.query) % four == 0 && p.q_batch_stride % 4 == 0 &&
-      p.pool_blocks <= 0xfffffffell / 2 / p.page_size)
-    return launch_quant_mma(p, dtype, s);
+  return p.head_dim % 16 == 0 && p.rows_head_stride == 0 &&
+         reinterpret_cast<uintptr_t>(p.query) % four == 0 && p.q_batch_stride % 4 == 0 &&
+         p.pool_blocks <= 0xfffffffell / 2 / p.page_size;
+}
+int launch_rows(const QuantAttendParams &p, int dtype, cudaStream_t s) {
+  if (on_tensor_cores(p, dtype)) return launch_quant_mma(p, dtype, s);
   switch (dtype) {
     case HS_FLOAT32: return launch_rows<float>(p, s);
     case HS_FLOAT16: return launch_rows<__half>(p, s);
@@ -364,7 +380,9 @@ extern "C" size_t hs_attend_quantized_workspace_bytes(int batch, int phases, int
   if (batch < 1 || phases < 1 || kv_heads < 1 || q_heads < kv_heads || head_dim < 1 || count < 0)
     return 0;
   const int splits = quant_splits(batch, q_heads, kv_heads, head_dim, count);
-  if (splits == 1 && phases == 1) return 0;
+  if (phases == 1 &&
+      splits <= splits_without_join(quant_mma_grid(q_heads, kv_heads, head_dim), head_dim))
+    return 0;
   const int64_t parts = (int64_t)phases * batch * q_heads * splits;
   return (size_t)parts * (sizeof(float4) + quant_pad(head_dim) * sizeof(float));
 }
@@ -396,13 +414,16 @@ extern "C" int hs_attend_quantized(int batch, const void *query, int64_t query_b
   p.rows_batch_stride = rows_batch_stride;
   p.rows_head_stride = rows_head_stride;
   p.counts32 = counts;
-  p.out = p.splits == 1 ? out : nullptr;
   p.page_size = page_size;
   p.page_shift = page_shift_of(page_size);
   p.status = device_status;
+  if (p.splits <= splits_without_join(quant_mma_grid(q_heads, kv_heads, head_dim), head_dim)) {
+    p.out = out;
+    if (!on_tensor_cores(p, dtype)) p.splits = 1;
+  }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int status = launch_rows(p, dtype, s);
-  return status != HS_OK || p.splits == 1 ? status : launch_merge(p, 1, out, dtype, true, s);
+  return status != HS_OK || p.out != nullptr ? status : launch_merge(p, 1, out, dtype, true, s);
 }
 
 extern "C" int hs_attend_quantized_phase(int batch, const void *query,

@@ -9,6 +9,7 @@
 namespace hs {
 
 constexpr int kQuantMaxSplits = 128;
+constexpr int kClusterSplits = 8;  // joined in the kernel, as a cluster
 constexpr float kSumLift = 10.f, kSumScale = 1024.f;  // 2^kSumLift
 
 struct QuantAttendParams {
@@ -22,7 +23,7 @@ struct QuantAttendParams {
   const int32_t *counts32;  // rows of a request: counts32, or the sum of counts64, or `count`
   const int64_t *counts64;
   int counts_stride, counts_first, counts_n;
-  void *out;            // written where there is one split and one phase, else NULL
+  void *out;            // written where no other kernel joins the splits, else NULL
   int q_heads, kv_heads, head_dim, page_size, page_shift;
   int groups;           // query heads of a KV head
   int splits, phase;
@@ -72,6 +73,7 @@ __device__ __forceinline__ float quant_share(float s, float e, float top_s, floa
 
 // attend_quantized_mma.cu: head_dim a multiple of 16, shared rows, query and its stride
 // multiples of four elements, fewer than 2^32 records
+// It joins up to kClusterSplits splits itself where p.out is given.
 struct QuantMmaGrid {
   int queries, chunks;         // query heads of a warp, such parts of a KV head's
   int heads, groups, places;   // KV heads of a block, such blocks, warps side by side

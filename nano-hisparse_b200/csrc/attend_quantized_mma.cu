@@ -149,7 +149,7 @@ template <typename T> __device__ __forceinline__ float4 load4(const T *from) {
 
 template <typename T, int kDim, int kQuads>
 __global__ void __launch_bounds__(kMmaThreads, MmaShape<T, kDim, kQuads>::resident)
-    quant_mma_kernel(QuantAttendParams p, int heads_of_block, int head_places) {
+    quant_mma_kernel(QuantAttendParams p, int heads_of_block, int head_places, bool cluster) {
   using Shape = MmaShape<T, kDim, kQuads>;
   constexpr int kChunks = kDim / 16, kQueries = Shape::queries;
   constexpr int kQueryTiles = Shape::query_tiles, kOutputTiles = Shape::output_tiles;
@@ -446,8 +446,7 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<T, kDim, kQuads>::reside
   asm volatile("cp.async.wait_all;\n" ::: "memory");
 
   // ---- results: out = o / l, in the join's terms o 2^-kSumLift / l 2^kSumLift ------------
-  const auto write = [&](int g, int d, float top, float sum, float2 x) {
-    const int h = h0 + g;
+  const auto write = [&](int h, int d, float top, float sum, float2 x) {
     if (p.out != nullptr) {
       const float inv = sum > 0.f || sum != sum ? kSumScale / sum : 0.f;
       T *out = static_cast<T *>(p.out) + ((int64_t)b * p.q_heads + h) * D + d;
@@ -470,17 +469,19 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<T, kDim, kQuads>::reside
   for (int n = 0; n < kQuads; ++n)
 #pragma unroll
     for (int i = 4; i < 32; i <<= 1) l[n] += __shfl_xor_sync(kFullMask, l[n], i);
-  if (slices == 1) {
+  if (slices == 1 && !cluster) {
 #pragma unroll
     for (int n = 0; n < kQuads; ++n)
 #pragma unroll
       for (int c = 0; c < kChunks; ++c) {
         const int g = n * 4 + lane % 4, d = c * 16 + lane / 4 * 2;
-        if (g < hn && d < D) write(g, d, -base[n], l[n], result(n, c));
+        if (g < hn && d < D) write(h0 + g, d, -base[n], l[n], result(n, c));
       }
     return;
   }
-  // the slices' results meet in shared memory: a query's maximum and sum, then its elements
+  // The results of the slices, and of the splits in a cluster, meet in shared memory: a
+  // query's maximum and sum, then its elements. Every thread of the cluster comes to both of
+  // its barriers.
   __syncthreads();
   float *mine = reinterpret_cast<float *>(smem + (size_t)warp * Shape::result);
 #pragma unroll
@@ -491,29 +492,66 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<T, kDim, kQuads>::reside
     for (int c = 0; c < kChunks; ++c)
       *reinterpret_cast<float2 *>(to_query + 4 + c * 16 + lane / 4 * 2) = result(n, c);
   }
-  __syncthreads();
-  // warp (place, slice) takes every slices-th query of its head
-  for (int g = slice; g < hn; g += slices) {
-    const auto of = [&](int s) {
-      return reinterpret_cast<const float *>(smem + (size_t)(s * head_places + place) *
-                                                        Shape::result) + g * (kDim + 4);
+  if (cluster) cluster_barrier();
+  else __syncthreads();
+  const int ranks = cluster ? p.splits : 1, rank = cluster ? split : 0, parts = ranks * slices;
+  const int queries = min(kQueries, p.groups - chunk * kQueries);
+  static_assert(kClusterSplits * kMmaWarps <= 64, "two parts a lane");
+  // a warp takes a query head at a time; part i is slice i % slices of rank i / slices
+  for (int i = rank + ranks * warp; i < sharing * queries; i += ranks * kMmaWarps) {
+    const int head = i % sharing, g = i / sharing;
+    const auto of = [&](int part) {
+      const int from = part / slices, slice_of = part - from * slices;
+      float *at = reinterpret_cast<float *>(
+                      smem + (size_t)(slice_of * head_places + head) * Shape::result) +
+                  g * (kDim + 4);
+      return cluster ? map_rank(at, from) : at;
     };
-    float top = -kNothing, sum = 0.f;
-    for (int s = 0; s < slices; ++s) top = fmaxf(top, of(s)[0]);
-    for (int s = 0; s < slices; ++s)
-      if (of(s)[1] != 0.f) sum = fmaf(of(s)[1], quant_exp2(of(s)[0] - top), sum);
-    for (int d = lane * 2; d < D; d += 64) {
-      float2 x = make_float2(0.f, 0.f);
-      for (int s = 0; s < slices; ++s) {
-        if (of(s)[1] == 0.f) continue;  // saw nothing
-        const float f = quant_exp2(of(s)[0] - top);
-        const float2 y = *reinterpret_cast<const float2 *>(of(s) + 4 + d);
-        x.x = fmaf(f, y.x, x.x);
-        x.y = fmaf(f, y.y, x.y);
-      }
-      write(g, d, top, sum, x);
+    float2 stat[2];
+    float weight[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      stat[k] = lane + 32 * k < parts ? *reinterpret_cast<const float2 *>(of(lane + 32 * k))
+                                      : make_float2(-kNothing, 0.f);
+    const float top = warp_max(fmaxf(stat[0].x, stat[1].x));
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {  // one that saw nothing left zeros
+      weight[k] = stat[k].y == 0.f ? 0.f : quant_exp2(stat[k].x - top);
+      sum = fmaf(stat[k].y, weight[k], sum);
     }
+    sum = warp_xor_tree_sum(sum);
+    float2 x[kDim / 64];
+#pragma unroll
+    for (int j = 0; j < kDim / 64; ++j) x[j] = make_float2(0.f, 0.f);
+    constexpr int kTogether = 8;  // parts read before the first is used
+    for (int part = 0; part < parts; part += kTogether) {
+      float2 y[kTogether][kDim / 64];
+#pragma unroll
+      for (int u = 0; u < kTogether; ++u) {
+        const float *from = of(min(part + u, parts - 1)) + 4 + lane * 2;
+#pragma unroll
+        for (int j = 0; j < kDim / 64; ++j) y[u][j] = *reinterpret_cast<const float2 *>(from + j * 64);
+      }
+#pragma unroll
+      for (int u = 0; u < kTogether; ++u) {
+        const int at = part + u;
+        const float w = __shfl_sync(kFullMask, at < 32 ? weight[0] : weight[1], at & 31);
+#pragma unroll
+        for (int j = 0; j < kDim / 64; ++j) {
+          if (at < parts) {
+            x[j].x = fmaf(w, y[u][j].x, x[j].x);
+            x[j].y = fmaf(w, y[u][j].y, x[j].y);
+          }
+        }
+      }
+    }
+    const int h = (group * heads_of_block + head) * p.groups + chunk * kQueries + g;
+#pragma unroll
+    for (int j = 0; j < kDim / 64; ++j)
+      if (lane * 2 + j * 64 < D) write(h, lane * 2 + j * 64, top, sum, x[j]);
   }
+  if (cluster) cluster_barrier();  // the others may still read this block's results
 }
 
 template <typename T, int kDim, int kQuads>
@@ -524,8 +562,20 @@ int launch(const QuantAttendParams &p, cudaStream_t s) {
     return e;
   const QuantMmaGrid g = quant_mma_grid(p.q_heads, p.kv_heads, p.head_dim);
   const int chunks = (p.groups + 4 * kQuads - 1) / (4 * kQuads);
-  const dim3 grid((unsigned)p.splits, (unsigned)(g.groups * chunks), (unsigned)p.batch);
-  kernel<<<grid, kMmaThreads, bytes, s>>>(p, g.heads, g.places);
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3((unsigned)p.splits, (unsigned)(g.groups * chunks), (unsigned)p.batch);
+  config.blockDim = dim3(kMmaThreads);
+  config.dynamicSmemBytes = bytes;
+  config.stream = s;
+  // the splits of a request are one cluster where they write its output
+  const bool cluster = p.out != nullptr && p.splits > 1;
+  cudaLaunchAttribute attribute{};
+  attribute.id = cudaLaunchAttributeClusterDimension;
+  attribute.val.clusterDim.x = (unsigned)p.splits;
+  attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+  config.attrs = &attribute;
+  config.numAttrs = cluster ? 1 : 0;
+  cudaLaunchKernelEx(&config, kernel, p, g.heads, g.places, cluster);
   return check_launch("quant_mma_kernel");
 }
 // Quads of a warp: as many as the query heads need and the registers hold.
