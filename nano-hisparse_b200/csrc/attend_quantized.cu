@@ -228,9 +228,10 @@ int splits_without_join(const QuantMmaGrid &g, int head_dim) {
 // of blocks do not hurt them (16 of 32,768: 18 splits 172, 37 splits 168), and small calls
 // want a unit a warp (1 of 2,048: 64 splits 9.5, 16 splits 12.5). A cluster saves the join's
 // launch and its traffic (4 requests of 1,000 rows: 8 splits 11.6, 14.5 with a join), but
-// those of more than 4 blocks crowd on some SMs while others idle (16 of 2,048: 8 splits
-// 23.8, 20.5 with a join): they count as two blocks an SM. One number for every type, so
-// that the workspace depends on the sizes alone. Times in ns.
+// its blocks crowd on some SMs while others idle, which counts once there is much to do (16
+// of 2,048: 8 splits 23.8, 20.5 with a join; 16 of 32,768: 288 and 198): such calls do not
+// take one. One number for every type, so that the workspace depends on the sizes alone.
+// Times in ns.
 int quant_splits(int batch, int q_heads, int kv_heads, int head_dim, int64_t count) {
   const QuantMmaGrid g = quant_mma_grid(q_heads, kv_heads, head_dim);
   const int64_t blocks = (int64_t)batch * g.groups * g.chunks, sms = sm_count();
@@ -246,9 +247,10 @@ int quant_splits(int batch, int q_heads, int kv_heads, int head_dim, int64_t cou
     const int64_t per = ceil_div(ceil_div(units, n), g.slices);
     if (per > 0) n = ceil_div(units, per * g.slices);  // the fewest with as many units a warp
     const bool join = n > splits_without_join(g, head_dim);
-    const int64_t all = blocks * n, beside = all > sms || (!join && n > 4) ? g.resident : 1;
+    const int64_t all = blocks * n, beside = all > sms || (!join && n > 1) ? g.resident : 1;
     const int64_t rounds = ceil_div(all, beside * sms);
     const int64_t unit = compute > beside * share ? compute : beside * share;
+    if (!join && n > 1 && rounds * per * unit > 15000) return;
     const int64_t time = rounds * (per * unit + 3000 / beside) +
                          (n == 1 ? 0 : join ? 2500 + 20 * n : 1000);
     if (least == 0 || time < least) {
