@@ -57,9 +57,12 @@ template <typename T, int kDim, int kQuads> struct MmaShape {
   static constexpr int stage = 2 * plane;  // K, V
   static constexpr int queries = 4 * kQuads;
   static constexpr int ring = kStages * stage;
-  // the warps' results at the end, in the place of the rings
-  static constexpr int result = queries * (kDim + 4) * 4;
-  static constexpr int rings = kMmaWarps * (ring > result ? ring : result);
+  // a warp's results at the end, in the place of its ring: its queries' elements (the rows'
+  // pitch keeps the stores of four queries in different banks) and statistics, and in the
+  // first slice's the statistics of all slices together
+  static constexpr int pitch = kDim + 16, result = queries * pitch * 4;
+  static_assert(result + 2 * queries * (int)sizeof(float2) <= ring, "the results fit a ring");
+  static constexpr int rings = kMmaWarps * ring;
   // the rings of scales, and their barriers: for each slice of the warps full and free
   static constexpr size_t bytes = rings + kScaleRoom + kMmaWarps * 2 * kSlots * sizeof(uint64_t);
   // blocks on an SM: two where the output and the queries leave the registers for it
@@ -126,25 +129,64 @@ __device__ __forceinline__ void copies_arrive(uint64_t *bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];\n" ::"r"(smem_addr(bar))
                : "memory");
 }
-// This lane's part (of the two of a column pair: `odd`) in each tile of columns
+// The parts of four query elements, two for each tile of columns
 template <typename T, int kTiles>
-__device__ __forceinline__ void split_query(float4 x, bool odd, uint32_t (&codes)[kTiles]) {
+__device__ __forceinline__ void split_query(float4 x, uint32_t (&codes)[2 * kTiles]) {
 #pragma unroll
-  for (int part = 0; part < kQueryParts<T>; ++part) {
-    const uint32_t code = encode4(x.x, x.y, x.z, x.w);
-    if ((part & 1) == (int)odd) codes[part / 2] = code;
-    const float4 y = decode4_f32(code);
+  for (int part = 0; part < 2 * kTiles; ++part) {
+    codes[part] = part < kQueryParts<T> ? encode4(x.x, x.y, x.z, x.w) : 0u;
+    const float4 y = decode4_f32(codes[part]);
     x = make_float4((x.x - y.x) * 16.f, (x.y - y.y) * 16.f, (x.z - y.z) * 16.f,
                     (x.w - y.w) * 16.f);
   }
 }
-__device__ __forceinline__ float4 load4(const float *from) {
-  return __ldg(reinterpret_cast<const float4 *>(from));
-}
-template <typename T> __device__ __forceinline__ float4 load4(const T *from) {
-  const uint2 raw = __ldg(reinterpret_cast<const uint2 *>(from));
-  const T *x = reinterpret_cast<const T *>(&raw);
-  return make_float4(to_f32(x[0]), to_f32(x[1]), to_f32(x[2]), to_f32(x[3]));
+// Four query elements as they lie in memory
+template <typename T> struct Raw4 {
+  uint2 raw;
+  __device__ __forceinline__ void load(const T *from) {
+    raw = __ldg(reinterpret_cast<const uint2 *>(from));
+  }
+  __device__ __forceinline__ void clear() { raw = make_uint2(0u, 0u); }
+  __device__ __forceinline__ float4 get() const {
+    const T *x = reinterpret_cast<const T *>(&raw);
+    return make_float4(to_f32(x[0]), to_f32(x[1]), to_f32(x[2]), to_f32(x[3]));
+  }
+};
+template <> struct Raw4<float> {
+  float4 raw;
+  __device__ __forceinline__ void load(const float *from) {
+    raw = __ldg(reinterpret_cast<const float4 *>(from));
+  }
+  __device__ __forceinline__ void clear() { raw = make_float4(0.f, 0.f, 0.f, 0.f); }
+  __device__ __forceinline__ float4 get() const { return raw; }
+};
+// A query's results of n <= 8 parts of its rows, joined: stat(i) is part i's maximum and
+// sum, element(i) a pair of its elements. A part that saw nothing has left zeros.
+struct Joined {
+  float top, sum;
+  float2 x;
+};
+template <typename Stat, typename Element>
+__device__ __forceinline__ Joined join(int n, Stat stat, Element element) {
+  constexpr int kMost = 8;
+  static_assert(kClusterSplits <= kMost && kMmaWarps <= kMost, "the parts of a join");
+  float2 s[kMost], x[kMost];
+#pragma unroll
+  for (int i = 0; i < kMost; ++i) {
+    s[i] = i < n ? stat(i) : make_float2(-kNothing, 0.f);
+    x[i] = i < n ? element(i) : make_float2(0.f, 0.f);
+  }
+  Joined all{s[0].x, 0.f, make_float2(0.f, 0.f)};
+#pragma unroll
+  for (int i = 1; i < kMost; ++i) all.top = fmaxf(all.top, s[i].x);
+#pragma unroll
+  for (int i = 0; i < kMost; ++i) {
+    const float w = s[i].y == 0.f ? 0.f : quant_exp2(s[i].x - all.top);
+    all.sum = fmaf(w, s[i].y, all.sum);
+    all.x.x = fmaf(w, x[i].x, all.x.x);
+    all.x.y = fmaf(w, x[i].y, all.x.y);
+  }
+  return all;
 }
 
 template <typename T, int kDim, int kQuads>
@@ -168,6 +210,25 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<T, kDim, kQuads>::reside
   const bool here = place < heads_of_block && kh < p.kv_heads;
   const int h0 = kh * p.groups + chunk * kQueries;
   const int hn = here ? min(kQueries, p.groups - chunk * kQueries) : 0;  // query heads
+
+  // Q is read first and used after the first copies are on their way. A column lane / 4 of
+  // a tile is query head lane / 8 of a quad, part lane / 4 % 2; of every 16 elements the
+  // lane has those at 4 * (lane % 4) on. It reads and takes apart every other 16 elements,
+  // which its neighbour 4 lanes on has too, and gives it the parts that are its own.
+  const bool odd = lane & 4;
+  Raw4<T> raw[kQuads][kChunks / 2];
+#pragma unroll
+  for (int n = 0; n < kQuads; ++n) {
+    const int g = n * 4 + lane / 8;
+    const T *from = static_cast<const T *>(p.query) + (int64_t)b * p.q_batch_stride +
+                    (int64_t)(h0 + g) * D + lane % 4 * 4;
+#pragma unroll
+    for (int c = 0; c < kChunks / 2; ++c) {
+      const int at = (2 * c + odd) * 16;
+      if (g < hn && at < D) raw[n][c].load(from + at);
+      else raw[n][c].clear();
+    }
+  }
 
   // this warp's units: first, first + slices, ... < last
   const int valid = (int)quant_rows(p, b), units = (valid + kUnitRows - 1) / kUnitRows;
@@ -270,40 +331,40 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<T, kDim, kQuads>::reside
   copy_half(first, 0);
   copy_half(first, 1);
 
-  // Q: column lane / 4 of a tile is query head lane / 8 of a quad, part lane / 4 % 2; of
-  // every 16 elements this lane has those at 4 * (lane % 4) on
   uint32_t q[kQuads][kQueryTiles][kChunks];
   float factor[kQuads];  // of the scores of query head lane % 4
 #pragma unroll
   for (int n = 0; n < kQuads; ++n) {
-    const int g = n * 4 + lane / 8;
-    const T *from = static_cast<const T *>(p.query) + (int64_t)b * p.q_batch_stride +
-                    (int64_t)(h0 + g) * D + lane % 4 * 4;
     float largest = 0.f;
-    float4 x[kChunks];
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
-      x[c] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (g < hn && c * 16 < D) x[c] = load4(from + c * 16);
-      largest = fmaxf(fmaxf(largest, fmaxf(fabsf(x[c].x), fabsf(x[c].y))),
-                      fmaxf(fabsf(x[c].z), fabsf(x[c].w)));
+    for (int c = 0; c < kChunks / 2; ++c) {
+      const float4 x = raw[n][c].get();
+      largest = fmaxf(fmaxf(largest, fmaxf(fabsf(x.x), fabsf(x.y))),
+                      fmaxf(fabsf(x.z), fabsf(x.w)));
     }
-    largest = fmaxf(largest, __shfl_xor_sync(kFullMask, largest, 1));
-    largest = fmaxf(largest, __shfl_xor_sync(kFullMask, largest, 2));
+#pragma unroll
+    for (int i = 1; i < 8; i <<= 1)
+      largest = fmaxf(largest, __shfl_xor_sync(kFullMask, largest, i));
     // to between 128 and 256: what is 2^13 times smaller is still a normal e4m3 number. An
     // infinity leaves NaN, as its scores are
     const int e = (__float_as_int(largest) >> 23) - 127 - 7;
     const float scale = largest > 0.f ? power_of_two(max(-126, min(127, -e))) : 1.f;
+    const bool finite = largest < INFINITY;
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
-      uint32_t codes[kQueryTiles];
-      const float4 y = make_float4(x[c].x * scale, x[c].y * scale, x[c].z * scale,
-                                   x[c].w * scale);
-      for (int t = 0; t < kQueryTiles; ++t) codes[t] = 0;
-      split_query<T, kQueryTiles>(y, lane & 4, codes);
-      const bool finite = largest < INFINITY;
+    for (int c = 0; c < kChunks / 2; ++c) {
+      const float4 x = raw[n][c].get();
+      uint32_t codes[2 * kQueryTiles];
+      split_query<T, kQueryTiles>(
+          make_float4(x.x * scale, x.y * scale, x.z * scale, x.w * scale), codes);
 #pragma unroll
-      for (int t = 0; t < kQueryTiles; ++t) q[n][t][c] = finite ? codes[t] : 0x7f7f7f7fu;
+      for (int t = 0; t < kQueryTiles; ++t) {
+        const uint32_t even_part = finite ? codes[2 * t] : 0x7f7f7f7fu;
+        const uint32_t odd_part = finite ? codes[2 * t + 1] : 0x7f7f7f7fu;
+        const uint32_t own = odd ? odd_part : even_part;
+        const uint32_t other = __shfl_xor_sync(kFullMask, odd ? even_part : odd_part, 4);
+        q[n][t][2 * c] = odd ? other : own;
+        q[n][t][2 * c + 1] = odd ? own : other;
+      }
     }
     factor[n] = __shfl_sync(kFullMask, p.scale_log2 / scale, lane % 4 * 8);
   }
@@ -479,79 +540,60 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<T, kDim, kQuads>::reside
       }
     return;
   }
-  // The results of the slices, and of the splits in a cluster, meet in shared memory: a
-  // query's maximum and sum, then its elements. Every thread of the cluster comes to both of
-  // its barriers.
-  __syncthreads();
-  float *mine = reinterpret_cast<float *>(smem + (size_t)warp * Shape::result);
+  // The results of the slices meet in shared memory, then those of the splits in a cluster:
+  // a thread takes pairs of elements and reads the statistics beside them. Every thread of
+  // the cluster comes to both of its barriers.
+  constexpr int kPitch = Shape::pitch, kPairs = kDim / 2, kStep = kMmaThreads / kPairs;
+  // of warp w: elements, statistics and, of the first slice's, all slices' statistics
+  const auto elements = [&](int w) { return reinterpret_cast<float *>(smem + w * Shape::ring); };
+  const auto stats = [&](int w, int of) {
+    return reinterpret_cast<float2 *>(smem + w * Shape::ring + Shape::result) + of * kQueries;
+  };
 #pragma unroll
   for (int n = 0; n < kQuads; ++n) {
-    float *to_query = mine + (n * 4 + lane % 4) * (kDim + 4);
-    if (lane < 4) *reinterpret_cast<float2 *>(to_query) = make_float2(-base[n], l[n]);
+    float *to_query = elements(warp) + (n * 4 + lane % 4) * kPitch;
+    if (lane < 4) stats(warp, 0)[n * 4 + lane] = make_float2(-base[n], l[n]);
 #pragma unroll
     for (int c = 0; c < kChunks; ++c)
-      *reinterpret_cast<float2 *>(to_query + 4 + c * 16 + lane / 4 * 2) = result(n, c);
+      *reinterpret_cast<float2 *>(to_query + c * 16 + lane / 4 * 2) = result(n, c);
   }
-  if (cluster) cluster_barrier();
-  else __syncthreads();
-  const int ranks = cluster ? p.splits : 1, rank = cluster ? split : 0, parts = ranks * slices;
   const int queries = min(kQueries, p.groups - chunk * kQueries);
-  static_assert(kClusterSplits * kMmaWarps <= 64, "two parts a lane");
-  // a warp takes a query head at a time; part i is slice i % slices of rank i / slices
-  for (int i = rank + ranks * warp; i < sharing * queries; i += ranks * kMmaWarps) {
-    const int head = i % sharing, g = i / sharing;
-    const auto of = [&](int part) {
-      const int from = part / slices, slice_of = part - from * slices;
-      float *at = reinterpret_cast<float *>(
-                      smem + (size_t)(slice_of * head_places + head) * Shape::result) +
-                  g * (kDim + 4);
-      return cluster ? map_rank(at, from) : at;
-    };
-    float2 stat[2];
-    float weight[2];
-#pragma unroll
-    for (int k = 0; k < 2; ++k)
-      stat[k] = lane + 32 * k < parts ? *reinterpret_cast<const float2 *>(of(lane + 32 * k))
-                                      : make_float2(-kNothing, 0.f);
-    const float top = warp_max(fmaxf(stat[0].x, stat[1].x));
-    float sum = 0.f;
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {  // one that saw nothing left zeros
-      weight[k] = stat[k].y == 0.f ? 0.f : quant_exp2(stat[k].x - top);
-      sum = fmaf(stat[k].y, weight[k], sum);
-    }
-    sum = warp_xor_tree_sum(sum);
-    float2 x[kDim / 64];
-#pragma unroll
-    for (int j = 0; j < kDim / 64; ++j) x[j] = make_float2(0.f, 0.f);
-    constexpr int kTogether = 8;  // parts read before the first is used
-    for (int part = 0; part < parts; part += kTogether) {
-      float2 y[kTogether][kDim / 64];
-#pragma unroll
-      for (int u = 0; u < kTogether; ++u) {
-        const float *from = of(min(part + u, parts - 1)) + 4 + lane * 2;
-#pragma unroll
-        for (int j = 0; j < kDim / 64; ++j) y[u][j] = *reinterpret_cast<const float2 *>(from + j * 64);
-      }
-#pragma unroll
-      for (int u = 0; u < kTogether; ++u) {
-        const int at = part + u;
-        const float w = __shfl_sync(kFullMask, at < 32 ? weight[0] : weight[1], at & 31);
-#pragma unroll
-        for (int j = 0; j < kDim / 64; ++j) {
-          if (at < parts) {
-            x[j].x = fmaf(w, y[u][j].x, x[j].x);
-            x[j].y = fmaf(w, y[u][j].y, x[j].y);
-          }
-        }
+  const int d = threadIdx.x % kPairs * 2, first_query = threadIdx.x / kPairs;
+  const int all = d < D ? sharing * kQueries : 0;
+  if (slices > 1) {
+    __syncthreads();
+    for (int i = first_query; i < all; i += kStep) {
+      const int head = i / kQueries, g = i % kQueries;
+      if (g >= queries) continue;
+      const Joined x = join(
+          slices, [&](int k) { return stats(k * head_places + head, 0)[g]; },
+          [&](int k) {
+            return *reinterpret_cast<const float2 *>(elements(k * head_places + head) +
+                                                     g * kPitch + d);
+          });
+      if (!cluster) {
+        write((group * heads_of_block + head) * p.groups + chunk * kQueries + g, d, x.top, x.sum,
+              x.x);
+      } else {  // read by this thread alone so far
+        *reinterpret_cast<float2 *>(elements(head) + g * kPitch + d) = x.x;
+        if (d == 0) stats(head, 1)[g] = make_float2(x.top, x.sum);
       }
     }
-    const int h = (group * heads_of_block + head) * p.groups + chunk * kQueries + g;
-#pragma unroll
-    for (int j = 0; j < kDim / 64; ++j)
-      if (lane * 2 + j * 64 < D) write(h, lane * 2 + j * 64, top, sum, x[j]);
   }
-  if (cluster) cluster_barrier();  // the others may still read this block's results
+  if (!cluster) return;
+  cluster_barrier();
+  for (int i = split * kStep + first_query; i < all; i += p.splits * kStep) {
+    const int head = i / kQueries, g = i % kQueries;
+    if (g >= queries) continue;
+    const Joined x = join(
+        p.splits, [&](int k) { return *map_rank(stats(head, slices > 1 ? 1 : 0) + g, k); },
+        [&](int k) {
+          return *reinterpret_cast<const float2 *>(
+              map_rank(elements(head) + g * kPitch + d, k));
+        });
+    write((group * heads_of_block + head) * p.groups + chunk * kQueries + g, d, x.top, x.sum, x.x);
+  }
+  cluster_barrier();  // the others may still read this block's results
 }
 
 template <typename T, int kDim, int kQuads>
