@@ -160,16 +160,14 @@ template <> struct Raw4<float> {
   __device__ __forceinline__ void clear() { raw = make_float4(0.f, 0.f, 0.f, 0.f); }
   __device__ __forceinline__ float4 get() const { return raw; }
 };
-// A query's results of n <= 8 parts of its rows, joined: stat(i) is part i's maximum and
+// A query's results of n <= kMost parts of its rows, joined: stat(i) is part i's maximum and
 // sum, element(i) a pair of its elements. A part that saw nothing has left zeros.
 struct Joined {
   float top, sum;
   float2 x;
 };
-template <typename Stat, typename Element>
+template <int kMost, typename Stat, typename Element>
 __device__ __forceinline__ Joined join(int n, Stat stat, Element element) {
-  constexpr int kMost = 8;
-  static_assert(kClusterSplits <= kMost && kMmaWarps <= kMost, "the parts of a join");
   float2 s[kMost], x[kMost];
 #pragma unroll
   for (int i = 0; i < kMost; ++i) {
@@ -204,8 +202,9 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<T, kDim, kQuads>::reside
   const int split = blockIdx.x, b = blockIdx.z;
   const int chunks = (p.groups + kQueries - 1) / kQueries;  // of a KV head's query heads
   const int group = blockIdx.y / chunks, chunk = blockIdx.y - group * chunks;
-  const int slices = kMmaWarps / head_places;  // warps that share a head's rows
-  const int place = warp % head_places, slice = warp / head_places;
+  const int place_bits = __popc(head_places - 1);  // head_places is a power of two
+  const int slices = kMmaWarps >> place_bits;      // warps that share a head's rows
+  const int place = warp & (head_places - 1), slice = warp >> place_bits;
   const int kh = group * heads_of_block + place;
   const bool here = place < heads_of_block && kh < p.kv_heads;
   const int h0 = kh * p.groups + chunk * kQueries;
@@ -232,8 +231,9 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<T, kDim, kQuads>::reside
 
   // this warp's units: first, first + slices, ... < last
   const int valid = (int)quant_rows(p, b), units = (valid + kUnitRows - 1) / kUnitRows;
-  const int first = (int)((int64_t)units * split / p.splits) + slice;
-  const int last = here ? (int)((int64_t)units * (split + 1) / p.splits) : 0;
+  const int share = units / p.splits, rest = units - share * p.splits;
+  const int first = share * split + rest * split / p.splits + slice;
+  const int last = here ? share * (split + 1) + rest * (split + 1) / p.splits : 0;
 
   // A lane has the row number of one row of a unit, read one unit before its copies.
   const int64_t *rows = p.rows + b * p.rows_batch_stride;
@@ -258,11 +258,8 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<T, kDim, kQuads>::reside
   uint64_t *full = reinterpret_cast<uint64_t *>(smem + Shape::rings + kScaleRoom) +
                    slice * 2 * kSlots, *free = full + kSlots;
   const int sharing = min(head_places, min(heads_of_block, p.kv_heads - group * heads_of_block));
-  if (place == 0 && lane == 0) {
-    for (int i = 0; i < kSlots; ++i) {
-      mbar_init(&full[i], 32);
-      mbar_init(&free[i], sharing);
-    }
+  if (place == 0 && lane < 2 * kSlots) {
+    mbar_init(&full[lane], lane < kSlots ? 32 : sharing);  // free follows full
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
   __syncthreads();
@@ -325,9 +322,9 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<T, kDim, kQuads>::reside
     to = to == kStages - 1 ? 0 : to + 1;
     asm volatile("cp.async.commit_group;\n" ::: "memory");
   };
-  for (int i = 0; i < kAhead; ++i)
-    if (i % sharing == place && first + i * slices < last)
-      copy_scales(i, record_of(i == 0 ? next : later));
+  static_assert(kAhead == 2, "next and later");
+  if (place == 0 && first < last) copy_scales(0, record_of(next));
+  if (place == (sharing > 1) && first + slices < last) copy_scales(1, record_of(later));
   copy_half(first, 0);
   copy_half(first, 1);
 
@@ -386,12 +383,15 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<T, kDim, kQuads>::reside
   const uint32_t matrix = ring + tile_place<kDim>(lane & 15, lane / 16);
   const unsigned char *scale_byte = scales + lane / 4 * width + (kh - scale0);
   int stage = 0, count = 0;
+  // whose turn the scales of the unit kAhead units on are
+  int turn = sharing > 2 ? 2 : 0;
   for (int unit = first; unit < last && ok; unit += slices, ++count) {
     // row numbers of unit + 2 * slices are in `next` until the copies below move on
-    if ((count + kAhead) % sharing == place && unit + kAhead * slices < last) {
+    if (turn == place && unit + kAhead * slices < last) {
       copy_scales(count + kAhead, record_of(later));
       if (!ok) break;
     }
+    turn = turn == sharing - 1 ? 0 : turn + 1;
     const int slot = count % kSlots;
     ok = __all_sync(kFullMask, wait_phase(&full[slot], count / kSlots & 1, p.status));
     if (!ok) break;
@@ -507,6 +507,8 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<T, kDim, kQuads>::reside
   asm volatile("cp.async.wait_all;\n" ::: "memory");
 
   // ---- results: out = o / l, in the join's terms o 2^-kSumLift / l 2^kSumLift ------------
+  const int64_t part0 = quant_part(p, p.phase, b, 0, split);
+  const int pad = quant_pad(D);
   const auto write = [&](int h, int d, float top, float sum, float2 x) {
     if (p.out != nullptr) {
       const float inv = sum > 0.f || sum != sum ? kSumScale / sum : 0.f;
@@ -514,9 +516,9 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<T, kDim, kQuads>::reside
       out[0] = from_f32<T>(x.x * inv);
       out[1] = from_f32<T>(x.y * inv);
     } else {
-      const int64_t part = quant_part(p, p.phase, b, h, split);
+      const int64_t part = part0 + (unsigned)(h * p.splits);
       if (d == 0) p.stats[part] = make_float4(top, 0.f, sum, 0.f);
-      *reinterpret_cast<float2 *>(p.partials + part * quant_pad(D) + d) = x;
+      *reinterpret_cast<float2 *>(p.partials + part * pad + d) = x;
     }
   };
   // elements 16 c + 2 * (lane / 4) + 0, 1 of query head lane % 4 of quad n
@@ -560,13 +562,12 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<T, kDim, kQuads>::reside
   const int queries = min(kQueries, p.groups - chunk * kQueries);
   const int d = threadIdx.x % kPairs * 2, first_query = threadIdx.x / kPairs;
   const int all = d < D ? sharing * kQueries : 0;
-  if (slices > 1) {
-    __syncthreads();
+  const auto join_slices = [&](auto n) {
     for (int i = first_query; i < all; i += kStep) {
       const int head = i / kQueries, g = i % kQueries;
       if (g >= queries) continue;
-      const Joined x = join(
-          slices, [&](int k) { return stats(k * head_places + head, 0)[g]; },
+      const Joined x = join<n()>(
+          n(), [&](int k) { return stats(k * head_places + head, 0)[g]; },
           [&](int k) {
             return *reinterpret_cast<const float2 *>(elements(k * head_places + head) +
                                                      g * kPitch + d);
@@ -579,13 +580,20 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<T, kDim, kQuads>::reside
         if (d == 0) stats(head, 1)[g] = make_float2(x.top, x.sum);
       }
     }
+  };
+  static_assert(kMmaWarps == 8, "the numbers of slices");
+  if (slices > 1) {
+    __syncthreads();
+    if (slices == 2) join_slices(std::integral_constant<int, 2>());
+    else if (slices == 4) join_slices(std::integral_constant<int, 4>());
+    else join_slices(std::integral_constant<int, 8>());
   }
   if (!cluster) return;
   cluster_barrier();
   for (int i = split * kStep + first_query; i < all; i += p.splits * kStep) {
     const int head = i / kQueries, g = i % kQueries;
     if (g >= queries) continue;
-    const Joined x = join(
+    const Joined x = join<kClusterSplits>(
         p.splits, [&](int k) { return *map_rank(stats(head, slices > 1 ? 1 : 0) + g, k); },
         [&](int k) {
           return *reinterpret_cast<const float2 *>(
