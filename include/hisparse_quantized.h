@@ -96,8 +96,9 @@ HS_API int hs_read_quantized(const void *pool, int64_t pool_blocks, const int64_
  * The workspace (for `phases` phases, 1 for the plain form) is 16-byte aligned and
  * needs no initialisation; calls that may overlap on the GPU need separate ones.
  */
-HS_API size_t hs_attend_quantized_workspace_bytes(int batch, int phases, int q_heads,
-                                                  int kv_heads, int head_dim, int64_t count);
+HS_API size_t hs_attend_quantized_workspace_bytes(int batch, int phases, int dtype,
+                                                  int q_heads, int kv_heads, int head_dim,
+                                                  int64_t count);
 
 HS_API int hs_attend_quantized(int batch, const void *query, int64_t query_batch_stride,
                                int dtype, const void *pool, int64_t pool_blocks,

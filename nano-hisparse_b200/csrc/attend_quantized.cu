@@ -220,39 +220,41 @@ __global__ void __launch_bounds__(kJoinThreads) quant_merge_kernel(QuantAttendPa
 int splits_without_join(const QuantMmaGrid &g, int head_dim) {
   return head_dim % 16 == 0 && g.resident == 2 ? kClusterSplits : 1;
 }
-// Splits of a request's rows, from what was measured of the tensor-core kernel: a warp takes
-// 1.45 us for a unit of 32 rows (2.5 above head_dim 128) while memory keeps up, the blocks
-// of an SM together 1.73 us for 67.6 KB of records; a block takes 3 us besides (half of it
-// beside another block's work), the join 2.5 and 0.02 for each split. More blocks than one an SM thus do not help large calls
-// (4 requests of 8,192 rows, 8 heads of 128: 37 splits 18.2 us, 74 splits 19.9), more rounds
-// of blocks do not hurt them (16 of 32,768: 18 splits 172, 37 splits 168), and small calls
-// want a unit a warp (1 of 2,048: 64 splits 9.5, 16 splits 12.5). A cluster saves the join's
-// launch and its traffic (4 requests of 1,000 rows: 8 splits 11.6, 14.5 with a join), but
-// its blocks crowd on some SMs while others idle, which counts once there is much to do (16
-// of 2,048: 8 splits 23.8, 20.5 with a join; 16 of 32,768: 288 and 198): such calls do not
-// take one. One number for every type, so that the workspace depends on the sizes alone.
-// Times in ns.
-int quant_splits(int batch, int q_heads, int kv_heads, int head_dim, int64_t count) {
-  const QuantMmaGrid g = quant_mma_grid(q_heads, kv_heads, head_dim);
+// Splits of a request's rows, from what was measured of the tensor-core kernel, in ns: a
+// warp takes 1,450 for a unit of 32 rows (2,500 above head_dim 128) while memory keeps up,
+// the blocks of an SM together 1,730 for 67.6 KB of records. A block takes 3,000 besides
+// (half of it beside another block's work), one whose warps share a head's rows 250 more for
+// each query to join them, and the second kernel 2,500 and 20 for each split. So more blocks
+// than one an SM do not help large calls (16 requests of 2,048 rows, 8 heads of 128: 9 splits
+// 18.9 us, 18 splits 18.2, 37 splits 22.5), and small ones want a unit a warp (1 of 8,192:
+// 64 splits 12.7, 18 splits 26.2) or less where warps share a head (2 of 2,000, one head of
+// 256: 4 splits 20.3, 18 splits 14.2). A cluster saves the second launch and its traffic (4
+// requests of 1,000 rows: 8 splits 9.5, 10.6 with 9 splits and a join). But its blocks crowd
+// on some SMs while others idle: they count for a third more (16 of 2,048: 8 splits 21.5),
+// and with much to do only a grid that fills the SMs once takes one (53 of 3,057, 4 heads of
+// 128: 5 splits 39.2, 11 splits with a join 47.6; but 16 of 32,768, 8 heads: 8 splits 288, 18
+// with a join 168).
+int quant_splits(const QuantMmaGrid &g, int batch, int head_dim, int64_t count) {
   const int64_t blocks = (int64_t)batch * g.groups * g.chunks, sms = sm_count();
   const int64_t units = ceil_div(count, 32);
-  int64_t most = units / g.slices;  // a unit for each warp
-  if (most > kQuantMaxSplits) most = kQuantMaxSplits;
+  const int64_t most = units < kQuantMaxSplits ? units : kQuantMaxSplits;
   const int64_t compute = head_dim > 128 ? 2500 : 1450;
   const int64_t share = (int64_t)64 * g.heads * (head_dim + 1) * 1730 / 67584;
   int64_t best = 1, least = 0;
   const auto consider = [&](int64_t n) {
     if (n > most) n = most;
     if (n < 1) n = 1;
-    const int64_t per = ceil_div(ceil_div(units, n), g.slices);
-    if (per > 0) n = ceil_div(units, per * g.slices);  // the fewest with as many units a warp
-    const bool join = n > splits_without_join(g, head_dim);
-    const int64_t all = blocks * n, beside = all > sms || (!join && n > 1) ? g.resident : 1;
+    const int64_t own = ceil_div(units, n);  // units of a split
+    if (own > 0) n = ceil_div(units, own);   // the fewest such
+    const bool join = n > splits_without_join(g, head_dim), cluster = !join && n > 1;
+    const int64_t all = blocks * n, beside = all > sms ? g.resident : 1;
     const int64_t rounds = ceil_div(all, beside * sms);
-    const int64_t unit = compute > beside * share ? compute : beside * share;
-    if (!join && n > 1 && rounds * per * unit > 15000) return;
-    const int64_t time = rounds * (per * unit + 3000 / beside) +
-                         (n == 1 ? 0 : join ? 2500 + 20 * n : 1000);
+    const int64_t alone = ceil_div(own, g.slices) * compute, shared = own * beside * share;
+    int64_t time = rounds * (alone > shared ? alone : shared);
+    if (cluster && all <= sms) time = time * 4 / 3;
+    if (cluster && time > 15000 && (all <= sms || rounds > 1)) return;
+    time += rounds * (g.slices > 1 ? 3000 + 250 * g.queries : 3000 / beside);
+    time += join ? 2500 + 20 * n : cluster ? 1000 : 0;
     if (least == 0 || time < least) {
       least = time;
       best = n;
@@ -283,10 +285,13 @@ int check_sizes(int batch, int dtype, int64_t pool_blocks, int64_t count, int q_
   return HS_OK;
 }
 
-// Puts the workspace's parts into p; `phases` phases have to fit.
-int place_workspace(QuantAttendParams &p, int phases, void *workspace, size_t bytes) {
-  const size_t need = hs_attend_quantized_workspace_bytes(p.batch, phases, p.q_heads, p.kv_heads,
-                                                          p.head_dim, p.count);
+size_t workspace_of(const QuantAttendParams &p, int phases) {
+  const int64_t parts = p.join ? (int64_t)phases * p.batch * p.q_heads * p.splits : 0;
+  return (size_t)parts * (sizeof(float4) + quant_pad(p.head_dim) * sizeof(float));
+}
+// Whether the workspace holds `phases` phases
+int check_workspace(const QuantAttendParams &p, int phases, void *workspace, size_t bytes) {
+  const size_t need = workspace_of(p, phases);
   if (need == 0) return HS_OK;
   if ((reinterpret_cast<uintptr_t>(workspace) & 15) != 0)
     return set_error(HS_ERR_WORKSPACE, "attend_quantized: the workspace must be 16-byte aligned");
@@ -355,8 +360,8 @@ int launch_merge(const QuantAttendParams &p, int phases, void *out, int dtype, b
 }
 
 // The parameters that every form has; the workspace holds `phases` phases.
-QuantAttendParams params_of(int batch, int phases, int q_heads, int kv_heads, int head_dim,
-                            int64_t count, void *workspace) {
+QuantAttendParams params_of(int batch, int phases, int dtype, int q_heads, int kv_heads,
+                            int head_dim, int64_t count, void *workspace) {
   QuantAttendParams p{};
   p.batch = batch;
   p.count = count;
@@ -364,7 +369,9 @@ QuantAttendParams params_of(int batch, int phases, int q_heads, int kv_heads, in
   p.kv_heads = kv_heads;
   p.head_dim = head_dim;
   p.groups = q_heads / kv_heads;
-  p.splits = quant_splits(batch, q_heads, kv_heads, head_dim, count);
+  const QuantMmaGrid g = quant_mma_grid(dtype, q_heads, kv_heads, head_dim);
+  p.splits = quant_splits(g, batch, head_dim, count);
+  p.join = phases > 1 || p.splits > splits_without_join(g, head_dim);
   p.record = record_bytes(kv_heads, head_dim);
   p.scale_log2 = (float)(1.4426950408889634 / sqrt((double)head_dim));
   p.stats = static_cast<float4 *>(workspace);
@@ -375,18 +382,15 @@ QuantAttendParams params_of(int batch, int phases, int q_heads, int kv_heads, in
 }  // namespace
 }  // namespace hs
 
-extern "C" size_t hs_attend_quantized_workspace_bytes(int batch, int phases, int q_heads,
-                                                      int kv_heads, int head_dim,
+extern "C" size_t hs_attend_quantized_workspace_bytes(int batch, int phases, int dtype,
+                                                      int q_heads, int kv_heads, int head_dim,
                                                       int64_t count) {
   using namespace hs;
   if (batch < 1 || phases < 1 || kv_heads < 1 || q_heads < kv_heads || head_dim < 1 || count < 0)
     return 0;
-  const int splits = quant_splits(batch, q_heads, kv_heads, head_dim, count);
-  if (phases == 1 &&
-      splits <= splits_without_join(quant_mma_grid(q_heads, kv_heads, head_dim), head_dim))
-    return 0;
-  const int64_t parts = (int64_t)phases * batch * q_heads * splits;
-  return (size_t)parts * (sizeof(float4) + quant_pad(head_dim) * sizeof(float));
+  const QuantAttendParams p =
+      params_of(batch, phases, dtype, q_heads, kv_heads, head_dim, count, nullptr);
+  return workspace_of(p, phases);
 }
 
 extern "C" int hs_attend_quantized(int batch, const void *query, int64_t query_batch_stride,
@@ -406,8 +410,8 @@ extern "C" int hs_attend_quantized(int batch, const void *query, int64_t query_b
   if ((reinterpret_cast<uintptr_t>(pool) & 15) != 0)
     return set_error(HS_ERR_INVALID_ARGUMENT,
                      "attend_quantized: the pool must be 16-byte aligned");
-  QuantAttendParams p = params_of(batch, 1, q_heads, kv_heads, head_dim, count, workspace);
-  if (int e = place_workspace(p, 1, workspace, workspace_bytes)) return e;
+  QuantAttendParams p = params_of(batch, 1, dtype, q_heads, kv_heads, head_dim, count, workspace);
+  if (int e = check_workspace(p, 1, workspace, workspace_bytes)) return e;
   p.query = query;
   p.q_batch_stride = query_batch_stride;
   p.pool = static_cast<const unsigned char *>(pool);
@@ -419,7 +423,7 @@ extern "C" int hs_attend_quantized(int batch, const void *query, int64_t query_b
   p.page_size = page_size;
   p.page_shift = page_shift_of(page_size);
   p.status = device_status;
-  if (p.splits <= splits_without_join(quant_mma_grid(q_heads, kv_heads, head_dim), head_dim)) {
+  if (!p.join) {
     p.out = out;
     if (!on_tensor_cores(p, dtype)) p.splits = 1;
   }
@@ -449,8 +453,8 @@ extern "C" int hs_attend_quantized_phase(int batch, const void *query,
   if ((reinterpret_cast<uintptr_t>(pool) & 15) != 0)
     return set_error(HS_ERR_INVALID_ARGUMENT,
                      "attend_quantized: the pool must be 16-byte aligned");
-  QuantAttendParams p = params_of(batch, 2, q_heads, kv_heads, head_dim, count, workspace);
-  if (int e = place_workspace(p, 2, workspace, workspace_bytes)) return e;
+  QuantAttendParams p = params_of(batch, 2, dtype, q_heads, kv_heads, head_dim, count, workspace);
+  if (int e = check_workspace(p, 2, workspace, workspace_bytes)) return e;
   p.query = query;
   p.q_batch_stride = query_batch_stride;
   p.pool = static_cast<const unsigned char *>(pool);
@@ -478,7 +482,7 @@ extern "C" int hs_attend_quantized_merge(int batch, int phases, void *out, int d
     return set_error(HS_ERR_INVALID_ARGUMENT, "attend_quantized: invalid number of phases");
   if (batch == 0) return HS_OK;
   if (!out) return set_error(HS_ERR_INVALID_ARGUMENT, "attend_quantized: null pointer");
-  QuantAttendParams p = params_of(batch, 2, q_heads, kv_heads, head_dim, count, workspace);
-  if (int e = place_workspace(p, 2, workspace, workspace_bytes)) return e;
+  QuantAttendParams p = params_of(batch, 2, dtype, q_heads, kv_heads, head_dim, count, workspace);
+  if (int e = check_workspace(p, 2, workspace, workspace_bytes)) return e;
   return launch_merge(p, phases, out, dtype, false, static_cast<cudaStream_t>(stream));
 }

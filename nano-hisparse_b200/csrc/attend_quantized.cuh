@@ -27,6 +27,7 @@ struct QuantAttendParams {
   int q_heads, kv_heads, head_dim, page_size, page_shift;
   int groups;           // query heads of a KV head
   int splits, phase;
+  bool join;            // the splits' results go by way of the workspace
   float scale_log2;     // log2(e) / sqrt(head_dim): scores are kept in powers of two
   // [phases][batch][q_heads][splits]: the maximum's score and V exponent, the sum; and
   // [.. , quads of 4] outputs
@@ -80,7 +81,7 @@ struct QuantMmaGrid {
   int slices;                  // warps that share a head's rows
   int resident;                // blocks on an SM
 };
-QuantMmaGrid quant_mma_grid(int q_heads, int kv_heads, int head_dim);
+QuantMmaGrid quant_mma_grid(int dtype, int q_heads, int kv_heads, int head_dim);
 int launch_quant_mma(const QuantAttendParams &p, int dtype, cudaStream_t s);
 
 }  // namespace hs

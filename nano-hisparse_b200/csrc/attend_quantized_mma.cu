@@ -563,11 +563,12 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<T, kDim, kQuads>::reside
   const int d = threadIdx.x % kPairs * 2, first_query = threadIdx.x / kPairs;
   const int all = d < D ? sharing * kQueries : 0;
   const auto join_slices = [&](auto n) {
+    constexpr int kParts = decltype(n)::value;
     for (int i = first_query; i < all; i += kStep) {
       const int head = i / kQueries, g = i % kQueries;
       if (g >= queries) continue;
-      const Joined x = join<n()>(
-          n(), [&](int k) { return stats(k * head_places + head, 0)[g]; },
+      const Joined x = join<kParts>(
+          kParts, [&](int k) { return stats(k * head_places + head, 0)[g]; },
           [&](int k) {
             return *reinterpret_cast<const float2 *>(elements(k * head_places + head) +
                                                      g * kPitch + d);
@@ -604,16 +605,20 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<T, kDim, kQuads>::reside
   cluster_barrier();  // the others may still read this block's results
 }
 
+// Quads of a warp at most: what the registers hold
+template <typename T, int kDim>
+constexpr int kMostQuads = kDim == 64 || std::is_same<T, __nv_bfloat16>::value ? 4
+                           : std::is_same<T, __half>::value                    ? 2
+                                                                               : 256 / kDim;
+
 template <typename T, int kDim, int kQuads>
-int launch(const QuantAttendParams &p, cudaStream_t s) {
+int launch(const QuantAttendParams &p, const QuantMmaGrid &g, cudaStream_t s) {
   auto kernel = quant_mma_kernel<T, kDim, kQuads>;
   const size_t bytes = MmaShape<T, kDim, kQuads>::bytes;
   if (int e = reserve_smem(reinterpret_cast<const void *>(kernel), bytes, "attend_quantized"))
     return e;
-  const QuantMmaGrid g = quant_mma_grid(p.q_heads, p.kv_heads, p.head_dim);
-  const int chunks = (p.groups + 4 * kQuads - 1) / (4 * kQuads);
   cudaLaunchConfig_t config{};
-  config.gridDim = dim3((unsigned)p.splits, (unsigned)(g.groups * chunks), (unsigned)p.batch);
+  config.gridDim = dim3((unsigned)p.splits, (unsigned)(g.groups * g.chunks), (unsigned)p.batch);
   config.blockDim = dim3(kMmaThreads);
   config.dynamicSmemBytes = bytes;
   config.stream = s;
@@ -628,42 +633,57 @@ int launch(const QuantAttendParams &p, cudaStream_t s) {
   cudaLaunchKernelEx(&config, kernel, p, g.heads, g.places, cluster);
   return check_launch("quant_mma_kernel");
 }
-// Quads of a warp: as many as the query heads need and the registers hold.
-template <typename T, int kDim, int kMost>
-int launch_quads(const QuantAttendParams &p, cudaStream_t s) {
-  if constexpr (kMost >= 4)
-    if (p.groups > 8) return launch<T, kDim, 4>(p, s);
-  if constexpr (kMost >= 2)
-    if (p.groups > 4) return launch<T, kDim, 2>(p, s);
-  return launch<T, kDim, 1>(p, s);
+// Calls f with kDim and kQuads for a KV head's `per` query heads.
+template <typename T, int kDim, typename F> auto with_quads(int per, F f) {
+  constexpr int most = kMostQuads<T, kDim>;
+  if constexpr (most >= 4)
+    if (per > 8) return f(std::integral_constant<int, kDim>(), std::integral_constant<int, 4>());
+  if constexpr (most >= 2)
+    if (per > 4) return f(std::integral_constant<int, kDim>(), std::integral_constant<int, 2>());
+  return f(std::integral_constant<int, kDim>(), std::integral_constant<int, 1>());
 }
-template <typename T, int kWide> int launch(const QuantAttendParams &p, cudaStream_t s) {
-  if (p.head_dim <= 64) return launch_quads<T, 64, 4>(p, s);
-  if (p.head_dim <= 128) return launch_quads<T, 128, kWide>(p, s);
-  return launch_quads<T, 256, kWide / 2>(p, s);
+template <typename T, typename F> auto with_shape(int per, int head_dim, F f) {
+  if (head_dim <= 64) return with_quads<T, 64>(per, f);
+  if (head_dim <= 128) return with_quads<T, 128>(per, f);
+  return with_quads<T, 256>(per, f);
 }
-
-}  // namespace
-
-QuantMmaGrid quant_mma_grid(int q_heads, int kv_heads, int head_dim) {
-  QuantMmaGrid g;
-  const int per = q_heads / kv_heads;
-  const int queries = per <= 4 ? 4 : per <= 8 ? 8 : head_dim <= 128 ? 16 : 8;
-  g.chunks = (per + queries - 1) / queries;
+template <typename T> QuantMmaGrid grid_of(int per, int kv_heads, int head_dim) {
+  QuantMmaGrid g = with_shape<T>(per, head_dim, [](auto dim, auto quads) {
+    QuantMmaGrid shape{};
+    shape.queries = 4 * quads();
+    shape.resident = MmaShape<T, dim(), quads()>::resident;
+    return shape;
+  });
+  g.chunks = (per + g.queries - 1) / g.queries;
   g.groups = (kv_heads + kMmaWarps - 1) / kMmaWarps;
   g.heads = (kv_heads + g.groups - 1) / g.groups;
   g.groups = (kv_heads + g.heads - 1) / g.heads;
   for (g.places = 1; g.places < g.heads; g.places <<= 1) {}
-  g.resident = head_dim <= 128 && queries <= 8 ? 2 : 1;
   g.slices = kMmaWarps / g.places;
   return g;
+}
+template <typename T> int launch(const QuantAttendParams &p, cudaStream_t s) {
+  return with_shape<T>(p.groups, p.head_dim, [&](auto dim, auto quads) {
+    return launch<T, dim(), quads()>(p, grid_of<T>(p.groups, p.kv_heads, p.head_dim), s);
+  });
+}
+
+}  // namespace
+
+QuantMmaGrid quant_mma_grid(int dtype, int q_heads, int kv_heads, int head_dim) {
+  const int per = q_heads / kv_heads;
+  switch (dtype) {
+    case HS_FLOAT32: return grid_of<float>(per, kv_heads, head_dim);
+    case HS_FLOAT16: return grid_of<__half>(per, kv_heads, head_dim);
+    default: return grid_of<__nv_bfloat16>(per, kv_heads, head_dim);
+  }
 }
 
 int launch_quant_mma(const QuantAttendParams &p, int dtype, cudaStream_t s) {
   switch (dtype) {
-    case HS_FLOAT32: return launch<float, 2>(p, s);
-    case HS_FLOAT16: return launch<__half, 2>(p, s);
-    default: return launch<__nv_bfloat16, 4>(p, s);
+    case HS_FLOAT32: return launch<float>(p, s);
+    case HS_FLOAT16: return launch<__half>(p, s);
+    default: return launch<__nv_bfloat16>(p, s);
   }
 }
 

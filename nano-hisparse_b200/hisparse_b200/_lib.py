@@ -85,7 +85,7 @@ _QUANTIZED_SIGNATURES = {
     "hs_append_quantized": ([_INT, _I64, _P, _P, _I64, _INT, _P, _P, _P, _P, _I64, _P, _P, _I64, _P, _P,
                              _P, _INT, _INT, _INT, _P, _P], _INT),
     "hs_read_quantized": ([_P, _I64, _P, _I64, _P, _INT, _INT, _INT, _INT, _P, _P], _INT),
-    "hs_attend_quantized_workspace_bytes": ([_INT, _INT, _INT, _INT, _INT, _I64], _SZ),
+    "hs_attend_quantized_workspace_bytes": ([_INT, _INT, _INT, _INT, _INT, _INT, _I64], _SZ),
     "hs_attend_quantized": ([_INT, _P, _I64, _INT, _P, _I64, _P, _I64, _I64, _I64, _P, _P, _INT,
                              _INT, _INT, _INT, _P, _SZ, _P, _P], _INT),
     "hs_attend_quantized_phase": ([_INT, _P, _I64, _INT, _P, _I64, _P, _I64, _I64, _P, _INT, _INT,

@@ -110,8 +110,9 @@ class DecodeBatch:
         self.resolve_ws_bytes = lib.hs_resolve_workspace_bytes(b, self.width, self.hot_rows)
         self.resolve_ws = _lib.workspace(self.resolve_ws_bytes, dev)
         if held_in_8_bits(cfg):
-            self.attend_ws_bytes = lib.hs_attend_quantized_workspace_bytes(
-                b, 2, q_heads, cfg.kv_heads, cfg.head_dim, self.width)
+            self.attend_ws_bytes = max(lib.hs_attend_quantized_workspace_bytes(
+                b, 2, code, q_heads, cfg.kv_heads, cfg.head_dim, self.width)
+                for code in (_lib.HS_FLOAT32, _lib.HS_FLOAT16, _lib.HS_BFLOAT16))
         else:
             self.attend_ws_bytes = lib.hs_attend_workspace_bytes(b, q_heads, cfg.kv_heads,
                                                                  cfg.head_dim, self.width)

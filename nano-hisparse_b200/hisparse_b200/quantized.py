@@ -175,7 +175,8 @@ def attend_quantized(query, pool, rows, config, counts=None):
     out = torch.empty_like(query, memory_format=torch.contiguous_format)
     lib = _lib.load()
     with _lib.on_device(index):
-        nbytes = lib.hs_attend_quantized_workspace_bytes(batch, 1, q_heads, kv_heads, dim, count)
+        nbytes = lib.hs_attend_quantized_workspace_bytes(batch, 1, code, q_heads, kv_heads, dim,
+                                                         count)
         ws = query.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
         status = lib.hs_attend_quantized(
             batch, query.data_ptr(), q_batch, code, pool.data_ptr(), blocks, rows.data_ptr(),

@@ -79,7 +79,7 @@ def test_host_side_validation_needs_no_device():
     assert attend(q_heads=5) == attend(count=-1) == attend(dtype=9) == attend(pool=None) == bad
     assert attend(pool=24) == bad
     assert attend(dim=257) == attend(batch=65536) == unsupported
-    assert lib.hs_attend_quantized_workspace_bytes(1, 1, 4, 2, 32, 4096) > 0
+    assert lib.hs_attend_quantized_workspace_bytes(1, 1, _lib.HS_FLOAT32, 4, 2, 32, 4096) > 0
     assert attend(ws=None) == attend(nbytes=8) == attend(ws=8) == workspace
 
     def phase(phase=0, counts_n=1, nbytes=1 << 30):
@@ -92,8 +92,9 @@ def test_host_side_validation_needs_no_device():
     assert lib.hs_attend_quantized_merge(1, 3, 16, 0, 4, 2, 32, 64, 16, 1 << 30, None) == bad
     assert lib.hs_attend_quantized_merge(1, 2, None, 0, 4, 2, 32, 64, 16, 1 << 30, None) == bad
     assert lib.hs_attend_quantized_merge(1, 2, 16, 0, 4, 2, 32, 64, 16, 8, None) == workspace
-    assert lib.hs_attend_quantized_workspace_bytes(2, 2, 4, 2, 32, 4096) >= \
-        2 * lib.hs_attend_quantized_workspace_bytes(2, 1, 4, 2, 32, 4096) > 0
+    sizes = _lib.HS_FLOAT32, 4, 2, 32, 4096
+    assert lib.hs_attend_quantized_workspace_bytes(2, 2, *sizes) >= \
+        2 * lib.hs_attend_quantized_workspace_bytes(2, 1, *sizes) > 0
 
 
 def test_operators_refuse_cpu_tensors():
