@@ -2,14 +2,21 @@
 //
 // append: one block serves a chunk's K or V of up to 8 KV heads. A head's row is spread
 // over kLanes lanes, 8 elements a lane, so that a warp has 32 / kLanes rows of a head at
-// once and kBatch such groups of rows in flight: the reads are what bounds it, as long as
-// enough of them are on their way. The largest elements meet in shuffles, the exponent
+// once and kBatch such groups of rows in flight. The largest elements meet in shuffles, the exponent
 // follows from their bits, the codes leave as 8 bytes a lane. The scales' bytes of a row
 // meet in shared memory and are written together with the padding: a byte at a time they
 // would be separate transfers over the host link. Bounds and mean come from the values
 // held, so that they do not depend on how the rows were split over calls; the page's
 // earlier rows are read back for the mean. Where a chunk may have many rows, several
 // warps (slices) share a head.
+//
+// A prompt (2,048 pages of 16 rows, 8 heads of 128, bf16: 227 MB) takes 60 us, 58 % of a
+// copy's rate. Its instructions bound it, about 170 for two rows of a head (issue slots
+// busy 70 %, the integer pipe 56 %): unpacking, the largest element, the codes and, for K,
+// their values and bounds. With one row in flight it took 142, four rows 112; bounds in
+// pairs of bf16 halve their instructions and leave registers for four blocks an SM. A decode
+// step (a row of each of 16 requests) takes 5 us with its launch: page, row and bounds are
+// read side by side, so that one wait for memory is left.
 #include "quantized.cuh"
 
 namespace hs {

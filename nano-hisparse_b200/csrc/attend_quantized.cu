@@ -18,8 +18,10 @@ constexpr int kSimtWarps = kSimtThreads / 32;
 constexpr int kSimtHeads = 8;    // query heads of a block
 constexpr int kSimtAhead = 4;    // rows of a warp in flight
 
-// CUDA cores, every type and shape. A warp takes four rows at a time, a lane C
-// neighbouring elements of each.
+// CUDA cores, every type and shape: rows of their own for each query head, head_dims that
+// are no multiple of 16. A warp takes four rows at a time, a lane C neighbouring elements of
+// each. Its reads by the byte and a shuffle tree for each score bound it: 16 requests of
+// 2,048 rows, 32/8 heads of 128, take 213 us, 18 on tensor cores.
 template <typename T, int C>
 __global__ void __launch_bounds__(kSimtThreads) quant_simt_kernel(QuantAttendParams p) {
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
@@ -142,7 +144,8 @@ constexpr int kJoinThreads = 256, kJoinAhead = 4;
 // One block a query head. A thread reads the statistics of one partial result (at most two
 // phases of kQuantMaxSplits), whose weights meet in shared memory; then kLanes threads
 // have four elements each, and kJoinThreads / kLanes groups of them a share of the
-// results, kJoinAhead loads in flight.
+// results, kJoinAhead loads in flight. Its launch overlaps the end of the kernel before it;
+// latencies bound what is left, 2.5 to 5 us for 9 to 128 splits.
 template <typename T, int kLanes>
 __global__ void __launch_bounds__(kJoinThreads) quant_merge_kernel(QuantAttendParams p, int phases,
                                                                    T *out) {

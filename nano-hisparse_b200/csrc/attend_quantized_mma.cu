@@ -25,6 +25,15 @@
 //                   a step of a weight (2^-11) is an eighth of such a result's rounding.
 // A weight is kept times 2^7 of the current maximum's, which is raised only when one would
 // pass it by more than 2^8.
+//
+// 16 requests of 32,768 rows, 32/8 heads of 128, bf16 (959 MB) take 167 us: 5.7 TB/s, 88 % of
+// a copy's rate. Rows in runs reach 5.8, single rows in any order 5.5. What else was measured
+// of that call: scores in fp16, codes converted, 213; scales copied by each warp for itself
+// 197, since 32 of its 96 requests a tile were for one byte; whole records copied by one
+// warp of the block 208, by all warps 208; boxes of tiled copies 185 (75 clocks of the copy
+// engine a box); fragments straight from global memory 250. With 7 query heads a KV head the
+// warps' instructions are level with the reads (8 requests of 16,384 rows, 4 KV heads: 35 us,
+// floor 20.7; issue slots busy 54 %), with more of them ahead.
 #include <type_traits>
 
 #include "attend_quantized.cuh"

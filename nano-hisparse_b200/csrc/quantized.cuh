@@ -56,12 +56,7 @@ __device__ __forceinline__ float decode1(unsigned char code) {
   return decode4_f32((uint32_t)code).x;
 }
 
-__device__ __forceinline__ float min_nan(float a, float b) {  // NaN if one is
-  float r;
-  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float max_nan(float a, float b) {
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if one is
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;

@@ -97,6 +97,11 @@ def attend_tolerance(out, spread, size, dim, rows, dtype):
     power by 2^-21; sums of `rows` weights by that many steps (tensor cores may cut
     instead of rounding: whole steps). 16-bit queries: weights are rounded to fp16 for the
     second product, by half a step or, near zero, by 2^-25 of the largest (2^8 at most).
+    fp32 queries: a weight is two fp16 numbers, whose rounding is part of the 2^-20 but for
+    their smallest step, 2^-24, so half of that, 2^-25. The largest weight is kept at 2^7 or
+    more, so this is 2^-32 of it; with codes up to 448 in the other rows and at least 224
+    in its own row's largest element, each row adds at most 2^-32 * 448 / 224 = 2^-31 of the
+    largest element's sum of |v| to any element, one with a far smaller sum among them.
     The result's own rounding is half a step of its type, and half the distance of its
     subnormal numbers (finfo's smallest normal times eps) where it is below the normal ones."""
     info = torch.finfo(dtype)
@@ -104,7 +109,9 @@ def attend_tolerance(out, spread, size, dim, rows, dtype):
     share = 2 * (dim + 4) * step * size + 2.0 ** -20 + (rows + 8) * step
     if dtype != torch.float32:
         share = share + 2.0 ** -11
-    near_zero = 0.0 if dtype == torch.float32 else 2.0 ** -25 * 2.0 ** 8 * rows
-    absolute = near_zero * np.abs(spread).max(initial=0.0) + 2.0 ** -126
+    if dtype == torch.float32:
+        absolute = 2.0 ** -31 * rows * spread.max(axis=-1, keepdims=True) + 2.0 ** -126
+    else:
+        absolute = 2.0 ** -25 * 2.0 ** 8 * rows * np.abs(spread).max(initial=0.0) + 2.0 ** -126
     absolute += info.smallest_normal * info.eps / 2
     return share * spread + absolute + info.eps / 2 * (np.abs(out) + share * spread)

@@ -346,6 +346,31 @@ def test_attend(dtype, batch, q_heads, heads, dim, page, count):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("batch,q_heads,heads,dim,count", [
+    # 8, 4, 2 and 1 warps to a head; joined by a second kernel, in a cluster, or not at all
+    (2, 7, 1, 128, 1000), (1, 12, 1, 256, 2000), (1, 5, 1, 64, 100), (160, 12, 1, 256, 100),
+    (3, 14, 2, 128, 400), (60, 6, 2, 96, 900), (80, 24, 2, 256, 300),
+    (2, 28, 4, 128, 300), (53, 28, 4, 128, 700), (1, 28, 4, 128, 2500), (160, 4, 4, 64, 250),
+    (2, 16, 8, 64, 500), (1, 32, 16, 80, 3000), (150, 8, 8, 32, 260)])
+def test_attend_joins(dtype, batch, q_heads, heads, dim, count):
+    """Requests share a pool; one of them has a few rows only, so that most of the parts
+    that are joined saw nothing."""
+    config = make_config(70, 16, heads, dim)
+    pool = make_pool(config, seed=dim + heads)
+    rows = np.random.default_rng(41).integers(0, 70 * 16, (batch, count))
+    rows[0, 3:] = -1
+    query = normal(batch, q_heads, dim, seed=42, dtype=dtype)
+    some = sorted({0, batch // 3, batch - 1})  # compared
+    for counts in (None, [count - i % 45 for i in range(batch - 1)] + [33]):
+        got = attend_quantized(query.to(DEV), torch.from_numpy(pool).to(DEV),
+                               torch.from_numpy(rows).to(DEV), config,
+                               counts=None if counts is None else ints(counts))
+        check_attend(query[some], pool, rows[some], config,
+                     None if counts is None else [counts[i] for i in some],
+                     run=lambda *_, **__: got[some])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_attend_nothing_to_see(dtype):
     config = make_config(4, 16, 2, 64)
     pool = make_pool(config, seed=31)
