@@ -10,13 +10,13 @@
 // earlier rows are read back for the mean. Where a chunk may have many rows, several
 // warps (slices) share a head.
 //
-// A prompt (2,048 pages of 16 rows, 8 heads of 128, bf16: 227 MB) takes 60 us, 58 % of a
+// A prompt (2,048 pages of 16 rows, 8 heads of 128, bf16: 227 MB) takes 61 us, 57 % of a
 // copy's rate. Its instructions bound it, about 170 for two rows of a head (issue slots
 // busy 70 %, the integer pipe 56 %): unpacking, the largest element, the codes and, for K,
 // their values and bounds. With one row in flight it took 142, four rows 112; bounds in
-// pairs of bf16 halve their instructions and leave registers for four blocks an SM. A decode
-// step (a row of each of 16 requests) takes 5 us with its launch: page, row and bounds are
-// read side by side, so that one wait for memory is left.
+// pairs of bf16 halve their instructions and leave registers for four blocks an SM (three: 70;
+// five with half the rows in flight: 63). A decode step (a row of each of 16 requests) takes
+// 4.2 us with its launch: row and bounds are read side by side, behind one wait for the page.
 #include "quantized.cuh"
 
 namespace hs {
@@ -42,18 +42,17 @@ struct QuantAppendParams {
   int32_t *status;
 };
 
-// This lane's 8 elements of a row as they are in memory
+// This lane's 8 elements of a row as they are in memory, the first n
 template <typename T> struct Raw {
   uint4 words[sizeof(T) / 2];
   template <bool kWide> __device__ __forceinline__ void load(const T *from, int n) {
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) words[i] = make_uint4(0, 0, 0, 0);
     if constexpr (kWide) {
-      if (n > 0)
 #pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; ++i)
-          words[i] = __ldg(reinterpret_cast<const uint4 *>(from) + i);
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+        words[i] = __ldg(reinterpret_cast<const uint4 *>(from) + i);
     } else {
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) words[i] = make_uint4(0, 0, 0, 0);
       T *x = reinterpret_cast<T *>(words);
 #pragma unroll
       for (int i = 0; i < 8; ++i)
@@ -138,12 +137,15 @@ __global__ void __launch_bounds__(32 * kAppendWarps, sizeof(T) == 2 ? 4 : 2)
   const T *from = static_cast<const T *>(plane ? p.v : p.k) + (int64_t)b * p.kv_batch_stride + at;
 
   Raw<T> raw[kBatch];
-  const int64_t from_step = (int64_t)step * E, to_step = (int64_t)step * p.record;
-  const T *load_at = from + (int64_t)first * E;  // of the next row to load
-  const auto load = [&](int r) {  // rows r, r + step, ..., below cnt
+  // Rows r, r + step, ... Nothing is read past the last row, nor by lanes and warps past the
+  // row's end and the last head: they read what others read and write nothing, and their
+  // row's largest element is the same.
+  const int row_size = (int)E, record_size = (int)p.record;
+  const T *load_from = kWide && n <= 0 ? from - (here ? d0 : at) : from;
+  const auto load = [&](int r) {
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u, load_at += from_step)
-      raw[u].template load<kWide>(load_at, r + u * step < cnt ? n : 0);
+    for (int u = 0; u < kBatch; ++u)
+      raw[u].template load<kWide>(load_from + (int64_t)min(r + u * step, cnt - 1) * row_size, n);
   };
   load(first);
   // the bounds so far, by the lanes that will write them
@@ -199,7 +201,7 @@ __global__ void __launch_bounds__(32 * kAppendWarps, sizeof(T) == 2 ? 4 : 2)
   const bool last_group = h0 + heads == p.kv_heads;
   const int own = last_group ? tail - h0 : heads;  // those that this block writes
   // where the next row goes
-  const int64_t place = (int64_t)(w + first) * p.record + at;
+  const int64_t place = (int64_t)w * p.record + at;
   unsigned char *pool_at = pool != nullptr ? pool + place : nullptr;
   unsigned char *host_at = host != nullptr ? host + place : nullptr;
   for (int r0 = 0; r0 < cnt; r0 += kTailRows) {
@@ -207,9 +209,9 @@ __global__ void __launch_bounds__(32 * kAppendWarps, sizeof(T) == 2 ? 4 : 2)
     for (int i0 = 0; i0 < rows; i0 += kBatch * step) {
       if (r0 + i0 > 0) load(r0 + i0 + first);
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u, pool_at += to_step, host_at += to_step) {
-        if (i0 + u * step >= rows) continue;  // the same for the whole block
-        const int r = i0 + u * step + first;
+      for (int u = 0; u < kBatch; ++u) {
+        if (i0 + u * step >= rows) break;  // the same for the whole block
+        const int r = i0 + u * step + first;  // of the tile
         float2 x[4];
         float largest = 0.f;
 #pragma unroll
@@ -240,8 +242,9 @@ __global__ void __launch_bounds__(32 * kAppendWarps, sizeof(T) == 2 ? 4 : 2)
         const uint2 codes = make_uint2(encode4(x[0].x, x[0].y, x[1].x, x[1].y),
                                        encode4(x[2].x, x[2].y, x[3].x, x[3].y));
         if (r >= rows || !here) continue;
-        if (pool != nullptr) store8<kWide>(pool_at, n, codes);
-        if (host != nullptr) store8<kWide>(host_at, n, codes);
+        const int64_t to = (int64_t)(r0 + r) * record_size;
+        if (pool != nullptr) store8<kWide>(pool_at + to, n, codes);
+        if (host != nullptr) store8<kWide>(host_at + to, n, codes);
         if (lane % kLanes == 0) scales[r][head] = (unsigned char)(e + 127);
         if (metadata) {
           decode8(codes, power_of_two(e), x);
@@ -495,6 +498,8 @@ extern "C" int hs_append_quantized(int batch, int64_t tokens, const void *k, con
   if (head_dim > kQuantMaxDim)
     return set_error(HS_ERR_UNSUPPORTED, "append: head_dim %d > %d is not supported", head_dim,
                      kQuantMaxDim);
+  if ((int64_t)kv_heads * head_dim > (1 << 24))
+    return set_error(HS_ERR_UNSUPPORTED, "append: heads too many");
   if (batch == 0 || tokens == 0) return HS_OK;
   if (!k || !v || !within || !count || !pool_block || !pool ||
       !minimum_ptrs != !maximum_ptrs || !minimum_ptrs != !summary_ptrs)

@@ -61,7 +61,7 @@ def test_host_side_validation_needs_no_device():
     # bounds without the mean
     assert lib.hs_append_quantized(1, 1, 16, 16, 64, 0, 16, 16, 16, 16, 4, 16, None, 0, 16, 16,
                                    None, 2, 32, 16, None, None) == bad
-    assert append(dim=257) == append(batch=65536) == unsupported
+    assert append(dim=257) == append(batch=65536) == append(heads=1 << 20) == unsupported
 
     def read(count=4, dtype=_lib.HS_FLOAT32, dim=32, pool=16):
         return lib.hs_read_quantized(pool, 4, 16, count, 16, dtype, 2, dim, 16, None, None)
