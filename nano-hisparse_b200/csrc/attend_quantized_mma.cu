@@ -442,8 +442,8 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<T, kDim, kQuads>::reside
         // byte - 127 as a float: the byte under 2^23's exponent
         v_exponent[r] = __uint_as_float(0x4b000000u | ev[r]) - (8388608.f + 127.f);
       }
-      float x[kQuads][2], y[kQuads][2];  // exponents of the weights in the sum and in the output
-      bool raise = false;
+      // exponents of the weights: x in the sum, y in the output, lifted
+      float x[kQuads][2], y[kQuads][2], lifted[kQuads][2], top_lifted = -INFINITY;
 #pragma unroll
       for (int n = 0; n < kQuads; ++n)
 #pragma unroll
@@ -454,9 +454,10 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<T, kDim, kQuads>::reside
             dot = fmaf(dot, 1.f / 256.f, fmaf(s[n][t][2 * r + 1], 1.f / 16.f, s[n][t][2 * r]));
           x[n][r] = fmaf(dot, k_scale[r] * factor[n], hidden[r]);
           y[n][r] = x[n][r] + v_exponent[r];
-          raise = raise || y[n][r] + base[n] > kRaise;
+          lifted[n][r] = y[n][r] + base[n];
+          top_lifted = fmaxf(top_lifted, lifted[n][r]);
         }
-      if (__any_sync(kFullMask, raise)) {
+      if (__any_sync(kFullMask, top_lifted > kRaise)) {
         float f[kQuads];
 #pragma unroll
         for (int n = 0; n < kQuads; ++n) {
@@ -468,6 +469,8 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<T, kDim, kQuads>::reside
           f[n] = quant_exp2(to_base - base[n]);
           base[n] = to_base;
           l[n] *= f[n];
+#pragma unroll
+          for (int r = 0; r < 2; ++r) lifted[n][r] = y[n][r] + to_base;
         }
 #pragma unroll
         for (int n = 0; n < kOutputTiles; ++n)
@@ -481,7 +484,7 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<T, kDim, kQuads>::reside
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           l[n] += quant_exp2(x[n][r] + base[n]);
-          y[n][r] = quant_exp2(y[n][r] + base[n]);
+          y[n][r] = quant_exp2(lifted[n][r]);
         }
       uint32_t w[kOutputTiles][2];
 #pragma unroll
@@ -499,7 +502,7 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<T, kDim, kQuads>::reside
 #pragma unroll
       for (int c = 0; c < kChunks; c += 2) {
         uint32_t v[4];
-        ldmatrix4_trans(v, tile_chunk<kDim>(tile + Shape::plane, c));
+        ldmatrix4_trans(v, tile_chunk<kDim>(tile, c) + Shape::plane);
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const uint2 lo = decode4(__byte_perm(v[2 * u], 0, 0x3120));
