@@ -76,12 +76,21 @@ __global__ void __launch_bounds__(kGatherThreads, 16) gather_kernel(GatherParams
         const V *v_src = reinterpret_cast<const V *>(src + plane_stride);
         V *k_dst = reinterpret_cast<V *>(dst);
         V *v_dst = reinterpret_cast<V *>(dst + plane_stride);
-        for (int c_ = lane; c_ < vecs; c_ += 32 * kUnroll) {
+        // The vectors of a row that begins inside a line of 128 bytes are counted from the
+        // line's start, so that no line is asked for twice (rows of 1,056 bytes: 46.3 GB/s,
+        // 44.8 counted from the row's). V's row begins at the same place of a line where a
+        // plane is whole lines, as those of pages of 4, 8, ... records of an 8-bit cache are.
+        const int skew = (int)(reinterpret_cast<uintptr_t>(src) % 128 / sizeof(V));
+        k_src -= skew;
+        k_dst -= skew;
+        v_src -= skew;
+        v_dst -= skew;
+        for (int c_ = lane; c_ < vecs + skew; c_ += 32 * kUnroll) {
           V kv[kUnroll], vv[kUnroll];
 #pragma unroll
           for (int u = 0; u < kUnroll; ++u) {
             const int c = c_ + 32 * u;
-            if (c < vecs) {
+            if ((unsigned)(c - skew) < (unsigned)vecs) {
               kv[u] = __ldcs(k_src + c);  // host rows are read once: stream past the caches
               vv[u] = __ldcs(v_src + c);
             }
@@ -89,7 +98,7 @@ __global__ void __launch_bounds__(kGatherThreads, 16) gather_kernel(GatherParams
 #pragma unroll
           for (int u = 0; u < kUnroll; ++u) {
             const int c = c_ + 32 * u;
-            if (c < vecs) {
+            if ((unsigned)(c - skew) < (unsigned)vecs) {
               k_dst[c] = kv[u];
               v_dst[c] = vv[u];
             }

@@ -9,8 +9,9 @@ import torch
 
 import quantized_reference as ref
 from hisparse_b200 import (CacheConfig, MappedHost, _lib, append_quantized, attend_quantized,
-                           attend_rows, read_quantized)
+                           attend_rows, gather_rows, read_quantized)
 from hisparse_b200.append import append_chunks, append_page
+from hisparse_b200.row_index import RowPlan
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -304,6 +305,26 @@ def test_read_shapes_bad_rows_and_nan():
     assert "beyond the pool" in _lib.device_flags(DEV)[0]
     strided = read_quantized(torch.from_numpy(pool).to(DEV), rows.flatten()[::2], config)
     assert torch.equal(strided[0, 0].nan_to_num(9.0), got[0, 0, 0, 0].nan_to_num(9.0))
+
+
+@pytest.mark.parametrize("heads,dim,page", [(1, 33, 3), (2, 32, 16), (8, 128, 16), (16, 256, 5),
+                                            (3, 80, 12)])
+def test_gather_of_records(heads, dim, page):
+    """Records begin anywhere in a line of 128 bytes, K's and V's not always at the same
+    place; those that are not asked for stay as they are."""
+    config = make_config(6, page, heads, dim)
+    rng = np.random.default_rng(81)
+    host = torch.from_numpy(rng.integers(0, 256, (9, *config.page_shape), dtype=np.uint8))
+    pool0 = rng.integers(0, 256, (6, *config.page_shape), dtype=np.uint8)
+    n = min(13, 2 * page)
+    source, target = rng.permutation(9 * page)[:n], rng.permutation(6 * page)[:n]
+    plan = [torch.from_numpy(np.append(x, [-1, -1])).to(DEV) for x in (source, target)]
+    pool = torch.from_numpy(pool0).to(DEV)
+    mapped = MappedHost(host.pin_memory())
+    gather_rows(mapped, pool, RowPlan(None, *plan, None), config)
+    for a, b in zip(source, target):
+        pool0[b // page, :, b % page] = host[a // page, :, a % page]
+    assert np.array_equal(pool.cpu().numpy(), pool0)
 
 
 # ---- attention ----------------------------------------------------------------------------------
