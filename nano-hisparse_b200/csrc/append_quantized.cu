@@ -16,7 +16,7 @@
 // their values and bounds. With one row in flight it took 142, four rows 112; bounds in
 // pairs of bf16 halve their instructions and leave registers for four blocks an SM (three: 70;
 // five with half the rows in flight: 63). A decode step (a row of each of 16 requests) takes
-// 4.2 us with its launch: row and bounds are read side by side, behind one wait for the page.
+// 4.5 us with its launch: row and bounds are read side by side, behind one wait for the page.
 #include "quantized.cuh"
 
 namespace hs {
@@ -304,13 +304,13 @@ __global__ void __launch_bounds__(32 * kAppendWarps, sizeof(T) == 2 ? 4 : 2)
   }
   if (!writes) return;
   float *summary = reinterpret_cast<float *>(entries[2]) + at;
-  const float share = 1.f / (float)(w + cnt);  // two roundings instead of a division's one
+  const float page_rows = (float)(w + cnt);
   if (vectors) {
     *reinterpret_cast<uint4 *>(minimum) = *reinterpret_cast<const uint4 *>(low);
     *reinterpret_cast<uint4 *>(maximum) = *reinterpret_cast<const uint4 *>(high);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      reinterpret_cast<float2 *>(summary)[i] = make_float2(sum[i].x * share, sum[i].y * share);
+      reinterpret_cast<float2 *>(summary)[i] = make_float2(sum[i].x / page_rows, sum[i].y / page_rows);
     return;
   }
 #pragma unroll
@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(32 * kAppendWarps, sizeof(T) == 2 ? 4 : 2)
     if (i >= n) break;
     minimum[i] = reinterpret_cast<const __nv_bfloat16 *>(low)[i];
     maximum[i] = reinterpret_cast<const __nv_bfloat16 *>(high)[i];
-    summary[i] = (i % 2 ? sum[i / 2].y : sum[i / 2].x) * share;
+    summary[i] = (i % 2 ? sum[i / 2].y : sum[i / 2].x) / page_rows;
   }
 }
 
