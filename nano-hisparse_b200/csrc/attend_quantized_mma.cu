@@ -20,9 +20,13 @@
 //   O^T += V^T P^T  m16n8k16 in fp16, which holds every e4m3 number. V through
 //                   ldmatrix.trans, whose 16-bit unit is two neighbouring elements of a
 //                   row: a byte permutation makes pairs of rows of each. P is the weight
-//                   rounded to fp16 and, in the column beside it, what that left (22 bits
-//                   together). Two quads of bf16 queries share the columns instead: half
-//                   a step of a weight (2^-11) is an eighth of such a result's rounding.
+//                   rounded to fp16 and what that left (22 bits together), in the column
+//                   beside it or, where two quads of bf16 queries share the columns, in a
+//                   second product into the same sums: half the registers for the output,
+//                   as many products. (A single product, 11 bits, took 39.5 us where this
+//                   takes 40.7, 8 requests of 16,384 rows, 28/4 heads of 128, and 66.6 where
+//                   this takes 72.8, 16 of 18,348, 12 heads of 256; but one result in thirty
+//                   then differed from the weights' own by a step of bf16.)
 // A weight is kept times 2^7 of the current maximum's, which is raised only when one would
 // pass it by more than 2^8.
 //
@@ -32,8 +36,8 @@
 // 197, since 32 of its 96 requests a tile were for one byte; whole records copied by one
 // warp of the block 208, by all warps 208; boxes of tiled copies 185 (75 clocks of the copy
 // engine a box); fragments straight from global memory 250. With 7 query heads a KV head the
-// warps' instructions are level with the reads (8 requests of 16,384 rows, 4 KV heads: 35 us,
-// floor 20.7; issue slots busy 54 %), with more of them ahead.
+// warps' instructions are level with the reads (8 requests of 16,384 rows, 4 KV heads: 41 us,
+// floor 20.7), with more of them ahead.
 #include <type_traits>
 
 #include "attend_quantized.cuh"
@@ -486,13 +490,17 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<T, kDim, kQuads>::reside
           l[n] += quant_exp2(x[n][r] + base[n]);
           y[n][r] = quant_exp2(lifted[n][r]);
         }
-      uint32_t w[kOutputTiles][2];
+      uint32_t w[kOutputTiles][2], left[kOutputTiles][2];  // left: what rounding left, if paired
 #pragma unroll
       for (int n = 0; n < kOutputTiles; ++n)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           if constexpr (kPaired) {
-            w[n][r] = transpose8(pack_half(y[2 * n][r], y[2 * n + 1][r]));
+            const float even = y[2 * n][r], odd = y[2 * n + 1][r];
+            const __half2 rounded = __floats2half2_rn(even, odd);
+            w[n][r] = transpose8(*reinterpret_cast<const uint32_t *>(&rounded));
+            left[n][r] = transpose8(
+                pack_half(even - __low2float(rounded), odd - __high2float(rounded)));
           } else {
             const __half rounded = __float2half_rn(y[n][r]);
             w[n][r] = transpose8(pack_half(y[n][r], y[n][r] - __half2float(rounded)));
@@ -508,8 +516,10 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<T, kDim, kQuads>::reside
           const uint2 lo = decode4(__byte_perm(v[2 * u], 0, 0x3120));
           const uint2 hi = decode4(__byte_perm(v[2 * u + 1], 0, 0x3120));
 #pragma unroll
-          for (int n = 0; n < kOutputTiles; ++n)
+          for (int n = 0; n < kOutputTiles; ++n) {
             mma_f16(o[n][c + u], lo.x, lo.y, hi.x, hi.y, w[n][0], w[n][1]);
+            if constexpr (kPaired) mma_f16(o[n][c + u], lo.x, lo.y, hi.x, hi.y, left[n][0], left[n][1]);
+          }
         }
       }
     }

@@ -1,0 +1,74 @@
+"""attend_quantized within bounds that one missing row, or a weight in fewer bits, exceeds."""
+
+import numpy as np
+import pytest
+import torch
+
+import quantized_bounds as bounds
+from hisparse_b200 import CacheConfig, _lib, attend_quantized
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+# batch, query heads, KV heads, head_dim, rows: 8, 4, 2 and 1 warps to a head, one to four quads
+# of query heads, splits joined by a second kernel, in a cluster, or none
+FLAT = [(1, 28, 4, 128, 1200), (60, 28, 4, 128, 700), (3, 32, 8, 128, 300), (2, 16, 1, 128, 1000),
+        (2, 14, 1, 64, 1200), (150, 10, 2, 80, 260), (2, 12, 1, 256, 600), (1, 32, 16, 64, 900),
+        (2, 8, 8, 32, 500), (2, 6, 2, 33, 400)]
+CANCELLING = [(1, 28, 4, 128, 40), (1, 16, 2, 64, 64), (1, 16, 1, 128, 33), (1, 12, 1, 256, 50),
+              (1, 8, 2, 32, 24), (1, 32, 8, 128, 40)]
+
+
+def normal(*shape, seed, dtype):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).to(dtype)
+
+
+def flat(batch, q_heads, heads, dim, count, dtype):
+    """Scores of about 0.3: weights from a half to twice their mean."""
+    pool = bounds.pool_of(-(-count // 16) + 2, 16, heads, dim, seed=count + dim)
+    rng = np.random.default_rng(dim)
+    rows = np.stack([rng.permutation(len(pool) * 16)[:count] for _ in range(batch)])
+    return normal(batch, q_heads, dim, seed=1, dtype=dtype), pool, rows
+
+
+def cancelling(batch, q_heads, heads, dim, count, dtype):
+    """Scores of two products; results of one query head of each KV head nearly cancel."""
+    pool = bounds.pool_of(-(-count // 16) + 1, 16, heads, dim, seed=7 + count, key_size=1.5,
+                          key_elements=2)
+    query = normal(batch, q_heads, dim, seed=dim, dtype=dtype) * dim ** 0.5 / 4
+    rows = np.random.default_rng(count).permutation(len(pool) * 16)[:count]
+    some = bounds.cancel(query[0].double().numpy(), pool, rows, heads, q_heads // heads - 1)
+    return query, pool, rows[None], some
+
+
+def run(query, pool, rows, heads, counts=None):
+    config = CacheConfig(gpu_pages=len(pool), page_size=pool.shape[2], kv_heads=heads,
+                         head_dim=query.shape[-1], device=DEV, dtype=torch.float8_e4m3fn)
+    got = attend_quantized(query.to(DEV), torch.from_numpy(pool).to(DEV),
+                           torch.from_numpy(rows).to(DEV), config, counts)
+    assert got.dtype == query.dtype and not _lib.device_flags(DEV)
+    return got.double().cpu().numpy()
+
+
+def check(got, query, pool, rows, heads, dtype):
+    out, bound = bounds.attend(query.double().numpy(), pool, rows, heads, dtype)
+    error = np.abs(got - out)
+    assert np.all(error <= bound), (error / bound).max()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("case", FLAT)
+def test_every_row_counts(dtype, case):
+    query, pool, rows = flat(*case, dtype)
+    got = run(query, pool, rows, case[2])
+    some = sorted({0, case[0] // 2, case[0] - 1})
+    check(got[some], query[some], pool, rows[some], case[2], dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("case", CANCELLING)
+def test_small_differences(dtype, case):
+    query, pool, rows, some = cancelling(*case, dtype)
+    got = run(query, pool, rows, case[2])
+    check(got, query, pool, rows, case[2], dtype)
