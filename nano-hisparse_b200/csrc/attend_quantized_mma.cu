@@ -438,11 +438,10 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<T, kDim, kQuads>::reside
       // a row that is not seen has zeros in the place of its scale, which is never 0
       const unsigned ek[2] = {bytes[0], bytes[8 * width]};
       const unsigned ev[2] = {bytes[kUnitRows * width], bytes[(kUnitRows + 8) * width]};
-      float k_scale[2], hidden[2], v_exponent[2];
+      float k_scale[2], v_exponent[2];
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         k_scale[r] = scale_of(ek[r]);
-        hidden[r] = ek[r] != 0 ? 0.f : -INFINITY;
         // byte - 127 as a float: the byte under 2^23's exponent
         v_exponent[r] = __uint_as_float(0x4b000000u | ev[r]) - (8388608.f + 127.f);
       }
@@ -456,7 +455,8 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<T, kDim, kQuads>::reside
 #pragma unroll
           for (int t = kQueryTiles - 1; t >= 0; --t)
             dot = fmaf(dot, 1.f / 256.f, fmaf(s[n][t][2 * r + 1], 1.f / 16.f, s[n][t][2 * r]));
-          x[n][r] = fmaf(dot, k_scale[r] * factor[n], hidden[r]);
+          // chosen, not added: the product is NaN for a query that is not finite
+          x[n][r] = ek[r] != 0 ? dot * (k_scale[r] * factor[n]) : -INFINITY;
           y[n][r] = x[n][r] + v_exponent[r];
           lifted[n][r] = y[n][r] + base[n];
           top_lifted = fmaxf(top_lifted, lifted[n][r]);

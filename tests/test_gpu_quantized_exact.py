@@ -72,3 +72,32 @@ def test_small_differences(dtype, case):
     query, pool, rows, some = cancelling(*case, dtype)
     got = run(query, pool, rows, case[2])
     check(got, query, pool, rows, case[2], dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("q_heads,heads,dim", [(8, 2, 64), (28, 4, 128), (12, 1, 256), (6, 2, 33)])
+def test_nothing_seen_whatever_the_query(dtype, q_heads, heads, dim):
+    """Zeros where no row is seen (masked, beyond the pool, never written, behind the counts),
+    also for queries that are not finite; those are NaN where a row is seen."""
+    pool = bounds.pool_of(4, 16, heads, dim, seed=5)
+    pool[3] = 0
+    rows = np.stack([np.full(70, -1), np.arange(70) % 16 + 48, np.full(70, 64), np.arange(70) % 48,
+                     np.arange(70) % 48, np.full(70, -1)])
+    rows[4, 1:] = -1
+    query = normal(6, q_heads, dim, seed=6, dtype=dtype)
+    query[:5, 0, 0], query[:5, -1, -1], query[:5, 1] = np.inf, np.nan, -np.inf
+    config = CacheConfig(gpu_pages=4, page_size=16, kv_heads=heads, head_dim=dim, device=DEV,
+                         dtype=torch.float8_e4m3fn)
+    counts = torch.tensor([70, 70, 70, 0, 70, 70], dtype=torch.int32, device=DEV)
+    some = [0, 1, q_heads - 1]  # the heads that are not finite
+    for limit in (counts, None):
+        got = attend_quantized(query.to(DEV), torch.from_numpy(pool).to(DEV),
+                               torch.from_numpy(rows).to(DEV), config, limit)
+        assert torch.all(got[[0, 1, 2, 5]] == 0)
+        seen = got[4:5] if limit is not None else got[3:5]
+        assert torch.isnan(seen[:, some]).all()
+        others = [h for h in range(q_heads) if h not in some]
+        assert torch.isfinite(seen[:, others]).all()
+        if limit is not None:
+            assert torch.all(got[3] == 0)
+    assert "beyond the pool" in _lib.device_flags(DEV)[0]
