@@ -20,10 +20,14 @@
 //   O^T += V^T P^T  m16n8k16 in fp16, which holds every e4m3 number. V through
 //                   ldmatrix.trans, whose 16-bit unit is two neighbouring elements of a
 //                   row: a byte permutation makes pairs of rows of each. P is the weight
-//                   rounded to fp16 and what that left (22 bits together), in the column
-//                   beside it or, where two quads of bf16 queries share the columns, in a
+//                   rounded to fp16 and, in the column beside it, 2^11 times what that left:
+//                   22 bits together, and steps of 2^-35 where the first one's are of 2^-24
+//                   (2^-43 of the largest weight; unscaled, 2^-32, the weights of a long flat
+//                   tail behind one large row were all cut alike). Where two quads of bf16
+//                   queries share the columns, what was left goes, as it is, through a
 //                   second product into the same sums: half the registers for the output,
-//                   as many products. (A single product, 11 bits, took 39.5 us where this
+//                   as many products, 2^-32 of the largest weight a row where a result's
+//                   own rounding is 2^-8. (A single product, 11 bits, took 39.5 us where this
 //                   takes 40.7, 8 requests of 16,384 rows, 28/4 heads of 128, and 66.6 where
 //                   this takes 72.8, 16 of 18,348, 12 heads of 256; but one result in thirty
 //                   then differed from the weights' own by a step of bf16.)
@@ -55,6 +59,7 @@ constexpr int kAhead = 2;        // units that scales are copied ahead
 // one or two 16-byte chunks of a row that have the block's heads
 constexpr int kScaleRoom = 16 * 1024;  // of all rings of scales: 8 of words or 1 of two chunks
 constexpr float kWeightLift = 7.f, kRaise = 15.f;  // lifted weights stay below 2^kRaise
+constexpr float kLeftLift = 2048.f;                // of what a weight's rounding to fp16 left
 constexpr float kNothing = 1e38f;                  // base of a query that has seen nothing
 
 // parts of a query element
@@ -503,7 +508,8 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<T, kDim, kQuads>::reside
                 pack_half(even - __low2float(rounded), odd - __high2float(rounded)));
           } else {
             const __half rounded = __float2half_rn(y[n][r]);
-            w[n][r] = transpose8(pack_half(y[n][r], y[n][r] - __half2float(rounded)));
+            w[n][r] = transpose8(
+                pack_half(y[n][r], (y[n][r] - __half2float(rounded)) * kLeftLift));
           }
         }
       // ---- O^T: elements 16 c + 2 * (lane / 4) + 0, 1, columns 2 * (lane % 4) + 0, 1
@@ -547,7 +553,8 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<T, kDim, kQuads>::reside
   const auto result = [&](int n, int c) {
     const float(&x)[4] = o[kPaired ? n / 2 : n][c];
     const float2 sum = kPaired ? make_float2(x[n & 1], x[2 + (n & 1)])
-                               : make_float2(x[0] + x[1], x[2] + x[3]);
+                               : make_float2(fmaf(x[1], 1.f / kLeftLift, x[0]),
+                                             fmaf(x[3], 1.f / kLeftLift, x[2]));
     return make_float2(sum.x * (1.f / kSumScale), sum.y * (1.f / kSumScale));
   };
 #pragma unroll

@@ -16,9 +16,15 @@ STEP = 2.0 ** -23  # of fp32
 # leaves half a step, with the largest element at 2^7 or more and numbers below 2^-6 in steps
 # of 2^-9. Part j works on 16^(j-1) of the rest, so n parts leave 2^-10 / 16^(n-1) / 2^7.
 QUERY = {torch.bfloat16: 2.0 ** -21, torch.float16: 2.0 ** -25, torch.float32: 2.0 ** -37}
-# What a weight loses besides its share, of the largest: its second fp16 number has steps of
-# 2^-24, and the largest weight is kept at 2^7 or more.
-SMALLEST = 2.0 ** -32
+
+
+def smallest(dtype, group, dim):
+    """What a weight loses besides its share, of the largest, which is kept at 2^7 or more. Its
+    second fp16 number has steps of 2^-24, of which rounding loses half, and is kept times 2^11;
+    with two quads of bf16 queries to a KV head it is kept as it is. (Weights stay in fp32
+    where head_dim is no multiple of 16.)"""
+    together = dtype == torch.bfloat16 and group > 4 and dim % 16 == 0
+    return 2.0 ** -32 if together else 2.0 ** -43
 
 
 def pool_of(blocks, page, heads, dim, seed, key_size=0.3, key_elements=None):
@@ -43,7 +49,7 @@ def attend(query, pool, rows, heads, dtype, counts=None):
     share, in the numerator and in the sum (twice). The power itself, the factors of a moved
     maximum and of a join, the weight as two fp16 numbers: 2^-20 together. Sums of n rows: a
     step each. What is small against a weight's second number counts with the codes of its
-    row, up to 448 where the largest weight's row has at least 224: twice SMALLEST of the
+    row, up to 448 where the largest weight's row has at least 224: twice `smallest` of the
     largest element's sum of |v|. Then the result's own rounding."""
     b, hq, d = query.shape
     info = torch.finfo(dtype)
@@ -70,7 +76,7 @@ def attend(query, pool, rows, heads, dtype, counts=None):
             exponents = records[:, heads * d + kh].astype(int) - 127
             number = np.abs(s).max() * 1.4427 + np.abs(exponents).max() + 32
             share = 2 * score + 5 * STEP / 2 * number + 2.0 ** -20 + (len(at) + 8) * STEP
-            error = share * spread + 2 * SMALLEST * len(at) * spread.max() + 2.0 ** -126
+            error = share * spread + 2 * smallest(dtype, hq // heads, d) * len(at) * spread.max() + 2.0 ** -126
             bound[i, h] = error + info.eps / 2 * (np.abs(out[i, h]) + error) + \
                 info.smallest_normal * info.eps / 2
     return out, bound

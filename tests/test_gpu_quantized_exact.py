@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import quantized_bounds as bounds
+import quantized_reference as ref
 from hisparse_b200 import CacheConfig, _lib, attend_quantized
 
 pytestmark = pytest.mark.gpu
@@ -101,3 +102,21 @@ def test_nothing_seen_whatever_the_query(dtype, q_heads, heads, dim):
         if limit is not None:
             assert torch.all(got[3] == 0)
     assert "beyond the pool" in _lib.device_flags(DEV)[0]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("q_heads,heads,dim", [(8, 2, 64), (8, 2, 128), (28, 4, 128), (4, 1, 256),
+                                               (6, 2, 33)])
+def test_tail_behind_one_row(dtype, q_heads, heads, dim):
+    """Rows of one small weight behind a row that takes nearly all, which has no part in half of
+    the elements. The weights, 2^-24 of the largest, differ from head to head."""
+    rng = np.random.default_rng(dim)
+    x = np.zeros((3, 2, 16, heads, dim))
+    x[0, 0, 3, :, 0] = 1.0
+    x[:, 1] = 256 * rng.standard_normal((3, 16, heads, dim))
+    x[0, 1, 3, :, dim // 2:] = 0
+    pool, rows = ref.records(x), np.arange(32)[None]
+    query = torch.zeros(1, q_heads, dim)
+    query[0, :, 0] = (24 + torch.arange(q_heads) / q_heads) * np.log(2) * dim ** 0.5
+    query = query.to(dtype)
+    check(run(query, pool, rows, heads), query, pool, rows, heads, dtype)
