@@ -241,9 +241,11 @@ class DecodeBatch:
         over the physical rows and the nodes' own key/value, on the batch's compute
         stream. query [B, T, Hq, D], key/value [B, T, Hkv, D], mask int64 [B, T],
         nodes int32 [B] (see attend_tree); positions int32 [B, width], -1 padded
-        behind row_counts int32 [B] leading ones. Returns [B, T, Hq, D]. Rows held
-        in 8 bits are read back in the query's dtype first (``read_quantized``), and
-        the nodes' own are taken as they will be held."""
+        behind row_counts int32 [B] leading ones. Returns [B, T, Hq, D] of the query's
+        dtype. Rows held in 8 bits are read back first (``read_quantized``) into a
+        temporary of 2 * B * width * Hkv * D elements, and the nodes' own are taken as
+        they will be held: in the query's dtype, or in fp32, attention too, for fp16,
+        whose range a held value may leave (65,504 is held as 65,536)."""
         from .quantized import held_values, read_quantized
         from .tree import attend_tree
 
@@ -260,19 +262,23 @@ class DecodeBatch:
             compute.wait_event(st.ready)
         self._resolve_and_gather(layer, positions.data_ptr(), st.counts)
         compute.wait_event(st.ready)
-        pool, rows = self.cache.pool, self.physical
+        pool, rows, dtype = self.cache.pool, self.physical, query.dtype
         if held_in_8_bits(cfg):
+            if key.dtype != dtype or value.dtype != dtype:
+                raise ValueError("query, key and value must have one dtype")
+            held = torch.float32 if dtype == torch.float16 else dtype
             # one page of all rows, in the order of the requests; padding has none
             page = self.batch * self.width
             order = torch.arange(page, device=self.device).view(self.batch, self.width)
-            pool = read_quantized(pool, rows, cfg, query.dtype).view(
+            pool = read_quantized(pool, rows, cfg, held).view(
                 1, 2, page, cfg.kv_heads, cfg.head_dim)
             rows = torch.where(rows >= 0, order, rows)
-            key, value = held_values(key, value, cfg)
+            key, value = held_values(key, value, cfg, held)
+            query = query.to(held)
             cfg = CacheConfig(gpu_pages=1, page_size=page, kv_heads=cfg.kv_heads,
-                              head_dim=cfg.head_dim, device=cfg.device, dtype=query.dtype)
+                              head_dim=cfg.head_dim, device=cfg.device, dtype=held)
         out = attend_tree(query, key, value, mask, pool, rows, cfg, counts=row_counts,
-                          nodes=nodes)
+                          nodes=nodes).to(dtype)
         st.last_use = torch.cuda.Event()
         st.last_use.record(compute)
         return out

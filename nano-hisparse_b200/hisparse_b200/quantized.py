@@ -96,10 +96,11 @@ def append_quantized(k, v, within, count, pool_block, pool, minimum_ptrs, maximu
         _lib.check(status)
 
 
-def held_values(k, v, config):
-    """The values that K and V rows [B, T, Hkv, D] will be held as, in their own dtype:
-    [2, B, T, Hkv, D]. Drafted rows that are not appended yet are attended to as those,
-    so that a drafted turn computes what the plain turns after it will."""
+def held_values(k, v, config, dtype=None):
+    """The values that K and V rows [B, T, Hkv, D] will be held as, in `dtype` (theirs without):
+    [2, B, T, Hkv, D] (exact in bfloat16 and float32; those of float16 rows may leave its
+    range). Drafted rows that are not appended yet are attended to as those, so that a
+    drafted turn computes what the plain turns after it will."""
     batch, tokens = k.shape[:2]
     page = replace(config, gpu_pages=max(1, batch), page_size=max(1, tokens))
     pool = k.new_empty((batch, *page.page_shape), dtype=torch.uint8)
@@ -108,7 +109,7 @@ def held_values(k, v, config):
     append_quantized(k, v, within, torch.full_like(within, tokens), blocks, pool, None, None,
                      None, page)
     rows = torch.arange(batch * tokens, device=k.device).view(batch, tokens)
-    return read_quantized(pool, rows, page, k.dtype)
+    return read_quantized(pool, rows, page, k.dtype if dtype is None else dtype)
 
 
 def read_quantized(pool, rows, config, dtype=torch.bfloat16):
