@@ -258,14 +258,15 @@ class DecodeBatch:
                 or positions.device != self.device or not positions.is_contiguous()):
             raise ValueError("positions must be a contiguous int32 [batch, width] tensor "
                              "on the batch's device")
+        quantized, dtype = held_in_8_bits(cfg), query.dtype
+        if quantized and not dtype == key.dtype == value.dtype:
+            raise ValueError("query, key and value must have one dtype")
         if st.ready is not None:
             compute.wait_event(st.ready)
         self._resolve_and_gather(layer, positions.data_ptr(), st.counts)
         compute.wait_event(st.ready)
-        pool, rows, dtype = self.cache.pool, self.physical, query.dtype
-        if held_in_8_bits(cfg):
-            if key.dtype != dtype or value.dtype != dtype:
-                raise ValueError("query, key and value must have one dtype")
+        pool, rows = self.cache.pool, self.physical
+        if quantized:
             held = torch.float32 if dtype == torch.float16 else dtype
             # one page of all rows, in the order of the requests; padding has none
             page = self.batch * self.width
@@ -278,7 +279,9 @@ class DecodeBatch:
             cfg = CacheConfig(gpu_pages=1, page_size=page, kv_heads=cfg.kv_heads,
                               head_dim=cfg.head_dim, device=cfg.device, dtype=held)
         out = attend_tree(query, key, value, mask, pool, rows, cfg, counts=row_counts,
-                          nodes=nodes).to(dtype)
+                          nodes=nodes)
+        if quantized:
+            out = out.to(dtype)
         st.last_use = torch.cuda.Event()
         st.last_use.record(compute)
         return out
