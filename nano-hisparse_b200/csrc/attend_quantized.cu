@@ -21,12 +21,14 @@ constexpr int kSimtAhead = 4;    // rows of a warp in flight
 // CUDA cores, every type and shape: rows of their own for each query head, head_dims that
 // are no multiple of 16. A warp takes four rows at a time, a lane C neighbouring elements of
 // each. Its reads by the byte and a shuffle tree for each score bound it: 16 requests of
-// 2,048 rows, 32/8 heads of 128, take 213 us, 18 on tensor cores.
-template <typename T, int C>
+// 2,048 rows, 32/8 heads of 128, take 213 us, 18 on tensor cores. kCluster: a request's splits
+// are a cluster that joins them, without a workspace (simt_splits).
+template <typename T, int C, bool kCluster>
 __global__ void __launch_bounds__(kSimtThreads) quant_simt_kernel(QuantAttendParams p) {
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
   __shared__ float4 red[kSimtWarps][kSimtHeads];  // a maximum's score, exponent; the sum
   __shared__ float red_o[kSimtWarps][kSimtHeads][32 * C];
+  __shared__ float4 block_stats[kSimtHeads];  // of all warps
   const int split = blockIdx.x, b = blockIdx.z, D = p.head_dim;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, d0 = lane * C;
   int kh, h0, hn;
@@ -105,6 +107,10 @@ __global__ void __launch_bounds__(kSimtThreads) quant_simt_kernel(QuantAttendPar
       }
     }
   }
+  const auto write = [&](int g, int d, float x, float sum) {
+    const float y = sum > 0.f || sum != sum ? x / sum * kSumScale : 0.f;
+    static_cast<T *>(p.out)[((int64_t)b * p.q_heads + h0 + g) * D + d] = from_f32<T>(y);
+  };
   // the warps' results
 #pragma unroll
   for (int g = 0; g < kSimtHeads; ++g) {
@@ -127,15 +133,37 @@ __global__ void __launch_bounds__(kSimtThreads) quant_simt_kernel(QuantAttendPar
       sum = fmaf(part.z, f, sum);
       x = fmaf(red_o[w][g][d], f, x);
     }
-    if (p.out != nullptr) {
-      const float y = sum > 0.f || sum != sum ? x / sum * kSumScale : 0.f;
-      static_cast<T *>(p.out)[((int64_t)b * p.q_heads + h0 + g) * D + d] = from_f32<T>(y);
+    if constexpr (kCluster) {
+      if (d == 0) block_stats[g] = make_float4(top.x, top.y, sum, 0.f);
+      red_o[0][g][d] = x;  // read by this thread alone so far
+    } else if (p.out != nullptr) {
+      write(g, d, x, sum);
     } else {
       const int64_t part = quant_part(p, p.phase, b, h0 + g, split);
       if (d == 0) p.stats[part] = make_float4(top.x, top.y, sum, 0.f);
       p.partials[part * quant_pad(D) + d] = x;
     }
   }
+  if constexpr (!kCluster) return;
+  // the splits' results; every thread of the cluster comes to both barriers
+  cluster_barrier();
+  for (int i = split * kSimtThreads + threadIdx.x; i < hn * 32 * C;
+       i += p.splits * kSimtThreads) {
+    const int g = i / (32 * C), d = i % (32 * C);
+    if (d >= D) continue;
+    float4 top = *map_rank(&block_stats[g], 0);
+    float sum = 0.f, x = 0.f;
+    for (int k = 1; k < p.splits; ++k) top = quant_larger(top, *map_rank(&block_stats[g], k));
+    for (int k = 0; k < p.splits; ++k) {
+      const float4 part = *map_rank(&block_stats[g], k);
+      if (part.z == 0.f) continue;  // saw nothing
+      const float f = quant_share(part.x, part.y, top.x, top.y);
+      sum = fmaf(part.z, f, sum);
+      x = fmaf(*map_rank(&red_o[0][g][d], k), f, x);
+    }
+    write(g, d, x, sum);
+  }
+  cluster_barrier();  // the others may still read this block's results
 }
 
 // ---- the join of splits and phases ----------------------------------------------------------
@@ -219,7 +247,7 @@ __global__ void __launch_bounds__(kJoinThreads) quant_merge_kernel(QuantAttendPa
 // Splits that a call in one phase may have without a join and without a workspace: those of
 // a cluster, for the tensor-core kernel's head_dims and two blocks an SM (with one, clusters
 // leave SMs idle: 4 requests of 4,096 rows, one head of 256: 22.7 us as a cluster of 8, 17.1
-// with a join). A call that cannot take that kernel all the same has one split.
+// with a join). A call without a join that cannot take that kernel has simt_splits.
 int splits_without_join(const QuantMmaGrid &g, int head_dim) {
   return head_dim % 16 == 0 && g.resident == 2 ? kClusterSplits : 1;
 }
@@ -304,19 +332,46 @@ int check_workspace(const QuantAttendParams &p, int phases, void *workspace, siz
   return HS_OK;
 }
 
-template <typename T> int launch_rows(const QuantAttendParams &p, cudaStream_t s) {
+// Splits of a call on CUDA cores without a join, as a cluster: while one round of blocks
+// takes them all (registers leave an SM four blocks up to head_dim 64, three up to 128, two
+// above) and each has 16 rows. Of 32/8 heads of 128 with rows of their own, 200 rows: 1
+// request 8 splits 11 us, 1 split 42; 4 requests 2 splits 25, 1 split 42, 8 splits 32;
+// 64 requests 1 split 186, 4 splits 260.
+int simt_splits(const QuantAttendParams &p) {
   const int per = (p.groups + kSimtHeads - 1) / kSimtHeads;
-  const dim3 grid((unsigned)p.splits,
-                  (unsigned)(p.rows_head_stride == 0 ? p.kv_heads * per : p.q_heads),
-                  (unsigned)p.batch);
+  const int64_t blocks = (int64_t)p.batch *
+                         (p.rows_head_stride == 0 ? p.kv_heads * per : p.q_heads);
+  const int64_t places = (int64_t)sm_count() * (p.head_dim <= 64 ? 4 : p.head_dim <= 128 ? 3 : 2);
+  int n = kClusterSplits;
+  while (n > 1 && (blocks * n > places || (int64_t)n * 16 > p.count + 15)) n >>= 1;
+  return n;
+}
+template <typename T, bool kCluster> int launch_rows(const QuantAttendParams &p, cudaStream_t s) {
+  const int per = (p.groups + kSimtHeads - 1) / kSimtHeads;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3((unsigned)p.splits,
+                        (unsigned)(p.rows_head_stride == 0 ? p.kv_heads * per : p.q_heads),
+                        (unsigned)p.batch);
+  config.blockDim = dim3(kSimtThreads);
+  config.stream = s;
+  cudaLaunchAttribute attribute{};
+  attribute.id = cudaLaunchAttributeClusterDimension;
+  attribute.val.clusterDim.x = (unsigned)p.splits;
+  attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+  config.attrs = &attribute;
+  config.numAttrs = kCluster ? 1 : 0;
   switch (ceil_div(p.head_dim, 32)) {
-    case 1: quant_simt_kernel<T, 1><<<grid, kSimtThreads, 0, s>>>(p); break;
-    case 2: quant_simt_kernel<T, 2><<<grid, kSimtThreads, 0, s>>>(p); break;
+    case 1: cudaLaunchKernelEx(&config, quant_simt_kernel<T, 1, kCluster>, p); break;
+    case 2: cudaLaunchKernelEx(&config, quant_simt_kernel<T, 2, kCluster>, p); break;
     case 3:
-    case 4: quant_simt_kernel<T, 4><<<grid, kSimtThreads, 0, s>>>(p); break;
-    default: quant_simt_kernel<T, 8><<<grid, kSimtThreads, 0, s>>>(p); break;
+    case 4: cudaLaunchKernelEx(&config, quant_simt_kernel<T, 4, kCluster>, p); break;
+    default: cudaLaunchKernelEx(&config, quant_simt_kernel<T, 8, kCluster>, p); break;
   }
   return check_launch("quant_simt_kernel");
+}
+template <typename T> int launch_rows(const QuantAttendParams &p, cudaStream_t s) {
+  return p.out != nullptr && p.splits > 1 ? launch_rows<T, true>(p, s)
+                                          : launch_rows<T, false>(p, s);
 }
 // beside: whether its launch may overlap the end of the kernel before it, which it waits
 // for itself
@@ -428,7 +483,7 @@ extern "C" int hs_attend_quantized(int batch, const void *query, int64_t query_b
   p.status = device_status;
   if (!p.join) {
     p.out = out;
-    if (!on_tensor_cores(p, dtype)) p.splits = 1;
+    if (!on_tensor_cores(p, dtype)) p.splits = simt_splits(p);
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int status = launch_rows(p, dtype, s);

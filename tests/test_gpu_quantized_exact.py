@@ -120,3 +120,34 @@ def test_tail_behind_one_row(dtype, q_heads, heads, dim):
     query[0, :, 0] = (24 + torch.arange(q_heads) / q_heads) * np.log(2) * dim ** 0.5
     query = query.to(dtype)
     check(run(query, pool, rows, heads), query, pool, rows, heads, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("batch,q_heads,heads,dim,count", [
+    (4, 32, 8, 128, 1000), (1, 8, 2, 64, 3000), (3, 16, 16, 80, 400), (2, 6, 6, 32, 250),
+    (60, 4, 2, 96, 100), (1, 12, 1, 256, 300), (2, 5, 1, 48, 33), (1, 18, 2, 16, 8000)])
+def test_joins_of_the_cuda_core_kernel(dtype, batch, q_heads, heads, dim, count):
+    """Rows of each head, and queries off their vectors' boundary with shared rows: splits in a
+    cluster, with a workspace, or none; few rows, so that some splits see nothing, and none."""
+    pool = bounds.pool_of(40, 16, heads, dim, seed=count + dim)
+    rng = np.random.default_rng(count)
+    rows = rng.integers(0, 640, (batch, q_heads, count))
+    rows[0, 0, 20:] = -1
+    rows[-1, -1] = -1
+    query = normal(batch, q_heads, dim, seed=2, dtype=dtype)
+    some = sorted({0, batch - 1})
+    got = run(query, pool, rows, heads)
+    check(got[some], query[some], pool, rows[some], heads, dtype)
+    assert np.all(got[-1, -1] == 0)
+    counts = torch.full((batch,), count // 2, dtype=torch.int32, device=DEV)
+    got = run(query, pool, rows, heads, counts)
+    check(got[some], query[some], pool, rows[some][..., :count // 2], heads, dtype)
+    shared = rows[:, 0]
+    device = torch.zeros(batch * q_heads * dim + 1, dtype=dtype, device=DEV)
+    aside = device[1:].view(batch, q_heads, dim)  # an element past the boundary
+    aside.copy_(query)
+    config = CacheConfig(gpu_pages=len(pool), page_size=16, kv_heads=heads, head_dim=dim,
+                         device=DEV, dtype=torch.float8_e4m3fn)
+    got = attend_quantized(aside, torch.from_numpy(pool).to(DEV),
+                           torch.from_numpy(shared).to(DEV), config).double().cpu().numpy()
+    check(got[some], query[some], pool, shared[some], heads, dtype)
