@@ -6,8 +6,10 @@
 //   o += 2^(s_i + ev_i - m) v_i     l += 2^(s_i - m + kSumLift)     out = o / l 2^kSumLift
 // The two powers are taken apart: a row with a small scale may weigh nothing in o and
 // most in l. As scales are 2^-100 to 2^120, the largest term of l lies between 2^-110 and
-// 2^110, and l stays inside fp32. The maximum is kept as its row's score and exponent,
-// whose rounded sum would cost digits of the weights.
+// 2^110, and l stays inside fp32: on CUDA cores a block has at most 2^17 rows (of requests of up
+// to 2^24; it takes that many of zeros to make the sum too large), on tensor cores a large
+// sum is lowered. The maximum is kept as its row's score and exponent, whose
+// rounded sum would cost digits of the weights.
 #include "attend_quantized.cuh"
 
 namespace hs {
@@ -244,6 +246,12 @@ __global__ void __launch_bounds__(kJoinThreads) quant_merge_kernel(QuantAttendPa
   out[((int64_t)b * p.q_heads + h) * D + tid] = from_f32<T>(y * inv);
 }
 
+// Splits that leave a block of the CUDA-core kernel at most 2^17 rows: the sum of their weights
+// stays inside fp32 whatever the rows hold.
+int64_t fewest_splits(int64_t count) {
+  const int64_t n = ceil_div(count, (int64_t)1 << 17);
+  return n < kQuantMaxSplits ? n : kQuantMaxSplits;
+}
 // Splits that a call in one phase may have without a join and without a workspace: those of
 // a cluster, for the tensor-core kernel's head_dims and two blocks an SM (with one, clusters
 // leave SMs idle: 4 requests of 4,096 rows, one head of 256: 22.7 us as a cluster of 8, 17.1
@@ -296,7 +304,7 @@ int quant_splits(const QuantMmaGrid &g, int batch, int head_dim, int64_t count) 
   consider(kClusterSplits);
   for (int i = 1; i <= 4; ++i) consider(sms * i / blocks);
   consider(most);
-  return (int)best;
+  return (int)(best > fewest_splits(count) ? best : fewest_splits(count));
 }
 
 int check_sizes(int batch, int dtype, int64_t pool_blocks, int64_t count, int q_heads,
@@ -343,7 +351,9 @@ int simt_splits(const QuantAttendParams &p) {
                          (p.rows_head_stride == 0 ? p.kv_heads * per : p.q_heads);
   const int64_t places = (int64_t)sm_count() * (p.head_dim <= 64 ? 4 : p.head_dim <= 128 ? 3 : 2);
   int n = kClusterSplits;
-  while (n > 1 && (blocks * n > places || (int64_t)n * 16 > p.count + 15)) n >>= 1;
+  while (n > 1 && (blocks * n > places || (int64_t)n * 16 > p.count + 15) &&
+         n / 2 >= fewest_splits(p.count))
+    n >>= 1;
   return n;
 }
 template <typename T, bool kCluster> int launch_rows(const QuantAttendParams &p, cudaStream_t s) {

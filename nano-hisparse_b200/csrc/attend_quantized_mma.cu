@@ -32,7 +32,9 @@
 //                   this takes 72.8, 16 of 18,348, 12 heads of 256; but one result in thirty
 //                   then differed from the weights' own by a step of bf16.)
 // A weight is kept times 2^7 of the current maximum's, which is raised only when one would
-// pass it by more than 2^8.
+// pass it by more than 2^8. A row whose V has the smallest scale (zeros) adds up to 2^115 to
+// the sum: a sum that has passed 2^100 raises the maximum by 2^24, since 16,384 such rows of a
+// warp would take it past fp32, and with it what other rows hold.
 //
 // 16 requests of 32,768 rows, 32/8 heads of 128, bf16 (959 MB) take 167 us: 5.7 TB/s, 88 % of
 // a copy's rate. Rows in runs reach 5.8, single rows in any order 5.5. What else was measured
@@ -60,6 +62,7 @@ constexpr int kAhead = 2;        // units that scales are copied ahead
 constexpr int kScaleRoom = 16 * 1024;  // of all rings of scales: 8 of words or 1 of two chunks
 constexpr float kWeightLift = 7.f, kRaise = 15.f;  // lifted weights stay below 2^kRaise
 constexpr float kLeftLift = 2048.f;                // of what a weight's rounding to fp16 left
+constexpr float kSumShare = 0x1p-96f, kSumStep = 24.f;  // of a sum to compare with kRaise
 constexpr float kNothing = 1e38f;                  // base of a query that has seen nothing
 
 // parts of a query element
@@ -453,7 +456,8 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<T, kDim, kQuads>::reside
       // exponents of the weights: x in the sum, y in the output, lifted
       float x[kQuads][2], y[kQuads][2], lifted[kQuads][2], top_lifted = -INFINITY;
 #pragma unroll
-      for (int n = 0; n < kQuads; ++n)
+      for (int n = 0; n < kQuads; ++n) {
+        top_lifted = fmaxf(top_lifted, l[n] * kSumShare);
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           float dot = 0.f;
@@ -466,11 +470,13 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<T, kDim, kQuads>::reside
           lifted[n][r] = y[n][r] + base[n];
           top_lifted = fmaxf(top_lifted, lifted[n][r]);
         }
+      }
       if (__any_sync(kFullMask, top_lifted > kRaise)) {
         float f[kQuads];
 #pragma unroll
         for (int n = 0; n < kQuads; ++n) {
           float top = fmaxf(y[n][0], y[n][1]);
+          if (l[n] * kSumShare > kRaise) top = fmaxf(top, kWeightLift + kSumStep - base[n]);
 #pragma unroll
           for (int i = 4; i < 32; i <<= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, i));
           // (a base of kNothing makes f 0)

@@ -151,3 +151,50 @@ def test_joins_of_the_cuda_core_kernel(dtype, batch, q_heads, heads, dim, count)
     got = attend_quantized(aside, torch.from_numpy(pool).to(DEV),
                            torch.from_numpy(shared).to(DEV), config).double().cpu().numpy()
     check(got[some], query[some], pool, shared[some], heads, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("q_heads,dim", [(8, 16), (64, 16), (8, 128), (8, 256), (8, 24)])
+def test_millions_of_rows_of_zeros(dtype, q_heads, dim):
+    """V rows of zeros have the smallest scale, which makes their terms of the sum the largest
+    numbers, more so when scores rise by less than what moves the maximum; the last rows of the
+    request hold something."""
+    count, heads = 1 << 21, 8
+    x = np.zeros((1, 2, 3, heads, dim))
+    x[0, 0, 0, :, 0], x[0, 0, 1:, :, 0] = -1.0, 1.0
+    x[0, 1, 2] = 256 * np.random.default_rng(dim).standard_normal((heads, dim))
+    pool = ref.records(x)
+    query = torch.zeros(1, q_heads, dim)
+    query[..., 0] = 3.75 * np.log(2) * dim ** 0.5  # weights of 2^3.75 and 2^-3.75
+    query = query.to(dtype)
+    # row 0 in the first unit of every part that the request may be split into, row 2 at its end
+    rows = torch.where(torch.arange(count, device=DEV) // 32 % 512 == 0, 0, 1)[None]
+    rows[0, -32:] = 2
+    config = CacheConfig(gpu_pages=1, page_size=3, kv_heads=heads, head_dim=dim, device=DEV,
+                         dtype=torch.float8_e4m3fn)
+    got = attend_quantized(query.to(DEV), torch.from_numpy(pool).to(DEV), rows, config)
+    k, v = (ref.values(pool[0, plane], heads, dim) for plane in range(2))
+    w = np.exp(k[:, 0] @ query[0, 0].double().numpy() / np.sqrt(dim))
+    w *= [128 * 32, count - 129 * 32, 32]
+    want = np.repeat(w[2] / w.sum() * v[2], q_heads // heads, 0)
+    # a sum of 2^21 terms in fp32, a step each at most; every other error is far below
+    bound = 2.0 ** -2 * np.abs(want) + torch.finfo(dtype).smallest_normal
+    assert np.all(np.abs(got[0].double().cpu().numpy() - want) <= bound)
+
+
+def test_a_million_rows_of_zeros_on_cuda_cores():
+    """So many requests that each would have one split, whose sums fp32 could not hold."""
+    count, batch, dim = (1 << 20) + 64, 296, 9
+    x = np.zeros((1, 2, 2, 1, dim))
+    x[0, 1, 1] = np.arange(1, dim + 1)
+    pool = ref.records(x)
+    query = torch.ones(batch, 1, dim)
+    rows = torch.zeros(count, dtype=torch.int64, device=DEV)
+    rows[-16:] = 1
+    config = CacheConfig(gpu_pages=1, page_size=2, kv_heads=1, head_dim=dim, device=DEV,
+                         dtype=torch.float8_e4m3fn)
+    got = attend_quantized(query.to(DEV), torch.from_numpy(pool).to(DEV), rows.expand(batch, count),
+                           config).double().cpu().numpy()
+    want = 16 / count * x[0, 1, 1, 0]
+    # sums of 2^20 equal terms, a step of fp32 each at most
+    assert np.all(np.abs(got - want) <= 2.0 ** -3 * want)
