@@ -63,9 +63,10 @@ class _LayerState:
 class DecodeBatch:
     """Decode hot path for a fixed set of requests of a RowCache.
 
-    minimum / maximum: {request_id: [layers, pages, Hkv, D]} Quest metadata.
-    Queries have the cache's dtype; those over a cache held in 8 bits may be
-    float32, float16 or bfloat16.
+    minimum / maximum: {request_id: [layers, pages, Hkv, D]} Quest metadata of the
+    config's ``metadata_dtype`` (bfloat16 where rows are held in 8 bits). Queries have
+    the cache's dtype; those over a cache held in 8 bits may be float32, float16 or
+    bfloat16.
     """
 
     def __init__(self, cache: RowCache, request_ids, layers, minimum, maximum, top_pages,
@@ -95,6 +96,9 @@ class DecodeBatch:
         self.width = top_pages * cfg.page_size
         if self.width > cache.hot_config.max_union_rows:
             raise ValueError("top-k width/union exceeds the admitted max_union_rows")
+        if any(t[r].dtype != cfg.metadata_dtype for t in (minimum, maximum)
+               for r in self.request_ids):  # the kernels read addresses
+            raise ValueError(f"minimum and maximum must be {cfg.metadata_dtype}")
         self.max_pages = max(int(minimum[r].shape[1]) for r in self.request_ids)
         self.hot_rows = cache.hot_config.hot_rows
         self.layers = [_LayerState(self, layer) for layer in range(layers)]
@@ -192,6 +196,8 @@ class DecodeBatch:
             raise ValueError("query must be [batch, q_heads, head_dim]")
         if out is None:
             out = torch.empty_like(query)
+        elif out.shape != query.shape or out.dtype != query.dtype or not out.is_contiguous():
+            raise ValueError("out must be contiguous, of the query's shape and dtype")
         if counts is None:
             counts = st.counts
         elif counts.shape != (b, 3) or counts.dtype != torch.int64 or not counts.is_contiguous():
