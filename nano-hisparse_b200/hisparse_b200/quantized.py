@@ -25,7 +25,8 @@ from . import _lib
 _VALUES = (torch.float32, torch.float16, torch.bfloat16)
 
 
-def _check_pool(pool, config):
+def check_pool(pool, config):
+    """Blocks of a pool held in 8 bits; raises if it is not one of `config`."""
     if not config.quantized:
         raise ValueError("config must hold its rows in 8 bits (dtype torch.float8_e4m3fn)")
     shape = pool.shape
@@ -50,7 +51,7 @@ def append_quantized(k, v, within, count, pool_block, pool, minimum_ptrs, maximu
     """
     index = _lib.one_device(k, v, within, count, pool_block, pool, minimum_ptrs, maximum_ptrs,
                             summary_ptrs, host_block)
-    blocks = _check_pool(pool, config)
+    blocks = check_pool(pool, config)
     shape = k.shape
     if v.shape != shape or len(shape) != 4 or shape[2:] != (config.kv_heads, config.head_dim):
         raise ValueError("expected matching [batch, tokens, kv_heads, head_dim] K/V")
@@ -119,7 +120,7 @@ def read_quantized(pool, rows, config, dtype=torch.bfloat16):
     one beyond the pool too, and raises the device flag. Runs on the current
     stream."""
     index = _lib.one_device(pool, rows)
-    blocks = _check_pool(pool, config)
+    blocks = check_pool(pool, config)
     if rows.dtype != torch.int64:
         raise ValueError("rows must be int64")
     if dtype not in _VALUES:
@@ -147,7 +148,7 @@ def attend_quantized(query, pool, rows, config, counts=None):
     the current stream.
     """
     index = _lib.one_device(query, pool, rows, counts)
-    blocks = _check_pool(pool, config)
+    blocks = check_pool(pool, config)
     shape, kv_heads = query.shape, config.kv_heads
     if len(shape) != 3 or shape[2] != config.head_dim:
         raise ValueError("query must be [batch, heads, head_dim]")

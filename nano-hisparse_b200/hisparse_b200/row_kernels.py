@@ -53,12 +53,17 @@ def gather_rows(host, pool, plan, config):
     host: MappedHost (or pinned tensor) [host_pages, 2, P, Hkv, D]; pool: CUDA
     tensor [gpu_pages, 2, P, Hkv, D] of the same dtype; plan: RowPlan whose
     miss_host_rows / miss_device_rows are the resolver's compact prefix.
+    A cache held in 8 bits: uint8 stores of the config's page_shape.
     Runs on the current stream.
     """
     mapped = _host_alias(host)
     _lib.require_cuda(pool, plan.miss_host_rows, plan.miss_device_rows)
     if mapped.tensor.dtype != pool.dtype or mapped.tensor.shape[1:] != pool.shape[1:]:
         raise ValueError("host store and pool layouts differ")
+    if held_in_8_bits(config):
+        from .quantized import check_pool
+
+        check_pool(pool, config)
     lib = _lib.load()
     miss_host = plan.miss_host_rows.contiguous()
     miss_device = plan.miss_device_rows.contiguous()
@@ -76,9 +81,10 @@ def gather_rows(host, pool, plan, config):
 def attend_rows(query, pool, rows, config):
     """Decode attention of query [Hq, D] over physical rows of the pool.
 
-    On a pool held in 8 bits this is ``attend_quantized``. rows: int64 [Hq, K] (a stride-0 expansion of a shared [K] vector is read
-    once per GQA group) or [K]; -1 entries are masked; a head with no valid row
-    gets zeros. Output has the query's dtype.
+    On a pool held in 8 bits this is ``attend_quantized``. rows: int64 [Hq, K] (a
+    stride-0 expansion of a shared [K] vector is read once per GQA group) or [K]; -1
+    entries are masked; a head with no valid row gets zeros. Output has the query's
+    dtype.
     """
     _lib.require_cuda(query, pool, rows)
     if rows.ndim == 1:

@@ -7,8 +7,10 @@ import torch
 
 import quantized_bounds as bounds
 import quantized_reference as ref
-from hisparse_b200 import CacheConfig, DecodeBatch, HotConfig, RowCache, _lib
+from hisparse_b200 import (CacheConfig, DecodeBatch, HotConfig, MappedHost, RowCache, _lib,
+                           gather_rows)
 from hisparse_b200.batched import DecodeGraph
+from hisparse_b200.row_index import RowPlan
 from hisparse_b200.sharded import head_slice
 
 pytestmark = pytest.mark.gpu
@@ -161,3 +163,20 @@ def test_graph_of_a_plain_cache_takes_its_dtype():
     with pytest.raises(ValueError, match="the cache's dtype"):
         DecodeGraph([batch], 1, dtype=torch.float32)
     assert DecodeGraph([batch], 1, dtype=torch.bfloat16).outputs[0].dtype == torch.bfloat16
+
+
+def test_gather_refuses_other_records():
+    """Pool and host store agree with each other but not with the configuration."""
+    def store(dim, page):
+        config = CacheConfig(gpu_pages=2, page_size=page, kv_heads=2, head_dim=dim, device=DEV,
+                             dtype=torch.float8_e4m3fn)
+        return config, torch.zeros((2, *config.page_shape), dtype=torch.uint8)
+
+    config, own = store(64, 8)
+    row = torch.zeros(1, dtype=torch.int64, device=DEV)
+    plan = RowPlan(None, row, row, None)
+    others = [store(32, 8)[1], store(64, 4)[1], torch.zeros(2, 2, 8, 2, 64, dtype=torch.float16)]
+    for other in others:
+        with pytest.raises(ValueError, match="pool must be"):
+            gather_rows(MappedHost(other.pin_memory()), other.to(DEV), plan, config)
+    gather_rows(MappedHost(own.pin_memory()), own.to(DEV), plan, config)
