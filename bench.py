@@ -10,7 +10,8 @@ the rest only in pinned host memory. Weak scaling: every rank decodes its own
 
   python bench.py [--gpus N] [--steps K] [--warmup W] [--impl reference]
 
-Prints one JSON line on rank 0. `--impl reference` times the CPU restatement
+Prints one JSON line on rank 0. `--kv-dtype e4m3` holds the cache in 8 bits (a
+line of its own beside the bench line). `--impl reference` times the CPU restatement
 of the reference's path (the oracle) on the host cores instead.
 """
 
@@ -41,6 +42,7 @@ TOP_PAGES = 2048 // PAGE          # Quest budget of 2048 tokens incl. sink and t
 HOT_ROWS = 2 * 2048               # reference default: 2 x max_union_rows
 RESIDENT_FRACTION = 0.25
 DTYPE = torch.bfloat16
+KV = "bf16"  # how the cache holds rows; "e4m3": in 8 bits (--kv-dtype)
 MICRO = 2  # request groups pipelined on separate streams
 TRANSFER = "shared"  # the micro-batches' gathers share one transfer stream
 SETTLE_STEPS = 12  # untimed steps that fill the hot buffers before the warm-up steps
@@ -62,9 +64,11 @@ def workload_config():
         "requests_per_gpu": REQUESTS, "layers": LAYERS, "context": CONTEXT,
         "q_heads": Q_HEADS, "kv_heads": KV_HEADS, "head_dim": HEAD_DIM, "page_size": PAGE,
         "quest_budget_tokens": TOP_PAGES * PAGE, "hot_rows": HOT_ROWS,
-        "resident_fraction": RESIDENT_FRACTION, "kv_dtype": "bf16", "accumulate": "fp32",
+        "resident_fraction": RESIDENT_FRACTION, "kv_dtype": KV, "accumulate": "fp32",
         "queries": "N(0,1) per request, layer and step (seed 1)",
-        "kv": "N(0,1) bf16, page min/max metadata from K (seed 1)",
+        "kv": "N(0,1) bf16, page min/max metadata from K (seed 1)" if KV == "bf16" else
+              "N(0,1) bf16 held as e4m3 codes with a scale for each row and head, page min/max "
+              "metadata from the held K (seed 1)",
         "l2": "inputs larger than L2 (about 12 GiB of metadata and KV rows read per step)",
         "parallelism": "requests sharded over ranks, no collective on the hot path",
         "microbatches": MICRO, "transfer_streams": TRANSFER,
@@ -207,26 +211,45 @@ def host_store_pages(wanted_pages, page_bytes, log):
     return pages
 
 
+def quantized_pages(kv, minimum, maximum, config):
+    """Pages kv [n, 2, P, Hkv, D] as they are held in 8 bits; the pages' bounds [n, Hkv, D] become
+    those of the held K."""
+    from hisparse_b200 import append_quantized
+
+    n, device = len(kv), kv.device
+    pages = torch.empty((n, *config.page_shape), dtype=torch.uint8, device=device)
+    minimum.fill_(math.inf)
+    maximum.fill_(-math.inf)
+    mean = torch.empty(minimum.shape, device=device)
+    first = torch.zeros(n, dtype=torch.int32, device=device)
+    pointers = [t.data_ptr() + torch.arange(n, device=device) * t[0].nbytes
+                for t in (minimum, maximum, mean)]
+    append_quantized(kv[:, 0], kv[:, 1], first, first + config.page_size,
+                     torch.arange(n, device=device), pages, *pointers, config)
+    return pages
+
+
 def build_workload(device, seed, log):
-    from hisparse_b200 import CacheConfig, DecodeBatch, HotConfig, RowCache
+    from hisparse_b200 import CacheConfig, HotConfig, RowCache
 
     n = math.ceil(CONTEXT / PAGE)
     hot = HotConfig(TOP_PAGES * PAGE, HOT_ROWS)
     hot_blocks = hot.hot_blocks(PAGE)
     resident_pages = int(round(n * RESIDENT_FRACTION))
     units = REQUESTS * LAYERS
-    page_bytes = 2 * PAGE * KV_HEADS * HEAD_DIM * 2
+    dtype = torch.float8_e4m3fn if KV == "e4m3" else DTYPE
+    page_bytes = 2 * PAGE * CacheConfig(kv_heads=KV_HEADS, head_dim=HEAD_DIM, dtype=dtype).row_bytes
     host_pages = host_store_pages(units * n, page_bytes, log)
     HOST_STORE.update(gib_per_rank=round(host_pages * page_bytes / 2**30, 2),
                       shared_by_units=host_pages < units * n)
     config = CacheConfig(gpu_pages=units * (resident_pages + hot_blocks), host_pages=host_pages,
                          page_size=PAGE, kv_heads=KV_HEADS, head_dim=HEAD_DIM,
-                         device=str(device), dtype=DTYPE,
+                         device=str(device), dtype=dtype,
                          index_budget_bytes=1 << 40)
     t0 = time.time()
-    host = torch.empty((config.host_pages, 2, PAGE, KV_HEADS, HEAD_DIM), dtype=DTYPE,
+    host = torch.empty((config.host_pages, *config.page_shape), dtype=config.storage_dtype,
                        pin_memory=True)
-    log(f"pinned host store {host.numel() * 2 / 2**30:.1f} GiB in {time.time() - t0:.1f}s")
+    log(f"pinned host store {host.nbytes / 2**30:.1f} GiB in {time.time() - t0:.1f}s")
     cache = RowCache(config, hot, host=host)
     gen = torch.Generator(device=device).manual_seed(seed)
     rng = np.random.default_rng(seed)
@@ -240,8 +263,11 @@ def build_workload(device, seed, log):
             base = ((r * LAYERS + layer) * n) % (host_pages - n + 1)
             kv = torch.randn((n, 2, PAGE, KV_HEADS, HEAD_DIM), generator=gen, device=device,
                              dtype=torch.float32).to(DTYPE)
-            mins[r][layer] = kv[:, 0].amin(1)
-            maxs[r][layer] = kv[:, 0].amax(1)
+            if KV == "e4m3":
+                kv = quantized_pages(kv, mins[r][layer], maxs[r][layer], config)
+            else:
+                mins[r][layer] = kv[:, 0].amin(1)
+                maxs[r][layer] = kv[:, 0].amax(1)
             host[base:base + n].copy_(kv, non_blocking=True)
             # 25% of the pages resident: the two tail pages plus a uniform sample
             chosen = rng.choice(n - 2, size=resident_pages - 2, replace=False)
@@ -278,10 +304,9 @@ def make_batches(cache, mins, maxs, micro, device):
     return groups, batches
 
 
-def bytes_per_unit(valid_rows, misses):
+def bytes_per_unit(valid_rows, misses, row):
     """Algorithmic HBM bytes of one (request, layer): Quest metadata (min+max),
-    K+V of every selected row, and the miss rows written into the pool."""
-    row = 2 * KV_HEADS * HEAD_DIM * 2
+    K+V (`row` bytes) of every selected row, and the miss rows written into the pool."""
     meta = 2 * math.ceil(CONTEXT / PAGE) * KV_HEADS * HEAD_DIM * 2
     return meta + valid_rows * row + misses * row
 
@@ -409,7 +434,7 @@ def run_gpu(args, rank, world, local_rank, log):
     clocks = sampler.stop()
     elapsed_ms = max_over_ranks(start.elapsed_time(end))
     timed_counts = counts[warmup:].cpu().numpy()  # [steps, L, B, 3]
-    row_bytes = 2 * KV_HEADS * HEAD_DIM * 2
+    row_bytes = 2 * cache.config.row_bytes  # K and V
 
     # ---- gather roofline: the same step captured with CUDA events around every
     # gather launch (on the transfer stream it runs on), replayed W + K times on
@@ -499,7 +524,8 @@ def run_gpu(args, rank, world, local_rank, log):
     # micro-batches' gathers overlap on the one host link: the link's rate is
     # the bytes over the time any gather is running
     gather_gbs = eager_gather_bytes / (gather_busy_ms * 1e-3) / 1e9
-    hbm_bytes = sum(bytes_per_unit(int(timed_counts[s, l, b].sum()), int(timed_counts[s, l, b, 2]))
+    hbm_bytes = sum(bytes_per_unit(int(timed_counts[s, l, b].sum()), int(timed_counts[s, l, b, 2]),
+                                   row_bytes)
                     for s in range(steps) for l in range(LAYERS) for b in range(REQUESTS))
     attend_ms = kernel_ms["attend_ready"] + kernel_ms["attend_gathered"]
     attend_bytes = int(eager.sum()) * row_bytes
@@ -546,7 +572,8 @@ def run_gpu(args, rank, world, local_rank, log):
     value = tokens / (elapsed_ms * 1e-3)
     io_bytes = LAYERS * REQUESTS * Q_HEADS * HEAD_DIM * 2
     result = {
-        "metric": METRIC, "value": round(value, 2), "unit": "tok/s", "n_gpus": world,
+        "metric": METRIC if KV == "bf16" else METRIC + " (cache held in 8 bits)",
+        "value": round(value, 2), "unit": "tok/s", "n_gpus": world,
         "steps": steps, "warmup": warmup, "ms_per_step": round(elapsed_ms / steps, 3),
         "higher_is_better": True, "scaling": "weak", "vs_baseline": None, "dtype": "bf16",
         "data": "synthetic", "config": workload_config(),
@@ -562,10 +589,13 @@ def run_gpu(args, rank, world, local_rank, log):
             "peak": round(link_peak, 2), "unit": "GB/s", "frac": round(live_gbs / link_peak, 4),
             "peak_source": "measured in bench.py: pinned host->device cudaMemcpyAsync, 1 GiB, "
                            "this GPU alone (hostlink: the same with every rank copying)",
-            "traffic": round(PCIE_READ_PER_GATHERED_BYTE * live_bytes / len(live)),
-            "traffic_definition": "PCIe read bytes per launch (ncu pcie__read_bytes.sum, scaled "
-                                  "from a one-layer capture by the bytes gathered)",
-            "achieved_definition": "miss rows x 4 KiB per launch / launch duration, CUDA events "
+            # the ratio was captured with rows of 2,048 bytes
+            **({"traffic": round(PCIE_READ_PER_GATHERED_BYTE * live_bytes / len(live)),
+                "traffic_definition": "PCIe read bytes per launch (ncu pcie__read_bytes.sum, "
+                                      "scaled from a one-layer capture by the bytes gathered)"}
+               if KV == "bf16" else {}),
+            "achieved_definition": f"miss rows x {'4 KiB' if KV == 'bf16' else f'{row_bytes} bytes'}"
+                                   " per launch / launch duration, CUDA events "
                                    "around each gather on its transfer stream, captured in an "
                                    "instrumented copy of the step graph replayed W+K steps "
                                    "after the headline region; the last step's launches",
@@ -1273,7 +1303,7 @@ def cpu_sample(seed=1, budget_s=10.0, threads=None, log=print):
 
 
 def main():
-    global REQUESTS, LAYERS, MICRO, TRANSFER
+    global REQUESTS, LAYERS, MICRO, TRANSFER, KV
     parser = argparse.ArgumentParser(description=__doc__.split("\n\n")[0])
     parser.add_argument("--gpus", type=int, default=1)
     parser.add_argument("--steps", type=int, default=10)
@@ -1295,11 +1325,16 @@ def main():
                              "resident-fraction sweep), config4 (256 requests sharded over the "
                              "GPUs) or config5 (one 1M-token request, KV heads split over 1, 2 "
                              "or 4 GPUs)")
+    parser.add_argument("--kv-dtype", choices=["bf16", "e4m3"], default=KV,
+                        help="how config2's cache holds rows: bf16 (the bench line) or e4m3 (in 8 "
+                             "bits: a line of its own, without a baseline)")
     parser.add_argument("--requests", type=int, default=REQUESTS)
     parser.add_argument("--layers", type=int, default=LAYERS)
     args = parser.parse_args()
+    if args.kv_dtype != KV and (args.workload != "config2" or args.impl == "reference"):
+        parser.error("--kv-dtype goes with config2 on this library")
     REQUESTS, LAYERS, MICRO = args.requests, args.layers, args.microbatches
-    TRANSFER = args.transfer
+    TRANSFER, KV = args.transfer, args.kv_dtype
     rank = int(os.environ.get("RANK", 0))
     world = int(os.environ.get("WORLD_SIZE", 1))
     local_rank = int(os.environ.get("LOCAL_RANK", 0))
@@ -1343,7 +1378,7 @@ def main():
                 print(json.dumps(result), flush=True)
             return
         result = run_gpu(args, rank, world, local_rank, log)
-        if world in (2, 4) and not args.no_config5:
+        if world in (2, 4) and not args.no_config5 and KV == "bf16":
             # configuration 5 (one 1M-token request, its KV heads split over these
             # ranks) measured after the configuration-2 line, with that workload's
             # device and pinned host memory released first
@@ -1363,7 +1398,7 @@ def main():
                                                     "per_rank")}
         os.sched_setaffinity(0, all_cpus)  # the CPU baseline uses every host core
         if rank == 0:
-            if world == 1 and not args.no_cpu_baseline:
+            if world == 1 and not args.no_cpu_baseline and KV == "bf16":
                 result["cpu_baseline"] = cpu_sample(log=log)
             print(json.dumps(result), flush=True)
     finally:
