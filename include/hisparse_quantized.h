@@ -82,7 +82,8 @@ HS_API int hs_read_quantized(const void *pool, int64_t pool_blocks, const int64_
  * are the values held; query head h reads KV head h / (q_heads / kv_heads). fp32
  * sums; zeros where nothing is seen. rows int64: head h of request b starts at
  * b * rows_batch_stride + h * rows_head_stride (0: the heads share their rows,
- * which is the fast form). query [batch, q_heads, head_dim] with heads adjacent
+ * which is the fast form, where head_dim is also a multiple of 16 and query and its
+ * stride are multiples of four elements; other calls run on CUDA cores). query [batch, q_heads, head_dim] with heads adjacent
  * and requests query_batch_stride elements apart, out contiguous, both of `dtype`.
  * counts below 0 or above `count` are clamped. A row beyond the pool is skipped
  * and raises HS_DEV_ROW_OUT_OF_RANGE.
@@ -93,8 +94,8 @@ HS_API int hs_read_quantized(const void *pool, int64_t pool_blocks, const int64_
  * (counts NULL: count). phase is 0 or 1 and a merge of `phases` joins phases
  * 0 .. phases - 1, all of one batch, dtype, sizes and `count`.
  *
- * The workspace (for `phases` phases, 1 for the plain form) is 16-byte aligned and
- * needs no initialisation; calls that may overlap on the GPU need separate ones.
+ * The workspace (phases: 1 for the plain form, 2 for the phase form and its merge, however
+ * many phases that joins) is 16-byte aligned and needs no initialisation; calls that may overlap on the GPU need separate ones.
  */
 HS_API size_t hs_attend_quantized_workspace_bytes(int batch, int phases, int dtype,
                                                   int q_heads, int kv_heads, int head_dim,

@@ -13,9 +13,11 @@
 //   S^T = K Q^T     m16n8k32 in e4m3: the codes go from ldmatrix to the tensor core as
 //                   they are. Q is taken apart into e4m3 numbers, each a sixteenth of the
 //                   one before it (q = q0 + q1 / 16 + ...): 2 parts hold bf16, 3 fp16 and
-//                   6 fp32 exactly, since each part leaves at most 2^-4 of what it takes.
-//                   Two parts of a query are neighbouring columns, whose sums meet in one
-//                   lane. The products are exact and added in fp32 (measured: within
+//                   6 fp32 exactly, since each part leaves at most 2^-4 of what it takes,
+//                   but for elements below 2^-13 of the query's largest: those are off by up
+//                   to 2^-21 of it in bf16 (e4m3 numbers end there), 2^-25 in fp16. Two
+//                   parts of a query are neighbouring columns, whose sums meet in one lane.
+//                   The products are exact and added in fp32 (measured: within
 //                   2^-20 of the largest, as fp16 products are).
 //   O^T += V^T P^T  m16n8k16 in fp16, which holds every e4m3 number. V through
 //                   ldmatrix.trans, whose 16-bit unit is two neighbouring elements of a
@@ -29,7 +31,7 @@
 //                   as many products, 2^-32 of the largest weight a row where a result's
 //                   own rounding is 2^-8. (A single product, 11 bits, took 39.5 us where this
 //                   takes 40.7, 8 requests of 16,384 rows, 28/4 heads of 128, and 66.6 where
-//                   this takes 72.8, 16 of 18,348, 12 heads of 256; but one result in thirty
+//                   this takes 72.8, 16 of 18,348, 12 heads of 256; but one result in twelve
 //                   then differed from the weights' own by a step of bf16.)
 // A weight is kept times 2^7 of the current maximum's, which is raised only when one would
 // pass it by more than 2^8. A row whose V has the smallest scale (zeros) adds up to 2^115 to
@@ -42,8 +44,8 @@
 // 197, since 32 of its 96 requests a tile were for one byte; whole records copied by one
 // warp of the block 208, by all warps 208; boxes of tiled copies 185 (75 clocks of the copy
 // engine a box); fragments straight from global memory 250. With 7 query heads a KV head the
-// warps' instructions are level with the reads (8 requests of 16,384 rows, 4 KV heads: 41 us,
-// floor 20.7), with more of them ahead.
+// warps' instructions are level with the reads (8 requests of 16,384 rows, 4 KV heads: 38 to
+// 41 us, floor 20.7), with more of them ahead.
 #include <type_traits>
 
 #include "attend_quantized.cuh"
