@@ -151,6 +151,32 @@ def test_kv_heads_split_over_shards(monkeypatch, dtype):
     assert not _lib.device_flags(DEV)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [64, 33])
+def test_merge_of_one_phase(dtype, dim):
+    """A merge joins as many phases as it is told; what the other one left is not looked at."""
+    batch, q_heads, heads, count = 3, 8, 2, 300
+    pool = bounds.pool_of(25, PAGE, heads, dim, seed=dim)
+    rows = np.stack([np.random.default_rng(s).permutation(400)[:count] for s in range(batch)])
+    query = torch.randn(batch, q_heads, dim, generator=torch.Generator().manual_seed(5)).to(DEV, dtype)
+    lib, code, stream = _lib.load(), _lib.dtype_code(dtype), _lib.stream_of(DEV)
+    nbytes = lib.hs_attend_quantized_workspace_bytes(batch, 2, code, q_heads, heads, dim, count)
+    workspace = torch.full((nbytes,), 255, dtype=torch.uint8, device=DEV)  # NaN
+    device, at = torch.from_numpy(pool).to(DEV), torch.from_numpy(rows).to(DEV)
+    given = torch.tensor([[300, 7], [150, 7], [0, 7]], device=DEV)
+    out = torch.empty_like(query)
+    _lib.check(lib.hs_attend_quantized_phase(
+        batch, query.data_ptr(), q_heads * dim, code, device.data_ptr(), 25, at.data_ptr(), count,
+        count, given.data_ptr(), 2, 0, 1, 0, q_heads, heads, dim, PAGE, workspace.data_ptr(), nbytes,
+        None, stream))
+    _lib.check(lib.hs_attend_quantized_merge(batch, 1, out.data_ptr(), code, q_heads, heads, dim,
+                                             count, workspace.data_ptr(), nbytes, stream))
+    want, bound = bounds.attend(query.double().cpu().numpy(), pool, rows, heads, dtype,
+                                [300, 150, 0])
+    assert np.all(np.abs(out.double().cpu().numpy() - want) <= bound)
+    assert torch.all(out[2] == 0)
+
+
 def test_graph_of_a_plain_cache_takes_its_dtype():
     hot = HotConfig(TOP * PAGE, TOP * PAGE)
     config = CacheConfig(gpu_pages=40, host_pages=8, page_size=PAGE, kv_heads=2, head_dim=32,

@@ -198,3 +198,22 @@ def test_a_million_rows_of_zeros_on_cuda_cores():
     want = 16 / count * x[0, 1, 1, 0]
     # sums of 2^20 equal terms, a step of fp32 each at most
     assert np.all(np.abs(got - want) <= 2.0 ** -3 * want)
+
+
+def test_cluster_of_the_cuda_core_kernel_in_a_graph():
+    """Captured with rows of each head and replayed with others."""
+    pool = bounds.pool_of(20, 16, 2, 64, seed=3)
+    config = CacheConfig(gpu_pages=20, page_size=16, kv_heads=2, head_dim=64, device=DEV,
+                         dtype=torch.float8_e4m3fn)
+    device = torch.from_numpy(pool).to(DEV)
+    query = normal(2, 8, 64, seed=4, dtype=torch.bfloat16).to(DEV)
+    rows = torch.zeros(2, 8, 200, dtype=torch.int64, device=DEV)
+    attend_quantized(query, device, rows, config)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = attend_quantized(query, device, rows, config)
+    for seed in range(3):
+        rows.copy_(torch.from_numpy(np.random.default_rng(seed).integers(-1, 320, rows.shape)))
+        graph.replay()
+        check(captured.double().cpu().numpy(), query.cpu(), pool, rows.cpu().numpy(), 2,
+              torch.bfloat16)
