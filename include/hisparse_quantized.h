@@ -83,7 +83,8 @@ HS_API int hs_read_quantized(const void *pool, int64_t pool_blocks, const int64_
  * sums; zeros where nothing is seen. rows int64: head h of request b starts at
  * b * rows_batch_stride + h * rows_head_stride (0: the heads share their rows,
  * which is the fast form, where head_dim is also a multiple of 16 and query and its
- * stride are multiples of four elements; other calls run on CUDA cores). query [batch, q_heads, head_dim] with heads adjacent
+ * stride are multiples of four elements; other calls run on CUDA cores). query
+ * [batch, q_heads, head_dim] with heads adjacent
  * and requests query_batch_stride elements apart, out contiguous, both of `dtype`.
  * counts below 0 or above `count` are clamped. A row beyond the pool is skipped
  * and raises HS_DEV_ROW_OUT_OF_RANGE.
@@ -95,7 +96,8 @@ HS_API int hs_read_quantized(const void *pool, int64_t pool_blocks, const int64_
  * 0 .. phases - 1, all of one batch, dtype, sizes and `count`.
  *
  * The workspace (phases: 1 for the plain form, 2 for the phase form and its merge, however
- * many phases that joins) is 16-byte aligned and needs no initialisation; calls that may overlap on the GPU need separate ones.
+ * many phases that joins) is 16-byte aligned and needs no initialisation; calls that may
+ * overlap on the GPU need separate ones.
  */
 HS_API size_t hs_attend_quantized_workspace_bytes(int batch, int phases, int dtype,
                                                   int q_heads, int kv_heads, int head_dim,

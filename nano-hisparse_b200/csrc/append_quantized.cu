@@ -7,8 +7,8 @@
 // meet in shared memory and are written together with the padding: a byte at a time they
 // would be separate transfers over the host link. Bounds and mean come from the values
 // held, so that they do not depend on how the rows were split over calls (the mean but for
-// the order of its sum); the page's earlier rows are read back for the mean. Where a chunk may have many rows, several
-// warps (slices) share a head.
+// the order of its sum); the page's earlier rows are read back for the mean. Where a chunk
+// may have many rows, several warps (slices) share a head.
 //
 // A prompt (2,048 pages of 16 rows, 8 heads of 128, bf16: 227 MB) takes 61 us, 57 % of a
 // copy's rate. Its instructions bound it, about 170 for two rows of a head (issue slots

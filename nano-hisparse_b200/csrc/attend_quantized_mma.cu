@@ -532,7 +532,8 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<T, kDim, kQuads>::reside
 #pragma unroll
           for (int n = 0; n < kOutputTiles; ++n) {
             mma_f16(o[n][c + u], lo.x, lo.y, hi.x, hi.y, w[n][0], w[n][1]);
-            if constexpr (kPaired) mma_f16(o[n][c + u], lo.x, lo.y, hi.x, hi.y, left[n][0], left[n][1]);
+            if constexpr (kPaired)
+              mma_f16(o[n][c + u], lo.x, lo.y, hi.x, hi.y, left[n][0], left[n][1]);
           }
         }
       }
